@@ -54,6 +54,20 @@ class Matrix(C.Structure):
     _fields_ = [("data", vp), ("rs", i64), ("cs", i64), ("bstride", i64 * FA_MAX_BATCH_DIMS)]
 
 
+FA_KV_BLOCK = 64
+
+
+class KvCache(C.Structure):
+    """fa_kv_cache: a pool of key/value blocks in device memory."""
+    _fields_ = [("codes", vp), ("scales", vp), ("blocks", i32), ("kv_heads", i32), ("head_dim", i32)]
+
+
+class KvBatch(C.Structure):
+    """fa_kv_batch: the sequences of one call (block tables, lengths, row starts)."""
+    _fields_ = [("tables", vp), ("table_stride", i32), ("lengths", vp), ("cu_rows", vp), ("nseq", i32),
+                ("rows", i64)]
+
+
 class GemmaConfig(C.Structure):
     _fields_ = [("hidden_size", i32), ("num_hidden_layers", i32), ("num_attention_heads", i32),
                 ("num_key_value_heads", i32), ("head_dim", i32), ("intermediate_size", i32), ("vocab_size", i32),
@@ -64,6 +78,9 @@ class GemmaConfig(C.Structure):
                 ("layer_head_dim", i32 * 64), ("layer_kv_heads", i32 * 64), ("layer_sliding", i32 * 64),
                 ("dense_act", i32 * 4)]
 
+
+P_kvc = C.POINTER(KvCache)
+P_kvb = C.POINTER(KvBatch)
 
 _SIGS = {
     "fa_create": (C.c_int, [C.c_int, C.POINTER(vp)]),
@@ -91,6 +108,15 @@ _SIGS = {
                                i64, i64, f32, vp]),
     "fa_attention_dev": (C.c_int, [vp, vp, vp, vp, i32, i32, i32, i32, i32, i64, i64, i64, i64, i64, i64, vp, i64,
                                    i64, i64, i64, f32, vp]),
+    "fa_kv_codes_bytes": (C.c_size_t, [i32, i32, i32]),
+    "fa_kv_write": (C.c_int, [vp, P_kvc, P_kvb, C.c_int, vp, i64, i64, vp, i64, i64]),
+    "fa_kv_write_dev": (C.c_int, [vp, P_kvc, P_kvb, C.c_int, vp, i64, i64, vp, i64, i64]),
+    "fa_kv_read": (C.c_int, [vp, P_kvc, P_kvb, C.c_int, vp, vp]),
+    "fa_kv_read_dev": (C.c_int, [vp, P_kvc, P_kvb, C.c_int, vp, vp]),
+    "fa_kv_attention": (C.c_int, [vp, P_kvc, P_kvb, C.c_int, vp, i64, i64, i32, C.c_int, i32, f32, vp]),
+    "fa_kv_attention_dev": (C.c_int, [vp, P_kvc, P_kvb, C.c_int, vp, i64, i64, i32, C.c_int, i32, f32, vp, vp,
+                                      C.c_size_t]),
+    "fa_kv_attention_work": (C.c_int, [P_kvc, P_kvb, i32, C.POINTER(C.c_size_t)]),
     "fa_similarities_topk": (C.c_int, [vp, vp, i64, vp, i64, i32, i32, vp, vp]),
     "fa_similarities_topk_dev": (C.c_int, [vp, vp, i64, vp, i64, i32, i32, vp, vp]),
     "fa_similarities_topk_dev_noalloc": (C.c_int, [vp, vp, i64, vp, i64, i32, i32, vp, vp]),

@@ -58,6 +58,8 @@ enum : size_t {
   S_BPLANES,                            // B operand as bf16 [n x k] planes (matmul drop-in)
   S_APACK,                              // A operand packed to [nb][m][kp] (strided matmul)
   S_ATTN,                               // key and value images (attention drop-in)
+  S_KV,                                 // batch arrays of the key/value cache's host entry points
+  S_KV_PARTS,                           // parts of a split token axis (attention over the cache)
   S_COUNT
 };
 }  // namespace slots

@@ -1,0 +1,623 @@
+// Attention of new tokens over the 8-bit key/value cache:
+//   o_i = sum_j softmax_j(scale * q_i . k_j) v_j
+// over the tokens j that query i sees, one pass over the cached blocks with
+// the running maximum and sum of the softmax.
+//
+// A query row is (new token, query head of the key/value head's group):
+// heads that share keys share a tile. Scores are computed transposed, S^T =
+// K . Q^T, and so is the output, O^T = V^T . P^T: the MFMA leaves a lane the
+// scores of its row against the tokens whose values it needs next as an
+// operand (the value layout is permuted to that order), so weights stay in
+// registers. Codes become bf16 exactly; a block's key scale multiplies its
+// scores, its value scale its weights (both powers of two).
+//
+// float32 queries, and the weights for them, enter as three exact bf16 terms
+// (24 bits, the whole range of float32), bf16 queries as they are and their
+// weights rounded to bf16, as many bits as the outputs keep. Scores,
+// statistics and sums are float32.
+#include <algorithm>
+
+#include "device_math.h"
+#include "kvcache.h"
+
+namespace fa {
+namespace {
+
+constexpr int kTileRows = 16;   // query rows of a work item
+constexpr int kWaves = 4;       // waves of a workgroup: each every fourth block
+constexpr int kMinChunk = 4;    // blocks of a split part, at least (one per wave)
+constexpr int kTarget = 1024;   // split parts aimed at: two rounds of two workgroups on each of 256 CUs
+constexpr int kMergeDims = 128; // dims that the waves' results are merged at a time
+// Weights are multiplied by the value scale 2^e and this, so that sums of 2^20
+// times float32's largest values stay finite; the result is multiplied back.
+constexpr float kWeightScale = 0x1p-24f;
+
+// The work of one call: tiles of kTileRows rows of a sequence's n * G, for
+// each key/value head, over the blocks they see; in a planned call the blocks
+// are cut into parts of about equal size over the whole batch.
+struct AttnArgs {
+  KvArgs c;
+  const void* q;
+  int64_t q_st, q_sh;
+  int32_t H, G;
+  int32_t causal, window;
+  float scale2;  // scale * log2 e
+  void* out;
+  float* part;    // planned: [parts][16][Dp] sums, then [parts][16][2] maximum, sum
+  int64_t parts;  // parts that the scratch holds
+  int32_t vec;
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Tokens that the rows of new tokens t0 .. t1 (positions len - n + t) see at
+// all: [lo, hi).
+__device__ __forceinline__ void seen_range(const AttnArgs& a, const KvSeq& s, int t0, int t1, int* lo, int* hi) {
+  const int64_t p0 = (int64_t)s.len - s.n + t0, p1 = (int64_t)s.len - s.n + t1;
+  int64_t l = a.window ? p0 - a.window + 1 : 0;
+  int64_t h = a.causal ? p1 + 1 : a.window ? p1 + a.window : s.len;
+  l = max(l, (int64_t)0);
+  h = min(h, (int64_t)s.len);
+  *lo = (int)l;
+  *hi = (int)max(h, l);
+}
+
+// The number of blocks that sequence b's rows see.
+__device__ __forceinline__ int seen_blocks(const AttnArgs& a, const KvSeq& s) {
+  if (s.n == 0) return 0;
+  int lo, hi;
+  seen_range(a, s, 0, s.n - 1, &lo, &hi);
+  hi = (int)min((int64_t)hi, (int64_t)a.c.tstride * 64);
+  return hi <= lo ? 0 : ((hi + 63) >> 6) - (lo >> 6);
+}
+
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o, 64);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// Blocks to a part: the batch's blocks over kTarget, kMinChunk at least.
+// Every wave computes it from the lengths.
+__device__ __forceinline__ int plan_chunk(const AttnArgs& a) {
+  const int lane = threadIdx.x & 63;
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
+    const int b = b0 + lane;
+    if (b < a.c.nseq) {
+      const KvSeq s = kv_seq(a.c, b);
+      total += (int64_t)ceil_div(s.n * a.G, kTileRows) * a.c.hkv * seen_blocks(a, s);
+    }
+  }
+  total = wave_sum64(total);
+  return (int)max((total + kTarget - 1) / kTarget, (int64_t)kMinChunk);
+}
+
+struct Item {
+  int b, tile, h, chunk, chunks;
+  int64_t first;  // planned: the part of chunk 0
+  bool ok;
+};
+
+// Parts are numbered by sequence, tile, head, chunk. The item of part w, or
+// (w < 0) the first part of the tile and head that are asked for.
+__device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want_b, int want_tile, int want_h) {
+  const int lane = threadIdx.x & 63;
+  const int chunk = plan_chunk(a);
+  Item r = {0, 0, 0, 0, 1, 0, false};
+  int64_t before = 0;
+  for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
+    const int b = b0 + lane;
+    int tiles = 0, cb = 1;
+    if (b < a.c.nseq) {
+      const KvSeq s = kv_seq(a.c, b);
+      tiles = ceil_div(s.n * a.G, kTileRows);
+      cb = max(1, ceil_div(seen_blocks(a, s), chunk));
+    }
+    const int cnt = tiles * a.c.hkv * cb;
+    const int incl = wave_scan(cnt);
+    const int64_t all = __shfl(incl, 63, 64);
+    const bool mine = w >= 0 ? (w < before + incl) : (b == want_b);
+    const uint64_t m = __ballot(mine && b < a.c.nseq);
+    if (m) {
+      const int src = __ffsll((unsigned long long)m) - 1;
+      r.b = b0 + src;
+      r.chunks = __shfl(cb, src, 64);
+      const int64_t base = before + __shfl(incl - cnt, src, 64);
+      if (w >= 0) {
+        const int64_t i = w - base;
+        const int64_t th = i / r.chunks;
+        r.chunk = (int)(i - th * r.chunks);
+        r.h = (int)(th % a.c.hkv);
+        r.tile = (int)(th / a.c.hkv);
+      } else {
+        r.tile = want_tile;
+        r.h = want_h;
+      }
+      r.first = base + ((int64_t)r.tile * a.c.hkv + r.h) * r.chunks;
+      // (row starts that are not in order number more parts than there are: those have no place)
+      r.ok = r.tile >= 0 && r.tile < __shfl(tiles, src, 64) && r.chunk >= 0 && r.h >= 0 && r.first >= 0 &&
+             r.first + r.chunks <= a.parts;
+      break;
+    }
+    before += all;
+  }
+  r.b = __builtin_amdgcn_readfirstlane(r.b);
+  r.tile = __builtin_amdgcn_readfirstlane(r.tile);
+  r.h = __builtin_amdgcn_readfirstlane(r.h);
+  r.chunk = __builtin_amdgcn_readfirstlane(r.chunk);
+  r.chunks = __builtin_amdgcn_readfirstlane(r.chunks);
+  return r;
+}
+
+// Unplanned: tile slots of sequence b start at cu[b] * G / 16 + b.
+__device__ __forceinline__ Item direct_item(const AttnArgs& a, int64_t slot, int h) {
+  Item r = {0, 0, h, 0, 1, 0, false};
+  const int32_t* cu = a.c.cu;
+  const int G = a.G;
+  auto base = [&](int b) { return (((int64_t)cu[b] * G) >> 4) + b; };
+  r.b = kv_find(a.c.nseq, slot, base);
+  const KvSeq s = kv_seq(a.c, r.b);
+  const int64_t t = slot - base(r.b);
+  r.ok = t >= 0 && t * kTileRows < (int64_t)s.n * G;
+  r.tile = (int)t;
+  return r;
+}
+
+// Eight codes (two dwords) as a bf16 operand.
+__device__ __forceinline__ bf16x8 widen(uint32_t a, uint32_t b) {
+  const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false);
+  const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
+  const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false);
+  const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true);
+  return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+
+__device__ __forceinline__ kvf4 mfma(bf16x8 a, bf16x8 b, kvf4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// The bf16 terms of eight float32 values as operands: all 24 bits in three
+// (TERMS 3), or rounded to nearest (TERMS 1).
+template <int TERMS>
+__device__ __forceinline__ void terms_of(const float (&v)[8], bf16x8 (&t)[TERMS]) {
+  if constexpr (TERMS == 1) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) t[0][i] = (__bf16)v[i];
+  } else {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const Split3 x = split3(v[2 * i]), y = split3(v[2 * i + 1]);
+      w[0][i] = pack_hi16(x.h, y.h);
+      w[1][i] = pack_hi16(x.m, y.m);
+      w[2][i] = pack_hi16(x.l, y.l);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; k++) t[k] = __builtin_bit_cast(bf16x8, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
+  }
+}
+
+__device__ __forceinline__ float ld(const float* p) { return *p; }
+__device__ __forceinline__ float ld(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+__device__ __forceinline__ void st(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st(uint16_t* p, float v) { *p = __builtin_bit_cast(uint16_t, (__bf16)v); }
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int d, int D, bool vec, float (&v)[8]) {
+  if (vec && d + 8 <= D) {
+    if constexpr (sizeof(T) == 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + d), y = *reinterpret_cast<const f32x4*>(p + d + 4);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = x[i], v[4 + i] = y[i];
+    } else {
+      const uint4 x = *reinterpret_cast<const uint4*>(p + d);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = d + i < D ? ld(p + d + i) : 0.f;
+  }
+}
+
+// Maximum over the four lane groups of a row (lanes 16 apart).
+__device__ __forceinline__ float row_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// Bytes that are a NaN code, as 0x80 each.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
+// One work item: 16 query rows of one key/value head over a run of blocks.
+// Lane l: row l % 16, group l / 16. NC: slices of 64 dims (at most; nc in use).
+template <typename T, int TERMS, int NC>
+__global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
+  const int nc = NC <= 4 ? NC : a.c.nc;
+  constexpr int kQ = TERMS * NC * 2 * 64;           // operands of 16 bytes
+  constexpr int kM = kWaves * kTileRows * (kMergeDims + 4);  // floats
+  __shared__ __align__(16) char lds[kQ * 16 > kM * 4 ? kQ * 16 : kM * 4];
+  __shared__ float stat[kWaves][kTileRows][2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 15, grp = lane >> 4;
+  const bool planned = a.part != nullptr;
+  const Item it = planned ? plan_item(a, blockIdx.x, 0, 0, 0) : direct_item(a, blockIdx.x, blockIdx.y);
+  if (!it.ok) return;
+  const KvSeq s = kv_seq(a.c, it.b);
+  const int rows = s.n * a.G, r0 = it.tile * kTileRows;
+  const int valid = min(kTileRows, rows - r0);
+  T* out = (T*)a.out;
+  const bool too_long = (int64_t)s.len > (int64_t)a.c.tstride * 64;  // tokens without a table entry: NaN, not a guess
+
+  // what the tile sees, and this lane's row of it
+  int lo, hi;
+  const int ta = r0 / a.G, tb = (r0 + valid - 1) / a.G;
+  seen_range(a, s, ta, tb, &lo, &hi);
+  if (too_long) hi = lo;
+  const int t = min(r0 + row, rows - 1) / a.G;
+  int rlo, rhi, alo, ahi;  // the row's range, and what every row of the tile sees
+  seen_range(a, s, t, t, &rlo, &rhi);
+  {
+    int l0, h0, l1, h1;
+    seen_range(a, s, ta, ta, &l0, &h0);
+    seen_range(a, s, tb, tb, &l1, &h1);
+    alo = max(l0, l1);
+    ahi = min(h0, h1);
+  }
+  int pg0 = lo >> 6, pg1 = hi <= lo ? pg0 : (hi + 63) >> 6;
+  {
+    const int np = pg1 - pg0;
+    const int c0 = (int)((int64_t)np * it.chunk / it.chunks), c1 = (int)((int64_t)np * (it.chunk + 1) / it.chunks);
+    pg1 = pg0 + c1;
+    pg0 += c0;
+  }
+
+  // the tile's queries as operands in LDS: [term][slice of 32 dims][lane]
+  uint4* qf = reinterpret_cast<uint4*>(lds);
+  for (int i = tid; i < nc * 2 * 64; i += 256) {
+    const int ks = i >> 6, l = i & 63, r = r0 + (l & 15);
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r < rows) {
+      const int tok = r / a.G, head = it.h * a.G + (r - tok * a.G);
+      const T* p = (const T*)a.q + (s.row0 + tok) * a.q_st + head * a.q_sh;
+      load8(p, (ks >> 1) * 64 + (l >> 4) * 16 + (ks & 1) * 8, a.c.D, a.vec, v);
+    }
+    bf16x8 tm[TERMS];
+    terms_of<TERMS>(v, tm);
+#pragma unroll
+    for (int k = 0; k < TERMS; k++) qf[(k * NC * 2 + ks) * 64 + l] = __builtin_bit_cast(uint4, tm[k]);
+  }
+  __syncthreads();
+
+  kvf4 acc[NC * 4];
+#pragma unroll
+  for (int i = 0; i < NC * 4; i++) acc[i] = kvf4{0.f, 0.f, 0.f, 0.f};
+  float m = -__builtin_inff(), l = 0.f;
+
+  for (int p = pg0 + wave; p < pg1; p += kWaves) {
+    const int id = kv_block(a.c, it.b, p);
+    const bool bad = id < 0;
+    const uint8_t* base = kv_part(a.c, bad ? 0 : id, it.h, 0);
+    const float* sc = a.c.scales + ((int64_t)(bad ? 0 : id) * a.c.hkv + it.h) * 2;
+    const float ks = bad ? 1.f : sc[0], vs = bad ? 1.f : sc[1];
+    const uint4* kp = reinterpret_cast<const uint4*>(base) + row * 4 + grp;
+    const uint4* vp = reinterpret_cast<const uint4*>(base + kv_part_bytes(a.c)) + row * 4 + grp;
+    const int j0 = p * 64;
+
+    // S^T: four tiles of 16 tokens
+    kvf4 sc4[4];
+#pragma unroll
+    for (int tt = 0; tt < 4; tt++) sc4[tt] = kvf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+      if (NC > 4 && c >= nc) continue;
+      uint4 kr[4];
+#pragma unroll
+      for (int tt = 0; tt < 4; tt++)
+        kr[tt] = bad ? make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu) : kp[c * 256 + tt * 64];
+#pragma unroll
+      for (int k = 0; k < TERMS; k++) {
+        const bf16x8 q0 = __builtin_bit_cast(bf16x8, qf[(k * NC * 2 + c * 2) * 64 + lane]);
+        const bf16x8 q1 = __builtin_bit_cast(bf16x8, qf[(k * NC * 2 + c * 2 + 1) * 64 + lane]);
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++) {
+          sc4[tt] = mfma(widen(kr[tt].x, kr[tt].y), q0, sc4[tt]);
+          sc4[tt] = mfma(widen(kr[tt].z, kr[tt].w), q1, sc4[tt]);
+        }
+      }
+    }
+    const float mul = a.scale2 * ks;
+    const bool edge = j0 < alo || j0 + 64 > ahi;  // some row does not see some token
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float x = sc4[tt][i] * mul;
+        if (edge) {
+          const int j = j0 + tt * 16 + grp * 4 + i;
+          x = j >= rlo && j < rhi ? x : -__builtin_inff();
+        }
+        sc4[tt][i] = x;
+        top = fmaxf(top, x);
+      }
+    const float mn = fmaxf(m, row_max(top));
+    const float mu = mn == -__builtin_inff() ? 0.f : mn;  // a row that has seen nothing yet: weights 0, not NaN
+    const float alpha = __builtin_amdgcn_exp2f(m - mu);
+    if (__ballot(mn != m)) {
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < NC * 4; i++) {
+        acc[i] *= alpha;
+      }
+    }
+    m = mn;
+    // weights and their operands: two steps of 32 tokens
+    const float f = vs * kWeightScale;
+    bf16x8 pt[2][TERMS];
+#pragma unroll
+    for (int st2 = 0; st2 < 2; st2++) {
+      float w[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float x = __builtin_amdgcn_exp2f(sc4[st2 * 2 + (i >> 2)][i & 3] - mu);
+        l += x;
+        w[i] = x * f;
+      }
+      terms_of<TERMS>(w, pt[st2]);
+    }
+    // Tokens that no row of the tile sees may hold anything (a length ends
+    // inside the block): their value codes become zero. Tokens that some rows
+    // see and others do not may be NaN: a zero weight times NaN would reach
+    // the others, so NaN codes go aside and are counted by a product of their
+    // own against the rows that see them.
+    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+    if (edge) {
+#pragma unroll
+      for (int tt = 0; tt < 4; tt++) {
+        keep[tt] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int j = j0 + tt * 16 + grp * 4 + i;
+          if (j >= lo && j < hi) keep[tt] |= 0xFFu << (8 * i);
+        }
+      }
+    }
+    bf16x8 see[2];
+    const bool mixed = edge && ta != tb;
+    if (mixed) {
+#pragma unroll
+      for (int st2 = 0; st2 < 2; st2++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int j = j0 + (st2 * 2 + (i >> 2)) * 16 + grp * 4 + (i & 3);
+          see[st2][i] = (__bf16)(j >= rlo && j < rhi ? 1.f : 0.f);
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < NC * 4; dt++) {
+      if (NC > 4 && dt >= nc * 4) continue;
+      uint4 vr = bad ? make_uint4(0, 0, 0, 0) : vp[dt * 64];
+      if (edge) {
+        vr.x &= keep[0]; vr.y &= keep[1]; vr.z &= keep[2]; vr.w &= keep[3];
+        const uint4 nb = make_uint4(nan_bytes(vr.x), nan_bytes(vr.y), nan_bytes(vr.z), nan_bytes(vr.w));
+        if (mixed && __ballot((nb.x | nb.y | nb.z | nb.w) != 0)) {
+          // 0x80 of a NaN byte -> 0x38, the code of one
+          auto one = [](uint32_t b) { return (b >> 7) * 0x38u; };
+          kvf4 cnt = {0.f, 0.f, 0.f, 0.f};
+          cnt = mfma(widen(one(nb.x), one(nb.y)), see[0], cnt);
+          cnt = mfma(widen(one(nb.z), one(nb.w)), see[1], cnt);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (cnt[i] > 0.f) acc[dt][i] = __builtin_nanf("");
+          auto drop = [](uint32_t w, uint32_t b) { return w & ~((b >> 7) * 0xFFu); };
+          vr = make_uint4(drop(vr.x, nb.x), drop(vr.y, nb.y), drop(vr.z, nb.z), drop(vr.w, nb.w));
+        }
+      }
+      const bf16x8 v0 = widen(vr.x, vr.y), v1 = widen(vr.z, vr.w);
+#pragma unroll
+      for (int k = 0; k < TERMS; k++) {
+        acc[dt] = mfma(v0, pt[0][k], acc[dt]);
+        acc[dt] = mfma(v1, pt[1][k], acc[dt]);
+      }
+    }
+  }
+
+  // merge the waves: maxima and sums, then the outputs kMergeDims at a time
+  l = row_sum(l);
+  if (grp == 0) {
+    stat[wave][row][0] = m;
+    stat[wave][row][1] = l;
+  }
+  __syncthreads();
+  float M = -__builtin_inff();
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) M = fmaxf(M, stat[w][row][0]);
+  const float Mu = M == -__builtin_inff() ? 0.f : M;
+  const float mine = __builtin_amdgcn_exp2f(m - Mu);
+  // the output rows: thread tid -> row tid / 16, dims 8 (tid % 16) .. + 7 of each kMergeDims
+  const int orow = tid >> 4;
+  float oM = -__builtin_inff(), L = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) oM = fmaxf(oM, stat[w][orow][0]);
+  const float oMu = oM == -__builtin_inff() ? 0.f : oM;
+#pragma unroll
+  for (int w = 0; w < kWaves; w++) L += stat[w][orow][1] * __builtin_amdgcn_exp2f(stat[w][orow][0] - oMu);
+  const bool split = it.chunks > 1;
+  const int Dp = nc * 64;
+  const int otok = (r0 + orow) / a.G, ohead = it.h * a.G + (r0 + orow) - otok * a.G;
+  float fin = 1.f;
+  if (!split) {
+    int l0, h0;
+    seen_range(a, s, min(otok, s.n - 1), min(otok, s.n - 1), &l0, &h0);
+    fin = too_long ? __builtin_nanf("") : h0 <= l0 ? 0.f : (1.f / kWeightScale) / L;
+  }
+  const bool empty = !split && fin == 0.f;
+  float* buf = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int c = 0; c < (NC + 1) / 2; c++) {
+    if (NC > 4 && c * 2 >= nc) continue;
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < 8; dt++) {
+      if (c * 8 + dt < NC * 4)
+        *reinterpret_cast<kvf4*>(buf + (wave * kTileRows + row) * (kMergeDims + 4) + dt * 16 + grp * 4) =
+            acc[c * 8 + dt] * mine;
+    }
+    __syncthreads();
+    const int d = c * kMergeDims + (tid & 15) * 8;
+    if (orow < valid && d < Dp) {
+      float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWaves; w++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] += buf[(w * kTileRows + orow) * (kMergeDims + 4) + (tid & 15) * 8 + i];
+      if (split) {
+        float* to = a.part + ((it.first + it.chunk) * kTileRows + orow) * Dp + d;
+        *reinterpret_cast<kvf4*>(to) = kvf4{o[0], o[1], o[2], o[3]};
+        *reinterpret_cast<kvf4*>(to + 4) = kvf4{o[4], o[5], o[6], o[7]};
+      } else {
+        T* to = out + ((s.row0 + otok) * a.H + ohead) * (int64_t)a.c.D;
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          if (d + i < a.c.D) st(to + d + i, empty ? 0.f : o[i] * fin);
+      }
+    }
+  }
+  if (split && (tid & 15) == 0 && orow < valid) {
+    float* to = a.part + a.parts * kTileRows * Dp + ((it.first + it.chunk) * kTileRows + orow) * 2;
+    to[0] = oM;
+    to[1] = L;
+  }
+}
+
+// Joins the parts of a planned call's split tiles: one workgroup for each
+// row and head; 16 nc lanes by four dims, the rest of the workgroup by parts.
+template <typename T>
+__global__ __launch_bounds__(256) void kv_merge_kernel(AttnArgs a) {
+  __shared__ float w[kTarget + 1];
+  __shared__ float red[4], red2[4];
+  __shared__ float sum[256 * 4];
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const int head = blockIdx.y, h = head / a.G;
+  const int32_t* cu = a.c.cu;
+  const int b = kv_find(a.c.nseq, row, [&](int i) { return (int64_t)cu[i]; });
+  const KvSeq s = kv_seq(a.c, b);
+  const int64_t tok = row - s.row0;
+  if (tok < 0 || tok >= s.n) return;
+  const int r = (int)tok * a.G + (head - h * a.G), tile = r / kTileRows, tr = r - tile * kTileRows;
+  const Item it = plan_item(a, -1, b, tile, h);
+  if (!it.ok || it.chunks <= 1) return;
+  const int Dp = a.c.nc * 64, n = it.chunks;
+  const float* stat = a.part + a.parts * kTileRows * Dp + (it.first * kTileRows + tr) * 2;
+  float M = -__builtin_inff();
+  for (int i = tid; i < n; i += 256) M = fmaxf(M, stat[(int64_t)i * kTileRows * 2]);
+  M = wave_max(M);
+  if ((tid & 63) == 0) red[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float Mu = M == -__builtin_inff() ? 0.f : M;
+  float L = 0.f;
+  for (int i = tid; i < n; i += 256) {
+    const float f = __builtin_amdgcn_exp2f(stat[(int64_t)i * kTileRows * 2] - Mu);
+    w[i] = f;
+    L += f * stat[(int64_t)i * kTileRows * 2 + 1];
+  }
+  L = wave_sum(L);
+  if ((tid & 63) == 0) red2[tid >> 6] = L;
+  __syncthreads();
+  L = (red2[0] + red2[1]) + (red2[2] + red2[3]);
+  const int lanes = a.c.nc * 16, groups = 256 / lanes, g = tid / lanes, ln = tid - g * lanes;
+  kvf4 o = {0.f, 0.f, 0.f, 0.f};
+  if (g < groups) {
+    const float* src = a.part + (it.first * kTileRows + tr) * Dp + ln * 4;
+#pragma unroll 8
+    for (int i = g; i < n; i += groups)
+      o += *reinterpret_cast<const kvf4*>(src + (int64_t)i * kTileRows * Dp) * w[i];
+  }
+  *reinterpret_cast<kvf4*>(sum + tid * 4) = o;
+  __syncthreads();
+  if (g != 0) return;
+  for (int i = 1; i < groups; i++) o += *reinterpret_cast<const kvf4*>(sum + (i * lanes + ln) * 4);
+  int l0, h0;
+  seen_range(a, s, (int)tok, (int)tok, &l0, &h0);
+  const bool too_long = (int64_t)s.len > (int64_t)a.c.tstride * 64;
+  const float fin = too_long ? __builtin_nanf("") : (1.f / kWeightScale) / L;
+  T* to = (T*)a.out + (row * a.H + head) * (int64_t)a.c.D;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (ln * 4 + i < a.c.D) st(to + ln * 4 + i, h0 <= l0 ? 0.f : o[i] * fin);
+}
+
+int64_t tile_slots(const KvAttnArgs& a) { return a.c.rows * (a.H / a.c.hkv) / kTileRows + a.c.nseq; }
+
+// Parts that a planned call can have, 0 where the token axis is not split:
+// enough tiles without, or no sequence that could be cut.
+int64_t plan_parts(const KvAttnArgs& a) {
+  const int64_t items = tile_slots(a) * a.c.hkv;
+  if (items >= kTarget || a.c.tstride <= kMinChunk) return 0;
+  const int64_t most = (a.c.tstride + kMinChunk - 1) / kMinChunk;
+  return std::min((int64_t)kTarget + items, items * most);
+}
+
+template <typename T, int TERMS>
+int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
+  const dim3 grid = a.part ? dim3((unsigned)a.parts) : dim3((unsigned)slots, (unsigned)a.c.hkv);
+#define FA_KV_A(N) kv_attn_kernel<T, TERMS, N><<<grid, 256, 0, s>>>(a)
+  if (a.c.nc == 1) FA_KV_A(1);
+  else if (a.c.nc == 2) FA_KV_A(2);
+  else if (a.c.nc == 3) FA_KV_A(3);
+  else if (a.c.nc == 4) FA_KV_A(4);
+  else FA_KV_A(8);
+#undef FA_KV_A
+  FA_CHECK_LAUNCH(ctx);
+  if (a.part) {
+    kv_merge_kernel<T><<<dim3((unsigned)a.c.rows, (unsigned)a.H), 256, 0, s>>>(a);
+    FA_CHECK_LAUNCH(ctx);
+  }
+  return FA_OK;
+}
+
+}  // namespace
+
+size_t kv_attention_scratch(const KvAttnArgs& a) {
+  return (size_t)plan_parts(a) * kTileRows * (a.c.nc * 64 + 2) * sizeof(float);
+}
+
+int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStream_t s) {
+  AttnArgs a;
+  a.c = k.c;
+  a.q = k.q;
+  a.q_st = k.q_st;
+  a.q_sh = k.q_sh;
+  a.H = k.H;
+  a.G = k.H / k.c.hkv;
+  a.causal = k.causal;
+  a.window = k.window;
+  a.scale2 = (float)((double)k.scale * 1.4426950408889634);
+  a.out = k.out;
+  a.parts = plan_parts(k);
+  a.part = a.parts ? static_cast<float*>(scratch) : nullptr;
+  a.vec = (reinterpret_cast<uintptr_t>(k.q) & 15) == 0 && (k.q_st | k.q_sh) % (k.dtype == FA_DT_F32 ? 4 : 8) == 0;
+  return k.dtype == FA_DT_F32 ? attn_t<float, 3>(ctx, a, tile_slots(k), s)
+                              : attn_t<uint16_t, 1>(ctx, a, tile_slots(k), s);
+}
+
+}  // namespace fa

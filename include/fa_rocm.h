@@ -21,8 +21,8 @@
  * documented as goroutine-safe either, models/gemma/embed.go:15). Distinct
  * contexts may be used from distinct threads.
  *
- * HIP graphs: fa_similarities_topk_dev_noalloc is the entry point meant for
- * capture. The others are not capture-safe (they may grow device buffers on
+ * HIP graphs: fa_similarities_topk_dev_noalloc and the fa_kv_*_dev entry
+ * points (fa_kv_attention_dev with work) can be captured. The others are not capture-safe (they may grow device buffers on
  * a call, and fa_gemma_embed_ids_dev uploads its per-call plan from a pinned
  * host buffer that the next call rewrites and records events of the model):
  * they check hipStreamIsCapturing on the context's stream and return
@@ -225,6 +225,106 @@ int fa_attention_dev(fa_ctx* ctx, const float* q, const float* k, const float* v
                      int32_t S, int32_t D, int64_t q_sb, int64_t q_sh, int64_t k_sb, int64_t k_sh, int64_t v_sb,
                      int64_t v_sh, const float* mask, int64_t m_sb, int64_t m_sh, int64_t m_sr, int64_t m_sc,
                      float scale, float* out);
+
+/* ---- key/value cache in 8 bits ------------------------------------------ */
+
+/* Keys and values of many sequences, quantised as they are written, read
+ * back, and attended to: what attention of new tokens over the tokens before
+ * them keeps (beside fa_attention, which takes keys and values whole).
+ *
+ * A cache is a pool of blocks of FA_KV_BLOCK tokens that the caller
+ * allocates (fa_device_alloc) and hands out: a sequence is a row of a block
+ * table and a length, token j of it being place j % 64 of block
+ * table[j / 64]. For every block, key/value head and part (keys, values)
+ * there are 64 x head_dim e4m3 codes and one scale, a power of two; a value
+ * is code * scale. Nothing need be initialised.
+ *
+ * codes: fa_kv_codes_bytes(...) bytes, 16-byte aligned: [blocks][kv_heads][2]
+ *   parts of 64 * Dp bytes, Dp = head_dim rounded up to whole slices of 64.
+ *   keys:   dim d of token t at (d / 64) * 4096 + t * 64 + d % 64
+ *   values: dim d of token t = 16 a + 4 b + c at d * 64 + 16 b + 4 a + c
+ * scales: [blocks][kv_heads][2] floats. */
+#define FA_KV_BLOCK 64
+typedef struct fa_kv_cache {
+  void* codes;   /* device memory, also in the host entry points */
+  float* scales; /* likewise */
+  int32_t blocks;
+  int32_t kv_heads; /* 1..65535 */
+  int32_t head_dim; /* 1..512 */
+} fa_kv_cache;
+/* Bytes of a cache's codes; 0 for sizes outside the ranges above. */
+size_t fa_kv_codes_bytes(int32_t blocks, int32_t kv_heads, int32_t head_dim);
+
+/* The sequences of one call. Rows cu_rows[b] .. cu_rows[b + 1] - 1 of the
+ * call's tensors are the last tokens of sequence b: with n of them, positions
+ * lengths[b] - n .. lengths[b] - 1. One batch serves a step's calls: write the
+ * new tokens' keys and values, then attend with their queries. */
+typedef struct fa_kv_batch {
+  const int32_t* tables;  /* [nseq][table_stride] block indexes */
+  int32_t table_stride;   /* blocks that a table row has room for */
+  const int32_t* lengths; /* [nseq] tokens of each sequence, the call's included */
+  const int32_t* cu_rows; /* [nseq + 1], from 0, not falling */
+  int32_t nseq;
+  int64_t rows; /* rows of the tensors; those from cu_rows[nseq] on are neither read nor written */
+} fa_kv_batch;
+
+/* The calls below come in two forms. Without _dev, the batch's arrays and the
+ * tensors are host memory, and what the batch asks for is checked: FA_ERR_ARG
+ * for row starts that fall, more rows than tokens, a table entry outside the
+ * pool or missing, a block that would be written twice. With _dev they are
+ * device memory (nothing of them is seen by the host: the call can be captured
+ * into a HIP graph, and replayed with other contents of the same arrays), the
+ * work is enqueued on fa_stream(ctx), and what cannot be done is left out:
+ * rows whose token has no block inside the table and the pool are not written,
+ * read back as NaN, and make the outputs of the queries that see them NaN (all
+ * outputs of a sequence longer than its table row). Two sequences of a call
+ * must not write the same block: the block's contents would be undefined.
+ * dtype (of the tensors): FA_DT_F32 or FA_DT_BF16. rows * heads < 2^31.
+ * k, v, q: row r, head h at r * st + h * sh elements, dims contiguous.
+ *
+ * fa_kv_write quantises rows into the cache. A block that receives new tokens
+ * takes, per head and part, the smallest scale 2^e (-80 <= e <= 120) under
+ * which the largest finite magnitude among them is at most 448 (e4m3's
+ * largest); where tokens at places below the first new one stay (the block is
+ * continued), it keeps its own scale if that is larger, and otherwise their
+ * codes are rounded again to the new one. Places from the first new one on
+ * count as empty: writing at an earlier position drops what followed.
+ * Rounding is to nearest, ties to even: within 2^-4 of a value, or 2^-10 of
+ * the scale; magnitudes above 240 * 2^120 (3.19e38) become that. NaN and
+ * infinities are stored as NaN. */
+int fa_kv_write(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, const void* k,
+                int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh);
+int fa_kv_write_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, const void* k,
+                    int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh);
+
+/* fa_kv_read fills k and v, [rows][kv_heads][head_dim] contiguous, with what
+ * the cache holds for the batch's rows (exact in either type). Whole
+ * sequences: as many rows as lengths. */
+int fa_kv_read(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, void* k, void* v);
+int fa_kv_read_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, void* k, void* v);
+
+/* out = softmax(scale * q . k^T) . v for each row and each of `heads` query
+ * heads, of which heads / kv_heads neighbours share a key/value head. A query
+ * at position p sees the tokens j of its sequence with j <= p (causal != 0) or
+ * all of them, and of those, with window > 0, only the ones with |p - j| <
+ * window. A row that sees nothing gives zeros; a token it does not see has no
+ * part in its output, whatever the cache holds there. out: [rows][heads][head_dim]
+ * contiguous, of dtype. Sums, statistics and scores in float32; float32
+ * queries and weights enter the matrix units as three exact bf16 terms; with
+ * bf16 tensors weights are rounded to bf16.
+ *
+ * work (_dev): scratch of at least fa_kv_attention_work(...) bytes, 16-byte
+ * aligned, used until the call's work is done: calls that may overlap (graphs
+ * replayed on different streams) need one each. NULL: the context's own, which
+ * may grow, so that a call under capture needs work (FA_ERR_STATE otherwise,
+ * if any is needed). fa_kv_attention_work reads only the sizes in cache and
+ * batch (blocks, kv_heads, head_dim, table_stride, nseq, rows). */
+int fa_kv_attention(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, const void* q,
+                    int64_t q_st, int64_t q_sh, int32_t heads, int causal, int32_t window, float scale, void* out);
+int fa_kv_attention_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, const void* q,
+                        int64_t q_st, int64_t q_sh, int32_t heads, int causal, int32_t window, float scale, void* out,
+                        void* work, size_t work_bytes);
+int fa_kv_attention_work(const fa_kv_cache* cache, const fa_kv_batch* batch, int32_t heads, size_t* bytes);
 
 /* Scores queries [nq x d] against docs [nd x d] (dot products, the rows
  * being unit length as cluster.Similarities requires, cluster.go:180-190) and
