@@ -24,10 +24,9 @@ namespace fa {
 namespace {
 
 constexpr int kTileRows = 16;   // query rows of a work item
-constexpr int kWaves = 4;       // waves of a workgroup: each every fourth block
 constexpr int kMinChunk = 4;    // blocks of a split part, at least (one per wave)
+constexpr int kWhole = 32;      // tables of up to this many blocks are not split
 constexpr int kTarget = 1024;   // split parts aimed at: two rounds of two workgroups on each of 256 CUs
-constexpr int kMergeDims = 128; // dims that the waves' results are merged at a time
 // Weights are multiplied by the value scale 2^e and this, so that sums of 2^20
 // times float32's largest values stay finite; the result is multiplied back.
 constexpr float kWeightScale = 0x1p-24f;
@@ -71,36 +70,29 @@ __device__ __forceinline__ int seen_blocks(const AttnArgs& a, const KvSeq& s) {
   return hi <= lo ? 0 : ((hi + 63) >> 6) - (lo >> 6);
 }
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
-  return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
+}
+// Inclusive sums over the lanes: within rows of 16 by row shifts, then the
+// last lane of a row added to the rows after it (row broadcasts).
+__device__ __forceinline__ int wave_scan(int v) {
+  v = dpp_add<0x111, 0xF>(v);
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+  return dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
-__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-
-// Blocks to a part: the batch's blocks over kTarget, kMinChunk at least.
-// Every wave computes it from the lengths.
-__device__ __forceinline__ int plan_chunk(const AttnArgs& a) {
-  const int lane = threadIdx.x & 63;
-  int64_t total = 0;
-  for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
-    const int b = b0 + lane;
-    if (b < a.c.nseq) {
-      const KvSeq s = kv_seq(a.c, b);
-      total += (int64_t)ceil_div(s.n * a.G, kTileRows) * a.c.hkv * seen_blocks(a, s);
-    }
-  }
-  total = wave_sum64(total);
-  return (int)max((total + kTarget - 1) / kTarget, (int64_t)kMinChunk);
+// What lane % 64 = b - b0 knows of sequence b: its tiles and the blocks they see.
+struct Seen {
+  int tiles, blocks;
+};
+__device__ __forceinline__ Seen seen_by(const AttnArgs& a, int b) {
+  if (b >= a.c.nseq) return {0, 0};
+  const KvSeq s = kv_seq(a.c, b);
+  return {ceil_div(s.n * a.G, kTileRows), seen_blocks(a, s)};
 }
 
 struct Item {
@@ -110,53 +102,52 @@ struct Item {
 };
 
 // Parts are numbered by sequence, tile, head, chunk. The item of part w, or
-// (w < 0) the first part of the tile and head that are asked for.
+// (w < 0) the first part of the tile and head that are asked for. A part has
+// the batch's blocks over kTarget, kMinChunk at least (a float32 sum in a
+// fixed order: the same in every wave); every wave finds its own from the
+// lengths, one load for up to 64 sequences.
 __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want_b, int want_tile, int want_h) {
   const int lane = threadIdx.x & 63;
-  const int chunk = plan_chunk(a);
+  const Seen first = seen_by(a, lane);
+  float total = (float)first.tiles * (float)first.blocks;
+  for (int b0 = 64; b0 < a.c.nseq; b0 += 64) {
+    const Seen x = seen_by(a, b0 + lane);
+    total += (float)x.tiles * (float)x.blocks;
+  }
+  total = wave_sum(total) * (float)a.c.hkv;
+  const int chunk = max((int)ceilf(fminf(total * (1.f / kTarget), 1e9f)), kMinChunk);
   Item r = {0, 0, 0, 0, 1, 0, false};
   int64_t before = 0;
   for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
-    const int b = b0 + lane;
-    int tiles = 0, cb = 1;
-    if (b < a.c.nseq) {
-      const KvSeq s = kv_seq(a.c, b);
-      tiles = ceil_div(s.n * a.G, kTileRows);
-      cb = max(1, ceil_div(seen_blocks(a, s), chunk));
-    }
-    const int cnt = tiles * a.c.hkv * cb;
+    const Seen x = b0 ? seen_by(a, b0 + lane) : first;
+    const int cb = max(1, ceil_div(x.blocks, chunk));
+    const int cnt = x.tiles * a.c.hkv * cb;
     const int incl = wave_scan(cnt);
-    const int64_t all = __shfl(incl, 63, 64);
-    const bool mine = w >= 0 ? (w < before + incl) : (b == want_b);
-    const uint64_t m = __ballot(mine && b < a.c.nseq);
+    const bool mine = w >= 0 ? w < before + incl : b0 + lane == want_b;
+    const uint64_t m = __ballot(mine && b0 + lane < a.c.nseq);
     if (m) {
-      const int src = __ffsll((unsigned long long)m) - 1;
+      const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)m) - 1);
+      const int tiles = __builtin_amdgcn_readlane(x.tiles, src);
       r.b = b0 + src;
-      r.chunks = __shfl(cb, src, 64);
-      const int64_t base = before + __shfl(incl - cnt, src, 64);
+      r.chunks = __builtin_amdgcn_readlane(cb, src);
+      const int64_t base = before + __builtin_amdgcn_readlane(incl - cnt, src);
       if (w >= 0) {
-        const int64_t i = w - base;
-        const int64_t th = i / r.chunks;
-        r.chunk = (int)(i - th * r.chunks);
-        r.h = (int)(th % a.c.hkv);
-        r.tile = (int)(th / a.c.hkv);
+        const int i = (int)(w - base), th = i / r.chunks;
+        r.chunk = i - th * r.chunks;
+        r.tile = th / a.c.hkv;
+        r.h = th - r.tile * a.c.hkv;
       } else {
         r.tile = want_tile;
         r.h = want_h;
       }
       r.first = base + ((int64_t)r.tile * a.c.hkv + r.h) * r.chunks;
       // (row starts that are not in order number more parts than there are: those have no place)
-      r.ok = r.tile >= 0 && r.tile < __shfl(tiles, src, 64) && r.chunk >= 0 && r.h >= 0 && r.first >= 0 &&
+      r.ok = r.tile >= 0 && r.tile < tiles && r.chunk >= 0 && r.h >= 0 && r.chunks <= kTarget + 1 && r.first >= 0 &&
              r.first + r.chunks <= a.parts;
       break;
     }
-    before += all;
+    before += __builtin_amdgcn_readlane(incl, 63);
   }
-  r.b = __builtin_amdgcn_readfirstlane(r.b);
-  r.tile = __builtin_amdgcn_readfirstlane(r.tile);
-  r.h = __builtin_amdgcn_readfirstlane(r.h);
-  r.chunk = __builtin_amdgcn_readfirstlane(r.chunk);
-  r.chunks = __builtin_amdgcn_readfirstlane(r.chunks);
   return r;
 }
 
@@ -248,14 +239,23 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7
 
 // One work item: 16 query rows of one key/value head over a run of blocks.
 // Lane l: row l % 16, group l / 16. NC: slices of 64 dims (at most; nc in use).
-template <typename T, int TERMS, int NC>
-__global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
+// Its blocks go to the W waves in turn. A wave loads a block's keys
+// while it turns the block before into weights and sums, and its values likewise, as registers
+// allow: the loads of one block (D = 128: 16 KB) are always under way.
+template <typename T, int TERMS, int NC, int W>
+__global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs a) {
+  // registers: what is loaded a block ahead (2: keys and values, 1: keys)
+  constexpr int AHEAD = NC > 4 ? 0 : NC <= 2 || W == 4 ? 2 : TERMS == 1 || NC == 3 ? 1 : 0;
+  constexpr int kWaves = W, kThreads = W * 64;
+  constexpr int kMergeDims = W == 4 ? 128 : 64;      // dims that the waves' results are merged at a time
+  constexpr int kLane = kMergeDims / (W * 4);        // and a thread's of them, W * 4 threads a row
   const int nc = NC <= 4 ? NC : a.c.nc;
   constexpr int kQ = TERMS * NC * 2 * 64;           // operands of 16 bytes
   constexpr int kM = kWaves * kTileRows * (kMergeDims + 4);  // floats
   __shared__ __align__(16) char lds[kQ * 16 > kM * 4 ? kQ * 16 : kM * 4];
   __shared__ float stat[kWaves][kTileRows][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 15, grp = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = lane & 15, grp = lane >> 4;
   const bool planned = a.part != nullptr;
   const Item it = planned ? plan_item(a, blockIdx.x, 0, 0, 0) : direct_item(a, blockIdx.x, blockIdx.y);
   if (!it.ok) return;
@@ -288,9 +288,48 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
     pg0 += c0;
   }
 
+  // a block's codes, 16 bytes a lane: kr[slice * 4 + tile of 16 tokens], vr[tile of 16 dims]
+  uint4 kr[AHEAD >= 1 ? NC * 4 : 1], vr[AHEAD == 2 ? NC * 4 : 1];
+  auto part = [&](int id, int which) {
+    return reinterpret_cast<const uint4*>(kv_part(a.c, id, it.h, which)) + row * 4 + grp;
+  };
+  auto key = [&](const uint4* p, int i) {  // no such block: keys that are NaN
+    return p && (NC <= 4 || i < nc * 4) ? p[(i >> 2) * 256 + (i & 3) * 64]
+                                        : make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+  };
+  auto value = [&](const uint4* p, int i) {
+    return p && (NC <= 4 || i < nc * 4) ? p[i * 64] : make_uint4(0, 0, 0, 0);
+  };
+  auto load_k = [&](int id) {
+    if constexpr (AHEAD >= 1) {
+      const uint4* p = id >= 0 ? part(id, 0) : nullptr;
+#pragma unroll
+      for (int i = 0; i < NC * 4; i++) kr[i] = key(p, i);
+    }
+  };
+  auto load_v = [&](int id) {
+    if constexpr (AHEAD == 2) {
+      const uint4* p = id >= 0 ? part(id, 1) : nullptr;
+#pragma unroll
+      for (int i = 0; i < NC * 4; i++) vr[i] = value(p, i);
+    }
+  };
+  auto scales = [&](int id) {
+    return id >= 0 ? *reinterpret_cast<const float2*>(a.c.scales + ((int64_t)id * a.c.hkv + it.h) * 2)
+                   : make_float2(1.f, 1.f);
+  };
+  auto block = [&](int p) { return __builtin_amdgcn_readfirstlane(p < pg1 ? kv_block(a.c, it.b, p) : -1); };
+  int id = block(pg0 + wave), id1 = block(pg0 + wave + kWaves);
+  float2 ksv = make_float2(1.f, 1.f);
+  if (pg0 + wave < pg1) {
+    ksv = scales(id);
+    load_k(id);
+    load_v(id);
+  }
+
   // the tile's queries as operands in LDS: [term][slice of 32 dims][lane]
   uint4* qf = reinterpret_cast<uint4*>(lds);
-  for (int i = tid; i < nc * 2 * 64; i += 256) {
+  for (int i = tid; i < nc * 2 * 64; i += kThreads) {
     const int ks = i >> 6, l = i & 63, r = r0 + (l & 15);
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (r < rows) {
@@ -311,14 +350,11 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
   float m = -__builtin_inff(), l = 0.f;
 
   for (int p = pg0 + wave; p < pg1; p += kWaves) {
-    const int id = kv_block(a.c, it.b, p);
-    const bool bad = id < 0;
-    const uint8_t* base = kv_part(a.c, bad ? 0 : id, it.h, 0);
-    const float* sc = a.c.scales + ((int64_t)(bad ? 0 : id) * a.c.hkv + it.h) * 2;
-    const float ks = bad ? 1.f : sc[0], vs = bad ? 1.f : sc[1];
-    const uint4* kp = reinterpret_cast<const uint4*>(base) + row * 4 + grp;
-    const uint4* vp = reinterpret_cast<const uint4*>(base + kv_part_bytes(a.c)) + row * 4 + grp;
+    const int id2 = block(p + 2 * kWaves);  // ahead of the keys that need it
+    const float ks = ksv.x, vs = ksv.y;
     const int j0 = p * 64;
+    const uint4* kp = id >= 0 ? part(id, 0) : nullptr;
+    const uint4* vp = id >= 0 ? part(id, 1) : nullptr;
 
     // S^T: four tiles of 16 tokens
     kvf4 sc4[4];
@@ -327,20 +363,27 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int c = 0; c < NC; c++) {
       if (NC > 4 && c >= nc) continue;
-      uint4 kr[4];
+      uint4 kc[4];
 #pragma unroll
-      for (int tt = 0; tt < 4; tt++)
-        kr[tt] = bad ? make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu) : kp[c * 256 + tt * 64];
+      for (int tt = 0; tt < 4; tt++) {
+        if constexpr (AHEAD >= 1) kc[tt] = kr[c * 4 + tt];
+        else kc[tt] = key(kp, c * 4 + tt);
+      }
 #pragma unroll
       for (int k = 0; k < TERMS; k++) {
         const bf16x8 q0 = __builtin_bit_cast(bf16x8, qf[(k * NC * 2 + c * 2) * 64 + lane]);
         const bf16x8 q1 = __builtin_bit_cast(bf16x8, qf[(k * NC * 2 + c * 2 + 1) * 64 + lane]);
 #pragma unroll
         for (int tt = 0; tt < 4; tt++) {
-          sc4[tt] = mfma(widen(kr[tt].x, kr[tt].y), q0, sc4[tt]);
-          sc4[tt] = mfma(widen(kr[tt].z, kr[tt].w), q1, sc4[tt]);
+          sc4[tt] = mfma(widen(kc[tt].x, kc[tt].y), q0, sc4[tt]);
+          sc4[tt] = mfma(widen(kc[tt].z, kc[tt].w), q1, sc4[tt]);
         }
       }
+    }
+    const bool more = p + kWaves < pg1;
+    if (more) {
+      ksv = scales(id1);
+      load_k(id1);
     }
     const float mul = a.scale2 * ks;
     const bool edge = j0 < alo || j0 + 64 > ahi;  // some row does not see some token
@@ -413,10 +456,12 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int dt = 0; dt < NC * 4; dt++) {
       if (NC > 4 && dt >= nc * 4) continue;
-      uint4 vr = bad ? make_uint4(0, 0, 0, 0) : vp[dt * 64];
+      uint4 v;
+      if constexpr (AHEAD == 2) v = vr[dt];
+      else v = value(vp, dt);
       if (edge) {
-        vr.x &= keep[0]; vr.y &= keep[1]; vr.z &= keep[2]; vr.w &= keep[3];
-        const uint4 nb = make_uint4(nan_bytes(vr.x), nan_bytes(vr.y), nan_bytes(vr.z), nan_bytes(vr.w));
+        v.x &= keep[0]; v.y &= keep[1]; v.z &= keep[2]; v.w &= keep[3];
+        const uint4 nb = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
         if (mixed && __ballot((nb.x | nb.y | nb.z | nb.w) != 0)) {
           // 0x80 of a NaN byte -> 0x38, the code of one
           auto one = [](uint32_t b) { return (b >> 7) * 0x38u; };
@@ -427,16 +472,19 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
           for (int i = 0; i < 4; i++)
             if (cnt[i] > 0.f) acc[dt][i] = __builtin_nanf("");
           auto drop = [](uint32_t w, uint32_t b) { return w & ~((b >> 7) * 0xFFu); };
-          vr = make_uint4(drop(vr.x, nb.x), drop(vr.y, nb.y), drop(vr.z, nb.z), drop(vr.w, nb.w));
+          v = make_uint4(drop(v.x, nb.x), drop(v.y, nb.y), drop(v.z, nb.z), drop(v.w, nb.w));
         }
       }
-      const bf16x8 v0 = widen(vr.x, vr.y), v1 = widen(vr.z, vr.w);
+      const bf16x8 v0 = widen(v.x, v.y), v1 = widen(v.z, v.w);
 #pragma unroll
       for (int k = 0; k < TERMS; k++) {
         acc[dt] = mfma(v0, pt[0][k], acc[dt]);
         acc[dt] = mfma(v1, pt[1][k], acc[dt]);
       }
     }
+    if (more) load_v(id1);
+    id = id1;
+    id1 = id2;
   }
 
   // merge the waves: maxima and sums, then the outputs kMergeDims at a time
@@ -451,8 +499,8 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
   for (int w = 0; w < kWaves; w++) M = fmaxf(M, stat[w][row][0]);
   const float Mu = M == -__builtin_inff() ? 0.f : M;
   const float mine = __builtin_amdgcn_exp2f(m - Mu);
-  // the output rows: thread tid -> row tid / 16, dims 8 (tid % 16) .. + 7 of each kMergeDims
-  const int orow = tid >> 4;
+  // the output rows: W * 4 threads a row, each kLane dims of every kMergeDims
+  const int orow = tid / (W * 4), oat = (tid % (W * 4)) * kLane;
   float oM = -__builtin_inff(), L = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; w++) oM = fmaxf(oM, stat[w][orow][0]);
@@ -471,36 +519,38 @@ __global__ __launch_bounds__(256) void kv_attn_kernel(AttnArgs a) {
   const bool empty = !split && fin == 0.f;
   float* buf = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int c = 0; c < (NC + 1) / 2; c++) {
-    if (NC > 4 && c * 2 >= nc) continue;
+  for (int c = 0; c < (NC * 64 + kMergeDims - 1) / kMergeDims; c++) {
+    if (NC > 4 && c * kMergeDims >= nc * 64) continue;
     __syncthreads();
 #pragma unroll
-    for (int dt = 0; dt < 8; dt++) {
-      if (c * 8 + dt < NC * 4)
+    for (int dt = 0; dt < kMergeDims / 16; dt++) {
+      if (c * (kMergeDims / 16) + dt < NC * 4)
         *reinterpret_cast<kvf4*>(buf + (wave * kTileRows + row) * (kMergeDims + 4) + dt * 16 + grp * 4) =
-            acc[c * 8 + dt] * mine;
+            acc[c * (kMergeDims / 16) + dt] * mine;
     }
     __syncthreads();
-    const int d = c * kMergeDims + (tid & 15) * 8;
+    const int d = c * kMergeDims + oat;
     if (orow < valid && d < Dp) {
-      float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      float o[kLane];
+#pragma unroll
+      for (int i = 0; i < kLane; i++) o[i] = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; w++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[i] += buf[(w * kTileRows + orow) * (kMergeDims + 4) + (tid & 15) * 8 + i];
+        for (int i = 0; i < kLane; i++) o[i] += buf[(w * kTileRows + orow) * (kMergeDims + 4) + oat + i];
       if (split) {
         float* to = a.part + ((it.first + it.chunk) * kTileRows + orow) * Dp + d;
-        *reinterpret_cast<kvf4*>(to) = kvf4{o[0], o[1], o[2], o[3]};
-        *reinterpret_cast<kvf4*>(to + 4) = kvf4{o[4], o[5], o[6], o[7]};
+#pragma unroll
+        for (int i = 0; i < kLane; i++) to[i] = o[i];
       } else {
         T* to = out + ((s.row0 + otok) * a.H + ohead) * (int64_t)a.c.D;
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < kLane; i++)
           if (d + i < a.c.D) st(to + d + i, empty ? 0.f : o[i] * fin);
       }
     }
   }
-  if (split && (tid & 15) == 0 && orow < valid) {
+  if (split && oat == 0 && orow < valid) {
     float* to = a.part + a.parts * kTileRows * Dp + ((it.first + it.chunk) * kTileRows + orow) * 2;
     to[0] = oM;
     to[1] = L;
@@ -572,7 +622,7 @@ int64_t tile_slots(const KvAttnArgs& a) { return a.c.rows * (a.H / a.c.hkv) / kT
 // enough tiles without, or no sequence that could be cut.
 int64_t plan_parts(const KvAttnArgs& a) {
   const int64_t items = tile_slots(a) * a.c.hkv;
-  if (items >= kTarget || a.c.tstride <= kMinChunk) return 0;
+  if (items >= kTarget || a.c.tstride <= kWhole) return 0;
   const int64_t most = (a.c.tstride + kMinChunk - 1) / kMinChunk;
   return std::min((int64_t)kTarget + items, items * most);
 }
@@ -580,7 +630,14 @@ int64_t plan_parts(const KvAttnArgs& a) {
 template <typename T, int TERMS>
 int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
   const dim3 grid = a.part ? dim3((unsigned)a.parts) : dim3((unsigned)slots, (unsigned)a.c.hkv);
-#define FA_KV_A(N) kv_attn_kernel<T, TERMS, N><<<grid, 256, 0, s>>>(a)
+  // eight waves for a tile that is not split (its blocks end sooner), four
+  // where there are parts enough
+  const bool wide = !a.part;
+#define FA_KV_A(N)                                                              \
+  do {                                                                          \
+    if (wide && N <= 4) kv_attn_kernel<T, TERMS, N, N <= 4 ? 8 : 4><<<grid, 512, 0, s>>>(a); \
+    else kv_attn_kernel<T, TERMS, N, 4><<<grid, 256, 0, s>>>(a);                \
+  } while (0)
   if (a.c.nc == 1) FA_KV_A(1);
   else if (a.c.nc == 2) FA_KV_A(2);
   else if (a.c.nc == 3) FA_KV_A(3);
