@@ -38,7 +38,12 @@ HIP_FLAGS = [
 ]
 
 ROCM_SOURCES = ["context.cpp", "matmul.cpp", "model.cpp", "plan.cpp", "gemm.hip", "gemm_h2.hip", "rowops.hip", "attention.hip", "attention_split.hip", "score.hip", "score_few.hip", "cluster.hip",
-                "kvcache.cpp", "kvcache.hip", "kv_attention.hip"]
+                "kvcache.cpp", "kvcache.hip", "kv_attention.hip", "kv_attention_tile.hip"]
+
+# Products whose accumulators arithmetic reads too (the softmax's scores) stay
+# in the ordinary registers: left to itself the compiler keeps them in the
+# accumulation registers and copies each value there and back.
+SOURCE_FLAGS = {"kv_attention_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
 def _run(cmd: list[str], verbose: bool) -> None:
@@ -61,7 +66,7 @@ def build_rocm(verbose: bool = False) -> str:
         obj = os.path.join(BUILD, src.replace(".", "_") + ".o")
         objs.append(obj)
         lang = ["-x", "hip"] if src.endswith(".hip") else []
-        jobs.append([HIPCC, *HIP_FLAGS, *lang, "-c", os.path.join(CSRC, src), "-o", obj])
+        jobs.append([HIPCC, *HIP_FLAGS, *SOURCE_FLAGS.get(src, []), *lang, "-c", os.path.join(CSRC, src), "-o", obj])
     workers = min(len(jobs), max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(workers) as ex:
         for f in [ex.submit(_run, j, verbose) for j in jobs]:

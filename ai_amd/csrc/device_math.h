@@ -69,6 +69,12 @@ __device__ __forceinline__ float lane_xor32(float v) {
   return __uint_as_float((threadIdx.x & 63) < 32 ? r[1] : r[0]);
 }
 
+// v of the lane 16 apart (lane ^ 16), likewise by v_permlane16_swap.
+__device__ __forceinline__ float lane_xor16(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float((threadIdx.x & 16) == 0 ? r[1] : r[0]);
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp_f32(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false));

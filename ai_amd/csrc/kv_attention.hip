@@ -17,225 +17,10 @@
 // statistics and sums are float32.
 #include <algorithm>
 
-#include "device_math.h"
-#include "kvcache.h"
+#include "kv_attention.h"
 
 namespace fa {
 namespace {
-
-constexpr int kTileRows = 16;   // query rows of a work item
-constexpr int kMinChunk = 4;    // blocks of a split part, at least (one per wave)
-constexpr int kWhole = 32;      // tables of up to this many blocks are not split
-constexpr int kTarget = 1024;   // split parts aimed at: two rounds of two workgroups on each of 256 CUs
-// Weights are multiplied by the value scale 2^e and this, so that sums of 2^20
-// times float32's largest values stay finite; the result is multiplied back.
-constexpr float kWeightScale = 0x1p-24f;
-
-// The work of one call: tiles of kTileRows rows of a sequence's n * G, for
-// each key/value head, over the blocks they see; in a planned call the blocks
-// are cut into parts of about equal size over the whole batch.
-struct AttnArgs {
-  KvArgs c;
-  const void* q;
-  int64_t q_st, q_sh;
-  int32_t H, G;
-  int32_t causal, window;
-  float scale2;  // scale * log2 e
-  void* out;
-  float* part;    // planned: [parts][16][Dp] sums, then [parts][16][2] maximum, sum
-  int64_t parts;  // parts that the scratch holds
-  int32_t vec;
-};
-
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
-// Tokens that the rows of new tokens t0 .. t1 (positions len - n + t) see at
-// all: [lo, hi).
-__device__ __forceinline__ void seen_range(const AttnArgs& a, const KvSeq& s, int t0, int t1, int* lo, int* hi) {
-  const int64_t p0 = (int64_t)s.len - s.n + t0, p1 = (int64_t)s.len - s.n + t1;
-  int64_t l = a.window ? p0 - a.window + 1 : 0;
-  int64_t h = a.causal ? p1 + 1 : a.window ? p1 + a.window : s.len;
-  l = max(l, (int64_t)0);
-  h = min(h, (int64_t)s.len);
-  *lo = (int)l;
-  *hi = (int)max(h, l);
-}
-
-// The number of blocks that sequence b's rows see.
-__device__ __forceinline__ int seen_blocks(const AttnArgs& a, const KvSeq& s) {
-  if (s.n == 0) return 0;
-  int lo, hi;
-  seen_range(a, s, 0, s.n - 1, &lo, &hi);
-  hi = (int)min((int64_t)hi, (int64_t)a.c.tstride * 64);
-  return hi <= lo ? 0 : ((hi + 63) >> 6) - (lo >> 6);
-}
-
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_add(int v) {
-  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, true);
-}
-// Inclusive sums over the lanes: within rows of 16 by row shifts, then the
-// last lane of a row added to the rows after it (row broadcasts).
-__device__ __forceinline__ int wave_scan(int v) {
-  v = dpp_add<0x111, 0xF>(v);
-  v = dpp_add<0x112, 0xF>(v);
-  v = dpp_add<0x114, 0xF>(v);
-  v = dpp_add<0x118, 0xF>(v);
-  v = dpp_add<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
-  return dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
-}
-
-// What lane % 64 = b - b0 knows of sequence b: its tiles and the blocks they see.
-struct Seen {
-  int tiles, blocks;
-};
-__device__ __forceinline__ Seen seen_by(const AttnArgs& a, int b) {
-  if (b >= a.c.nseq) return {0, 0};
-  const KvSeq s = kv_seq(a.c, b);
-  return {ceil_div(s.n * a.G, kTileRows), seen_blocks(a, s)};
-}
-
-struct Item {
-  int b, tile, h, chunk, chunks;
-  int64_t first;  // planned: the part of chunk 0
-  bool ok;
-};
-
-// Parts are numbered by sequence, tile, head, chunk. The item of part w, or
-// (w < 0) the first part of the tile and head that are asked for. A part has
-// the batch's blocks over kTarget, kMinChunk at least (a float32 sum in a
-// fixed order: the same in every wave); every wave finds its own from the
-// lengths, one load for up to 64 sequences.
-__device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want_b, int want_tile, int want_h) {
-  const int lane = threadIdx.x & 63;
-  const Seen first = seen_by(a, lane);
-  float total = (float)first.tiles * (float)first.blocks;
-  for (int b0 = 64; b0 < a.c.nseq; b0 += 64) {
-    const Seen x = seen_by(a, b0 + lane);
-    total += (float)x.tiles * (float)x.blocks;
-  }
-  total = wave_sum(total) * (float)a.c.hkv;
-  const int chunk = max((int)ceilf(fminf(total * (1.f / kTarget), 1e9f)), kMinChunk);
-  Item r = {0, 0, 0, 0, 1, 0, false};
-  int64_t before = 0;
-  for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
-    const Seen x = b0 ? seen_by(a, b0 + lane) : first;
-    const int cb = max(1, ceil_div(x.blocks, chunk));
-    const int cnt = x.tiles * a.c.hkv * cb;
-    const int incl = wave_scan(cnt);
-    const bool mine = w >= 0 ? w < before + incl : b0 + lane == want_b;
-    const uint64_t m = __ballot(mine && b0 + lane < a.c.nseq);
-    if (m) {
-      const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)m) - 1);
-      const int tiles = __builtin_amdgcn_readlane(x.tiles, src);
-      r.b = b0 + src;
-      r.chunks = __builtin_amdgcn_readlane(cb, src);
-      const int64_t base = before + __builtin_amdgcn_readlane(incl - cnt, src);
-      if (w >= 0) {
-        const int i = (int)(w - base), th = i / r.chunks;
-        r.chunk = i - th * r.chunks;
-        r.tile = th / a.c.hkv;
-        r.h = th - r.tile * a.c.hkv;
-      } else {
-        r.tile = want_tile;
-        r.h = want_h;
-      }
-      r.first = base + ((int64_t)r.tile * a.c.hkv + r.h) * r.chunks;
-      // (row starts that are not in order number more parts than there are: those have no place)
-      r.ok = r.tile >= 0 && r.tile < tiles && r.chunk >= 0 && r.h >= 0 && r.chunks <= kTarget + 1 && r.first >= 0 &&
-             r.first + r.chunks <= a.parts;
-      break;
-    }
-    before += __builtin_amdgcn_readlane(incl, 63);
-  }
-  return r;
-}
-
-// Unplanned: tile slots of sequence b start at cu[b] * G / 16 + b.
-__device__ __forceinline__ Item direct_item(const AttnArgs& a, int64_t slot, int h) {
-  Item r = {0, 0, h, 0, 1, 0, false};
-  const int32_t* cu = a.c.cu;
-  const int G = a.G;
-  auto base = [&](int b) { return (((int64_t)cu[b] * G) >> 4) + b; };
-  r.b = kv_find(a.c.nseq, slot, base);
-  const KvSeq s = kv_seq(a.c, r.b);
-  const int64_t t = slot - base(r.b);
-  r.ok = t >= 0 && t * kTileRows < (int64_t)s.n * G;
-  r.tile = (int)t;
-  return r;
-}
-
-// Eight codes (two dwords) as a bf16 operand.
-__device__ __forceinline__ bf16x8 widen(uint32_t a, uint32_t b) {
-  const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false);
-  const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, true);
-  const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, false);
-  const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.f, true);
-  return bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
-}
-
-__device__ __forceinline__ kvf4 mfma(bf16x8 a, bf16x8 b, kvf4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-// The bf16 terms of eight float32 values as operands: all 24 bits in three
-// (TERMS 3), or rounded to nearest (TERMS 1).
-template <int TERMS>
-__device__ __forceinline__ void terms_of(const float (&v)[8], bf16x8 (&t)[TERMS]) {
-  if constexpr (TERMS == 1) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) t[0][i] = (__bf16)v[i];
-  } else {
-    uint32_t w[3][4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const Split3 x = split3(v[2 * i]), y = split3(v[2 * i + 1]);
-      w[0][i] = pack_hi16(x.h, y.h);
-      w[1][i] = pack_hi16(x.m, y.m);
-      w[2][i] = pack_hi16(x.l, y.l);
-    }
-#pragma unroll
-    for (int k = 0; k < 3; k++) t[k] = __builtin_bit_cast(bf16x8, make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]));
-  }
-}
-
-__device__ __forceinline__ float ld(const float* p) { return *p; }
-__device__ __forceinline__ float ld(const uint16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
-__device__ __forceinline__ void st(float* p, float v) { *p = v; }
-__device__ __forceinline__ void st(uint16_t* p, float v) { *p = __builtin_bit_cast(uint16_t, (__bf16)v); }
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, int d, int D, bool vec, float (&v)[8]) {
-  if (vec && d + 8 <= D) {
-    if constexpr (sizeof(T) == 4) {
-      const f32x4 x = *reinterpret_cast<const f32x4*>(p + d), y = *reinterpret_cast<const f32x4*>(p + d + 4);
-#pragma unroll
-      for (int i = 0; i < 4; i++) v[i] = x[i], v[4 + i] = y[i];
-    } else {
-      const uint4 x = *reinterpret_cast<const uint4*>(p + d);
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = d + i < D ? ld(p + d + i) : 0.f;
-  }
-}
-
-// Maximum over the four lane groups of a row (lanes 16 apart).
-__device__ __forceinline__ float row_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-__device__ __forceinline__ float row_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
-}
-
-// Bytes that are a NaN code, as 0x80 each.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
 // One work item: 16 query rows of one key/value head over a run of blocks.
 // Lane l: row l % 16, group l / 16. NC: slices of 64 dims (at most; nc in use).
@@ -318,8 +103,8 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
     return id >= 0 ? *reinterpret_cast<const float2*>(a.c.scales + ((int64_t)id * a.c.hkv + it.h) * 2)
                    : make_float2(1.f, 1.f);
   };
-  auto block = [&](int p) { return __builtin_amdgcn_readfirstlane(p < pg1 ? kv_block(a.c, it.b, p) : -1); };
-  int id = block(pg0 + wave), id1 = block(pg0 + wave + kWaves);
+  Blocks blocks(a, it.b, pg0 + wave, kWaves, pg1);
+  int id = blocks.at(a, it.b, 0), turn = 0;
   float2 ksv = make_float2(1.f, 1.f);
   if (pg0 + wave < pg1) {
     ksv = scales(id);
@@ -350,7 +135,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
   float m = -__builtin_inff(), l = 0.f;
 
   for (int p = pg0 + wave; p < pg1; p += kWaves) {
-    const int id2 = block(p + 2 * kWaves);  // ahead of the keys that need it
+    const int id1 = blocks.at(a, it.b, ++turn);
     const float ks = ksv.x, vs = ksv.y;
     const int j0 = p * 64;
     const uint4* kp = id >= 0 ? part(id, 0) : nullptr;
@@ -484,7 +269,6 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
     }
     if (more) load_v(id1);
     id = id1;
-    id1 = id2;
   }
 
   // merge the waves: maxima and sums, then the outputs kMergeDims at a time
@@ -572,13 +356,13 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(AttnArgs a) {
   const KvSeq s = kv_seq(a.c, b);
   const int64_t tok = row - s.row0;
   if (tok < 0 || tok >= s.n) return;
-  const int r = (int)tok * a.G + (head - h * a.G), tile = r / kTileRows, tr = r - tile * kTileRows;
+  const int r = (int)tok * a.G + (head - h * a.G), tile = r / a.tile, tr = r - tile * a.tile;
   const Item it = plan_item(a, -1, b, tile, h);
   if (!it.ok || it.chunks <= 1) return;
   const int Dp = a.c.nc * 64, n = it.chunks;
-  const float* stat = a.part + a.parts * kTileRows * Dp + (it.first * kTileRows + tr) * 2;
+  const float* stat = a.part + a.parts * a.tile * Dp + (it.first * a.tile + tr) * 2;
   float M = -__builtin_inff();
-  for (int i = tid; i < n; i += 256) M = fmaxf(M, stat[(int64_t)i * kTileRows * 2]);
+  for (int i = tid; i < n; i += 256) M = fmaxf(M, stat[(int64_t)i * a.tile * 2]);
   M = wave_max(M);
   if ((tid & 63) == 0) red[tid >> 6] = M;
   __syncthreads();
@@ -586,9 +370,9 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(AttnArgs a) {
   const float Mu = M == -__builtin_inff() ? 0.f : M;
   float L = 0.f;
   for (int i = tid; i < n; i += 256) {
-    const float f = __builtin_amdgcn_exp2f(stat[(int64_t)i * kTileRows * 2] - Mu);
+    const float f = __builtin_amdgcn_exp2f(stat[(int64_t)i * a.tile * 2] - Mu);
     w[i] = f;
-    L += f * stat[(int64_t)i * kTileRows * 2 + 1];
+    L += f * stat[(int64_t)i * a.tile * 2 + 1];
   }
   L = wave_sum(L);
   if ((tid & 63) == 0) red2[tid >> 6] = L;
@@ -597,10 +381,10 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(AttnArgs a) {
   const int lanes = a.c.nc * 16, groups = 256 / lanes, g = tid / lanes, ln = tid - g * lanes;
   kvf4 o = {0.f, 0.f, 0.f, 0.f};
   if (g < groups) {
-    const float* src = a.part + (it.first * kTileRows + tr) * Dp + ln * 4;
+    const float* src = a.part + (it.first * a.tile + tr) * Dp + ln * 4;
 #pragma unroll 8
     for (int i = g; i < n; i += groups)
-      o += *reinterpret_cast<const kvf4*>(src + (int64_t)i * kTileRows * Dp) * w[i];
+      o += *reinterpret_cast<const kvf4*>(src + (int64_t)i * a.tile * Dp) * w[i];
   }
   *reinterpret_cast<kvf4*>(sum + tid * 4) = o;
   __syncthreads();
@@ -616,19 +400,35 @@ __global__ __launch_bounds__(256) void kv_merge_kernel(AttnArgs a) {
     if (ln * 4 + i < a.c.D) st(to + ln * 4 + i, h0 <= l0 ? 0.f : o[i] * fin);
 }
 
-int64_t tile_slots(const KvAttnArgs& a) { return a.c.rows * (a.H / a.c.hkv) / kTileRows + a.c.nseq; }
+// Tiles of many rows are split only where they are fewer than this: joining
+// the parts of every row costs more than a partly filled card.
+constexpr int kWideItems = 200;
 
-// Parts that a planned call can have, 0 where the token axis is not split:
-// enough tiles without, or no sequence that could be cut.
-int64_t plan_parts(const KvAttnArgs& a) {
-  const int64_t items = tile_slots(a) * a.c.hkv;
-  if (items >= kTarget || a.c.tstride <= kWhole) return 0;
-  const int64_t most = (a.c.tstride + kMinChunk - 1) / kMinChunk;
-  return std::min((int64_t)kTarget + items, items * most);
+// How a call runs, from its sizes alone.
+struct Shape {
+  int tile;        // rows of a work item
+  int64_t slots;   // tiles, at most
+  int64_t parts;   // parts of a split token axis, at most; 0: not split
+};
+
+Shape shape_of(const KvAttnArgs& a) {
+  Shape r;
+  const int64_t all = a.c.rows * (a.H / a.c.hkv);
+  r.tile = kv_tile_rows(a.c.nc, all, a.c.nseq);
+  r.slots = all / r.tile + a.c.nseq;
+  const int64_t items = r.slots * a.c.hkv;
+  // enough tiles without, or no sequence that could be cut
+  if (items >= (r.tile == kTileRows ? kTarget : kWideItems) || a.c.tstride <= kWhole) {
+    r.parts = 0;
+  } else {
+    const int64_t most = (a.c.tstride + kMinChunk - 1) / kMinChunk;
+    r.parts = std::min((int64_t)kTarget + items, items * most);
+  }
+  return r;
 }
 
 template <typename T, int TERMS>
-int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
+int rows16_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
   const dim3 grid = a.part ? dim3((unsigned)a.parts) : dim3((unsigned)slots, (unsigned)a.c.hkv);
   // eight waves for a tile that is not split (its blocks end sooner), four
   // where there are parts enough
@@ -645,6 +445,14 @@ int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
   else FA_KV_A(8);
 #undef FA_KV_A
   FA_CHECK_LAUNCH(ctx);
+  return FA_OK;
+}
+
+template <typename T, int TERMS>
+int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
+  const int rc = a.tile == kTileRows ? rows16_t<T, TERMS>(ctx, a, slots, s)
+                                     : launch_kv_tiles_attn(ctx, a, TERMS == 3 ? FA_DT_F32 : FA_DT_BF16, slots, s);
+  if (rc) return rc;
   if (a.part) {
     kv_merge_kernel<T><<<dim3((unsigned)a.c.rows, (unsigned)a.H), 256, 0, s>>>(a);
     FA_CHECK_LAUNCH(ctx);
@@ -655,7 +463,8 @@ int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
 }  // namespace
 
 size_t kv_attention_scratch(const KvAttnArgs& a) {
-  return (size_t)plan_parts(a) * kTileRows * (a.c.nc * 64 + 2) * sizeof(float);
+  const Shape h = shape_of(a);
+  return (size_t)h.parts * h.tile * (a.c.nc * 64 + 2) * sizeof(float);
 }
 
 int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStream_t s) {
@@ -670,11 +479,14 @@ int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStre
   a.window = k.window;
   a.scale2 = (float)((double)k.scale * 1.4426950408889634);
   a.out = k.out;
-  a.parts = plan_parts(k);
+  const Shape h = shape_of(k);
+  a.tile = h.tile;
+  a.parts = h.parts;
   a.part = a.parts ? static_cast<float*>(scratch) : nullptr;
   a.vec = (reinterpret_cast<uintptr_t>(k.q) & 15) == 0 && (k.q_st | k.q_sh) % (k.dtype == FA_DT_F32 ? 4 : 8) == 0;
-  return k.dtype == FA_DT_F32 ? attn_t<float, 3>(ctx, a, tile_slots(k), s)
-                              : attn_t<uint16_t, 1>(ctx, a, tile_slots(k), s);
+  a.out_vec = (reinterpret_cast<uintptr_t>(k.out) & 15) == 0 && k.c.D % 4 == 0;
+  return k.dtype == FA_DT_F32 ? attn_t<float, 3>(ctx, a, h.slots, s)
+                              : attn_t<uint16_t, 1>(ctx, a, h.slots, s);
 }
 
 }  // namespace fa

@@ -267,7 +267,10 @@ int fa_kv_attention_work(const fa_kv_cache* cache, const fa_kv_batch* batch, int
   fa::KvAttnArgs a = {};
   a.c = args_of(cache, batch);
   a.H = heads;
-  if (!nothing(batch)) *bytes = fa::kv_attention_scratch(a);
+  for (int dtype : {FA_DT_F32, FA_DT_BF16}) {
+    a.dtype = dtype;
+    if (!nothing(batch)) *bytes = std::max(*bytes, fa::kv_attention_scratch(a));
+  }
   return FA_OK;
 }
 
