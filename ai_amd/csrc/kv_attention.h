@@ -11,7 +11,7 @@ constexpr int kTileRows = 16;   // query rows of a work item of the kernel for f
 constexpr int kWideRows = 128;  // and of the one for many
 
 constexpr int kMinChunk = 4;    // blocks of a split part, at least (one per wave)
-constexpr int kWhole = 32;      // tables of up to this many blocks are not split
+constexpr int kRound = 64;      // blocks of a part up to which one round of a part for each CU is aimed at
 constexpr int kTarget = 1024;   // split parts aimed at: two rounds of two workgroups on each of 256 CUs
 // Weights are multiplied by the value scale 2^e and this, so that sums of 2^20
 // times float32's largest values stay finite; the result is multiplied back.
@@ -31,8 +31,10 @@ struct AttnArgs {
   float scale2;  // scale * log2 e
   void* out;
   float* part;    // planned: [parts][tile][Dp] sums, then [parts][tile][2] maximum, sum
+  uint32_t* count;  // planned: per part 0 of a tile, how many of its parts are done
   int64_t parts;  // parts that the scratch holds
   int32_t tile;   // query rows of a work item
+  int32_t target, least, cap;  // planned: parts aimed at, blocks of a part at least
   int32_t vec, out_vec;  // rows of q / out aligned for one load / store
 };
 
@@ -92,19 +94,23 @@ struct Item {
 
 // Parts are numbered by sequence, tile, head, chunk. The item of part w, or
 // (w < 0) the first part of the tile and head that are asked for. A part has
-// the batch's blocks over kTarget, kMinChunk at least (a float32 sum in a
+// the batch's blocks over a.target, a.least at least (a float32 sum in a
 // fixed order: the same in every wave); every wave finds its own from the
 // lengths, one load for up to 64 sequences.
 __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want_b, int want_tile, int want_h) {
   const int lane = threadIdx.x & 63;
   const Seen first = seen_by(a, lane);
-  float total = (float)first.tiles * (float)first.blocks;
+  float total = (float)first.tiles * (float)first.blocks, tiles = (float)first.tiles;
   for (int b0 = 64; b0 < a.c.nseq; b0 += 64) {
     const Seen x = seen_by(a, b0 + lane);
     total += (float)x.tiles * (float)x.blocks;
+    tiles += (float)x.tiles;
   }
   total = wave_sum(total) * (float)a.c.hkv;
-  const int chunk = max((int)ceilf(fminf(total * (1.f / kTarget), 1e9f)), kMinChunk);
+  tiles = wave_sum(tiles) * (float)a.c.hkv;
+  const float round = total / fmaxf(256.f - tiles, 128.f);
+  const int chunk = max(max((int)ceilf(fminf(total / (float)a.target, 1e9f)), a.least),
+                        (int)ceilf(fminf(round, (float)a.cap)));
   Item r = {0, 0, 0, 0, 1, 0, false};
   int64_t before = 0;
   for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
@@ -131,7 +137,7 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want
       }
       r.first = base + ((int64_t)r.tile * a.c.hkv + r.h) * r.chunks;
       // (row starts that are not in order number more parts than there are: those have no place)
-      r.ok = r.tile >= 0 && r.tile < tiles && r.chunk >= 0 && r.h >= 0 && r.chunks <= kTarget + 1 && r.first >= 0 &&
+      r.ok = r.tile >= 0 && r.tile < tiles && r.chunk >= 0 && r.h >= 0 && r.first >= 0 &&
              r.first + r.chunks <= a.parts;
       break;
     }
@@ -140,11 +146,11 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want
   return r;
 }
 
-// Unplanned: tile slots of sequence b start at cu[b] * G / tile + b.
-__device__ __forceinline__ Item direct_item(const AttnArgs& a, int64_t slot, int h) {
+// Unplanned: the slots of sequence b's tiles of `rows` rows start at cu[b] * G / rows + b.
+__device__ __forceinline__ Item direct_item(const AttnArgs& a, int64_t slot, int h, int rows) {
   Item r = {0, 0, h, 0, 1, 0, false};
   const int32_t* cu = a.c.cu;
-  const int G = a.G, rows = a.tile;
+  const int G = a.G;
   auto base = [&](int b) { return (int64_t)(uint32_t)((uint32_t)cu[b] * (uint32_t)G / (uint32_t)rows) + b; };
   r.b = kv_find(a.c.nseq, slot, base);
   const KvSeq s = kv_seq(a.c, r.b);

@@ -22,18 +22,93 @@
 namespace fa {
 namespace {
 
+// Two floats of a part, written and read past the caches that XCDs do not
+// share (relaxed atomics of the device's scope): the workgroup that joins a
+// tile's parts may be on another XCD than those that wrote them, and a fence
+// for ordinary stores writes back a whole L2 (with one in each workgroup a
+// step of 16 sequences of 2048 tokens took 81 us instead of 16).
+__device__ __forceinline__ void put2(float* p, float a, float b) {
+  const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* p) {
+  const uint64_t v =
+      __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// Joins the parts of query row r of item it (row tr of its tile) in their
+// order, by 16 threads: thread ln the dims 64 c + 4 ln + 0..3. A few parts at
+// a time, whose loads go out together.
+template <typename T, int NC>
+__device__ __forceinline__ void join_row(const AttnArgs& a, const KvSeq& s, const Item& it, int r, int tr, int ln) {
+  const int n = it.chunks, nc = a.c.nc, Dp = nc * 64, rows = a.tile;
+  const float* jstat = a.part + a.parts * rows * Dp + (it.first * rows + tr) * 2;
+  const float* src = a.part + (it.first * rows + tr) * Dp + ln * 4;
+  constexpr int kBatch = NC <= 2 ? 8 : NC <= 4 ? 4 : 1;
+  float jM = -__builtin_inff(), jL = 0.f, o[NC * 4];
+#pragma unroll
+  for (int i = 0; i < NC * 4; i++) o[i] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += kBatch) {
+    float2 ml[kBatch], x[kBatch][NC * 2];
+    float top = jM;
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      ml[i] = make_float2(-__builtin_inff(), 0.f);
+#pragma unroll
+      for (int c = 0; c < NC * 2; c++) x[i][c] = make_float2(0.f, 0.f);
+      if (i0 + i < n) {
+        ml[i] = get2(jstat + (int64_t)(i0 + i) * rows * 2);
+#pragma unroll
+        for (int c = 0; c < NC * 2; c++)
+          if (c < nc * 2) x[i][c] = get2(src + (int64_t)(i0 + i) * rows * Dp + (c >> 1) * 64 + (c & 1) * 2);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) top = fmaxf(top, ml[i].x);
+    const float mu = top == -__builtin_inff() ? 0.f : top, alpha = __builtin_amdgcn_exp2f(jM - mu);
+    jM = top;
+    jL *= alpha;
+#pragma unroll
+    for (int c = 0; c < NC * 4; c++) o[c] *= alpha;
+#pragma unroll
+    for (int i = 0; i < kBatch; i++) {
+      const float f = __builtin_amdgcn_exp2f(ml[i].x - mu);
+      jL = fmaf(ml[i].y, f, jL);
+#pragma unroll
+      for (int c = 0; c < NC * 2; c++) {
+        o[c * 2] = fmaf(x[i][c].x, f, o[c * 2]);
+        o[c * 2 + 1] = fmaf(x[i][c].y, f, o[c * 2 + 1]);
+      }
+    }
+  }
+  const int tok = r / a.G, head = it.h * a.G + r - tok * a.G;
+  int l0, h0;
+  seen_range(a, s, tok, tok, &l0, &h0);
+  const bool too_long = (int64_t)s.len > (int64_t)a.c.tstride * 64;
+  const float fin = too_long ? __builtin_nanf("") : (1.f / kWeightScale) / jL;
+  T* to = (T*)a.out + ((s.row0 + tok) * a.H + head) * (int64_t)a.c.D;
+#pragma unroll
+  for (int c = 0; c < NC; c++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int d = c * 64 + ln * 4 + e;
+      if (d < a.c.D) st(to + d, h0 <= l0 ? 0.f : o[c * 4 + e] * fin);
+    }
+}
+
 // One work item: 16 query rows of one key/value head over a run of blocks.
 // Lane l: row l % 16, group l / 16. NC: slices of 64 dims (at most; nc in use).
-// Its blocks go to the W waves in turn. A wave loads a block's keys
+// Its blocks go to the four waves in turn. A wave loads a block's keys
 // while it turns the block before into weights and sums, and its values likewise, as registers
 // allow: the loads of one block (D = 128: 16 KB) are always under way.
-template <typename T, int TERMS, int NC, int W>
-__global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs a) {
-  // registers: what is loaded a block ahead (2: keys and values, 1: keys)
-  constexpr int AHEAD = NC > 4 ? 0 : NC <= 2 || W == 4 ? 2 : TERMS == 1 || NC == 3 ? 1 : 0;
-  constexpr int kWaves = W, kThreads = W * 64;
-  constexpr int kMergeDims = W == 4 ? 128 : 64;      // dims that the waves' results are merged at a time
-  constexpr int kLane = kMergeDims / (W * 4);        // and a thread's of them, W * 4 threads a row
+template <typename T, int TERMS, int NC>
+__global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs a) {
+  // what is loaded a block ahead, with room for two workgroups on a CU (2: keys and values, 1: keys, 0: nothing)
+  constexpr int AHEAD = NC <= 4 ? 2 : 0;
+  constexpr int W = 4, kWaves = W, kThreads = W * 64;
+  constexpr int kMergeDims = 128;              // dims that the waves' results are merged at a time
+  constexpr int kLane = kMergeDims / (W * 4);  // and a thread's of them, W * 4 threads a row
   const int nc = NC <= 4 ? NC : a.c.nc;
   constexpr int kQ = TERMS * NC * 2 * 64;           // operands of 16 bytes
   constexpr int kM = kWaves * kTileRows * (kMergeDims + 4);  // floats
@@ -42,7 +117,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = lane & 15, grp = lane >> 4;
   const bool planned = a.part != nullptr;
-  const Item it = planned ? plan_item(a, blockIdx.x, 0, 0, 0) : direct_item(a, blockIdx.x, blockIdx.y);
+  const Item it = planned ? plan_item(a, blockIdx.x, 0, 0, 0) : direct_item(a, blockIdx.x, blockIdx.y, kTileRows);
   if (!it.ok) return;
   const KvSeq s = kv_seq(a.c, it.b);
   const int rows = s.n * a.G, r0 = it.tile * kTileRows;
@@ -133,6 +208,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
 #pragma unroll
   for (int i = 0; i < NC * 4; i++) acc[i] = kvf4{0.f, 0.f, 0.f, 0.f};
   float m = -__builtin_inff(), l = 0.f;
+  uint64_t nan_sum[2] = {0, 0};  // sums that are NaN: bit 4 (tile % 16) + i of word tile / 16
 
   for (int p = pg0 + wave; p < pg1; p += kWaves) {
     const int id1 = blocks.at(a, it.b, ++turn);
@@ -213,8 +289,8 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
     // Tokens that no row of the tile sees may hold anything (a length ends
     // inside the block): their value codes become zero. Tokens that some rows
     // see and others do not may be NaN: a zero weight times NaN would reach
-    // the others, so NaN codes go aside and are counted by a product of their
-    // own against the rows that see them.
+    // the others, so NaN codes are dropped and counted by a product of their
+    // own against the rows that see them; those sums become NaN at the end.
     uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
     if (edge) {
 #pragma unroll
@@ -227,38 +303,22 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
         }
       }
     }
-    bf16x8 see[2];
     const bool mixed = edge && ta != tb;
-    if (mixed) {
-#pragma unroll
-      for (int st2 = 0; st2 < 2; st2++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int j = j0 + (st2 * 2 + (i >> 2)) * 16 + grp * 4 + (i & 3);
-          see[st2][i] = (__bf16)(j >= rlo && j < rhi ? 1.f : 0.f);
-        }
-    }
+    uint32_t nan = 0;
 #pragma unroll
     for (int dt = 0; dt < NC * 4; dt++) {
       if (NC > 4 && dt >= nc * 4) continue;
       uint4 v;
       if constexpr (AHEAD == 2) v = vr[dt];
       else v = value(vp, dt);
-      if (edge) {
-        v.x &= keep[0]; v.y &= keep[1]; v.z &= keep[2]; v.w &= keep[3];
-        const uint4 nb = make_uint4(nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w));
-        if (mixed && __ballot((nb.x | nb.y | nb.z | nb.w) != 0)) {
-          // 0x80 of a NaN byte -> 0x38, the code of one
-          auto one = [](uint32_t b) { return (b >> 7) * 0x38u; };
-          kvf4 cnt = {0.f, 0.f, 0.f, 0.f};
-          cnt = mfma(widen(one(nb.x), one(nb.y)), see[0], cnt);
-          cnt = mfma(widen(one(nb.z), one(nb.w)), see[1], cnt);
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (cnt[i] > 0.f) acc[dt][i] = __builtin_nanf("");
-          auto drop = [](uint32_t w, uint32_t b) { return w & ~((b >> 7) * 0xFFu); };
-          v = make_uint4(drop(v.x, nb.x), drop(v.y, nb.y), drop(v.z, nb.z), drop(v.w, nb.w));
-        }
+      if (edge) v = make_uint4(v.x & keep[0], v.y & keep[1], v.z & keep[2], v.w & keep[3]);
+      if (mixed) {
+        auto drop = [&](uint32_t w) {
+          const uint32_t n = nan_bytes(w);
+          nan |= n;
+          return w & ~((n >> 7) * 0xFFu);
+        };
+        v = make_uint4(drop(v.x), drop(v.y), drop(v.z), drop(v.w));
       }
       const bf16x8 v0 = widen(v.x, v.y), v1 = widen(v.z, v.w);
 #pragma unroll
@@ -267,10 +327,42 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
         acc[dt] = mfma(v1, pt[1][k], acc[dt]);
       }
     }
+    if (mixed && __ballot(nan != 0)) {
+#pragma unroll 1
+      for (int dt = 0; dt < nc * 4; dt++) {
+        const uint4 v = value(vp, dt);
+        const uint32_t n0 = nan_bytes(v.x & keep[0]) >> 7, n1 = nan_bytes(v.y & keep[1]) >> 7;
+        const uint32_t n2 = nan_bytes(v.z & keep[2]) >> 7, n3 = nan_bytes(v.w & keep[3]) >> 7;
+        if (__ballot((n0 | n1 | n2 | n3) != 0) == 0) continue;
+        kvf4 cnt = {0.f, 0.f, 0.f, 0.f};  // 0x01 of a NaN byte -> 0x38, the code of one
+#pragma unroll
+        for (int st2 = 0; st2 < 2; st2++) {
+          bf16x8 see;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const int j = j0 + (st2 * 2 + (i >> 2)) * 16 + grp * 4 + (i & 3);
+            see[i] = (__bf16)(j >= rlo && j < rhi ? 1.f : 0.f);
+          }
+          cnt = mfma(st2 ? widen(n2 * 0x38u, n3 * 0x38u) : widen(n0 * 0x38u, n1 * 0x38u), see, cnt);
+        }
+        uint64_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) bits |= (uint64_t)(cnt[i] > 0.f) << i;
+        nan_sum[0] |= dt < 16 ? bits << (4 * dt) : 0;
+        if (NC > 4) nan_sum[1] |= dt < 16 ? 0 : bits << (4 * (dt & 15));
+      }
+    }
     if (more) load_v(id1);
     id = id1;
   }
 
+  if (__ballot((nan_sum[0] | nan_sum[1]) != 0)) {
+#pragma unroll
+    for (int dt = 0; dt < NC * 4; dt++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (nan_sum[dt >> 4] >> (4 * (dt & 15) + i) & 1) acc[dt][i] = __builtin_nanf("");
+  }
   // merge the waves: maxima and sums, then the outputs kMergeDims at a time
   l = row_sum(l);
   if (grp == 0) {
@@ -325,7 +417,7 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
       if (split) {
         float* to = a.part + ((it.first + it.chunk) * kTileRows + orow) * Dp + d;
 #pragma unroll
-        for (int i = 0; i < kLane; i++) to[i] = o[i];
+        for (int i = 0; i < kLane; i += 2) put2(to + i, o[i], o[i + 1]);
       } else {
         T* to = out + ((s.row0 + otok) * a.H + ohead) * (int64_t)a.c.D;
 #pragma unroll
@@ -334,81 +426,51 @@ __global__ __launch_bounds__(W * 64, W == 4 && NC <= 2 ? 2 : 1) void kv_attn_ker
       }
     }
   }
-  if (split && oat == 0 && orow < valid) {
-    float* to = a.part + a.parts * kTileRows * Dp + ((it.first + it.chunk) * kTileRows + orow) * 2;
-    to[0] = oM;
-    to[1] = L;
+  if (!split) return;
+  const int64_t mine_at = (it.first + it.chunk) * kTileRows;
+  float* stats = a.part + a.parts * kTileRows * Dp;
+  if (oat == 0 && orow < valid) {
+    put2(stats + (mine_at + orow) * 2, oM, L);
   }
+  // The workgroup that ends last of a tile's joins its parts, in their order
+  // (the result does not depend on which one that is), and leaves the count
+  // at zero for the next call.
+  __shared__ int last;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's are where every workgroup finds them
+  __syncthreads();
+  if (tid == 0) {
+    last = __hip_atomic_fetch_add(a.count + it.first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           (uint32_t)it.chunks - 1;
+    if (last) __hip_atomic_store(a.count + it.first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last) return;
+  if (orow < valid) join_row<T, NC>(a, s, it, r0 + orow, orow, tid & 15);
 }
 
-// Joins the parts of a planned call's split tiles: one workgroup for each
-// row and head; 16 nc lanes by four dims, the rest of the workgroup by parts.
+// Joins the parts of split tiles of many rows: a workgroup for each 16 rows.
 template <typename T>
-__global__ __launch_bounds__(256) void kv_merge_kernel(AttnArgs a) {
-  __shared__ float w[kTarget + 1];
-  __shared__ float red[4], red2[4];
-  __shared__ float sum[256 * 4];
-  const int tid = threadIdx.x;
-  const int64_t row = blockIdx.x;
-  const int head = blockIdx.y, h = head / a.G;
-  const int32_t* cu = a.c.cu;
-  const int b = kv_find(a.c.nseq, row, [&](int i) { return (int64_t)cu[i]; });
-  const KvSeq s = kv_seq(a.c, b);
-  const int64_t tok = row - s.row0;
-  if (tok < 0 || tok >= s.n) return;
-  const int r = (int)tok * a.G + (head - h * a.G), tile = r / a.tile, tr = r - tile * a.tile;
-  const Item it = plan_item(a, -1, b, tile, h);
-  if (!it.ok || it.chunks <= 1) return;
-  const int Dp = a.c.nc * 64, n = it.chunks;
-  const float* stat = a.part + a.parts * a.tile * Dp + (it.first * a.tile + tr) * 2;
-  float M = -__builtin_inff();
-  for (int i = tid; i < n; i += 256) M = fmaxf(M, stat[(int64_t)i * a.tile * 2]);
-  M = wave_max(M);
-  if ((tid & 63) == 0) red[tid >> 6] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float Mu = M == -__builtin_inff() ? 0.f : M;
-  float L = 0.f;
-  for (int i = tid; i < n; i += 256) {
-    const float f = __builtin_amdgcn_exp2f(stat[(int64_t)i * a.tile * 2] - Mu);
-    w[i] = f;
-    L += f * stat[(int64_t)i * a.tile * 2 + 1];
-  }
-  L = wave_sum(L);
-  if ((tid & 63) == 0) red2[tid >> 6] = L;
-  __syncthreads();
-  L = (red2[0] + red2[1]) + (red2[2] + red2[3]);
-  const int lanes = a.c.nc * 16, groups = 256 / lanes, g = tid / lanes, ln = tid - g * lanes;
-  kvf4 o = {0.f, 0.f, 0.f, 0.f};
-  if (g < groups) {
-    const float* src = a.part + (it.first * a.tile + tr) * Dp + ln * 4;
-#pragma unroll 8
-    for (int i = g; i < n; i += groups)
-      o += *reinterpret_cast<const kvf4*>(src + (int64_t)i * a.tile * Dp) * w[i];
-  }
-  *reinterpret_cast<kvf4*>(sum + tid * 4) = o;
-  __syncthreads();
-  if (g != 0) return;
-  for (int i = 1; i < groups; i++) o += *reinterpret_cast<const kvf4*>(sum + (i * lanes + ln) * 4);
-  int l0, h0;
-  seen_range(a, s, (int)tok, (int)tok, &l0, &h0);
-  const bool too_long = (int64_t)s.len > (int64_t)a.c.tstride * 64;
-  const float fin = too_long ? __builtin_nanf("") : (1.f / kWeightScale) / L;
-  T* to = (T*)a.out + (row * a.H + head) * (int64_t)a.c.D;
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    if (ln * 4 + i < a.c.D) st(to + ln * 4 + i, h0 <= l0 ? 0.f : o[i] * fin);
+__global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
+  const Item t = direct_item(a, blockIdx.x, blockIdx.y, 16);
+  if (!t.ok) return;
+  const KvSeq s = kv_seq(a.c, t.b);
+  const int r = t.tile * 16 + (threadIdx.x >> 4), tile = r / a.tile;
+  const Item it = plan_item(a, -1, t.b, tile, t.h);
+  if (it.ok && it.chunks > 1 && r < s.n * a.G) join_row<T, 4>(a, s, it, r, r - tile * a.tile, threadIdx.x & 15);
 }
 
-// Tiles of many rows are split only where they are fewer than this: joining
-// the parts of every row costs more than a partly filled card.
-constexpr int kWideItems = 200;
+// Tiles of many rows are split only where they are fewer than kWideItems, in
+// about kWideTarget parts: writing and joining a part of every row costs more
+// than a partly filled card (139 tiles of float32 rows on up to 18 blocks:
+// 80 + 20 us in 332 parts, 100 us whole).
+constexpr int kWideItems = 128, kWideTarget = 512;
 
 // How a call runs, from its sizes alone.
 struct Shape {
-  int tile;        // rows of a work item
-  int64_t slots;   // tiles, at most
-  int64_t parts;   // parts of a split token axis, at most; 0: not split
+  int tile;           // rows of a work item
+  int target, least, cap;  // of a split: parts aimed at, blocks of a part at least
+  int64_t slots;      // tiles, at most
+  int64_t parts;      // parts, at most; 0: not split
 };
 
 Shape shape_of(const KvAttnArgs& a) {
@@ -417,12 +479,21 @@ Shape shape_of(const KvAttnArgs& a) {
   r.tile = kv_tile_rows(a.c.nc, all, a.c.nseq);
   r.slots = all / r.tile + a.c.nseq;
   const int64_t items = r.slots * a.c.hkv;
+  const bool wide = r.tile != kTileRows;
+  // blocks that a sequence's rows can see
+  int64_t blocks = a.c.tstride;
+  if (a.window) blocks = std::min(blocks, ((int64_t)a.window * (a.causal ? 1 : 2) + a.c.rows) / 64 + 2);
+  r.target = wide ? kWideTarget : kTarget;
+  r.least = kMinChunk;
+  r.cap = wide ? 0 : kRound;
   // enough tiles without, or no sequence that could be cut
-  if (items >= (r.tile == kTileRows ? kTarget : kWideItems) || a.c.tstride <= kWhole) {
+  if (items >= (wide ? kWideItems : kTarget) || blocks <= r.least) {
     r.parts = 0;
   } else {
-    const int64_t most = (a.c.tstride + kMinChunk - 1) / kMinChunk;
-    r.parts = std::min((int64_t)kTarget + items, items * most);
+    // (a part has at least least blocks, and total / 256 of them up to kRound)
+    const int64_t total = items * blocks, most = (blocks + r.least - 1) / r.least;
+    const int64_t cut = wide ? r.target : std::max((int64_t)256, std::min((int64_t)kTarget, total / kRound));
+    r.parts = std::min(cut + items, items * most);
   }
   return r;
 }
@@ -430,14 +501,7 @@ Shape shape_of(const KvAttnArgs& a) {
 template <typename T, int TERMS>
 int rows16_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
   const dim3 grid = a.part ? dim3((unsigned)a.parts) : dim3((unsigned)slots, (unsigned)a.c.hkv);
-  // eight waves for a tile that is not split (its blocks end sooner), four
-  // where there are parts enough
-  const bool wide = !a.part;
-#define FA_KV_A(N)                                                              \
-  do {                                                                          \
-    if (wide && N <= 4) kv_attn_kernel<T, TERMS, N, N <= 4 ? 8 : 4><<<grid, 512, 0, s>>>(a); \
-    else kv_attn_kernel<T, TERMS, N, 4><<<grid, 256, 0, s>>>(a);                \
-  } while (0)
+#define FA_KV_A(N) kv_attn_kernel<T, TERMS, N><<<grid, 256, 0, s>>>(a)
   if (a.c.nc == 1) FA_KV_A(1);
   else if (a.c.nc == 2) FA_KV_A(2);
   else if (a.c.nc == 3) FA_KV_A(3);
@@ -453,8 +517,9 @@ int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
   const int rc = a.tile == kTileRows ? rows16_t<T, TERMS>(ctx, a, slots, s)
                                      : launch_kv_tiles_attn(ctx, a, TERMS == 3 ? FA_DT_F32 : FA_DT_BF16, slots, s);
   if (rc) return rc;
-  if (a.part) {
-    kv_merge_kernel<T><<<dim3((unsigned)a.c.rows, (unsigned)a.H), 256, 0, s>>>(a);
+  if (a.part && a.tile != kTileRows) {
+    const dim3 grid((unsigned)(a.c.rows * a.G / 16 + a.c.nseq), (unsigned)a.c.hkv);
+    kv_join_kernel<T><<<grid, 256, 0, s>>>(a);
     FA_CHECK_LAUNCH(ctx);
   }
   return FA_OK;
@@ -464,7 +529,7 @@ int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
 
 size_t kv_attention_scratch(const KvAttnArgs& a) {
   const Shape h = shape_of(a);
-  return (size_t)h.parts * h.tile * (a.c.nc * 64 + 2) * sizeof(float);
+  return h.parts ? kKvCountBytes + (size_t)h.parts * h.tile * (a.c.nc * 64 + 2) * sizeof(float) : 0;
 }
 
 int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStream_t s) {
@@ -481,8 +546,12 @@ int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStre
   a.out = k.out;
   const Shape h = shape_of(k);
   a.tile = h.tile;
+  a.target = h.target;
+  a.least = h.least;
+  a.cap = h.cap;
   a.parts = h.parts;
-  a.part = a.parts ? static_cast<float*>(scratch) : nullptr;
+  a.count = static_cast<uint32_t*>(scratch);
+  a.part = a.parts ? reinterpret_cast<float*>(static_cast<char*>(scratch) + kKvCountBytes) : nullptr;
   a.vec = (reinterpret_cast<uintptr_t>(k.q) & 15) == 0 && (k.q_st | k.q_sh) % (k.dtype == FA_DT_F32 ? 4 : 8) == 0;
   a.out_vec = (reinterpret_cast<uintptr_t>(k.out) & 15) == 0 && k.c.D % 4 == 0;
   return k.dtype == FA_DT_F32 ? attn_t<float, 3>(ctx, a, h.slots, s)

@@ -22,9 +22,9 @@ template <int N, int M>
 __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
 #pragma unroll
-  for (int i = 0; i < N - kAhead; i++) {
-    __builtin_amdgcn_sched_group_barrier(0x8, M, 0);
-    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  for (int i = 0; i < (N - kAhead) / 2; i++) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 2 * M, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
   }
   __builtin_amdgcn_sched_group_barrier(0x8, M * kAhead, 0);
 }
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
   const bool planned = a.part != nullptr;
   // later tiles of a causal batch see more: they go first
   const Item it = planned ? plan_item(a, (int64_t)gridDim.x - 1 - blockIdx.x, 0, 0, 0)
-                          : direct_item(a, (int64_t)gridDim.y - 1 - blockIdx.y, blockIdx.x);
+                          : direct_item(a, (int64_t)gridDim.y - 1 - blockIdx.y, blockIdx.x, kRows);
   if (!it.ok) return;
   const KvSeq s = kv_seq(a.c, it.b);
   const int rows = s.n * a.G, r0 = it.tile * kRows;
@@ -278,13 +278,15 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
 #pragma unroll
         for (int j = 0; j < 16; j++) sc[tt][j] = 0.f;
 #pragma unroll
-      for (int k = 0; k < KS; k++)
+      for (int k = 0; k < KS; k++) {
+        const bf16x8 k0 = __builtin_bit_cast(bf16x8, kf[k * 128 + lane]);
+        const bf16x8 k1 = __builtin_bit_cast(bf16x8, kf[k * 128 + 64 + lane]);
 #pragma unroll
-        for (int tt = 0; tt < 2; tt++) {
-          const bf16x8 kk = __builtin_bit_cast(bf16x8, kf[(k * 2 + tt) * 64 + lane]);
-#pragma unroll
-          for (int x = 0; x < TERMS; x++) sc[tt] = mfma32(kk, qf[k][x], sc[tt]);
+        for (int x = 0; x < TERMS; x++) {
+          sc[0] = mfma32(k0, qf[k][x], sc[0]);
+          sc[1] = mfma32(k1, qf[k][x], sc[1]);
         }
+      }
       reads_ahead<KS * 2, TERMS>();
     }
     if (p + 1 < pg1) {
@@ -351,10 +353,14 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
 #pragma unroll
       for (int k = 0; k < 4; k++)
 #pragma unroll
-        for (int i = 0; i < DT; i++) {
-          const bf16x8 v = __builtin_bit_cast(bf16x8, vf[(k * DT + i) * 64 + lane]);
+        for (int i = 0; i < DT; i += 2) {
+          const bf16x8 v0 = __builtin_bit_cast(bf16x8, vf[(k * DT + i) * 64 + lane]);
+          const bf16x8 v1 = __builtin_bit_cast(bf16x8, vf[(k * DT + i + 1) * 64 + lane]);
 #pragma unroll
-          for (int x = 0; x < TERMS; x++) acc[i] = mfma32(v, pt[k][x], acc[i]);
+          for (int x = 0; x < TERMS; x++) {
+            acc[i] = mfma32(v0, pt[k][x], acc[i]);
+            acc[i + 1] = mfma32(v1, pt[k][x], acc[i + 1]);
+          }
         }
       reads_ahead<4 * DT, TERMS>();
     }

@@ -186,6 +186,16 @@ int need_ctx(fa_ctx* ctx, const char* op) {
   return ctx ? FA_OK : set_error(ctx, FA_ERR_ARG, "%s: ctx is NULL", op);
 }
 
+// The context's scratch for attention, its counters zero.
+int own_parts(fa_ctx* ctx, size_t need, void** work) {
+  fa::DevBuf& buf = ctx->slot(S_KV_PARTS);
+  const bool grows = buf.bytes < need;
+  int rc = buf.ensure(ctx, need);
+  if (rc) return rc;
+  *work = buf.ptr;
+  return grows ? fa::launch_zero(ctx, buf.ptr, fa::kKvCountBytes, ctx->stream) : FA_OK;
+}
+
 bool nothing(const fa_kv_batch* b) { return b->rows == 0 || b->nseq == 0; }
 
 }  // namespace
@@ -286,10 +296,10 @@ int fa_kv_attention_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch
     if (work_bytes < need || (reinterpret_cast<uintptr_t>(work) & 15))
       return set_error(ctx, FA_ERR_ARG, "KVAttention: work of %zu bytes, 16-byte aligned, is needed (%zu given)", need,
                        work_bytes);
+    if (need && (rc = fa::launch_zero(ctx, work, fa::kKvCountBytes, ctx->stream))) return rc;
   } else if (need) {
     if ((rc = fa::refuse_capture(ctx, ctx->stream, "KVAttention without work"))) return rc;
-    if ((rc = ctx->slot(S_KV_PARTS).ensure(ctx, need))) return rc;
-    work = ctx->slot(S_KV_PARTS).ptr;
+    if ((rc = own_parts(ctx, need, &work))) return rc;
   }
   return fa::launch_kv_attention(ctx, a, work, ctx->stream);
 }
@@ -316,8 +326,9 @@ int fa_kv_attention(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* ba
   a.q = dq;
   a.out = ctx->slot(S_OUT).ptr;
   const size_t need = fa::kv_attention_scratch(a);
-  if (need && (rc = ctx->slot(S_KV_PARTS).ensure(ctx, need))) return rc;
-  if ((rc = fa::launch_kv_attention(ctx, a, ctx->slot(S_KV_PARTS).ptr, ctx->stream))) return rc;
+  void* work = nullptr;
+  if (need && (rc = own_parts(ctx, need, &work))) return rc;
+  if ((rc = fa::launch_kv_attention(ctx, a, work, ctx->stream))) return rc;
   FA_HIP_CHECK(ctx, hipMemcpyAsync(out, a.out, bytes, hipMemcpyDeviceToHost, ctx->stream));
   FA_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
   return FA_OK;

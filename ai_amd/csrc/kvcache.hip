@@ -166,14 +166,16 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
           if (y < __builtin_inff()) big = fmaxf(big, y);
           else x[c][i][j] = __builtin_nanf("");  // not finite: stored as NaN
         }
+  uint8_t* dst = kv_part(a, id, h, part);
+  const bool whole = u.place == 0 && end == 64;
+  float* scale = a.scales + ((int64_t)id * a.hkv + h) * 2 + part;
+  const bool keep = u.place > 0;  // tokens below the first new one stay
+  const int e_old = keep ? stored_exp(*scale) : kKvMinExp;
   big = wave_max(big);
   if ((tid & 63) == 0) red[tid >> 6] = big;
   __syncthreads();
   big = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  float* scale = a.scales + ((int64_t)id * a.hkv + h) * 2 + part;
   const int e_new = scale_exp(big);
-  const bool keep = u.place > 0;  // tokens below the first new one stay
-  const int e_old = keep ? stored_exp(*scale) : kKvMinExp;
   const int e = max(e_new, e_old);
   const bool grow = keep && e > e_old;
   const float inv = exp2_int(-e), shrink = exp2_int(max(e_old - e, -126));
@@ -188,9 +190,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
           if (c < a.nc) x[c][i][j] = y > top ? top : y < -top ? -top : y;
         }
   }
-  __syncthreads();  // every thread has read the scale
-  if (tid == 0) *scale = exp2_int(e);
-  uint8_t* dst = kv_part(a, id, h, part);
+  if (tid == 0) *scale = exp2_int(e);  // (every thread read the old one before the maximum was joined)
 #pragma unroll
   for (int c = 0; c < NCM; c++) {
     if (c >= a.nc) continue;
@@ -201,6 +201,19 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
         uint32_t* w = reinterpret_cast<uint32_t*>(dst + c * 4096 + t * 64 + dq * 4);
         if (t >= u.place && t < end) *w = pack4(x[c][i][0] * inv, x[c][i][1] * inv, x[c][i][2] * inv, x[c][i][3] * inv);
         else if (grow && t < u.place) *w = rescale4(*w, shrink);
+      }
+    } else if (u.n <= 8 && !grow) {
+      // few tokens: their bytes alone (a token's step of 64 sequences, 8
+      // heads of 128 dims: 8.3 us with the value rows read and written whole)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int t = t0 + i;
+        if (t >= u.place && t < end) {
+          const uint32_t w = pack4(x[c][i][0] * inv, x[c][i][1] * inv, x[c][i][2] * inv, x[c][i][3] * inv);
+          uint8_t* to = dst + (int64_t)(c * 64 + dq * 4) * 64 + tb * 16 + ta * 4 + i;
+#pragma unroll
+          for (int j = 0; j < 4; j++) to[j * 64] = (uint8_t)(w >> (8 * j));
+        }
       }
     } else {
       // four tokens of one dim to a word, the slice's words through LDS so
@@ -217,10 +230,9 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
       uint32_t nw[4];
 #pragma unroll
       for (int q = 0; q < 4; q++) nw[q] = tile[row * 17 + b * 4 + q];
-      const bool whole = u.place == 0 && end == 64;
       if (!whole) {
-        const uint4 old4 = *w;
-        const uint32_t old[4] = {old4.x, old4.y, old4.z, old4.w};
+        const uint4 o4 = *w;
+        const uint32_t old[4] = {o4.x, o4.y, o4.z, o4.w};
 #pragma unroll
         for (int q = 0; q < 4; q++) {
           uint32_t fresh = 0, below = 0;  // byte masks: new tokens, kept ones
