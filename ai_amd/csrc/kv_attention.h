@@ -79,17 +79,19 @@ __device__ __forceinline__ int wave_scan(int v) {
 // What lane % 64 = b - b0 knows of sequence b: its tiles and the blocks they see.
 struct Seen {
   int tiles, blocks;
+  KvSeq s;
 };
 __device__ __forceinline__ Seen seen_by(const AttnArgs& a, int b) {
-  if (b >= a.c.nseq) return {0, 0};
+  if (b >= a.c.nseq) return {0, 0, {0, 0, 0}};
   const KvSeq s = kv_seq(a.c, b);
-  return {ceil_div(s.n * a.G, a.tile), seen_blocks(a, s)};
+  return {ceil_div(s.n * a.G, a.tile), seen_blocks(a, s), s};
 }
 
 struct Item {
   int b, tile, h, chunk, chunks;
   int64_t first;  // planned: the part of chunk 0
   bool ok;
+  KvSeq s;  // the sequence's rows and length
 };
 
 // Parts are numbered by sequence, tile, head, chunk. The item of part w, or
@@ -111,7 +113,7 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want
   const float round = total / fmaxf(256.f - tiles, 128.f);
   const int chunk = max(max((int)ceilf(fminf(total / (float)a.target, 1e9f)), a.least),
                         (int)ceilf(fminf(round, (float)a.cap)));
-  Item r = {0, 0, 0, 0, 1, 0, false};
+  Item r = {0, 0, 0, 0, 1, 0, false, {0, 0, 0}};
   int64_t before = 0;
   for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
     const Seen x = b0 ? seen_by(a, b0 + lane) : first;
@@ -124,6 +126,7 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want
       const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)m) - 1);
       const int tiles = __builtin_amdgcn_readlane(x.tiles, src);
       r.b = b0 + src;
+      r.s = lane_seq(x.s, src);
       r.chunks = __builtin_amdgcn_readlane(cb, src);
       const int64_t base = before + __builtin_amdgcn_readlane(incl - cnt, src);
       if (w >= 0) {
@@ -148,14 +151,14 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want
 
 // Unplanned: the slots of sequence b's tiles of `rows` rows start at cu[b] * G / rows + b.
 __device__ __forceinline__ Item direct_item(const AttnArgs& a, int64_t slot, int h, int rows) {
-  Item r = {0, 0, h, 0, 1, 0, false};
-  const int32_t* cu = a.c.cu;
+  Item r = {0, 0, h, 0, 1, 0, false, {0, 0, 0}};
   const int G = a.G;
-  auto base = [&](int b) { return (int64_t)(uint32_t)((uint32_t)cu[b] * (uint32_t)G / (uint32_t)rows) + b; };
-  r.b = kv_find(a.c.nseq, slot, base);
-  const KvSeq s = kv_seq(a.c, r.b);
-  const int64_t t = slot - base(r.b);
-  r.ok = t >= 0 && t * rows < (int64_t)s.n * G;
+  auto base = [&](int32_t c, int b) { return (int64_t)((uint32_t)c * (uint32_t)G / (uint32_t)rows) + b; };
+  const KvFound f = kv_find(a.c, slot, base);
+  r.b = f.b;
+  r.s = f.s;
+  const int64_t t = slot - base(f.cu0, f.b);
+  r.ok = t >= 0 && t * rows < (int64_t)f.s.n * G;
   r.tile = (int)t;
   return r;
 }

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
   const bool planned = a.part != nullptr;
   const Item it = planned ? plan_item(a, blockIdx.x, 0, 0, 0) : direct_item(a, blockIdx.x, blockIdx.y, kTileRows);
   if (!it.ok) return;
-  const KvSeq s = kv_seq(a.c, it.b);
+  const KvSeq s = it.s;
   const int rows = s.n * a.G, r0 = it.tile * kTileRows;
   const int valid = min(kTileRows, rows - r0);
   T* out = (T*)a.out;
@@ -453,7 +453,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
   const Item t = direct_item(a, blockIdx.x, blockIdx.y, 16);
   if (!t.ok) return;
-  const KvSeq s = kv_seq(a.c, t.b);
+  const KvSeq s = t.s;
   const int r = t.tile * 16 + (threadIdx.x >> 4), tile = r / a.tile;
   const Item it = plan_item(a, -1, t.b, tile, t.h);
   if (it.ok && it.chunks > 1 && r < s.n * a.G) join_row<T, 4>(a, s, it, r, r - tile * a.tile, threadIdx.x & 15);

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
   const Item it = planned ? plan_item(a, (int64_t)gridDim.x - 1 - blockIdx.x, 0, 0, 0)
                           : direct_item(a, (int64_t)gridDim.y - 1 - blockIdx.y, blockIdx.x, kRows);
   if (!it.ok) return;
-  const KvSeq s = kv_seq(a.c, it.b);
+  const KvSeq s = it.s;
   const int rows = s.n * a.G, r0 = it.tile * kRows;
   const int valid = min(kRows, rows - r0);
   const bool too_long = (int64_t)s.len > (int64_t)a.c.tstride * 64;

@@ -87,24 +87,46 @@ __device__ __forceinline__ uint8_t* kv_part(const KvArgs& a, int block, int h, i
   return a.codes + (((int64_t)block * a.hkv + h) * 2 + part) * kv_part_bytes(a);
 }
 
-// The largest b in [0, nseq) with base(b) <= u (base does not fall), found by
-// the 64 lanes of a wave together: one round of loads for up to 64
-// sequences, two up to 4096. Any array contents end the search in range.
+// The sequence that unit u belongs to: the largest b in [0, nseq) with
+// base(cu[b], b) <= u (base does not fall), found by the 64 lanes of a wave
+// together, and its rows and length. Up to 64 sequences: one round of loads
+// for all of it. Any array contents end the search in range.
+struct KvFound {
+  int b;
+  int32_t cu0;
+  KvSeq s;
+};
+__device__ __forceinline__ int64_t lane64(int64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ KvSeq lane_seq(const KvSeq& s, int lane) {
+  return {lane64(s.row0, lane), __builtin_amdgcn_readlane(s.n, lane), __builtin_amdgcn_readlane(s.len, lane)};
+}
 template <typename F>
-__device__ __forceinline__ int kv_find(int nseq, int64_t u, F base) {
+__device__ __forceinline__ KvFound kv_find(const KvArgs& a, int64_t u, F base) {
   const int lane = threadIdx.x & 63;
-  int lo = 0, n = nseq;
+  if (a.nseq <= 64) {
+    const int i = min(lane, a.nseq - 1);
+    const int32_t c = a.cu[i];
+    const KvSeq s = kv_seq(a, i);
+    const uint64_t m = __ballot(lane < a.nseq && base(c, lane) <= u);
+    const int b = __builtin_amdgcn_readfirstlane(max(1, (int)__popcll(m)) - 1);
+    return {b, __builtin_amdgcn_readlane(c, b), lane_seq(s, b)};
+  }
+  int lo = 0, n = a.nseq;
   while (n > 1) {
     const int step = (n + 63) >> 6;
     const int off = lane * step;
-    const bool at = off < n && base(lo + off) <= u;
+    const bool at = off < n && base(a.cu[lo + min(off, n - 1)], lo + off) <= u;
     const uint64_t m = __ballot(at);
     const int c = max(1, (int)__popcll(m));
     const int skip = (c - 1) * step;
     lo += skip;
     n = min(step, n - skip);
   }
-  return __builtin_amdgcn_readfirstlane(lo);
+  const int b = __builtin_amdgcn_readfirstlane(lo);
+  return {b, a.cu[b], kv_seq(a, b)};
 }
 #endif
 

@@ -40,11 +40,11 @@ int64_t kv_units(int64_t rows, int nseq, bool* by_row) {
 
 __device__ __forceinline__ KvUnit kv_unit(const KvArgs& a, int64_t u, bool by_row) {
   KvUnit r;
-  const int32_t* cu = a.cu;
   int64_t slot;
   if (by_row) {
-    r.b = kv_find(a.nseq, u, [&](int b) { return (int64_t)cu[b]; });
-    const KvSeq s = kv_seq(a, r.b);
+    const KvFound f = kv_find(a, u, [](int32_t c, int) { return (int64_t)c; });
+    const KvSeq s = f.s;
+    r.b = f.b;
     const int64_t start = (int64_t)s.len - s.n, pos = start + (u - s.row0);
     slot = pos >> 6;
     r.ok = u >= s.row0 && u < s.row0 + s.n && (u == s.row0 || (pos & 63) == 0);
@@ -52,10 +52,12 @@ __device__ __forceinline__ KvUnit kv_unit(const KvArgs& a, int64_t u, bool by_ro
     r.place = (int32_t)(pos & 63);
     r.n = (int32_t)min((int64_t)(64 - r.place), s.row0 + s.n - u);
   } else {
-    r.b = kv_find(a.nseq, u, [&](int b) { return ((int64_t)cu[b] >> 6) + 2 * b; });
-    const KvSeq s = kv_seq(a, r.b);
+    auto base = [](int32_t c, int b) { return ((int64_t)c >> 6) + 2 * b; };
+    const KvFound f = kv_find(a, u, base);
+    const KvSeq s = f.s;
+    r.b = f.b;
     const int64_t start = (int64_t)s.len - s.n, end = s.len;
-    slot = (start >> 6) + (u - (((int64_t)cu[r.b] >> 6) + 2 * r.b));
+    slot = (start >> 6) + (u - base(f.cu0, f.b));
     const int64_t p0 = max(start, slot * 64), p1 = min(end, slot * 64 + 64);
     r.ok = slot >= (start >> 6) && p0 < p1;
     r.row = s.row0 + (p0 - start);
@@ -191,6 +193,23 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
         }
   }
   if (tid == 0) *scale = exp2_int(e);  // (every thread read the old one before the maximum was joined)
+  if (part == 1 && u.n <= 8 && !grow) {
+    // few values: their bytes alone (one token of 64 sequences, 8 heads of
+    // 128 dims: 7.1 us, and 8.3 with the value rows read and written whole)
+#pragma unroll
+    for (int c = 0; c < NCM; c++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int t = t0 + i;
+        if (c < a.nc && t >= u.place && t < end) {
+          const uint32_t w = pack4(x[c][i][0] * inv, x[c][i][1] * inv, x[c][i][2] * inv, x[c][i][3] * inv);
+          uint8_t* to = dst + (int64_t)(c * 64 + dq * 4) * 64 + tb * 16 + ta * 4 + i;
+#pragma unroll
+          for (int j = 0; j < 4; j++) to[j * 64] = (uint8_t)(w >> (8 * j));
+        }
+      }
+    return;
+  }
 #pragma unroll
   for (int c = 0; c < NCM; c++) {
     if (c >= a.nc) continue;
@@ -201,19 +220,6 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
         uint32_t* w = reinterpret_cast<uint32_t*>(dst + c * 4096 + t * 64 + dq * 4);
         if (t >= u.place && t < end) *w = pack4(x[c][i][0] * inv, x[c][i][1] * inv, x[c][i][2] * inv, x[c][i][3] * inv);
         else if (grow && t < u.place) *w = rescale4(*w, shrink);
-      }
-    } else if (u.n <= 8 && !grow) {
-      // few tokens: their bytes alone (a token's step of 64 sequences, 8
-      // heads of 128 dims: 8.3 us with the value rows read and written whole)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int t = t0 + i;
-        if (t >= u.place && t < end) {
-          const uint32_t w = pack4(x[c][i][0] * inv, x[c][i][1] * inv, x[c][i][2] * inv, x[c][i][3] * inv);
-          uint8_t* to = dst + (int64_t)(c * 64 + dq * 4) * 64 + tb * 16 + ta * 4 + i;
-#pragma unroll
-          for (int j = 0; j < 4; j++) to[j * 64] = (uint8_t)(w >> (8 * j));
-        }
       }
     } else {
       // four tokens of one dim to a word, the slice's words through LDS so
