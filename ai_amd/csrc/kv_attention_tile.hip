@@ -1,5 +1,7 @@
 // Attention over the 8-bit key/value cache for many query rows (prompts and
 // chunks of them).
+#include <type_traits>
+
 #include "kv_attention.h"
 
 namespace fa {
@@ -30,9 +32,24 @@ __device__ __forceinline__ void reads_ahead() {
 }
 
 typedef float kvf16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ kvf16 mfma32(bf16x8 a, bf16x8 b, kvf16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ kvf16 mfma32(f16x8 a, f16x8 b, kvf16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Eight codes (two dwords) as an fp16 operand.
+__device__ __forceinline__ f16x8 widen_f16(uint32_t a, uint32_t b) {
+  const f16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false);
+  const f16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true);
+  const f16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false);
+  const f16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
+  return f16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 }
 
 // A workgroup of four waves takes 128 query rows of one key/value head, a wave
@@ -42,10 +59,17 @@ __device__ __forceinline__ kvf16 mfma32(bf16x8 a, bf16x8 b, kvf16 c) {
 // them as operands (1 KB in a row: no bank conflicts). The products are
 // transposed as in the kernel for few rows, on the 32x32x16 MFMA: it leaves
 // lane l (row l % 32, half l / 32) the scores of tokens 8 i + 4 half + 0..3.
+//
+// A float32 query enters as two fp16 terms of its row scaled by a power of two
+// to a largest magnitude of 2^13 .. 2^14: 22 bits of a value, or 2^-39 of the row's
+// largest, whichever is coarser (codes are exact in fp16, too). Its weights
+// keep three bf16 terms: with the value scales in them they need float32's range.
 template <typename T, int TERMS, int NC>
 __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_tile_kernel(AttnArgs a) {
   constexpr int W = 4, kThreads = W * 64, kRows = W * 32;
   constexpr int KS = NC * 4;            // steps of 16 dims
+  constexpr int QT = TERMS == 3 ? 2 : 1;  // terms of a query
+  using Op = typename std::conditional<TERMS == 3, f16x8, bf16x8>::type;
   constexpr int DT = NC * 2;            // tiles of 32 dims
   constexpr int kFrag = NC * 512;       // operands of a block's keys; as many of its values
   constexpr int kVals = (NC + 1) / 2;   // a thread's value loads of 2 x 16 codes; NC key loads of 16
@@ -141,8 +165,13 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
     uint4* to = tile_lds + buf * 2 * kFrag;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
-      to[kto[i]] = __builtin_bit_cast(uint4, widen(kraw[i].x, kraw[i].y));
-      to[kto[i] + 32] = __builtin_bit_cast(uint4, widen(kraw[i].z, kraw[i].w));
+      if constexpr (TERMS == 3) {
+        to[kto[i]] = __builtin_bit_cast(uint4, widen_f16(kraw[i].x, kraw[i].y));
+        to[kto[i] + 32] = __builtin_bit_cast(uint4, widen_f16(kraw[i].z, kraw[i].w));
+      } else {
+        to[kto[i]] = __builtin_bit_cast(uint4, widen(kraw[i].x, kraw[i].y));
+        to[kto[i] + 32] = __builtin_bit_cast(uint4, widen(kraw[i].z, kraw[i].w));
+      }
     }
     const int j0 = p * 64;
     if (j0 < galo || j0 + 64 > gahi) {
@@ -193,17 +222,42 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
   }
 
   // queries as operands, in registers; a negative scale turns their sign
-  bf16x8 qf[KS][TERMS];
+  Op qf[KS][QT];
+  float back = 1.f;  // what a score is to be multiplied by
   {
     const float sign = a.scale2 < 0.f ? -1.f : 1.f;
     const T* p = (const T*)a.q + (s.row0 + tok) * a.q_st + head * a.q_sh;
+    if constexpr (TERMS == 3) {
+      float v[KS][8], top = 0.f;
 #pragma unroll
-    for (int k = 0; k < KS; k++) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (on) load8(p, k * 16 + half * 8, a.c.D, a.vec, v);
+      for (int k = 0; k < KS; k++) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) v[i] *= sign;
-      terms_of<TERMS>(v, qf[k]);
+        for (int i = 0; i < 8; i++) v[k][i] = 0.f;
+        if (on) load8(p, k * 16 + half * 8, a.c.D, a.vec, v[k]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[k][i]));
+      }
+      top = fmaxf(top, lane_xor32(top));
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 14), 254);
+      const float up = sign * __uint_as_float((uint32_t)(267 - e) << 23);  // 2^(140 - e): the row's largest to 2^13 .. 2^14
+      back = __uint_as_float((uint32_t)max(e - 13, 1) << 23);
+#pragma unroll
+      for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float y = v[k][i] * up;
+          qf[k][0][i] = (_Float16)y;
+          qf[k][1][i] = (_Float16)(y - (float)qf[k][0][i]);
+        }
+    } else {
+#pragma unroll
+      for (int k = 0; k < KS; k++) {
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (on) load8(p, k * 16 + half * 8, a.c.D, a.vec, v);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] *= sign;
+        terms_of<1>(v, qf[k]);
+      }
     }
   }
 
@@ -279,15 +333,15 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
         for (int j = 0; j < 16; j++) sc[tt][j] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; k++) {
-        const bf16x8 k0 = __builtin_bit_cast(bf16x8, kf[k * 128 + lane]);
-        const bf16x8 k1 = __builtin_bit_cast(bf16x8, kf[k * 128 + 64 + lane]);
+        const Op k0 = __builtin_bit_cast(Op, kf[k * 128 + lane]);
+        const Op k1 = __builtin_bit_cast(Op, kf[k * 128 + 64 + lane]);
 #pragma unroll
-        for (int x = 0; x < TERMS; x++) {
+        for (int x = 0; x < QT; x++) {
           sc[0] = mfma32(k0, qf[k][x], sc[0]);
           sc[1] = mfma32(k1, qf[k][x], sc[1]);
         }
       }
-      reads_ahead<KS * 2, TERMS>();
+      reads_ahead<KS * 2, QT>();
     }
     if (p + 1 < pg1) {
       stage(buf ^ 1, p + 1);
@@ -299,7 +353,7 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
     }
     if (here) {
       // (not zero: a hidden score is -inf times it)
-      const float mul = fmaxf(fabsf(a.scale2) * ksv.x, 0x1p-126f);
+      const float mul = fmaxf(fabsf(a.scale2) * ksv.x * back, 0x1p-126f);
       const float f = ksv.y * kWeightScale;
       if (j0 < alo || j0 + 64 > ahi) {
 #pragma unroll
