@@ -99,16 +99,18 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const KvSeq& s, cons
 
 // One work item: 16 query rows of one key/value head over a run of blocks.
 // Lane l: row l % 16, group l / 16. NC: slices of 64 dims (at most; nc in use).
-// Its blocks go to the four waves in turn. A wave loads a block's keys
-// while it turns the block before into weights and sums, and its values likewise, as registers
-// allow: the loads of one block (D = 128: 16 KB) are always under way.
+// Its blocks go to the four waves in turn, their results are merged at the
+// end. A wave loads a block's keys while it works on the scores of the block
+// before, and its values while it works on the next scores, so that about a
+// block (D = 128: 16 KB) is always under way: 64 sequences of up to 8192
+// tokens (606 MB) take 126 us, 4.8 TB/s, against 219 without, and a large copy
+// moves 5.1 TB/s. Above 256 dims the registers do not hold it.
 template <typename T, int TERMS, int NC>
 __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs a) {
-  // what is loaded a block ahead, with room for two workgroups on a CU (2: keys and values, 1: keys, 0: nothing)
-  constexpr int AHEAD = NC <= 4 ? 2 : 0;
-  constexpr int W = 4, kWaves = W, kThreads = W * 64;
-  constexpr int kMergeDims = 128;              // dims that the waves' results are merged at a time
-  constexpr int kLane = kMergeDims / (W * 4);  // and a thread's of them, W * 4 threads a row
+  constexpr bool AHEAD = NC <= 4;  // loads a block ahead
+  constexpr int kWaves = 4, kThreads = kWaves * 64;
+  constexpr int kMergeDims = 128;         // dims that the waves' results are merged at a time
+  constexpr int kLane = kMergeDims / 16;  // and a thread's of them, 16 threads a row
   const int nc = NC <= 4 ? NC : a.c.nc;
   constexpr int kQ = TERMS * NC * 2 * 64;           // operands of 16 bytes
   constexpr int kM = kWaves * kTileRows * (kMergeDims + 4);  // floats
@@ -149,7 +151,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
   }
 
   // a block's codes, 16 bytes a lane: kr[slice * 4 + tile of 16 tokens], vr[tile of 16 dims]
-  uint4 kr[AHEAD >= 1 ? NC * 4 : 1], vr[AHEAD == 2 ? NC * 4 : 1];
+  uint4 kr[AHEAD ? NC * 4 : 1], vr[AHEAD ? NC * 4 : 1];
   auto part = [&](int id, int which) {
     return reinterpret_cast<const uint4*>(kv_part(a.c, id, it.h, which)) + row * 4 + grp;
   };
@@ -161,14 +163,14 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
     return p && (NC <= 4 || i < nc * 4) ? p[i * 64] : make_uint4(0, 0, 0, 0);
   };
   auto load_k = [&](int id) {
-    if constexpr (AHEAD >= 1) {
+    if constexpr (AHEAD) {
       const uint4* p = id >= 0 ? part(id, 0) : nullptr;
 #pragma unroll
       for (int i = 0; i < NC * 4; i++) kr[i] = key(p, i);
     }
   };
   auto load_v = [&](int id) {
-    if constexpr (AHEAD == 2) {
+    if constexpr (AHEAD) {
       const uint4* p = id >= 0 ? part(id, 1) : nullptr;
 #pragma unroll
       for (int i = 0; i < NC * 4; i++) vr[i] = value(p, i);
@@ -227,7 +229,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
       uint4 kc[4];
 #pragma unroll
       for (int tt = 0; tt < 4; tt++) {
-        if constexpr (AHEAD >= 1) kc[tt] = kr[c * 4 + tt];
+        if constexpr (AHEAD) kc[tt] = kr[c * 4 + tt];
         else kc[tt] = key(kp, c * 4 + tt);
       }
 #pragma unroll
@@ -309,7 +311,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
     for (int dt = 0; dt < NC * 4; dt++) {
       if (NC > 4 && dt >= nc * 4) continue;
       uint4 v;
-      if constexpr (AHEAD == 2) v = vr[dt];
+      if constexpr (AHEAD) v = vr[dt];
       else v = value(vp, dt);
       if (edge) v = make_uint4(v.x & keep[0], v.y & keep[1], v.z & keep[2], v.w & keep[3]);
       if (mixed) {
@@ -375,8 +377,8 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
   for (int w = 0; w < kWaves; w++) M = fmaxf(M, stat[w][row][0]);
   const float Mu = M == -__builtin_inff() ? 0.f : M;
   const float mine = __builtin_amdgcn_exp2f(m - Mu);
-  // the output rows: W * 4 threads a row, each kLane dims of every kMergeDims
-  const int orow = tid / (W * 4), oat = (tid % (W * 4)) * kLane;
+  // the output rows: 16 threads a row, each kLane dims of every kMergeDims
+  const int orow = tid >> 4, oat = (tid & 15) * kLane;
   float oM = -__builtin_inff(), L = 0.f;
 #pragma unroll
   for (int w = 0; w < kWaves; w++) oM = fmaxf(oM, stat[w][orow][0]);
@@ -490,10 +492,11 @@ Shape shape_of(const KvAttnArgs& a) {
   if (items >= (wide ? kWideItems : kTarget) || blocks <= r.least) {
     r.parts = 0;
   } else {
-    // (a part has at least least blocks, and total / 256 of them up to kRound)
+    // as plan_item: a part has at least `least` blocks, total / target of them, and
+    // total / 256 up to kRound; the last part of each item may be short
     const int64_t total = items * blocks, most = (blocks + r.least - 1) / r.least;
     const int64_t cut = wide ? r.target : std::max((int64_t)256, std::min((int64_t)kTarget, total / kRound));
-    r.parts = std::min(cut + items, items * most);
+    r.parts = std::min(cut + items + 8, items * most);  // (8: the kernel's sums are rounded)
   }
   return r;
 }

@@ -38,9 +38,9 @@ int check_batch(fa_ctx* ctx, const char* op, const fa_kv_batch* b, int dtype) {
 
 // Rows of a batch, units of work and int32 row indexes in the kernels.
 int check_sizes(fa_ctx* ctx, const char* op, const fa_kv_batch* b, int64_t heads) {
-  if (b->rows > kMaxGrid / heads || b->rows * heads + (int64_t)b->nseq * 2 > kMaxGrid)
-    return set_error(ctx, FA_ERR_ARG, "%s: %lld rows of %lld heads are more than one call takes", op,
-                     (long long)b->rows, (long long)heads);
+  if (b->rows > kMaxGrid / heads || b->rows * heads + (int64_t)b->nseq * std::max<int64_t>(heads, 2) > kMaxGrid)
+    return set_error(ctx, FA_ERR_ARG, "%s: %lld rows of %d sequences with %lld heads are more than one call takes", op,
+                     (long long)b->rows, b->nseq, (long long)heads);
   return FA_OK;
 }
 

@@ -45,7 +45,7 @@ struct KvAttnArgs {
 };
 // Scratch that a call needs (partial results of a split token axis); 0: none.
 // It begins with kKvCountBytes of counters that are zero between calls.
-constexpr size_t kKvCountBytes = 8192;
+constexpr size_t kKvCountBytes = 16384;
 size_t kv_attention_scratch(const KvAttnArgs& a);
 int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& a, void* scratch, hipStream_t s);
 

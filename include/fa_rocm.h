@@ -279,7 +279,7 @@ typedef struct fa_kv_batch {
  * read back as NaN, and make the outputs of the queries that see them NaN (all
  * outputs of a sequence longer than its table row). Two sequences of a call
  * must not write the same block: the block's contents would be undefined.
- * dtype (of the tensors): FA_DT_F32 or FA_DT_BF16. rows * heads < 2^31.
+ * dtype (of the tensors): FA_DT_F32 or FA_DT_BF16. (rows + nseq) * heads < 2^31.
  * k, v, q: row r, head h at r * st + h * sh elements, dims contiguous.
  *
  * fa_kv_write quantises rows into the cache. A block that receives new tokens
@@ -309,12 +309,13 @@ int fa_kv_read_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* bat
  * all of them, and of those, with window > 0, only the ones with |p - j| <
  * window. A row that sees nothing gives zeros; a token it does not see has no
  * part in its output, whatever the cache holds there. out: [rows][heads][head_dim]
- * contiguous, of dtype. Sums, statistics and scores in float32; float32
- * queries and weights enter the matrix units as three exact bf16 terms; with
- * bf16 tensors weights are rounded to bf16.
+ * contiguous, of dtype. Sums, statistics and scores are float32. With float32
+ * tensors queries and weights enter the matrix units as three exact bf16 terms
+ * (queries of many rows as two fp16 terms of the row scaled by a power of two, 22
+ * bits), with bf16 tensors weights are rounded to bf16.
  *
  * work (_dev): scratch of at least fa_kv_attention_work(...) bytes, 16-byte
- * aligned, used until the call's work is done: calls that may overlap (graphs
+ * aligned, of any contents, used until the call's work is done: calls that may overlap (graphs
  * replayed on different streams) need one each. NULL: the context's own, which
  * may grow, so that a call under capture needs work (FA_ERR_STATE otherwise,
  * if any is needed). fa_kv_attention_work reads only the sizes in cache and

@@ -75,10 +75,9 @@ class RefCache:
 
     def tokens(self, table, length):
         """Keys and values [length, kv_heads, D] of a sequence."""
-        got = []
+        got, used = [], np.asarray(table[:-(-length // BLOCK)], int)
         for part in (0, 1):
-            x = self.val[:, :, part] * 2.0 ** self.exp[:, :, part][:, :, None, None]
-            x = x[np.asarray(table[:-(-length // BLOCK)], int)]  # [blocks, heads, 64, D]
+            x = self.val[used, :, part] * 2.0 ** self.exp[used, :, part][:, :, None, None]  # [blocks, heads, 64, D]
             got.append(x.transpose(0, 2, 1, 3).reshape(-1, x.shape[1], x.shape[3])[:length])
         return got
 
@@ -100,7 +99,8 @@ def attention(q, k, v, mask, scale):
     output is rounded (float32 queries); the second bound is for bf16 tensors, whose weights are rounded to bf16.
 
     Scores: exact products of bf16 terms, sums of at most 3 D terms and three factors in float32, so off by at most
-    (3 D + 4) U times the sum of magnitudes; the largest such error among a row's tokens, dS, moves every weight by a
+    (3 D + 4) U times the sum of magnitudes (two fp16 terms leave 2^-22 = 4 U of a query value, with sums of 2 D terms:
+    no more from D = 4 on, and below that the bound of D = 4 is taken; or 2^-39 of the row's largest); the largest such error among a row's tokens, dS, moves every weight by a
     factor within e^(+-2 dS) (weight and sum), the hardware's exp2 by 2^-22 at most (its argument is rounded, too: U
     times its size, at most 150 where a weight counts). The sums over S tokens, of three terms each, and the joining of
     waves and parts add at most (3 S + 64) U. All relative to sum p |v|."""
@@ -121,7 +121,8 @@ def attention(q, k, v, mask, scale):
             p = np.exp(x - x.max())
             p /= p.sum()
             out[i, h] = p @ vh[on]
-            ds = (3 * D + 4) * U * mag[i, on].max()
+            ds = (3 * max(D, 4) + 4) * U * mag[i, on].max()
+            ds += 2.0 ** -39 * np.abs(q[i, h]).max() * np.abs(kh[on]).sum(1).max() * abs(scale)
             rel = np.expm1(2 * ds) + 2.0 ** -22 + 2 * 150 * U + (3 * on.sum() + 64) * U
             tol[i, h] = rel * (p @ np.abs(vh[on]))
     return out, tol

@@ -276,6 +276,93 @@ def test_attention_prompts(ctx, D, H, Hkv, lengths, ns, dtype):
     attention_case(ctx, D + H + 1, dtype, D, H, Hkv, lengths, ns, window=90)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D,H,Hkv,lengths,ns", [(128, 8, 2, [5000], [40]), (64, 2, 1, [2000, 9000], [100, 130]),
+                                                (256, 3, 1, [1500], [70]), (192, 1, 1, [3000], [129])])
+def test_attention_few_tiles_of_many_rows_split(ctx, D, H, Hkv, lengths, ns, dtype):
+    """Chunks on long contexts: few tiles of 128 rows, whose blocks are cut into parts and joined."""
+    attention_case(ctx, D + H, dtype, D, H, Hkv, lengths, ns, work=dtype == "f32")
+    attention_case(ctx, D + H + 1, dtype, D, H, Hkv, lengths, ns, causal=False, window=1100, work=dtype == "bf16")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_many_sequences(ctx, dtype):
+    """More sequences than a wave has lanes, some empty, some without rows; split and not."""
+    r = rng(77)
+    lengths = [int(x) for x in r.integers(0, 700, 130)]
+    lengths[5] = lengths[64] = 0
+    ns = [min(l, int(r.integers(0, 4))) for l in lengths]
+    attention_case(ctx, 78, dtype, 64, 2, 1, lengths, ns, width=11)
+    attention_case(ctx, 79, dtype, 64, 16, 16, lengths, [min(l, 1) for l in lengths])
+
+
+def test_thousands_of_sequences(ctx):
+    """Sequence starts found in two rounds and more, one row each: written, read back, attended to."""
+    r = rng(80)
+    B, D = 4500, 64
+    lengths = [int(x) for x in r.integers(1, 4, B)]
+    blocks = B
+    tables = r.permutation(blocks).astype(np.int32)[:, None]
+    cache, ref = K.Cache(ctx, blocks, 1, D), O.RefCache(blocks, 1, D)
+    for step in range(1, 4):
+        now = [min(l, step) for l in lengths]
+        ns = [int(l >= step) for l in lengths]
+        cu = K.cu_of(ns)
+        k, v = make(r, (int(cu[-1]), 1, D), "f32"), make(r, (int(cu[-1]), 1, D), "f32")
+        b = K.Batch(ctx, tables, now, cu)
+        K.write(cache, b, k, v)
+        ref.write(tables, now, cu, k, v)
+        b.free()
+    b = K.Batch(ctx, tables, lengths, K.cu_of(lengths))
+    gk, gv = K.read(cache, b)
+    q = make(r, (int(b.cu[-1]), 2, D), "f32")
+    out = K.attend(cache, b, q, scale=0.125)
+    for i in range(B):
+        wk, wv = ref.tokens(tables[i], lengths[i])
+        rows = slice(b.cu[i], b.cu[i + 1])
+        np.testing.assert_array_equal(gk[rows], wk)
+        np.testing.assert_array_equal(gv[rows], wv)
+        if i % 50 == 0:
+            want, tol = O.attention(q[rows], wk, wv, O.sees(lengths[i], lengths[i], True, 0), 0.125)
+            close(out[rows], want, tol, f"sequence {i}")
+    b.free()
+    cache.free()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [2, 150])
+def test_attention_scores_that_rise_and_fall(ctx, dtype, n):
+    """Scores that rise by thousands of times their weights' range from block to block, and fall again: the reference
+    of the weights follows, in both kernels, split and not."""
+    r = rng(90 + n)
+    for length, H in ((700, 4), (300, 1)):
+        D = 64
+        blocks, tables = K.tables_for(r, [length])
+        cache, ref = K.Cache(ctx, blocks, 1, D), O.RefCache(blocks, 1, D)
+        k = make(r, (length, 1, D), "f32", 0.1)
+        k[:, 0, 0] = np.concatenate([np.linspace(0, 60, length // 2), np.linspace(60, -20, length - length // 2)])
+        v = make(r, (length, 1, D), "f32")
+        q = make(r, (n, H, D), "f32", 0.1)
+        q[:, :, 0] = 1.0
+        if dtype == "bf16":
+            k, v, q = (S.f32_to_bf16(x) for x in (k, v, q))
+        b = K.Batch(ctx, tables, [length], [0, length])
+        K.write(cache, b, k, v)
+        b.free()
+        ref.write(tables, [length], [0, length], K.wide(k), K.wide(v))
+        b = K.Batch(ctx, tables, [length], [0, n])
+        wk, wv = ref.tokens(tables[0], length)
+        for scale in (1.0, -1.0):
+            got = K.attend(cache, b, q, scale=scale)
+            mask = O.sees(length, n, True, 0)
+            want, tol = O.attention(K.wide(q), wk, wv, mask, scale)
+            if dtype == "bf16":
+                tol = tol + BF * O.attention(K.wide(q), wk, np.abs(wv), mask, scale)[0]
+            close(got, want, tol, f"rising scores, {n} rows, scale {scale}")
+        b.free()
+        cache.free()
+
+
 def test_attention_score_range(ctx):
     """Scores of hundreds either way, scale 0, a negative scale."""
     for scale in (3.0, 0.0, -0.7):
@@ -299,6 +386,30 @@ def test_attention_value_scales_far_apart(ctx):
     wk, wv = ref.tokens(tables[0], 320)
     want, tol = O.attention(q, wk, wv, O.sees(320, 320, True, 64), 0.125)
     close(got, want, tol, "value scales")
+    b.free()
+    cache.free()
+
+
+def test_attention_value_scales_far_apart_few_rows(ctx):
+    """The same with three rows on a split axis."""
+    r = rng(32)
+    lengths, D = [64 * 20], 128
+    blocks, tables = K.tables_for(r, lengths)
+    cache, ref = K.Cache(ctx, blocks, 1, D), O.RefCache(blocks, 1, D)
+    k, v = make(r, (1280, 1, D), "f32"), make(r, (1280, 1, D), "f32")
+    for i in range(20):
+        v[i * 64:(i + 1) * 64] *= np.float32(2.0 ** (-3 * i))
+    b = K.Batch(ctx, tables, lengths, [0, 1280])
+    K.write(cache, b, k, v)
+    b.free()
+    ref.write(tables, lengths, [0, 1280], k, v)
+    q = make(r, (3, 1, D), "f32")
+    wk, wv = ref.tokens(tables[0], 1280)
+    b = K.Batch(ctx, tables, lengths, [0, 3])
+    for window in (0, 70):
+        got = K.attend(cache, b, q, True, window, 0.125)
+        want, tol = O.attention(q, wk, wv, O.sees(1280, 3, True, window), 0.125)
+        close(got, want, tol, f"value scales, window {window}")
     b.free()
     cache.free()
 
@@ -354,6 +465,35 @@ def test_attention_nan_stays_where_it_is_seen(ctx):
             want[100:120, :, 5] = True
             want[150:170, :, 33] = True
             want[180:200] = True
+            np.testing.assert_array_equal(np.isnan(out), want)
+            b.free()
+            cache.free()
+
+
+def test_attention_nan_among_drafted_tokens(ctx):
+    """The same with a tile of few rows: NaN at the positions of the last tokens, seen by those after them."""
+    r = rng(18)
+    for dtype in ("f32", "bf16"):
+        for D, length in ((64, 70), (256, 2000), (512, 131)):
+            blocks, tables = K.tables_for(r, [length])
+            cache = K.Cache(ctx, blocks, 1, D)
+            k, v = make(r, (length, 1, D), "f32"), make(r, (length, 1, D), "f32")
+            v[length - 4, 0, 5] = np.nan
+            v[length - 2, 0, 40] = -np.inf
+            k[length - 1, 0, 1] = np.nan
+            if dtype == "bf16":
+                k, v = S.f32_to_bf16(k), S.f32_to_bf16(v)
+                k[length - 1, 0, 1] = 0x7FC0
+            b = K.Batch(ctx, tables, [length], [0, length])
+            K.write(cache, b, k, v)
+            b.free()
+            b = K.Batch(ctx, tables, [length], [0, 5])
+            q = make(r, (5, 3, D), dtype)
+            out = K.wide(K.attend(cache, b, q, scale=0.05))
+            want = np.zeros(out.shape, bool)
+            want[1:, :, 5] = True
+            want[3:, :, 40] = True
+            want[4] = True
             np.testing.assert_array_equal(np.isnan(out), want)
             b.free()
             cache.free()
