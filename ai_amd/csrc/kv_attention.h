@@ -11,11 +11,13 @@ constexpr int kTileRows = 16;   // query rows of a work item of the kernel for f
 constexpr int kWideRows = 128;  // and of the one for many
 
 constexpr int kMinChunk = 4;    // blocks of a split part, at least (one per wave)
-constexpr int kRound = 64;      // blocks of a part up to which one round of a part for each CU is aimed at
-constexpr int kTarget = 1024;   // split parts aimed at: two rounds of two workgroups on each of 256 CUs
+constexpr int kRound = 64;      // blocks of a part up to which one part for each CU is aimed at
+constexpr int kTarget = 1024;   // else parts aimed at: two rounds of two workgroups on each of 256 CUs
 // Weights are multiplied by the value scale 2^e and this, so that sums of 2^20
 // times float32's largest values stay finite; the result is multiplied back.
 constexpr float kWeightScale = 0x1p-24f;
+// The least of these factors under which float32 holds scaled weights down to 2^-62.
+constexpr float kLeastFactor = 0x1p-64f;
 // The largest sum of a lane's weights in a block, relative to its row's reference.
 constexpr float kMostWeight = 0x1p8f;
 
@@ -95,10 +97,17 @@ struct Item {
 };
 
 // Parts are numbered by sequence, tile, head, chunk. The item of part w, or
-// (w < 0) the first part of the tile and head that are asked for. A part has
-// the batch's blocks over a.target, a.least at least (a float32 sum in a
-// fixed order: the same in every wave); every wave finds its own from the
-// lengths, one load for up to 64 sequences.
+// (w < 0) the first part of the tile and head that are asked for. Every wave
+// finds its own from the lengths, one load for up to 64 sequences (float32
+// sums in a fixed order: the same in every wave).
+//
+// A part has the batch's blocks over a.target, a.least at least; but up to
+// a.cap blocks, as many as leave one part for each CU: a part's beginning (its
+// lengths, its table entries, its first codes, each load after the one before)
+// takes as long as some ten blocks, and every part is written and read once
+// more. One sequence of 131072 tokens, 32 heads on 8 of 128 dims: 57 us in 256
+// parts, 63 in 512, 80 in 1024. Longer parts leave less to balance uneven
+// sequences with: those are cut by the target.
 __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want_b, int want_tile, int want_h) {
   const int lane = threadIdx.x & 63;
   const Seen first = seen_by(a, lane);

@@ -535,6 +535,11 @@ size_t kv_attention_scratch(const KvAttnArgs& a) {
   return h.parts ? kKvCountBytes + (size_t)h.parts * h.tile * (a.c.nc * 64 + 2) * sizeof(float) : 0;
 }
 
+int64_t kv_attention_grid(const KvAttnArgs& a) {
+  const Shape h = shape_of(a);
+  return h.parts ? h.parts : h.tile == kTileRows ? h.slots : h.slots * a.c.hkv;
+}
+
 int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStream_t s) {
   AttnArgs a;
   a.c = k.c;

@@ -60,6 +60,15 @@ __device__ __forceinline__ f16x8 widen_f16(uint32_t a, uint32_t b) {
 // them as operands (1 KB in a row: no bank conflicts). The products are
 // transposed as in the kernel for few rows, on the 32x32x16 MFMA: it leaves
 // lane l (row l % 32, half l / 32) the scores of tokens 8 i + 4 half + 0..3.
+// 128 rows: a block's widening is shared by four waves (a wave alone would
+// convert 2 * 64 * D codes for 32 rows, as many instructions as its softmax),
+// and two such workgroups fit a CU (bf16, up to 128 dims).
+//
+// A prompt of 8192 tokens, 32 heads on 8 of 128 dims in bf16: 519 to 551 us,
+// 1.0 to 1.06 PFLOP/s, where a large matrix product reaches 1.26. Bound by the
+// products (matrix units busy 0.41 of the time) and by the arithmetic of
+// softmax and widening (0.45) in two waves per SIMD, which overlap little: a
+// wave's own products wait for its weights.
 //
 // A float32 query enters as two fp16 terms of its row scaled by a power of two
 // to a largest magnitude of 2^13 .. 2^14: 22 bits of a value, or 2^-39 of the row's
@@ -366,9 +375,10 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
             sc[tt][j] = t >= rlo && t < rhi ? sc[tt][j] : -__builtin_inff();
           }
       }
-      // one term: the value scale enters the exponent, and the sum of the
-      // scaled weights is scaled back once a block
-      const float fe = TERMS == 1 ? (float)((int)(__float_as_uint(f) >> 23) - 127) : 0.f;
+      // one term: the value scale enters the exponent (down to kLeastFactor:
+      // below it, weights that count in the row's sum would be lost), and the
+      // sum of the scaled weights is scaled back once a block
+      const float fe = TERMS == 1 ? (float)((int)(__float_as_uint(fmaxf(f, kLeastFactor)) >> 23) - 127) : 0.f;
       float part;
       bf16x8 pt[4][TERMS];
       auto weights = [&]() {
@@ -406,6 +416,13 @@ __global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_ti
         weights();
       }
       l += part;
+      if (TERMS == 1 && f < kLeastFactor) {  // (rare: values all zero, or none over 2^-31)
+        const float rest = f * (1.f / kLeastFactor);
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) pt[k][0][i] = (__bf16)((float)pt[k][0][i] * rest);
+      }
 #pragma unroll
       for (int k = 0; k < 4; k++)
 #pragma unroll

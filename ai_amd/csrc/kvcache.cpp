@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <new>
 #include <vector>
 
 using fa::set_error;
@@ -11,6 +12,7 @@ using namespace fa::slots;
 namespace {
 
 constexpr int64_t kMaxGrid = 0x7FFFFFFF;
+constexpr int32_t kMaxTable = (1 << 25) - 1;  // positions stay below 2^31
 
 int check_cache(fa_ctx* ctx, const char* op, const fa_kv_cache* c) {
   if (!c) return set_error(ctx, FA_ERR_ARG, "%s: cache is NULL", op);
@@ -30,6 +32,8 @@ int check_batch(fa_ctx* ctx, const char* op, const fa_kv_batch* b, int dtype) {
   if (b->nseq < 0 || b->rows < 0 || b->table_stride < 0)
     return set_error(ctx, FA_ERR_ARG, "%s: negative size (%d sequences, %lld rows, table rows of %d)", op, b->nseq,
                      (long long)b->rows, b->table_stride);
+  if (b->table_stride > kMaxTable)
+    return set_error(ctx, FA_ERR_ARG, "%s: table rows of %d entries, at most %d", op, b->table_stride, kMaxTable);
   if (dtype != FA_DT_F32 && dtype != FA_DT_BF16) return set_error(ctx, FA_ERR_ARG, "%s: unknown dtype %d", op, dtype);
   if (b->nseq > 0 && (!b->lengths || !b->cu_rows || (b->table_stride > 0 && !b->tables)))
     return set_error(ctx, FA_ERR_ARG, "%s: NULL batch array", op);
@@ -44,11 +48,19 @@ int check_sizes(fa_ctx* ctx, const char* op, const fa_kv_batch* b, int64_t heads
   return FA_OK;
 }
 
+// Workgroups of a launch (of 256 threads, which are counted in 32 bits).
+int check_grid(fa_ctx* ctx, const char* op, int64_t workgroups) {
+  if (workgroups >= (int64_t)1 << 24)
+    return set_error(ctx, FA_ERR_ARG, "%s: %lld workgroups are more than one call takes", op, (long long)workgroups);
+  return FA_OK;
+}
+
 enum class Use { Write, Read, Attend };
 
 // The host entry points see the batch: everything that the kernels would
 // have to leave out is an error here.
-int check_host_batch(fa_ctx* ctx, const char* op, const fa_kv_cache* c, const fa_kv_batch* b, Use use) {
+int check_host_batch(fa_ctx* ctx, const char* op, const fa_kv_cache* c, const fa_kv_batch* b, Use use,
+                     int32_t window = 0) try {
   if (b->nseq == 0) return FA_OK;
   if (b->cu_rows[0] != 0) return set_error(ctx, FA_ERR_ARG, "%s: cu_rows starts at %d, not 0", op, b->cu_rows[0]);
   for (int i = 0; i < b->nseq; i++)
@@ -68,7 +80,8 @@ int check_host_batch(fa_ctx* ctx, const char* op, const fa_kv_cache* c, const fa
     if (used > b->table_stride)
       return set_error(ctx, FA_ERR_ARG, "%s: sequence %d of %lld tokens needs %lld table entries, has %d", op, i,
                        (long long)len, (long long)used, b->table_stride);
-    const int64_t first = use == Use::Attend ? 0 : (len - n) / FA_KV_BLOCK;
+    const int64_t from = use != Use::Attend ? len - n : window ? std::max<int64_t>(0, len - n - window + 1) : 0;
+    const int64_t first = from / FA_KV_BLOCK;
     for (int64_t p = first; p < used; p++) {
       const int32_t id = b->tables[(int64_t)i * b->table_stride + p];
       if (id < 0 || id >= c->blocks)
@@ -82,6 +95,8 @@ int check_host_batch(fa_ctx* ctx, const char* op, const fa_kv_cache* c, const fa
   if (twice != written.end())
     return set_error(ctx, FA_ERR_ARG, "%s: block %d would be written twice", op, *twice);
   return FA_OK;
+} catch (const std::bad_alloc&) {
+  return set_error(ctx, FA_ERR_OOM, "%s: no host memory to check the batch", op);
 }
 
 fa::KvArgs args_of(const fa_kv_cache* c, const fa_kv_batch* b) {
@@ -104,17 +119,14 @@ fa::KvArgs args_of(const fa_kv_cache* c, const fa_kv_batch* b) {
 // The batch's arrays in device scratch; dev.tables etc. point there.
 int stage_batch(fa_ctx* ctx, const fa_kv_batch* b, fa_kv_batch* dev) {
   const size_t nt = (size_t)b->nseq * b->table_stride, n = (size_t)b->nseq;
-  std::vector<int32_t> all;
-  all.reserve(nt + 2 * n + 1);
-  all.insert(all.end(), b->tables, b->tables + nt);
-  all.insert(all.end(), b->lengths, b->lengths + n);
-  all.insert(all.end(), b->cu_rows, b->cu_rows + n + 1);
-  void* p;
-  const int rc = fa::stage_h2d(ctx, S_KV, all.data(), all.size() * 4, &p);
+  fa::DevBuf& buf = ctx->slot(S_KV);
+  const int rc = buf.ensure(ctx, (nt + 2 * n + 1) * 4);
   if (rc) return rc;
-  FA_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));  // `all` goes out of scope
+  int32_t* d = static_cast<int32_t*>(buf.ptr);
+  if (nt) FA_HIP_CHECK(ctx, hipMemcpyAsync(d, b->tables, nt * 4, hipMemcpyHostToDevice, ctx->stream));
+  FA_HIP_CHECK(ctx, hipMemcpyAsync(d + nt, b->lengths, n * 4, hipMemcpyHostToDevice, ctx->stream));
+  FA_HIP_CHECK(ctx, hipMemcpyAsync(d + nt + n, b->cu_rows, (n + 1) * 4, hipMemcpyHostToDevice, ctx->stream));
   *dev = *b;
-  const int32_t* d = static_cast<const int32_t*>(p);
   dev->tables = d;
   dev->lengths = d + nt;
   dev->cu_rows = d + nt + n;
@@ -128,8 +140,12 @@ size_t span(int64_t rows, int64_t heads, int64_t st, int64_t sh, int64_t D, int 
   return (size_t)((rows - 1) * st + (heads - 1) * sh + D) * elem(dtype);
 }
 
-int check_strides(fa_ctx* ctx, const char* op, int64_t st, int64_t sh) {
+int check_strides(fa_ctx* ctx, const char* op, int64_t rows, int64_t heads, int64_t st, int64_t sh) {
   if (st < 0 || sh < 0) return set_error(ctx, FA_ERR_ARG, "%s: negative stride", op);
+  constexpr int64_t most = (int64_t)1 << 58;  // elements: offsets in bytes stay within 63 bits
+  if (st > most / std::max<int64_t>(rows, 1) || sh > most / heads)
+    return set_error(ctx, FA_ERR_ARG, "%s: strides of %lld and %lld elements are too large", op, (long long)st,
+                     (long long)sh);
   return FA_OK;
 }
 
@@ -137,14 +153,13 @@ int attn_args(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, i
               int64_t q_sh, int32_t heads, int causal, int32_t window, float scale, void* out, fa::KvAttnArgs* a) {
   const char* op = "KVAttention";
   int rc;
-  if ((rc = check_cache(ctx, op, cache)) || (rc = check_batch(ctx, op, batch, dtype)) ||
-      (rc = check_strides(ctx, op, q_st, q_sh)))
-    return rc;
+  if ((rc = check_cache(ctx, op, cache)) || (rc = check_batch(ctx, op, batch, dtype))) return rc;
   if (heads < 1 || heads % cache->kv_heads != 0 || heads > 65535)
     return set_error(ctx, FA_ERR_ARG, "%s: %d query heads on %d key/value heads", op, heads, cache->kv_heads);
   if (window < 0) return set_error(ctx, FA_ERR_ARG, "%s: window %d", op, window);
-  if (!std::isfinite(scale)) return set_error(ctx, FA_ERR_ARG, "%s: scale is not finite", op);
-  if ((rc = check_sizes(ctx, op, batch, heads))) return rc;
+  if (!(std::fabs(scale) <= 0x1p126f)) return set_error(ctx, FA_ERR_ARG, "%s: scale is not finite, or over 2^126", op);
+  if ((rc = check_strides(ctx, op, batch->rows, heads, q_st, q_sh)) || (rc = check_sizes(ctx, op, batch, heads)))
+    return rc;
   if (batch->rows > 0 && batch->nseq > 0 && (!q || !out)) return set_error(ctx, FA_ERR_ARG, "%s: NULL buffer", op);
   a->c = args_of(cache, batch);
   a->dtype = dtype;
@@ -156,7 +171,7 @@ int attn_args(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, i
   a->window = window;
   a->scale = scale;
   a->out = out;
-  return FA_OK;
+  return check_grid(ctx, op, fa::kv_attention_grid(*a));
 }
 
 int write_check(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, const void* k,
@@ -164,8 +179,9 @@ int write_check(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch,
   const char* op = "KVWrite";
   int rc;
   if ((rc = check_cache(ctx, op, cache)) || (rc = check_batch(ctx, op, batch, dtype)) ||
-      (rc = check_strides(ctx, op, k_st, k_sh)) || (rc = check_strides(ctx, op, v_st, v_sh)) ||
-      (rc = check_sizes(ctx, op, batch, cache->kv_heads)))
+      (rc = check_strides(ctx, op, batch->rows, cache->kv_heads, k_st, k_sh)) ||
+      (rc = check_strides(ctx, op, batch->rows, cache->kv_heads, v_st, v_sh)) ||
+      (rc = check_sizes(ctx, op, batch, cache->kv_heads)) || (rc = check_grid(ctx, op, fa::kv_grid(args_of(cache, batch)))))
     return rc;
   if (batch->rows > 0 && batch->nseq > 0 && (!k || !v)) return set_error(ctx, FA_ERR_ARG, "%s: NULL buffer", op);
   return FA_OK;
@@ -176,7 +192,7 @@ int read_check(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, 
   const char* op = "KVRead";
   int rc;
   if ((rc = check_cache(ctx, op, cache)) || (rc = check_batch(ctx, op, batch, dtype)) ||
-      (rc = check_sizes(ctx, op, batch, cache->kv_heads)))
+      (rc = check_sizes(ctx, op, batch, cache->kv_heads)) || (rc = check_grid(ctx, op, fa::kv_grid(args_of(cache, batch)))))
     return rc;
   if (batch->rows > 0 && batch->nseq > 0 && (!k || !v)) return set_error(ctx, FA_ERR_ARG, "%s: NULL buffer", op);
   return FA_OK;
@@ -269,8 +285,8 @@ int fa_kv_attention_work(const fa_kv_cache* cache, const fa_kv_batch* batch, int
   *bytes = 0;
   int rc;
   if ((rc = check_cache(nullptr, "KVAttention", cache))) return rc;
-  if (!batch || batch->nseq < 0 || batch->rows < 0 || batch->table_stride < 0)
-    return set_error(nullptr, FA_ERR_ARG, "KVAttention: batch is NULL or has a negative size");
+  if (!batch || batch->nseq < 0 || batch->rows < 0 || batch->table_stride < 0 || batch->table_stride > kMaxTable)
+    return set_error(nullptr, FA_ERR_ARG, "KVAttention: batch is NULL or has a negative size or too long table rows");
   if (heads < 1 || heads % cache->kv_heads != 0 || heads > 65535)
     return set_error(nullptr, FA_ERR_ARG, "KVAttention: %d query heads on %d key/value heads", heads, cache->kv_heads);
   if ((rc = check_sizes(nullptr, "KVAttention", batch, heads))) return rc;
@@ -308,7 +324,7 @@ int fa_kv_attention(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* ba
                     int64_t q_st, int64_t q_sh, int32_t heads, int causal, int32_t window, float scale, void* out) {
   fa::KvAttnArgs a;
   int rc = attn_args(ctx, cache, batch, dtype, q, q_st, q_sh, heads, causal, window, scale, out, &a);
-  if (rc || (rc = check_host_batch(ctx, "KVAttention", cache, batch, Use::Attend)) ||
+  if (rc || (rc = check_host_batch(ctx, "KVAttention", cache, batch, Use::Attend, window)) ||
       (rc = need_ctx(ctx, "KVAttention")) || nothing(batch))
     return rc;
   const int64_t rows = batch->cu_rows[batch->nseq];

@@ -31,6 +31,7 @@ struct KvArgs {
 
 int launch_kv_write(fa_ctx* ctx, const KvArgs& a, int dtype, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                     int64_t v_st, int64_t v_sh, hipStream_t s);
+int64_t kv_grid(const KvArgs& a);  // workgroups of both along a grid's x
 int launch_kv_read(fa_ctx* ctx, const KvArgs& a, int dtype, void* k, void* v, hipStream_t s);
 
 struct KvAttnArgs {
@@ -47,6 +48,7 @@ struct KvAttnArgs {
 // It begins with kKvCountBytes of counters that are zero between calls.
 constexpr size_t kKvCountBytes = 16384;
 size_t kv_attention_scratch(const KvAttnArgs& a);
+int64_t kv_attention_grid(const KvAttnArgs& a);  // workgroups along a grid's x
 int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& a, void* scratch, hipStream_t s);
 
 #ifdef __HIPCC__

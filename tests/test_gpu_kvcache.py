@@ -745,6 +745,58 @@ def test_captured_step_replays_with_new_contents(ctx):
         x.free()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_weights_on_zero_values_count(ctx, dtype):
+    """131071 tokens whose values are zero (their scale is the smallest), each with a weight of 2^-22.5: together they
+    take 2 % of a row's sum, in the kernels for many rows and for few. The tokens after the first 64 share one block."""
+    r = rng(52)
+    Hkv, G, D, tokens = 64, 32, 64, 131072
+    k, v = np.zeros((128, Hkv, D), np.float32), np.zeros((128, Hkv, D), np.float32)
+    k[0, :, 0] = 1.0
+    v[:64] = r.standard_normal((64, 1, D)).astype(np.float32)
+    k, v = (S.f32_to_bf16(x) if dtype == "bf16" else x for x in (k, v))
+    cache, ref = K.Cache(ctx, 2, Hkv, D), O.RefCache(2, Hkv, D)
+    first = K.Batch(ctx, [[0, 1]], [128], [0, 128])
+    K.write(cache, first, k, v)
+    ref.write([[0, 1]], [128], [0, 128], K.wide(k), K.wide(v))
+    assert (ref.exp[1, :, 1] == -80).all()
+    table = np.ones((1, tokens // 64), np.int32)
+    table[0, 0] = 0
+    scale = float(np.float32(22.5 * np.log(2.0)))
+    kk, vv = (x[:, :1] for x in ref.tokens(table[0], tokens))
+    for n in (4, 1):
+        q = np.repeat(make(r, (n, G, D), dtype)[:, None], Hkv, 1).reshape(n, Hkv * G, D)
+        q[..., 0] = S.f32_to_bf16(np.ones(1, np.float32)) if dtype == "bf16" else 1.0
+        b = K.Batch(ctx, table, [tokens], [0, n])
+        got = K.attend(cache, b, q, scale=scale)
+        q1, mask = K.wide(q[:, :G]), O.sees(tokens, n, True, 0)
+        want, tol = O.attention(q1, kk, vv, mask, scale)
+        if dtype == "bf16":
+            tol = tol + BF * O.attention(q1, kk, np.abs(vv), mask, scale)[0]
+        close(got[:, :G], want, tol, f"{dtype} n={n}")
+        for h in range(1, Hkv):
+            np.testing.assert_array_equal(got[:, h * G:(h + 1) * G], got[:, :G])
+        b.free()
+    first.free()
+    cache.free()
+
+
+def test_blocks_behind_the_window_are_not_needed(ctx):
+    """The host form with a window: table entries of blocks that no row sees may be outside the pool."""
+    r = rng(53)
+    cache, ref, tables = fill(ctx, r, [500], 2, 64)
+    b = K.Batch(ctx, tables, [500], [0, 3])
+    q = make(r, (3, 4, 64), "f32")
+    want, tol = O.attention(q, *ref.tokens(tables[0], 500), O.sees(500, 3, True, 100), 0.125)
+    b.tables[0, :6] = -1  # the first row, 497, sees 398 .. 497
+    hb, out = b.host(), np.empty_like(q)
+    N.check(ctx.h, N.lib().fa_kv_attention(ctx.h, C.byref(cache.c), C.byref(hb), 0, q.ctypes.data, *K.st(q), 4, 1, 100,
+                                           0.125, out.ctypes.data))
+    close(out, want, tol, "behind the window")
+    b.free()
+    cache.free()
+
+
 def test_two_contexts_at_once():
     """Calls of two contexts on one pool, enqueued side by side, each with scratch of its own."""
     a, c = N.Context(0), N.Context(0)

@@ -152,6 +152,40 @@ def test_refusals_of_host_batches():
     c.refused("tokens but", host=host)
 
 
+def test_refusals_of_sizes_past_a_launch():
+    """More workgroups than a launch counts, positions and offsets past their integers."""
+    c = Call()
+    c.batch.table_stride = 1 << 25
+    c.refused("table rows")
+    n = C.c_size_t(7)
+    assert L.fa_kv_attention_work(C.byref(c.cache), C.byref(c.batch), 4, C.byref(n)) == N.FA_ERR_ARG and n.value == 0
+    c = Call()
+    c.batch.nseq, c.batch.rows, c.H = 1 << 24, 1 << 24, 2
+    c.refused("workgroups", host=(False,))
+    c.batch.nseq = c.batch.rows = (1 << 24) - 1
+    c.refused("ctx is NULL", ("write", "read"), host=(False,))
+    c = Call()
+    c.cache.head_dim, c.batch.rows = 512, (1 << 28) - 64  # 16 rows a workgroup
+    c.refused("workgroups", ("attend",), host=(False,))
+    for st in ((1 << 58, 64), (64, 1 << 58), ((1 << 63) - 1, 0)):
+        c = Call()
+        c.st = st
+        c.refused("too large", ("write", "attend"))
+    for s in (3e38, -3e38):
+        c = Call()
+        c.scale = s
+        c.refused("scale", ("attend",))
+
+
+def test_blocks_behind_the_window_need_no_table_entry():
+    c = Call(lengths=(130, 5), ns=(2, 5), table=((-1, 2, 0), (1, -1, -1)))
+    c.refused("outside", ("attend",), (True,))
+    c.window = 65  # the first row, 128, sees 64 .. 129
+    c.refused("ctx is NULL", ("attend",), (True,))
+    c.window = 66
+    c.refused("outside", ("attend",), (True,))
+
+
 def test_work_size():
     n = C.c_size_t(7)
     c = Call()
