@@ -13,6 +13,7 @@ constexpr int kWideRows = 128;  // and of the one for many
 constexpr int kMinChunk = 4;    // blocks of a split part, at least (one per wave)
 constexpr int kRound = 64;      // blocks of a part up to which one part for each CU is aimed at
 constexpr int kTarget = 1024;   // else parts aimed at: two rounds of two workgroups on each of 256 CUs
+constexpr float kWideGain = 20.f;  // blocks (plan_item)
 // Weights are multiplied by the value scale 2^e and this, so that sums of 2^20
 // times float32's largest values stay finite; the result is multiplied back.
 constexpr float kWeightScale = 0x1p-24f;
@@ -37,6 +38,8 @@ struct AttnArgs {
   int64_t parts;  // parts that the scratch holds
   int32_t tile;   // query rows of a work item
   int32_t target, least, cap;  // planned: parts aimed at, blocks of a part at least
+  int32_t span;   // blocks that a tile sees at most, by its window
+  float places, uneven;  // planned: workgroups on the card at once, where a rule decides whether to split (see there)
   int32_t vec, out_vec;  // rows of q / out aligned for one load / store
 };
 
@@ -54,13 +57,13 @@ __device__ __forceinline__ void seen_range(const AttnArgs& a, const KvSeq& s, in
   *hi = (int)max(h, l);
 }
 
-// The number of blocks that sequence b's rows see.
+// The most blocks that a tile of sequence s sees.
 __device__ __forceinline__ int seen_blocks(const AttnArgs& a, const KvSeq& s) {
   if (s.n == 0) return 0;
   int lo, hi;
   seen_range(a, s, 0, s.n - 1, &lo, &hi);
   hi = (int)min((int64_t)hi, (int64_t)a.c.tstride * 64);
-  return hi <= lo ? 0 : ((hi + 63) >> 6) - (lo >> 6);
+  return hi <= lo ? 0 : min(((hi + 63) >> 6) - (lo >> 6), a.span);
 }
 
 template <int CTRL, int ROWS>
@@ -78,7 +81,7 @@ __device__ __forceinline__ int wave_scan(int v) {
   return dpp_add<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
 }
 
-// What lane % 64 = b - b0 knows of sequence b: its tiles and the blocks they see.
+// What lane % 64 = b - b0 knows of sequence b: its tiles and the blocks that one of them sees at most.
 struct Seen {
   int tiles, blocks;
   KvSeq s;
@@ -107,21 +110,32 @@ struct Item {
 // takes as long as some ten blocks, and every part is written and read once
 // more. One sequence of 131072 tokens, 32 heads on 8 of 128 dims: 57 us in 256
 // parts, 63 in 512, 80 in 1024. Longer parts leave less to balance uneven
-// sequences with: those are cut by the target.
+// sequences with: those are cut by the target. With a.places (many rows, a card
+// not far from full) parts are made only where the longest tile's blocks times
+// the free share of the card are kWideGain or more: a tile counts whole, or less
+// by a.uneven of the part of its sequence that is new, whose tiles see less.
 __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want_b, int want_tile, int want_h) {
   const int lane = threadIdx.x & 63;
   const Seen first = seen_by(a, lane);
-  float total = (float)first.tiles * (float)first.blocks, tiles = (float)first.tiles;
-  for (int b0 = 64; b0 < a.c.nseq; b0 += 64) {
-    const Seen x = seen_by(a, b0 + lane);
-    total += (float)x.tiles * (float)x.blocks;
-    tiles += (float)x.tiles;
-  }
+  float total = 0.f, tiles = 0.f, longest = 0.f, busy = 0.f;
+  auto count = [&](const Seen& x) {
+    const float t = (float)x.tiles, b = (float)x.blocks;
+    total += t * b;
+    tiles += t;
+    longest = fmaxf(longest, b);
+    busy += t * (1.f - a.uneven * (float)x.s.n / (float)max(x.s.len, 1));
+  };
+  count(first);
+  for (int b0 = 64; b0 < a.c.nseq; b0 += 64) count(seen_by(a, b0 + lane));
   total = wave_sum(total) * (float)a.c.hkv;
   tiles = wave_sum(tiles) * (float)a.c.hkv;
   const float round = total / fmaxf(256.f - tiles, 128.f);
-  const int chunk = max(max((int)ceilf(fminf(total / (float)a.target, 1e9f)), a.least),
-                        (int)ceilf(fminf(round, (float)a.cap)));
+  int chunk = max(max((int)ceilf(fminf(total / (float)a.target, 1e9f)), a.least),
+                  (int)ceilf(fminf(round, (float)a.cap)));
+  if (a.places > 0.f) {
+    busy = wave_sum(busy) * (float)a.c.hkv;
+    if (!(wave_max(longest) * (a.places - busy) >= kWideGain * a.places)) chunk = 1 << 30;
+  }
   Item r = {0, 0, 0, 0, 1, 0, false, {0, 0, 0}};
   int64_t before = 0;
   for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
@@ -275,6 +289,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7
 
 // Many rows (kv_attention_tile.hip): a.tile rows a work item.
 int kv_tile_rows(int nc, int64_t rows, int nseq);
+int kv_tiles_per_cu(int nc, int dtype);
 int launch_kv_tiles_attn(fa_ctx* ctx, const AttnArgs& a, int dtype, int64_t slots, hipStream_t s);
 
 }  // namespace fa

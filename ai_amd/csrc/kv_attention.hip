@@ -461,16 +461,27 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
   if (it.ok && it.chunks > 1 && r < s.n * a.G) join_row<T, 4>(a, s, it, r, r - tile * a.tile, threadIdx.x & 15);
 }
 
-// Tiles of many rows are split only where they are fewer than kWideItems, in
-// about kWideTarget parts: writing and joining a part of every row costs more
-// than a partly filled card (139 tiles of float32 rows on up to 18 blocks:
-// 80 + 20 us in 332 parts, 100 us whole).
-constexpr int kWideItems = 128, kWideTarget = 512;
+// Tiles of many rows are split, in about kWideTarget parts, where they are fewer
+// than kWideItems, and beyond that where plan_item's rule finds that a longest
+// tile is long and the card far from full: every row of a part is written, read
+// and joined. Prompts of 8 x 1100 tokens, 139 tiles of float32 rows of 256 dims on
+// up to 18 blocks: 96 us whole, 114 in parts; 2 x 3000, 142 tiles on 47 blocks: 209
+// and 124. In bf16, 512 tokens on 8000, 32 heads on 8 of 128 dims, 136 tiles on 125
+// blocks: 173 and 96; 1536 on 3000, 392 tiles on 47: 86 and 101. Where workgroups
+// have a CU each, a prompt's later tiles leave the earlier ones' CUs idle
+// (kUneven: 8 heads on 2 of 256 dims, 4000 tokens, 252 tiles: 171 and 152 us); where
+// two share one, the longer has it to itself then (16 on 4 of 128, 4000 tokens,
+// 502 tiles: 104 and 120). Parts of fewer than kWideMin blocks cost more (2 x 3000
+// in float32: 139 us with 8, 124 with 16).
+constexpr int kWideItems = 128, kWideTarget = 512, kWideMin = 16;
+constexpr float kUneven = 0.4f;
 
 // How a call runs, from its sizes alone.
 struct Shape {
   int tile;           // rows of a work item
   int target, least, cap;  // of a split: parts aimed at, blocks of a part at least
+  int span;                // blocks that a tile sees at most, by its window
+  float places, uneven;    // of a split that plan_item decides on
   int64_t slots;      // tiles, at most
   int64_t parts;      // parts, at most; 0: not split
 };
@@ -483,13 +494,23 @@ Shape shape_of(const KvAttnArgs& a) {
   const int64_t items = r.slots * a.c.hkv;
   const bool wide = r.tile != kTileRows;
   // blocks that a sequence's rows can see
-  int64_t blocks = a.c.tstride;
-  if (a.window) blocks = std::min(blocks, ((int64_t)a.window * (a.causal ? 1 : 2) + a.c.rows) / 64 + 2);
+  const int64_t seen = a.window ? (int64_t)a.window * (a.causal ? 1 : 2) + r.tile / (a.H / a.c.hkv) + 1 : 0;
+  r.span = a.window ? (int)((seen + 62) / 64 + 1) : 0x7FFFFFFF;
+  const int64_t blocks = std::min(a.c.tstride, r.span);
   r.target = wide ? kWideTarget : kTarget;
   r.least = kMinChunk;
   r.cap = wide ? 0 : kRound;
+  r.places = r.uneven = 0.f;
+  bool split = items < (wide ? kWideItems : kTarget);
+  if (wide && !split) {
+    const int per_cu = kv_tiles_per_cu(a.c.nc, a.dtype);
+    r.least = kWideMin;
+    r.places = 256.f * (float)per_cu;
+    r.uneven = per_cu == 1 && a.causal ? kUneven : 0.f;
+    split = (float)blocks * (r.places - (1.f - r.uneven) * (float)items) >= kWideGain * r.places;
+  }
   // enough tiles without, or no sequence that could be cut
-  if (items >= (wide ? kWideItems : kTarget) || blocks <= r.least) {
+  if (!split || blocks <= r.least) {
     r.parts = 0;
   } else {
     // as plan_item: a part has at least `least` blocks, total / target of them, and
@@ -557,6 +578,9 @@ int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStre
   a.target = h.target;
   a.least = h.least;
   a.cap = h.cap;
+  a.span = h.span;
+  a.places = h.places;
+  a.uneven = h.uneven;
   a.parts = h.parts;
   a.count = static_cast<uint32_t*>(scratch);
   a.part = a.parts ? reinterpret_cast<float*>(static_cast<char*>(scratch) + kKvCountBytes) : nullptr;

@@ -32,6 +32,9 @@ __device__ __forceinline__ void reads_ahead() {
   __builtin_amdgcn_sched_group_barrier(0x8, M * kAhead, 0);
 }
 
+// Workgroups that a CU holds, by their registers.
+constexpr int per_cu(int nc, int terms) { return terms == 1 && nc <= 2 ? 2 : 1; }
+
 typedef float kvf16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -75,7 +78,7 @@ __device__ __forceinline__ f16x8 widen_f16(uint32_t a, uint32_t b) {
 // largest, whichever is coarser (codes are exact in fp16, too). Its weights
 // keep three bf16 terms: with the value scales in them they need float32's range.
 template <typename T, int TERMS, int NC>
-__global__ __launch_bounds__(256, TERMS == 1 && NC <= 2 ? 2 : 1) void kv_attn_tile_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(AttnArgs a) {
   constexpr int W = 4, kThreads = W * 64, kRows = W * 32;
   constexpr int KS = NC * 4;            // steps of 16 dims
   constexpr int QT = TERMS == 3 ? 2 : 1;  // terms of a query
@@ -529,6 +532,8 @@ int tiles_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
 int kv_tile_rows(int nc, int64_t rows, int nseq) {
   return nc > 4 || rows < (int64_t)96 * nseq ? kTileRows : kWideRows;
 }
+
+int kv_tiles_per_cu(int nc, int dtype) { return per_cu(nc, dtype == FA_DT_F32 ? 3 : 1); }
 
 int launch_kv_tiles_attn(fa_ctx* ctx, const AttnArgs& a, int dtype, int64_t slots, hipStream_t s) {
   return dtype == FA_DT_F32 ? tiles_t<float, 3>(ctx, a, slots, s) : tiles_t<uint16_t, 1>(ctx, a, slots, s);

@@ -94,7 +94,7 @@ def sees(length, n, causal, window):
     return m
 
 
-def attention(q, k, v, mask, scale):
+def attention(q, k, v, mask, scale, chain=None):
     """q [n, H, D] on k, v [S, Hkv, D] -> out [n, H, D] and, elementwise, how far the kernel may be from it before its
     output is rounded (float32 queries); the second bound is for bf16 tensors, whose weights are rounded to bf16.
 
@@ -103,7 +103,8 @@ def attention(q, k, v, mask, scale):
     no more from D = 4 on, and below that the bound of D = 4 is taken; or 2^-39 of the row's largest); the largest such error among a row's tokens, dS, moves every weight by a
     factor within e^(+-2 dS) (weight and sum), the hardware's exp2 by 2^-22 at most (its argument is rounded, too: U
     times its size, at most 150 where a weight counts). The sums over S tokens, of three terms each, and the joining of
-    waves and parts add at most (3 S + 64) U. All relative to sum p |v|."""
+    waves and parts add at most (3 S + 64) U (chain: terms that are added one after another, if not S). All relative to
+    sum p |v|."""
     n, H, D = q.shape
     S, Hkv, _ = k.shape
     out = np.zeros((n, H, D))
@@ -123,6 +124,6 @@ def attention(q, k, v, mask, scale):
             out[i, h] = p @ vh[on]
             ds = (3 * max(D, 4) + 4) * U * mag[i, on].max()
             ds += 2.0 ** -39 * np.abs(q[i, h]).max() * np.abs(kh[on]).sum(1).max() * abs(scale)
-            rel = np.expm1(2 * ds) + 2.0 ** -22 + 2 * 150 * U + (3 * on.sum() + 64) * U
+            rel = np.expm1(2 * ds) + 2.0 ** -22 + 2 * 150 * U + (3 * (chain or on.sum()) + 64) * U
             tol[i, h] = rel * (p @ np.abs(vh[on]))
     return out, tol

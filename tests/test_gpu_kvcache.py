@@ -745,10 +745,24 @@ def test_captured_step_replays_with_new_contents(ctx):
         x.free()
 
 
+@pytest.mark.parametrize("dtype,D,H,lengths,ns,window,width", [
+    ("bf16", 64, 16, [2000, 1900, 2048, 70], [128, 100, 128, 70], 0, None),  # long enough to be split
+    ("bf16", 64, 16, [1000, 900, 64, 200], [128, 100, 64, 128], 0, 40),      # only the tables are
+    ("bf16", 64, 16, [2500, 2400, 2048, 2000], [100] * 4, 1700, None),
+    ("f32", 80, 16, [2000, 1900, 2048, 1990], [100] * 4, 0, None),
+    ("f32", 80, 8, [1900], [1900], 0, None),                                  # a prompt: later tiles see more
+    ("f32", 80, 8, [1900], [1900], 500, None)])
+def test_tiles_of_many_rows_cut_in_parts(ctx, dtype, D, H, lengths, ns, window, width):
+    """128 work items and more of 128 rows, which are cut where the longest sequence is long."""
+    attention_case(ctx, 54, dtype, D, H, H, lengths, ns, window=window, width=width, work=True)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_weights_on_zero_values_count(ctx, dtype):
     """131071 tokens whose values are zero (their scale is the smallest), each with a weight of 2^-22.5: together they
-    take 2 % of a row's sum, in the kernels for many rows and for few. The tokens after the first 64 share one block."""
+    take 2 % of a row's sum, in the kernels for many rows and for few. The tokens after the first 64 share one block. A
+    lane adds 32 weights of a block to a sum over the blocks, or 16 of every fourth block to one sum: at most tokens / 16
+    terms one after another, and of the values those of one block."""
     r = rng(52)
     Hkv, G, D, tokens = 64, 32, 64, 131072
     k, v = np.zeros((128, Hkv, D), np.float32), np.zeros((128, Hkv, D), np.float32)
@@ -769,13 +783,12 @@ def test_weights_on_zero_values_count(ctx, dtype):
         q[..., 0] = S.f32_to_bf16(np.ones(1, np.float32)) if dtype == "bf16" else 1.0
         b = K.Batch(ctx, table, [tokens], [0, n])
         got = K.attend(cache, b, q, scale=scale)
-        q1, mask = K.wide(q[:, :G]), O.sees(tokens, n, True, 0)
-        want, tol = O.attention(q1, kk, vv, mask, scale)
+        q1, mask = K.wide(q[:, :1]), O.sees(tokens, n, True, 0)
+        want, tol = O.attention(q1, kk, vv, mask, scale, chain=tokens // 16)
         if dtype == "bf16":
             tol = tol + BF * O.attention(q1, kk, np.abs(vv), mask, scale)[0]
-        close(got[:, :G], want, tol, f"{dtype} n={n}")
-        for h in range(1, Hkv):
-            np.testing.assert_array_equal(got[:, h * G:(h + 1) * G], got[:, :G])
+        close(got[:, :1], want, tol, f"{dtype} n={n}")
+        assert (got == got[:, :1]).all()  # (keys are zero where queries differ)
         b.free()
     first.free()
     cache.free()
