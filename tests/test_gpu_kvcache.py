@@ -757,6 +757,17 @@ def test_tiles_of_many_rows_cut_in_parts(ctx, dtype, D, H, lengths, ns, window, 
     attention_case(ctx, 54, dtype, D, H, H, lengths, ns, window=window, width=width, work=True)
 
 
+def test_tiles_of_many_rows_go_by_length(ctx):
+    """Whole tiles of sequences of many lengths, some without rows or tokens: every tile is some workgroup's."""
+    lengths = [1300, 0, 100, 700, 1299, 400, 90, 1000, 640, 130, 1300, 257]
+    ns = [130, 0, 100, 129, 200, 0, 90, 128, 96, 130, 257, 120]
+    attention_case(ctx, 55, "bf16", 64, 16, 16, lengths, ns, work=True)
+    r = rng(56)
+    lengths = [int(x) for x in r.integers(96, 260, 70)]
+    ns = [int(r.integers(96, x + 1)) for x in lengths]
+    attention_case(ctx, 57, "f32", 64, 2, 2, lengths, ns, causal=False)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_weights_on_zero_values_count(ctx, dtype):
     """131071 tokens whose values are zero (their scale is the smallest), each with a weight of 2^-22.5: together they
