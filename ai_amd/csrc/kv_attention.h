@@ -7,8 +7,9 @@
 
 namespace fa {
 
-constexpr int kTileRows = 16;   // query rows of a work item of the kernel for few rows
-constexpr int kWideRows = 128;  // and of the one for many
+constexpr int kTileRows = 16;   // query rows of a work item of the kernel for few rows,
+constexpr int kPairRows = 32;   // of its form for some more,
+constexpr int kWideRows = 128;  // and of the kernel for many
 
 constexpr int kMinChunk = 4;    // blocks of a split part, at least (one per wave)
 constexpr int kRound = 64;      // blocks of a part up to which one part for each CU is aimed at
@@ -22,7 +23,7 @@ constexpr float kLeastFactor = 0x1p-64f;
 // The largest sum of a lane's weights in a block, relative to its row's reference.
 constexpr float kMostWeight = 0x1p8f;
 
-// The work of one call: tiles of kTileRows rows of a sequence's n * G, for
+// The work of one call: tiles of `tile` rows of a sequence's n * G, for
 // each key/value head, over the blocks they see; in a planned call the blocks
 // are cut into parts of about equal size over the whole batch.
 struct AttnArgs {
@@ -39,6 +40,7 @@ struct AttnArgs {
   int32_t tile;   // query rows of a work item
   int32_t target, least, cap;  // planned: parts aimed at, blocks of a part at least
   int32_t span;   // blocks that a tile sees at most, by its window
+  float once;     // planned, with cap: workgroups aimed at in one round of short parts
   float places, uneven;  // planned: workgroups on the card at once, where a rule decides whether to split (see there)
   int32_t vec, out_vec;  // rows of q / out aligned for one load / store
 };
@@ -129,7 +131,7 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want
   for (int b0 = 64; b0 < a.c.nseq; b0 += 64) count(seen_by(a, b0 + lane));
   total = wave_sum(total) * (float)a.c.hkv;
   tiles = wave_sum(tiles) * (float)a.c.hkv;
-  const float round = total / fmaxf(256.f - tiles, 128.f);
+  const float round = total / fmaxf(a.once - tiles, a.once * 0.5f);
   int chunk = max(max((int)ceilf(fminf(total / (float)a.target, 1e9f)), a.least),
                   (int)ceilf(fminf(round, (float)a.cap)));
   if (a.places > 0.f) {

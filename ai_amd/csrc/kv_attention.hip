@@ -97,44 +97,51 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const KvSeq& s, cons
     }
 }
 
-// One work item: 16 query rows of one key/value head over a run of blocks.
-// Lane l: row l % 16, group l / 16. NC: slices of 64 dims (at most; nc in use).
+// Workgroups that a CU holds, by their registers.
+constexpr int few_per_cu(int nc) { return nc <= 2 ? 2 : 1; }
+
+// One work item: 16 RT query rows of one key/value head over a run of blocks.
+// Lane l: rows l % 16 of each 16, group l / 16. NC: slices of 64 dims (at most; nc in use).
 // Its blocks go to the four waves in turn, their results are merged at the
 // end. A wave loads a block's keys while it works on the scores of the block
 // before, and its values while it works on the next scores, so that about a
 // block (D = 128: 16 KB) is always under way: 64 sequences of up to 8192
 // tokens (606 MB) take 126 us, 4.8 TB/s, against 219 without, and a large copy
 // moves 5.1 TB/s. Above 256 dims the registers do not hold it.
-template <typename T, int TERMS, int NC>
-__global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs a) {
+template <typename T, int TERMS, int NC, int RT>
+__global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a) {
+  constexpr int kRows = 16 * RT;
   constexpr bool AHEAD = NC <= 4;  // loads a block ahead
   constexpr int kWaves = 4, kThreads = kWaves * 64;
   constexpr int kMergeDims = 128;         // dims that the waves' results are merged at a time
   constexpr int kLane = kMergeDims / 16;  // and a thread's of them, 16 threads a row
   const int nc = NC <= 4 ? NC : a.c.nc;
-  constexpr int kQ = TERMS * NC * 2 * 64;           // operands of 16 bytes
-  constexpr int kM = kWaves * kTileRows * (kMergeDims + 4);  // floats
+  constexpr int kQ = RT * TERMS * NC * 2 * 64;        // operands of 16 bytes
+  constexpr int kM = kWaves * 16 * (kMergeDims + 4);  // floats
   __shared__ __align__(16) char lds[kQ * 16 > kM * 4 ? kQ * 16 : kM * 4];
-  __shared__ float stat[kWaves][kTileRows][2];
+  __shared__ float stat[kWaves][kRows][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = lane & 15, grp = lane >> 4;
   const bool planned = a.part != nullptr;
-  const Item it = planned ? plan_item(a, blockIdx.x, 0, 0, 0) : direct_item(a, blockIdx.x, blockIdx.y, kTileRows);
+  const Item it = planned ? plan_item(a, blockIdx.x, 0, 0, 0) : direct_item(a, blockIdx.x, blockIdx.y, kRows);
   if (!it.ok) return;
   const KvSeq s = it.s;
-  const int rows = s.n * a.G, r0 = it.tile * kTileRows;
-  const int valid = min(kTileRows, rows - r0);
+  const int rows = s.n * a.G, r0 = it.tile * kRows;
+  const int valid = min(kRows, rows - r0);
   T* out = (T*)a.out;
   const bool too_long = (int64_t)s.len > (int64_t)a.c.tstride * 64;  // tokens without a table entry: NaN, not a guess
 
-  // what the tile sees, and this lane's row of it
+  // what the tile sees, and this lane's rows of it
   int lo, hi;
   const int ta = r0 / a.G, tb = (r0 + valid - 1) / a.G;
   seen_range(a, s, ta, tb, &lo, &hi);
   if (too_long) hi = lo;
-  const int t = min(r0 + row, rows - 1) / a.G;
-  int rlo, rhi, alo, ahi;  // the row's range, and what every row of the tile sees
-  seen_range(a, s, t, t, &rlo, &rhi);
+  int rlo[RT], rhi[RT], alo, ahi;  // its rows' ranges, and what every row of the tile sees
+#pragma unroll
+  for (int rt = 0; rt < RT; rt++) {
+    const int t = min(r0 + rt * 16 + row, rows - 1) / a.G;
+    seen_range(a, s, t, t, &rlo[rt], &rhi[rt]);
+  }
   {
     int l0, h0, l1, h1;
     seen_range(a, s, ta, ta, &l0, &h0);
@@ -189,10 +196,10 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
     load_v(id);
   }
 
-  // the tile's queries as operands in LDS: [term][slice of 32 dims][lane]
+  // the tile's queries as operands in LDS: [16 rows][term][slice of 32 dims][lane]
   uint4* qf = reinterpret_cast<uint4*>(lds);
-  for (int i = tid; i < nc * 2 * 64; i += kThreads) {
-    const int ks = i >> 6, l = i & 63, r = r0 + (l & 15);
+  for (int i = tid; i < RT * nc * 2 * 64; i += kThreads) {
+    const int rt = RT == 1 ? 0 : i / (nc * 2 * 64), ks = (i >> 6) - rt * nc * 2, l = i & 63, r = r0 + rt * 16 + (l & 15);
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (r < rows) {
       const int tok = r / a.G, head = it.h * a.G + (r - tok * a.G);
@@ -202,15 +209,21 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
     bf16x8 tm[TERMS];
     terms_of<TERMS>(v, tm);
 #pragma unroll
-    for (int k = 0; k < TERMS; k++) qf[(k * NC * 2 + ks) * 64 + l] = __builtin_bit_cast(uint4, tm[k]);
+    for (int k = 0; k < TERMS; k++) qf[((rt * TERMS + k) * NC * 2 + ks) * 64 + l] = __builtin_bit_cast(uint4, tm[k]);
   }
   __syncthreads();
 
-  kvf4 acc[NC * 4];
+  kvf4 acc[RT][NC * 4];
+  float m[RT], l[RT];
+  uint64_t nan_sum[RT][2];  // sums that are NaN: bit 4 (tile % 16) + i of word tile / 16
 #pragma unroll
-  for (int i = 0; i < NC * 4; i++) acc[i] = kvf4{0.f, 0.f, 0.f, 0.f};
-  float m = -__builtin_inff(), l = 0.f;
-  uint64_t nan_sum[2] = {0, 0};  // sums that are NaN: bit 4 (tile % 16) + i of word tile / 16
+  for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+    for (int i = 0; i < NC * 4; i++) acc[rt][i] = kvf4{0.f, 0.f, 0.f, 0.f};
+    m[rt] = -__builtin_inff();
+    l[rt] = 0.f;
+    nan_sum[rt][0] = nan_sum[rt][1] = 0;
+  }
 
   for (int p = pg0 + wave; p < pg1; p += kWaves) {
     const int id1 = blocks.at(a, it.b, ++turn);
@@ -220,9 +233,11 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
     const uint4* vp = id >= 0 ? part(id, 1) : nullptr;
 
     // S^T: four tiles of 16 tokens
-    kvf4 sc4[4];
+    kvf4 sc4[RT][4];
 #pragma unroll
-    for (int tt = 0; tt < 4; tt++) sc4[tt] = kvf4{0.f, 0.f, 0.f, 0.f};
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+      for (int tt = 0; tt < 4; tt++) sc4[rt][tt] = kvf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NC; c++) {
       if (NC > 4 && c >= nc) continue;
@@ -232,15 +247,41 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
         if constexpr (AHEAD) kc[tt] = kr[c * 4 + tt];
         else kc[tt] = key(kp, c * 4 + tt);
       }
+      if constexpr (TERMS == 1) {
+        bf16x8 q[RT][2];
 #pragma unroll
-      for (int k = 0; k < TERMS; k++) {
-        const bf16x8 q0 = __builtin_bit_cast(bf16x8, qf[(k * NC * 2 + c * 2) * 64 + lane]);
-        const bf16x8 q1 = __builtin_bit_cast(bf16x8, qf[(k * NC * 2 + c * 2 + 1) * 64 + lane]);
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+            q[rt][u] = __builtin_bit_cast(bf16x8, qf[(rt * NC * 2 + c * 2 + u) * 64 + lane]);
 #pragma unroll
         for (int tt = 0; tt < 4; tt++) {
-          sc4[tt] = mfma(widen(kc[tt].x, kc[tt].y), q0, sc4[tt]);
-          sc4[tt] = mfma(widen(kc[tt].z, kc[tt].w), q1, sc4[tt]);
+          const bf16x8 k0 = widen(kc[tt].x, kc[tt].y), k1 = widen(kc[tt].z, kc[tt].w);
+#pragma unroll
+          for (int rt = 0; rt < RT; rt++) {
+            sc4[rt][tt] = mfma(k0, q[rt][0], sc4[rt][tt]);
+            sc4[rt][tt] = mfma(k1, q[rt][1], sc4[rt][tt]);
+          }
         }
+      } else {
+        bf16x8 kw[4][2];
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++) {
+          kw[tt][0] = widen(kc[tt].x, kc[tt].y);
+          kw[tt][1] = widen(kc[tt].z, kc[tt].w);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+          for (int k = 0; k < TERMS; k++) {
+            const bf16x8 q0 = __builtin_bit_cast(bf16x8, qf[((rt * TERMS + k) * NC * 2 + c * 2) * 64 + lane]);
+            const bf16x8 q1 = __builtin_bit_cast(bf16x8, qf[((rt * TERMS + k) * NC * 2 + c * 2 + 1) * 64 + lane]);
+#pragma unroll
+            for (int tt = 0; tt < 4; tt++) {
+              sc4[rt][tt] = mfma(kw[tt][0], q0, sc4[rt][tt]);
+              sc4[rt][tt] = mfma(kw[tt][1], q1, sc4[rt][tt]);
+            }
+          }
       }
     }
     const bool more = p + kWaves < pg1;
@@ -250,43 +291,45 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
     }
     const float mul = a.scale2 * ks;
     const bool edge = j0 < alo || j0 + 64 > ahi;  // some row does not see some token
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int tt = 0; tt < 4; tt++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float x = sc4[tt][i] * mul;
-        if (edge) {
-          const int j = j0 + tt * 16 + grp * 4 + i;
-          x = j >= rlo && j < rhi ? x : -__builtin_inff();
-        }
-        sc4[tt][i] = x;
-        top = fmaxf(top, x);
-      }
-    const float mn = fmaxf(m, row_max(top));
-    const float mu = mn == -__builtin_inff() ? 0.f : mn;  // a row that has seen nothing yet: weights 0, not NaN
-    const float alpha = __builtin_amdgcn_exp2f(m - mu);
-    if (__ballot(mn != m)) {
-      l *= alpha;
-#pragma unroll
-      for (int i = 0; i < NC * 4; i++) {
-        acc[i] *= alpha;
-      }
-    }
-    m = mn;
-    // weights and their operands: two steps of 32 tokens
     const float f = vs * kWeightScale;
-    bf16x8 pt[2][TERMS];
+    bf16x8 pt[RT][2][TERMS];  // weights as operands: two steps of 32 tokens
 #pragma unroll
-    for (int st2 = 0; st2 < 2; st2++) {
-      float w[8];
+    for (int rt = 0; rt < RT; rt++) {
+      float top = -__builtin_inff();
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float x = __builtin_amdgcn_exp2f(sc4[st2 * 2 + (i >> 2)][i & 3] - mu);
-        l += x;
-        w[i] = x * f;
+      for (int tt = 0; tt < 4; tt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          float x = sc4[rt][tt][i] * mul;
+          if (edge) {
+            const int j = j0 + tt * 16 + grp * 4 + i;
+            x = j >= rlo[rt] && j < rhi[rt] ? x : -__builtin_inff();
+          }
+          sc4[rt][tt][i] = x;
+          top = fmaxf(top, x);
+        }
+      const float mn = fmaxf(m[rt], row_max(top));
+      const float mu = mn == -__builtin_inff() ? 0.f : mn;  // a row that has seen nothing yet: weights 0, not NaN
+      const float alpha = __builtin_amdgcn_exp2f(m[rt] - mu);
+      if (__ballot(mn != m[rt])) {
+        l[rt] *= alpha;
+#pragma unroll
+        for (int i = 0; i < NC * 4; i++) {
+          acc[rt][i] *= alpha;
+        }
       }
-      terms_of<TERMS>(w, pt[st2]);
+      m[rt] = mn;
+#pragma unroll
+      for (int st2 = 0; st2 < 2; st2++) {
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float x = __builtin_amdgcn_exp2f(sc4[rt][st2 * 2 + (i >> 2)][i & 3] - mu);
+          l[rt] += x;
+          w[i] = x * f;
+        }
+        terms_of<TERMS>(w, pt[rt][st2]);
+      }
     }
     // Tokens that no row of the tile sees may hold anything (a length ends
     // inside the block): their value codes become zero. Tokens that some rows
@@ -324,10 +367,12 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
       }
       const bf16x8 v0 = widen(v.x, v.y), v1 = widen(v.z, v.w);
 #pragma unroll
-      for (int k = 0; k < TERMS; k++) {
-        acc[dt] = mfma(v0, pt[0][k], acc[dt]);
-        acc[dt] = mfma(v1, pt[1][k], acc[dt]);
-      }
+      for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int k = 0; k < TERMS; k++) {
+          acc[rt][dt] = mfma(v0, pt[rt][0][k], acc[rt][dt]);
+          acc[rt][dt] = mfma(v1, pt[rt][1][k], acc[rt][dt]);
+        }
     }
     if (mixed && __ballot(nan != 0)) {
 #pragma unroll 1
@@ -336,104 +381,111 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
         const uint32_t n0 = nan_bytes(v.x & keep[0]) >> 7, n1 = nan_bytes(v.y & keep[1]) >> 7;
         const uint32_t n2 = nan_bytes(v.z & keep[2]) >> 7, n3 = nan_bytes(v.w & keep[3]) >> 7;
         if (__ballot((n0 | n1 | n2 | n3) != 0) == 0) continue;
-        kvf4 cnt = {0.f, 0.f, 0.f, 0.f};  // 0x01 of a NaN byte -> 0x38, the code of one
 #pragma unroll
-        for (int st2 = 0; st2 < 2; st2++) {
-          bf16x8 see;
+        for (int rt = 0; rt < RT; rt++) {
+          kvf4 cnt = {0.f, 0.f, 0.f, 0.f};  // 0x01 of a NaN byte -> 0x38, the code of one
 #pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int j = j0 + (st2 * 2 + (i >> 2)) * 16 + grp * 4 + (i & 3);
-            see[i] = (__bf16)(j >= rlo && j < rhi ? 1.f : 0.f);
+          for (int st2 = 0; st2 < 2; st2++) {
+            bf16x8 see;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const int j = j0 + (st2 * 2 + (i >> 2)) * 16 + grp * 4 + (i & 3);
+              see[i] = (__bf16)(j >= rlo[rt] && j < rhi[rt] ? 1.f : 0.f);
+            }
+            cnt = mfma(st2 ? widen(n2 * 0x38u, n3 * 0x38u) : widen(n0 * 0x38u, n1 * 0x38u), see, cnt);
           }
-          cnt = mfma(st2 ? widen(n2 * 0x38u, n3 * 0x38u) : widen(n0 * 0x38u, n1 * 0x38u), see, cnt);
-        }
-        uint64_t bits = 0;
+          uint64_t bits = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) bits |= (uint64_t)(cnt[i] > 0.f) << i;
-        nan_sum[0] |= dt < 16 ? bits << (4 * dt) : 0;
-        if (NC > 4) nan_sum[1] |= dt < 16 ? 0 : bits << (4 * (dt & 15));
+          for (int i = 0; i < 4; i++) bits |= (uint64_t)(cnt[i] > 0.f) << i;
+          nan_sum[rt][0] |= dt < 16 ? bits << (4 * dt) : 0;
+          if (NC > 4) nan_sum[rt][1] |= dt < 16 ? 0 : bits << (4 * (dt & 15));
+        }
       }
     }
     if (more) load_v(id1);
     id = id1;
   }
 
-  if (__ballot((nan_sum[0] | nan_sum[1]) != 0)) {
 #pragma unroll
-    for (int dt = 0; dt < NC * 4; dt++)
+  for (int rt = 0; rt < RT; rt++) {
+    if (__ballot((nan_sum[rt][0] | nan_sum[rt][1]) != 0)) {
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (nan_sum[dt >> 4] >> (4 * (dt & 15) + i) & 1) acc[dt][i] = __builtin_nanf("");
-  }
-  // merge the waves: maxima and sums, then the outputs kMergeDims at a time
-  l = row_sum(l);
-  if (grp == 0) {
-    stat[wave][row][0] = m;
-    stat[wave][row][1] = l;
+      for (int dt = 0; dt < NC * 4; dt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (nan_sum[rt][dt >> 4] >> (4 * (dt & 15) + i) & 1) acc[rt][dt][i] = __builtin_nanf("");
+    }
+    // merge the waves: maxima and sums, then the outputs kMergeDims at a time
+    l[rt] = row_sum(l[rt]);
+    if (grp == 0) {
+      stat[wave][rt * 16 + row][0] = m[rt];
+      stat[wave][rt * 16 + row][1] = l[rt];
+    }
   }
   __syncthreads();
-  float M = -__builtin_inff();
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) M = fmaxf(M, stat[w][row][0]);
-  const float Mu = M == -__builtin_inff() ? 0.f : M;
-  const float mine = __builtin_amdgcn_exp2f(m - Mu);
-  // the output rows: 16 threads a row, each kLane dims of every kMergeDims
-  const int orow = tid >> 4, oat = (tid & 15) * kLane;
-  float oM = -__builtin_inff(), L = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) oM = fmaxf(oM, stat[w][orow][0]);
-  const float oMu = oM == -__builtin_inff() ? 0.f : oM;
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) L += stat[w][orow][1] * __builtin_amdgcn_exp2f(stat[w][orow][0] - oMu);
   const bool split = it.chunks > 1;
   const int Dp = nc * 64;
-  const int otok = (r0 + orow) / a.G, ohead = it.h * a.G + (r0 + orow) - otok * a.G;
-  float fin = 1.f;
-  if (!split) {
-    int l0, h0;
-    seen_range(a, s, min(otok, s.n - 1), min(otok, s.n - 1), &l0, &h0);
-    fin = too_long ? __builtin_nanf("") : h0 <= l0 ? 0.f : (1.f / kWeightScale) / L;
-  }
-  const bool empty = !split && fin == 0.f;
+  float* stats = a.part + a.parts * kRows * Dp;
   float* buf = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int c = 0; c < (NC * 64 + kMergeDims - 1) / kMergeDims; c++) {
-    if (NC > 4 && c * kMergeDims >= nc * 64) continue;
-    __syncthreads();
+  for (int rt = 0; rt < RT; rt++) {
+    if (rt && rt * 16 >= valid) break;
+    float M = -__builtin_inff();
 #pragma unroll
-    for (int dt = 0; dt < kMergeDims / 16; dt++) {
-      if (c * (kMergeDims / 16) + dt < NC * 4)
-        *reinterpret_cast<kvf4*>(buf + (wave * kTileRows + row) * (kMergeDims + 4) + dt * 16 + grp * 4) =
-            acc[c * (kMergeDims / 16) + dt] * mine;
+    for (int w = 0; w < kWaves; w++) M = fmaxf(M, stat[w][rt * 16 + row][0]);
+    const float Mu = M == -__builtin_inff() ? 0.f : M;
+    const float mine = __builtin_amdgcn_exp2f(m[rt] - Mu);
+    // the output rows: 16 threads a row, each kLane dims of every kMergeDims
+    const int orow = rt * 16 + (tid >> 4), oat = (tid & 15) * kLane;
+    float oM = -__builtin_inff(), L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) oM = fmaxf(oM, stat[w][orow][0]);
+    const float oMu = oM == -__builtin_inff() ? 0.f : oM;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) L += stat[w][orow][1] * __builtin_amdgcn_exp2f(stat[w][orow][0] - oMu);
+    const int otok = (r0 + orow) / a.G, ohead = it.h * a.G + (r0 + orow) - otok * a.G;
+    float fin = 1.f;
+    if (!split) {
+      int l0, h0;
+      seen_range(a, s, min(otok, s.n - 1), min(otok, s.n - 1), &l0, &h0);
+      fin = too_long ? __builtin_nanf("") : h0 <= l0 ? 0.f : (1.f / kWeightScale) / L;
     }
-    __syncthreads();
-    const int d = c * kMergeDims + oat;
-    if (orow < valid && d < Dp) {
-      float o[kLane];
+    const bool empty = !split && fin == 0.f;
 #pragma unroll
-      for (int i = 0; i < kLane; i++) o[i] = 0.f;
+    for (int c = 0; c < (NC * 64 + kMergeDims - 1) / kMergeDims; c++) {
+      if (NC > 4 && c * kMergeDims >= nc * 64) continue;
+      __syncthreads();
 #pragma unroll
-      for (int w = 0; w < kWaves; w++)
+      for (int dt = 0; dt < kMergeDims / 16; dt++) {
+        if (c * (kMergeDims / 16) + dt < NC * 4)
+          *reinterpret_cast<kvf4*>(buf + (wave * 16 + row) * (kMergeDims + 4) + dt * 16 + grp * 4) =
+              acc[rt][c * (kMergeDims / 16) + dt] * mine;
+      }
+      __syncthreads();
+      const int d = c * kMergeDims + oat;
+      if (orow < valid && d < Dp) {
+        float o[kLane];
 #pragma unroll
-        for (int i = 0; i < kLane; i++) o[i] += buf[(w * kTileRows + orow) * (kMergeDims + 4) + oat + i];
-      if (split) {
-        float* to = a.part + ((it.first + it.chunk) * kTileRows + orow) * Dp + d;
+        for (int i = 0; i < kLane; i++) o[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < kLane; i += 2) put2(to + i, o[i], o[i + 1]);
-      } else {
-        T* to = out + ((s.row0 + otok) * a.H + ohead) * (int64_t)a.c.D;
+        for (int w = 0; w < kWaves; w++)
 #pragma unroll
-        for (int i = 0; i < kLane; i++)
-          if (d + i < a.c.D) st(to + d + i, empty ? 0.f : o[i] * fin);
+          for (int i = 0; i < kLane; i++) o[i] += buf[(w * 16 + (tid >> 4)) * (kMergeDims + 4) + oat + i];
+        if (split) {
+          float* to = a.part + ((it.first + it.chunk) * kRows + orow) * Dp + d;
+#pragma unroll
+          for (int i = 0; i < kLane; i += 2) put2(to + i, o[i], o[i + 1]);
+        } else {
+          T* to = out + ((s.row0 + otok) * a.H + ohead) * (int64_t)a.c.D;
+#pragma unroll
+          for (int i = 0; i < kLane; i++)
+            if (d + i < a.c.D) st(to + d + i, empty ? 0.f : o[i] * fin);
+        }
       }
     }
+    if (split && oat == 0 && orow < valid) put2(stats + ((it.first + it.chunk) * kRows + orow) * 2, oM, L);
   }
   if (!split) return;
-  const int64_t mine_at = (it.first + it.chunk) * kTileRows;
-  float* stats = a.part + a.parts * kTileRows * Dp;
-  if (oat == 0 && orow < valid) {
-    put2(stats + (mine_at + orow) * 2, oM, L);
-  }
   // The workgroup that ends last of a tile's joins its parts, in their order
   // (the result does not depend on which one that is), and leaves the count
   // at zero for the next call.
@@ -447,7 +499,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void kv_attn_kernel(AttnArgs 
   }
   __syncthreads();
   if (!last) return;
-  if (orow < valid) join_row<T, NC>(a, s, it, r0 + orow, orow, tid & 15);
+  for (int r = tid >> 4; r < valid; r += 16) join_row<T, NC>(a, s, it, r0 + r, r, tid & 15);
 }
 
 // Joins the parts of split tiles of many rows: a workgroup for each 16 rows.
@@ -476,32 +528,54 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
 constexpr int kWideItems = 128, kWideTarget = 512, kWideMin = 16;
 constexpr float kUneven = 0.4f;
 
+// Tiles of kPairRows rows load and widen a block once for twice the rows: with
+// bf16 (float32 has no registers for it: 64 sequences of up to 8192 tokens, 24
+// rows on each of 8 heads of 128 dims, 279 and 295 us; in bf16 260 and 187), where
+// they still fill the card, or are kPairItems and full and see kPairBlocks (64
+// sequences, 64 rows on one head: 73 and 52; on the other side 16 of 2000 tokens,
+// 32 rows on each of 8: 23 and 28, and 32 of 4000, 20 rows: 53 and 60).
+constexpr int kPairItems = 96, kPairBlocks = 64;
+
 // How a call runs, from its sizes alone.
 struct Shape {
   int tile;           // rows of a work item
   int target, least, cap;  // of a split: parts aimed at, blocks of a part at least
   int span;                // blocks that a tile sees at most, by its window
+  int once;                // of a split with cap: workgroups aimed at in one round
   float places, uneven;    // of a split that plan_item decides on
   int64_t slots;      // tiles, at most
   int64_t parts;      // parts, at most; 0: not split
 };
 
-Shape shape_of(const KvAttnArgs& a) {
+Shape shape_of(const KvAttnArgs& a, bool pairs = true) {
   Shape r;
-  const int64_t all = a.c.rows * (a.H / a.c.hkv);
+  const int G = a.H / a.c.hkv;
+  const int64_t all = a.c.rows * G, nseq = a.c.nseq;
+  // tiles, about and at most
+  auto tiles = [&](int rows) { return std::max((all + nseq * rows / 2) / rows, std::min(nseq, all)); };
+  auto most_tiles = [&](int rows) { return all / rows + nseq; };
+  // blocks that a tile of some rows can see
+  auto seen = [&](int rows) {
+    return a.window ? ((int64_t)a.window * (a.causal ? 1 : 2) + rows / G + 63) / 64 + 1 : (int64_t)0x7FFFFFFF;
+  };
   r.tile = kv_tile_rows(a.c.nc, all, a.c.nseq);
-  r.slots = all / r.tile + a.c.nseq;
+  if (r.tile == kTileRows && pairs && a.dtype == FA_DT_BF16 && a.c.nc <= 4 && all > kTileRows * nseq) {
+    const int64_t items = tiles(kPairRows) * a.c.hkv, blocks = std::min<int64_t>(a.c.tstride, seen(kPairRows));
+    if (items >= 256 * few_per_cu(a.c.nc) ||
+        (a.c.nc <= 2 && items >= kPairItems && blocks >= kPairBlocks && all >= kPairRows * nseq))
+      r.tile = kPairRows;
+  }
+  r.slots = most_tiles(r.tile);
   const int64_t items = r.slots * a.c.hkv;
-  const bool wide = r.tile != kTileRows;
-  // blocks that a sequence's rows can see
-  const int64_t seen = a.window ? (int64_t)a.window * (a.causal ? 1 : 2) + r.tile / (a.H / a.c.hkv) + 1 : 0;
-  r.span = a.window ? (int)((seen + 62) / 64 + 1) : 0x7FFFFFFF;
+  const bool wide = r.tile == kWideRows;
+  r.span = (int)seen(r.tile);
   const int64_t blocks = std::min(a.c.tstride, r.span);
   r.target = wide ? kWideTarget : kTarget;
   r.least = kMinChunk;
   r.cap = wide ? 0 : kRound;
+  r.once = r.tile == kPairRows ? 256 * few_per_cu(a.c.nc) : 256;
   r.places = r.uneven = 0.f;
-  bool split = items < (wide ? kWideItems : kTarget);
+  bool split = wide ? items < kWideItems : tiles(r.tile) * a.c.hkv < kTarget && items < 2 * kTarget;
   if (wide && !split) {
     const int per_cu = kv_tiles_per_cu(a.c.nc, a.dtype);
     r.least = kWideMin;
@@ -514,23 +588,27 @@ Shape shape_of(const KvAttnArgs& a) {
     r.parts = 0;
   } else {
     // as plan_item: a part has at least `least` blocks, total / target of them, and
-    // total / 256 up to kRound; the last part of each item may be short
+    // total / once up to kRound; the last part of each item may be short
     const int64_t total = items * blocks, most = (blocks + r.least - 1) / r.least;
-    const int64_t cut = wide ? r.target : std::max((int64_t)256, std::min((int64_t)kTarget, total / kRound));
+    const int64_t cut = wide ? r.target : std::max((int64_t)r.once, std::min((int64_t)kTarget, total / kRound));
     r.parts = std::min(cut + items + 8, items * most);  // (8: the kernel's sums are rounded)
   }
   return r;
 }
 
 template <typename T, int TERMS>
-int rows16_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
+int few_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
   const dim3 grid = a.part ? dim3((unsigned)a.parts) : dim3((unsigned)slots, (unsigned)a.c.hkv);
-#define FA_KV_A(N) kv_attn_kernel<T, TERMS, N><<<grid, 256, 0, s>>>(a)
-  if (a.c.nc == 1) FA_KV_A(1);
-  else if (a.c.nc == 2) FA_KV_A(2);
-  else if (a.c.nc == 3) FA_KV_A(3);
-  else if (a.c.nc == 4) FA_KV_A(4);
-  else FA_KV_A(8);
+#define FA_KV_A(N)                                                                       \
+  if (TERMS == 1 && a.tile == kPairRows)                                                 \
+    kv_attn_kernel<T, TERMS, N, TERMS == 1 ? 2 : 1><<<grid, 256, 0, s>>>(a);             \
+  else                                                                                   \
+    kv_attn_kernel<T, TERMS, N, 1><<<grid, 256, 0, s>>>(a)
+  if (a.c.nc == 1) { FA_KV_A(1); }
+  else if (a.c.nc == 2) { FA_KV_A(2); }
+  else if (a.c.nc == 3) { FA_KV_A(3); }
+  else if (a.c.nc == 4) { FA_KV_A(4); }
+  else kv_attn_kernel<T, TERMS, 8, 1><<<grid, 256, 0, s>>>(a);
 #undef FA_KV_A
   FA_CHECK_LAUNCH(ctx);
   return FA_OK;
@@ -538,10 +616,10 @@ int rows16_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
 
 template <typename T, int TERMS>
 int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
-  const int rc = a.tile == kTileRows ? rows16_t<T, TERMS>(ctx, a, slots, s)
+  const int rc = a.tile != kWideRows ? few_t<T, TERMS>(ctx, a, slots, s)
                                      : launch_kv_tiles_attn(ctx, a, TERMS == 3 ? FA_DT_F32 : FA_DT_BF16, slots, s);
   if (rc) return rc;
-  if (a.part && a.tile != kTileRows) {
+  if (a.part && a.tile == kWideRows) {
     const dim3 grid((unsigned)(a.c.rows * a.G / 16 + a.c.nseq), (unsigned)a.c.hkv);
     kv_join_kernel<T><<<grid, 256, 0, s>>>(a);
     FA_CHECK_LAUNCH(ctx);
@@ -551,14 +629,30 @@ int attn_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
 
 }  // namespace
 
-size_t kv_attention_scratch(const KvAttnArgs& a) {
-  const Shape h = shape_of(a);
+namespace {
+size_t scratch_of(const KvAttnArgs& a, const Shape& h) {
   return h.parts ? kKvCountBytes + (size_t)h.parts * h.tile * (a.c.nc * 64 + 2) * sizeof(float) : 0;
+}
+}  // namespace
+
+size_t kv_attention_scratch(const KvAttnArgs& a) { return scratch_of(a, shape_of(a)); }
+
+size_t kv_attention_scratch_any(KvAttnArgs a) {
+  size_t most = 0;
+  a.window = 0;  // the more blocks a tile sees, the more parts; a window can only take other tiles
+  for (int dtype : {FA_DT_F32, FA_DT_BF16})
+    for (bool pairs : {false, true})
+      for (int causal : {0, 1}) {
+        a.dtype = dtype;
+        a.causal = causal;
+        most = std::max(most, scratch_of(a, shape_of(a, pairs)));
+      }
+  return most;
 }
 
 int64_t kv_attention_grid(const KvAttnArgs& a) {
   const Shape h = shape_of(a);
-  return h.parts ? h.parts : h.tile == kTileRows ? h.slots : h.slots * a.c.hkv;
+  return h.parts ? h.parts : h.tile != kWideRows ? h.slots : h.slots * a.c.hkv;
 }
 
 int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStream_t s) {
@@ -579,6 +673,7 @@ int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& k, void* scratch, hipStre
   a.least = h.least;
   a.cap = h.cap;
   a.span = h.span;
+  a.once = (float)h.once;
   a.places = h.places;
   a.uneven = h.uneven;
   a.parts = h.parts;

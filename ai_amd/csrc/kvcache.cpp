@@ -293,10 +293,7 @@ int fa_kv_attention_work(const fa_kv_cache* cache, const fa_kv_batch* batch, int
   fa::KvAttnArgs a = {};
   a.c = args_of(cache, batch);
   a.H = heads;
-  for (int dtype : {FA_DT_F32, FA_DT_BF16}) {
-    a.dtype = dtype;
-    if (!nothing(batch)) *bytes = std::max(*bytes, fa::kv_attention_scratch(a));
-  }
+  if (!nothing(batch)) *bytes = fa::kv_attention_scratch_any(a);
   return FA_OK;
 }
 

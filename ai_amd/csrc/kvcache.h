@@ -48,6 +48,7 @@ struct KvAttnArgs {
 // It begins with kKvCountBytes of counters that are zero between calls.
 constexpr size_t kKvCountBytes = 16384;
 size_t kv_attention_scratch(const KvAttnArgs& a);
+size_t kv_attention_scratch_any(KvAttnArgs a);  // enough for either type, any window, causal or not
 int64_t kv_attention_grid(const KvAttnArgs& a);  // workgroups along a grid's x
 int launch_kv_attention(fa_ctx* ctx, const KvAttnArgs& a, void* scratch, hipStream_t s);
 
