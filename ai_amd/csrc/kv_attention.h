@@ -290,7 +290,6 @@ __device__ __forceinline__ float row_sum(float v) {
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
 
 // Many rows (kv_attention_tile.hip): a.tile rows a work item.
-int kv_tile_rows(int nc, int64_t rows, int nseq);
 int kv_tiles_per_cu(int nc, int dtype);
 int launch_kv_tiles_attn(fa_ctx* ctx, const AttnArgs& a, int dtype, int64_t slots, hipStream_t s);
 

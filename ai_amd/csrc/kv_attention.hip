@@ -513,18 +513,31 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
   if (it.ok && it.chunks > 1 && r < s.n * a.G) join_row<T, 4>(a, s, it, r, r - tile * a.tile, threadIdx.x & 15);
 }
 
-// Tiles of many rows are split, in about kWideTarget parts, where they are fewer
-// than kWideItems, and beyond that where plan_item's rule finds that a longest
-// tile is long and the card far from full: every row of a part is written, read
-// and joined. Prompts of 8 x 1100 tokens, 139 tiles of float32 rows of 256 dims on
-// up to 18 blocks: 96 us whole, 114 in parts; 2 x 3000, 142 tiles on 47 blocks: 209
-// and 124. In bf16, 512 tokens on 8000, 32 heads on 8 of 128 dims, 136 tiles on 125
-// blocks: 173 and 96; 1536 on 3000, 392 tiles on 47: 86 and 101. Where workgroups
-// have a CU each, a prompt's later tiles leave the earlier ones' CUs idle
+// The kernel for many rows is taken where the work of 16-row tiles, tiles times
+// blocks times slices of 64 dims, is kWideWork or more, and a sequence and head has
+// over 64 rows in bf16, 95 in float32. Less work than that is over before its 128
+// rows and the launch that joins its parts pay. us by it and by the kernel for few
+// rows, with the work: bf16, 128 dims, 8 heads, 8000 tokens, 128 rows 32 and 30 (16 k),
+// 256 rows 39 and 40 (32 k), 512 rows 44 and 56; one head, 30000 tokens, 256 rows 54
+// and 29 (15 k); 64 sequences of 8192, one head, 80 rows 56 and 79 (82 k). float32, 256
+// dims, 16 sequences of 500, 4 heads, 128 rows 52 and 42 (16 k), 256 rows 56 and 88
+// (33 k). At 64 rows the two are within a fifth of each other either way.
+constexpr int kWideWork = 32768;
+
+// Its tiles are split, in about a part for each workgroup that the card holds, where
+// they are fewer than kWideItems; beyond that, in kWideTarget, where plan_item's rule
+// finds that a longest tile is long and the card far from full: every row of a part is
+// written, read and joined. Prompts of 8 x 1100 tokens, 139 tiles of float32 rows of
+// 256 dims on up to 18 blocks: 96 us whole, 114 in parts; 2 x 3000, 142 tiles on 47
+// blocks: 209 and 124. In bf16, 512 tokens on 8000, 32 heads on 8 of 128 dims, 136
+// tiles on 125 blocks: 173 and 96; 1536 on 3000, 392 tiles on 47: 86 and 101. Where
+// workgroups have a CU each, a prompt's later tiles leave the earlier ones' CUs idle
 // (kUneven: 8 heads on 2 of 256 dims, 4000 tokens, 252 tiles: 171 and 152 us); where
 // two share one, the longer has it to itself then (16 on 4 of 128, 4000 tokens,
 // 502 tiles: 104 and 120). Parts of fewer than kWideMin blocks cost more (2 x 3000
-// in float32: 139 us with 8, 124 with 16).
+// in float32: 139 us with 8, 124 with 16), and so do more of them than fit at once
+// (512 tokens on 8000, 3 heads on one of 256 dims in float32, 13 tiles: 62 us in 256
+// parts, 90 in 512).
 constexpr int kWideItems = 128, kWideTarget = 512, kWideMin = 16;
 constexpr float kUneven = 0.4f;
 
@@ -547,37 +560,51 @@ struct Shape {
   int64_t parts;      // parts, at most; 0: not split
 };
 
-Shape shape_of(const KvAttnArgs& a, bool pairs = true) {
+// Whether a call's tiles can have 32 rows, 128.
+bool may_be_pairs(const KvAttnArgs& a) {
+  return a.dtype == FA_DT_BF16 && a.c.nc <= 4 && a.c.rows * (a.H / a.c.hkv) > (int64_t)kTileRows * a.c.nseq;
+}
+bool may_be_wide(const KvAttnArgs& a) {
+  return a.c.nc <= 4 && a.c.rows * (a.H / a.c.hkv) > (int64_t)(a.dtype == FA_DT_BF16 ? 64 : 95) * a.c.nseq;
+}
+
+Shape shape_of(const KvAttnArgs& a, int tile = 0) {
   Shape r;
   const int G = a.H / a.c.hkv;
   const int64_t all = a.c.rows * G, nseq = a.c.nseq;
   // tiles, about and at most
   auto tiles = [&](int rows) { return std::max((all + nseq * rows / 2) / rows, std::min(nseq, all)); };
   auto most_tiles = [&](int rows) { return all / rows + nseq; };
-  // blocks that a tile of some rows can see
-  auto seen = [&](int rows) {
-    return a.window ? ((int64_t)a.window * (a.causal ? 1 : 2) + rows / G + 63) / 64 + 1 : (int64_t)0x7FFFFFFF;
+  // blocks that a tile of some rows can see, by the window
+  auto span = [&](int rows) {
+    return a.window ? (int)(((int64_t)a.window * (a.causal ? 1 : 2) + rows / G + 63) / 64 + 1) : 0x7FFFFFFF;
   };
-  r.tile = kv_tile_rows(a.c.nc, all, a.c.nseq);
-  if (r.tile == kTileRows && pairs && a.dtype == FA_DT_BF16 && a.c.nc <= 4 && all > kTileRows * nseq) {
-    const int64_t items = tiles(kPairRows) * a.c.hkv, blocks = std::min<int64_t>(a.c.tstride, seen(kPairRows));
-    if (items >= 256 * few_per_cu(a.c.nc) ||
-        (a.c.nc <= 2 && items >= kPairItems && blocks >= kPairBlocks && all >= kPairRows * nseq))
+  auto seen = [&](int rows) { return (int64_t)std::min(a.c.tstride, span(rows)); };
+  r.tile = tile;
+  if (!tile) {
+    r.tile = kTileRows;
+    const int64_t pairs = tiles(kPairRows) * a.c.hkv;
+    if (may_be_wide(a) && tiles(kTileRows) * a.c.hkv * seen(kTileRows) * a.c.nc >= kWideWork)
+      r.tile = kWideRows;
+    else if (may_be_pairs(a) &&
+             (pairs >= 256 * few_per_cu(a.c.nc) || (a.c.nc <= 2 && pairs >= kPairItems &&
+                                                    seen(kPairRows) >= kPairBlocks && all >= kPairRows * nseq)))
       r.tile = kPairRows;
   }
   r.slots = most_tiles(r.tile);
   const int64_t items = r.slots * a.c.hkv;
   const bool wide = r.tile == kWideRows;
-  r.span = (int)seen(r.tile);
-  const int64_t blocks = std::min(a.c.tstride, r.span);
-  r.target = wide ? kWideTarget : kTarget;
+  r.span = span(r.tile);
+  const int64_t blocks = seen(r.tile);
+  const int per_cu = wide ? kv_tiles_per_cu(a.c.nc, a.dtype) : few_per_cu(a.c.nc);
+  r.target = wide ? 256 * per_cu : kTarget;
   r.least = kMinChunk;
   r.cap = wide ? 0 : kRound;
-  r.once = r.tile == kPairRows ? 256 * few_per_cu(a.c.nc) : 256;
+  r.once = r.tile == kPairRows ? 256 * per_cu : 256;
   r.places = r.uneven = 0.f;
   bool split = wide ? items < kWideItems : tiles(r.tile) * a.c.hkv < kTarget && items < 2 * kTarget;
   if (wide && !split) {
-    const int per_cu = kv_tiles_per_cu(a.c.nc, a.dtype);
+    r.target = kWideTarget;
     r.least = kWideMin;
     r.places = 256.f * (float)per_cu;
     r.uneven = per_cu == 1 && a.causal ? kUneven : 0.f;
@@ -641,11 +668,12 @@ size_t kv_attention_scratch_any(KvAttnArgs a) {
   size_t most = 0;
   a.window = 0;  // the more blocks a tile sees, the more parts; a window can only take other tiles
   for (int dtype : {FA_DT_F32, FA_DT_BF16})
-    for (bool pairs : {false, true})
-      for (int causal : {0, 1}) {
+    for (int causal : {0, 1})
+      for (int tile : {kTileRows, kPairRows, kWideRows}) {
         a.dtype = dtype;
         a.causal = causal;
-        most = std::max(most, scratch_of(a, shape_of(a, pairs)));
+        if (tile == kTileRows || (tile == kPairRows ? may_be_pairs(a) : may_be_wide(a)))
+          most = std::max(most, scratch_of(a, shape_of(a, tile)));
       }
   return most;
 }

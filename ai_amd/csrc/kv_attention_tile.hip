@@ -556,15 +556,6 @@ int tiles_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
 
 }  // namespace
 
-// Rows of a work item: 16, or the kernel above's where the sequences bring 96
-// or more each. 16 sequences of 4000 tokens, 32 heads on 8 of 128 dims in
-// bf16: 54 us by the kernel for few rows and 90 by this one at 64 rows a
-// sequence and head, 174 and 96 at 128; 3 heads on one of 256 dims in float32:
-// 35 and 44 at 48, 48 and 48 at 96.
-int kv_tile_rows(int nc, int64_t rows, int nseq) {
-  return nc > 4 || rows < (int64_t)96 * nseq ? kTileRows : kWideRows;
-}
-
 int kv_tiles_per_cu(int nc, int dtype) { return per_cu(nc, dtype == FA_DT_F32 ? 3 : 1); }
 
 int launch_kv_tiles_attn(fa_ctx* ctx, const AttnArgs& a, int dtype, int64_t slots, hipStream_t s) {
