@@ -143,12 +143,16 @@ def attend(cache, batch, q, causal=True, window=0, scale=1.0, work=False):
     return out
 
 
+SPARE = 0  # table entries of a sequence more than it uses, as in a program with longest lengths in mind
+
+
 def tables_for(r, lengths, extra=2, width=None):
     """A pool size and block tables that hand its blocks out in random order; unused entries are out of range."""
     used = [-(-l // 64) for l in lengths]
     blocks = sum(used) + extra
     perm = r.permutation(blocks)
-    t = np.full((len(lengths), max(max(used, default=0), 1) if width is None else width), 2 ** 31 - 1, np.int32)
+    width = max(max(used, default=0), 1) + SPARE if width is None else width
+    t = np.full((len(lengths), width), 2 ** 31 - 1, np.int32)
     at = 0
     for i, u in enumerate(used):
         t[i, :u] = perm[at:at + u]

@@ -23,6 +23,12 @@ pytestmark = pytest.mark.gpu
 BF = 2.0 ** -8  # half a step of bf16, relative
 
 
+@pytest.fixture(params=[0, 20000], ids=["tables as long as needed", "longer tables"])
+def spare(request, monkeypatch):
+    """Attention is divided by what the tables have room for: with long ones many rows take the kernel for them."""
+    monkeypatch.setattr(K, "SPARE", request.param)
+
+
 def rng(seed):
     return np.random.default_rng(seed)
 
@@ -185,6 +191,32 @@ def test_write_strides_and_rows_behind(ctx):
     cache.free()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_strides_of_many_rows(ctx, spare, dtype):
+    """Queries as a view of a q|k|v product with rows of any alignment; rows behind the last sequence stay as they are."""
+    r = rng(13)
+    for D, pad in ((80, 3), (128, 8)):
+        H, Hkv, rows = 4, 2, 330
+        lengths, cu = [200, 128], [0, 200, 320]
+        cache, ref, tables = fill(ctx, r, lengths, Hkv, D, dtype)
+        qkv = make(r, (rows, 6 * D + pad), dtype)
+        q = np.lib.stride_tricks.as_strided(qkv[:, D:], (rows, H, D), (qkv.strides[0], D * qkv.itemsize, qkv.itemsize))
+        b = K.Batch(ctx, tables, lengths, cu, rows=rows)
+        got = K.attend(cache, b, q, scale=0.1)
+        assert (got[320:].view(np.uint8) == 0x5A).all()
+        for i in range(2):
+            at = slice(cu[i], cu[i + 1])
+            qi, mask = K.wide(np.ascontiguousarray(q[at])), O.sees(lengths[i], cu[i + 1] - cu[i], True, 0)
+            wk, wv = ref.tokens(tables[i], lengths[i])
+            scale = float(np.float32(0.1))
+            want, tol = O.attention(qi, wk, wv, mask, scale)
+            if dtype == "bf16":
+                tol = tol + BF * O.attention(qi, wk, np.abs(wv), mask, scale)[0]
+            close(got[at], want, tol, f"strided, {D} dims, sequence {i}")
+        b.free()
+        cache.free()
+
+
 def test_write_special_values(ctx):
     """Zeros, the smallest and largest magnitudes, ties between codes, and values that are not finite."""
     D, Hkv = 64, 1
@@ -249,7 +281,7 @@ def test_attention_head_layouts(ctx, H, Hkv, dtype):
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 1), (True, 64), (True, 100), (False, 1),
                                            (False, 37), (False, 1000), (True, 2 ** 31 - 1), (False, 2 ** 31 - 1)])
-def test_attention_masks(ctx, causal, window, dtype):
+def test_attention_masks(ctx, spare, causal, window, dtype):
     """Chunks and whole prompts under each mask, windows shorter and longer than a block and than the sequence."""
     attention_case(ctx, 17 + window % 97, dtype, 128, 4, 2, [150, 64, 400, 10], [150, 7, 90, 1], causal, window)
 
@@ -271,7 +303,7 @@ def test_attention_split_token_axis(ctx, D, H, Hkv, lengths, ns, dtype):
     (128, 8, 2, [640, 200, 333], [640, 200, 333]), (64, 4, 4, [300] * 3, [257, 300, 128]),
     (256, 3, 1, [500, 129], [400, 129]), (192, 2, 1, [260], [260]), (96, 6, 2, [700], [130]),
     (320, 2, 1, [200], [200])])
-def test_attention_prompts(ctx, D, H, Hkv, lengths, ns, dtype):
+def test_attention_prompts(ctx, spare, D, H, Hkv, lengths, ns, dtype):
     attention_case(ctx, D + H, dtype, D, H, Hkv, lengths, ns)
     attention_case(ctx, D + H + 1, dtype, D, H, Hkv, lengths, ns, window=90)
 
@@ -279,7 +311,7 @@ def test_attention_prompts(ctx, D, H, Hkv, lengths, ns, dtype):
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("D,H,Hkv,lengths,ns", [(128, 8, 2, [5000], [40]), (64, 2, 1, [2000, 9000], [100, 130]),
                                                 (256, 3, 1, [1500], [70]), (192, 1, 1, [3000], [129])])
-def test_attention_few_tiles_of_many_rows_split(ctx, D, H, Hkv, lengths, ns, dtype):
+def test_attention_few_tiles_of_many_rows_split(ctx, spare, D, H, Hkv, lengths, ns, dtype):
     """Chunks on long contexts: few tiles of 128 rows, whose blocks are cut into parts and joined."""
     attention_case(ctx, D + H, dtype, D, H, Hkv, lengths, ns, work=dtype == "f32")
     attention_case(ctx, D + H + 1, dtype, D, H, Hkv, lengths, ns, causal=False, window=1100, work=dtype == "bf16")
@@ -331,7 +363,7 @@ def test_thousands_of_sequences(ctx):
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [2, 150])
-def test_attention_scores_that_rise_and_fall(ctx, dtype, n):
+def test_attention_scores_that_rise_and_fall(ctx, spare, dtype, n):
     """Scores that rise by thousands of times their weights' range from block to block, and fall again: the reference
     of the weights follows, in both kernels, split and not."""
     r = rng(90 + n)
@@ -363,13 +395,13 @@ def test_attention_scores_that_rise_and_fall(ctx, dtype, n):
         cache.free()
 
 
-def test_attention_score_range(ctx):
+def test_attention_score_range(ctx, spare):
     """Scores of hundreds either way, scale 0, a negative scale."""
     for scale in (3.0, 0.0, -0.7):
         attention_case(ctx, 23, "f32", 64, 4, 2, [200, 90], [3, 90], scale=scale)
 
 
-def test_attention_value_scales_far_apart(ctx):
+def test_attention_value_scales_far_apart(ctx, spare):
     """Blocks whose values are 2^60 apart, large and tiny ones: weights meet each block's own scale."""
     r = rng(31)
     lengths, D = [64 * 5], 64
@@ -414,7 +446,7 @@ def test_attention_value_scales_far_apart_few_rows(ctx):
     cache.free()
 
 
-def test_attention_empty_rows_and_lengths(ctx):
+def test_attention_empty_rows_and_lengths(ctx, spare):
     """A sequence of no tokens, one without rows, more rows than tokens: rows that see nothing are zeros."""
     r = rng(2)
     for dtype in ("f32", "bf16"):
@@ -434,7 +466,7 @@ def test_attention_empty_rows_and_lengths(ctx):
         cache.free()
 
 
-def test_attention_nan_stays_where_it_is_seen(ctx):
+def test_attention_nan_stays_where_it_is_seen(ctx, spare):
     """A NaN value or key that some rows of a tile see and others do not reaches those that do, in its dims (values) or
     whole (keys); NaN codes behind a length reach nobody (every cache here begins with them)."""
     r = rng(8)
@@ -499,7 +531,7 @@ def test_attention_nan_among_drafted_tokens(ctx):
             cache.free()
 
 
-def test_attention_nan_query_stays_in_its_row(ctx):
+def test_attention_nan_query_stays_in_its_row(ctx, spare):
     r = rng(9)
     cache, ref, tables = fill(ctx, r, [90], 2, 64)
     b = K.Batch(ctx, tables, [90], [0, 90])
@@ -516,7 +548,7 @@ def test_attention_nan_query_stays_in_its_row(ctx):
     cache.free()
 
 
-def test_bad_tables_give_nan_and_touch_nothing(ctx):
+def test_bad_tables_give_nan_and_touch_nothing(ctx, spare):
     """Entries outside the pool and lengths past the table row: NaN for those that see them, and no write."""
     r = rng(4)
     for dtype in ("f32", "bf16"):
@@ -550,19 +582,20 @@ def test_bad_tables_give_nan_and_touch_nothing(ctx):
         cache.free()
 
 
-def test_row_starts_out_of_order_stay_in_bounds(ctx):
+def test_row_starts_out_of_order_stay_in_bounds(ctx, spare):
     """Device arrays are not checked on the host: whatever row starts they hold, nothing outside the call's rows is
     written."""
     r = rng(6)
     cache, ref, tables = fill(ctx, r, [300, 300, 300], 1, 64)
     before = [x.copy() for x in cache.state()]
     for cu in ([0, 500, 20, 10 ** 9], [-7, -9, -2 ** 31, 4], [100, 50, 2, 1], [2 ** 31 - 1] * 4):
-        b = K.Batch(ctx, tables, [300, -5, 300], cu, rows=40)
-        q = make(r, (40, 2, 64), "f32")
-        out = K.attend(cache, b, q, scale=0.125)
-        assert out.shape == (40, 2, 64)
-        K.read(cache, b)
-        b.free()
+        for rows in (40, 500):
+            b = K.Batch(ctx, tables, [300, -5, 300], cu, rows=rows)
+            q = make(r, (rows, 2, 64), "f32")
+            out = K.attend(cache, b, q, scale=0.125)
+            assert out.shape == (rows, 2, 64)
+            K.read(cache, b)
+            b.free()
     for x0, x1 in zip(before, cache.state()):
         np.testing.assert_array_equal(x0, x1)
     cache.free()
@@ -598,7 +631,7 @@ def test_offsets_past_32_bits(ctx):
     c.free()
 
 
-def test_same_results_every_time(ctx):
+def test_same_results_every_time(ctx, spare):
     """No order that changes: equal bits from call to call, split axis included."""
     r = rng(12)
     cache, ref, tables = fill(ctx, r, [4000, 100, 1700], 2, 128)
@@ -824,15 +857,37 @@ def test_work_suffices_whatever_the_mask(ctx):
         cache.free()
 
 
-def test_tiles_of_many_rows_go_by_length(ctx):
-    """Whole tiles of sequences of many lengths, some without rows or tokens: every tile is some workgroup's."""
-    lengths = [1300, 0, 100, 700, 1299, 400, 90, 1000, 640, 130, 1300, 257]
-    ns = [130, 0, 100, 129, 200, 0, 90, 128, 96, 130, 257, 120]
-    attention_case(ctx, 55, "bf16", 64, 16, 16, lengths, ns, work=True)
-    r = rng(56)
-    lengths = [int(x) for x in r.integers(96, 260, 70)]
-    ns = [int(r.integers(96, x + 1)) for x in lengths]
-    attention_case(ctx, 57, "f32", 64, 2, 2, lengths, ns, causal=False)
+@pytest.mark.parametrize("dtype,Hkv,lengths,ns,width", [
+    ("bf16", 64, [1300, 0, 100, 700, 1299, 400, 90, 1000, 640, 130, 1300, 257],
+     [130, 0, 100, 129, 200, 0, 90, 128, 96, 130, 257, 120], 22),
+    ("f32", 32, [90 + 2 * i for i in range(70)], [90 + i for i in range(70)], 8),
+    ("bf16", 128, [70 * i for i in range(20)], [70] * 10 + [66] * 10, 30)])
+def test_whole_tiles_of_many_rows_go_by_length(ctx, dtype, Hkv, lengths, ns, width):
+    """More tiles than the card takes at once, of sequences of many lengths, some without rows or tokens: every tile is
+    some workgroup's. Heads have the same keys, values and queries; the first is compared with the reference."""
+    r = rng(55)
+    D, ns = 64, [min(n, l) for n, l in zip(ns, lengths)]
+    blocks, tables = K.tables_for(r, lengths, width=width)
+    cache, ref = K.Cache(ctx, blocks, Hkv, D), O.RefCache(blocks, 1, D)
+    cu = K.cu_of(lengths)
+    k, v = (make(r, (int(cu[-1]), 1, D), dtype) for _ in range(2))
+    full = K.Batch(ctx, tables, lengths, cu)
+    K.write(cache, full, np.repeat(k, Hkv, 1), np.repeat(v, Hkv, 1))
+    ref.write(tables, lengths, cu, K.wide(k), K.wide(v))
+    cu = K.cu_of(ns)
+    q = make(r, (int(cu[-1]), 1, D), dtype)
+    b = K.Batch(ctx, tables, lengths, cu)
+    got = K.attend(cache, b, np.repeat(q, Hkv, 1), scale=0.125)
+    assert (got == got[:, :1]).all()
+    for i, (length, n) in enumerate(zip(lengths, ns)):
+        at = slice(cu[i], cu[i + 1])
+        kk, vv = ref.tokens(tables[i], length)
+        want, tol = O.attention(K.wide(q[at]), kk, vv, O.sees(length, n, True, 0), 0.125)
+        if dtype == "bf16":
+            tol = tol + BF * O.attention(K.wide(q[at]), kk, np.abs(vv), O.sees(length, n, True, 0), 0.125)[0]
+        close(got[at, :1], want, tol, f"sequence {i} of {length}, {n} rows")
+    for x in (full, b, cache):
+        x.free()
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
@@ -842,7 +897,7 @@ def test_weights_on_zero_values_count(ctx, dtype):
     lane adds 32 weights of a block to a sum over the blocks, or 16 of every fourth block to one sum: at most tokens / 16
     terms one after another, and of the values those of one block."""
     r = rng(52)
-    Hkv, G, D, tokens = 64, 32, 64, 131072
+    Hkv, G, D, tokens = 256, 32, 64, 131072  # (as many heads as leave tiles whole)
     k, v = np.zeros((128, Hkv, D), np.float32), np.zeros((128, Hkv, D), np.float32)
     k[0, :, 0] = 1.0
     v[:64] = r.standard_normal((64, 1, D)).astype(np.float32)
