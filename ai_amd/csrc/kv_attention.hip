@@ -45,7 +45,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const KvSeq& s, cons
   const int n = it.chunks, nc = a.c.nc, Dp = nc * 64, rows = a.tile;
   const float* jstat = a.part + a.parts * rows * Dp + (it.first * rows + tr) * 2;
   const float* src = a.part + (it.first * rows + tr) * Dp + ln * 4;
-  constexpr int kBatch = NC <= 2 ? 8 : NC <= 4 ? 4 : 1;
+  constexpr int kBatch = NC <= 2 ? 8 : NC <= 4 ? 4 : 2;
   float jM = -__builtin_inff(), jL = 0.f, o[NC * 4];
 #pragma unroll
   for (int i = 0; i < NC * 4; i++) o[i] = 0.f;
@@ -101,7 +101,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const KvSeq& s, cons
 constexpr int few_per_cu(int nc) { return nc <= 2 ? 2 : 1; }
 
 // One work item: 16 RT query rows of one key/value head over a run of blocks.
-// Lane l: rows l % 16 of each 16, group l / 16. NC: slices of 64 dims (at most; nc in use).
+// Lane l: rows l % 16 of each 16, group l / 16. NC: slices of 64 dims.
 // Its blocks go to the four waves in turn, their results are merged at the
 // end. A wave loads a block's keys while it works on the scores of the block
 // before, and its values while it works on the next scores, so that about a
@@ -111,11 +111,11 @@ constexpr int few_per_cu(int nc) { return nc <= 2 ? 2 : 1; }
 template <typename T, int TERMS, int NC, int RT>
 __global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a) {
   constexpr int kRows = 16 * RT;
-  constexpr bool AHEAD = NC <= 4;  // loads a block ahead
+  constexpr bool AHEAD = NC <= 4 && NC * RT <= 6;  // loads a block ahead, else half of one
   constexpr int kWaves = 4, kThreads = kWaves * 64;
   constexpr int kMergeDims = 128;         // dims that the waves' results are merged at a time
   constexpr int kLane = kMergeDims / 16;  // and a thread's of them, 16 threads a row
-  const int nc = NC <= 4 ? NC : a.c.nc;
+  constexpr int nc = NC;
   constexpr int kQ = RT * TERMS * NC * 2 * 64;        // operands of 16 bytes
   constexpr int kM = kWaves * 16 * (kMergeDims + 4);  // floats
   __shared__ __align__(16) char lds[kQ * 16 > kM * 4 ? kQ * 16 : kM * 4];
@@ -158,27 +158,26 @@ __global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a
   }
 
   // a block's codes, 16 bytes a lane: kr[slice * 4 + tile of 16 tokens], vr[tile of 16 dims]
-  uint4 kr[AHEAD ? NC * 4 : 1], vr[AHEAD ? NC * 4 : 1];
+  // (not AHEAD: kr alone, a slice's values after its keys, the next keys after them)
+  uint4 kr[NC * 4], vr[AHEAD ? NC * 4 : 1];
   auto part = [&](int id, int which) {
-    return reinterpret_cast<const uint4*>(kv_part(a.c, id, it.h, which)) + row * 4 + grp;
+    return static_cast<const uint8_t*>(kv_part(a.c, id, it.h, which));
   };
-  auto key = [&](const uint4* p, int i) {  // no such block: keys that are NaN
-    return p && (NC <= 4 || i < nc * 4) ? p[(i >> 2) * 256 + (i & 3) * 64]
-                                        : make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+  const uint32_t mine16 = (uint32_t)(row * 4 + grp) * 16;  // (a base that all lanes share and 32 bits of each)
+  auto key = [&](const uint8_t* p, int i) {  // no such block: keys that are NaN
+    return p ? *reinterpret_cast<const uint4*>(p + ((i >> 2) * 4096 + (i & 3) * 1024) + mine16) : make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
   };
-  auto value = [&](const uint4* p, int i) {
-    return p && (NC <= 4 || i < nc * 4) ? p[i * 64] : make_uint4(0, 0, 0, 0);
+  auto value = [&](const uint8_t* p, int i) {
+    return p ? *reinterpret_cast<const uint4*>(p + i * 1024 + mine16) : make_uint4(0, 0, 0, 0);
   };
   auto load_k = [&](int id) {
-    if constexpr (AHEAD) {
-      const uint4* p = id >= 0 ? part(id, 0) : nullptr;
+    const uint8_t* p = id >= 0 ? part(id, 0) : nullptr;
 #pragma unroll
-      for (int i = 0; i < NC * 4; i++) kr[i] = key(p, i);
-    }
+    for (int i = 0; i < NC * 4; i++) kr[i] = key(p, i);
   };
   auto load_v = [&](int id) {
     if constexpr (AHEAD) {
-      const uint4* p = id >= 0 ? part(id, 1) : nullptr;
+      const uint8_t* p = id >= 0 ? part(id, 1) : nullptr;
 #pragma unroll
       for (int i = 0; i < NC * 4; i++) vr[i] = value(p, i);
     }
@@ -229,8 +228,8 @@ __global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a
     const int id1 = blocks.at(a, it.b, ++turn);
     const float ks = ksv.x, vs = ksv.y;
     const int j0 = p * 64;
-    const uint4* kp = id >= 0 ? part(id, 0) : nullptr;
-    const uint4* vp = id >= 0 ? part(id, 1) : nullptr;
+    const uint8_t* kp1 = id1 >= 0 ? part(id1, 0) : nullptr;
+    const uint8_t* vp = id >= 0 ? part(id, 1) : nullptr;
 
     // S^T: four tiles of 16 tokens
     kvf4 sc4[RT][4];
@@ -240,13 +239,9 @@ __global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a
       for (int tt = 0; tt < 4; tt++) sc4[rt][tt] = kvf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NC; c++) {
-      if (NC > 4 && c >= nc) continue;
       uint4 kc[4];
 #pragma unroll
-      for (int tt = 0; tt < 4; tt++) {
-        if constexpr (AHEAD) kc[tt] = kr[c * 4 + tt];
-        else kc[tt] = key(kp, c * 4 + tt);
-      }
+      for (int tt = 0; tt < 4; tt++) kc[tt] = kr[c * 4 + tt];
       if constexpr (TERMS == 1) {
         bf16x8 q[RT][2];
 #pragma unroll
@@ -283,11 +278,16 @@ __global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a
             }
           }
       }
+      if constexpr (!AHEAD) {
+#pragma unroll
+        for (int tt = 0; tt < 4; tt++) kr[c * 4 + tt] = value(vp, c * 4 + tt);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     const bool more = p + kWaves < pg1;
     if (more) {
       ksv = scales(id1);
-      load_k(id1);
+      if constexpr (AHEAD) load_k(id1);
     }
     const float mul = a.scale2 * ks;
     const bool edge = j0 < alo || j0 + 64 > ahi;  // some row does not see some token
@@ -352,10 +352,7 @@ __global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a
     uint32_t nan = 0;
 #pragma unroll
     for (int dt = 0; dt < NC * 4; dt++) {
-      if (NC > 4 && dt >= nc * 4) continue;
-      uint4 v;
-      if constexpr (AHEAD) v = vr[dt];
-      else v = value(vp, dt);
+      uint4 v = AHEAD ? vr[AHEAD ? dt : 0] : kr[dt];
       if (edge) v = make_uint4(v.x & keep[0], v.y & keep[1], v.z & keep[2], v.w & keep[3]);
       if (mixed) {
         auto drop = [&](uint32_t w) {
@@ -373,6 +370,13 @@ __global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a
           acc[rt][dt] = mfma(v0, pt[rt][0][k], acc[rt][dt]);
           acc[rt][dt] = mfma(v1, pt[rt][1][k], acc[rt][dt]);
         }
+      if constexpr (!AHEAD) {
+        if ((dt & 3) == 3) {
+#pragma unroll
+          for (int i = dt - 3; i <= dt; i++) kr[i] = key(kp1, i);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
     }
     if (mixed && __ballot(nan != 0)) {
 #pragma unroll 1
@@ -453,7 +457,6 @@ __global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a
     const bool empty = !split && fin == 0.f;
 #pragma unroll
     for (int c = 0; c < (NC * 64 + kMergeDims - 1) / kMergeDims; c++) {
-      if (NC > 4 && c * kMergeDims >= nc * 64) continue;
       __syncthreads();
 #pragma unroll
       for (int dt = 0; dt < kMergeDims / 16; dt++) {
@@ -635,6 +638,9 @@ int few_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
   else if (a.c.nc == 2) { FA_KV_A(2); }
   else if (a.c.nc == 3) { FA_KV_A(3); }
   else if (a.c.nc == 4) { FA_KV_A(4); }
+  else if (a.c.nc == 5) kv_attn_kernel<T, TERMS, 5, 1><<<grid, 256, 0, s>>>(a);
+  else if (a.c.nc == 6) kv_attn_kernel<T, TERMS, 6, 1><<<grid, 256, 0, s>>>(a);
+  else if (a.c.nc == 7) kv_attn_kernel<T, TERMS, 7, 1><<<grid, 256, 0, s>>>(a);
   else kv_attn_kernel<T, TERMS, 8, 1><<<grid, 256, 0, s>>>(a);
 #undef FA_KV_A
   FA_CHECK_LAUNCH(ctx);
