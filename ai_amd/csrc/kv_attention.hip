@@ -98,7 +98,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, const KvSeq& s, cons
 }
 
 // Workgroups that a CU holds, by their registers.
-constexpr int few_per_cu(int nc) { return nc <= 2 ? 2 : 1; }
+constexpr int few_per_cu(int nc, int rt) { return nc * rt <= 4 ? 2 : 1; }
 
 // One work item: 16 RT query rows of one key/value head over a run of blocks.
 // Lane l: rows l % 16 of each 16, group l / 16. NC: slices of 64 dims.
@@ -107,11 +107,16 @@ constexpr int few_per_cu(int nc) { return nc <= 2 ? 2 : 1; }
 // before, and its values while it works on the next scores, so that about a
 // block (D = 128: 16 KB) is always under way: 64 sequences of up to 8192
 // tokens (606 MB) take 126 us, 4.8 TB/s, against 219 without, and a large copy
-// moves 5.1 TB/s. Above 256 dims the registers do not hold it.
+// moves 5.1 TB/s. Where registers for that leave room for fewer workgroups, one
+// set serves both (not AHEAD): a slice's values are loaded where its keys were,
+// the next block's keys where its values were, so half a block is under way
+// (64 sequences of 2000 tokens, 16 heads on 4 of 512 dims: 207 us without, 88;
+// drafts of 2 to 5 tokens on windows of 512, 8 heads on 2 of 256 dims: 19.1 us a
+// block ahead, 17.7 half a block and two workgroups a CU).
 template <typename T, int TERMS, int NC, int RT>
-__global__ __launch_bounds__(256, few_per_cu(NC)) void kv_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, few_per_cu(NC, RT)) void kv_attn_kernel(AttnArgs a) {
   constexpr int kRows = 16 * RT;
-  constexpr bool AHEAD = NC <= 4 && NC * RT <= 6;  // loads a block ahead, else half of one
+  constexpr bool AHEAD = NC * RT <= 2;  // loads a block ahead, else half of one
   constexpr int kWaves = 4, kThreads = kWaves * 64;
   constexpr int kMergeDims = 128;         // dims that the waves' results are merged at a time
   constexpr int kLane = kMergeDims / 16;  // and a thread's of them, 16 threads a row
@@ -544,12 +549,12 @@ constexpr int kWideWork = 32768;
 constexpr int kWideItems = 128, kWideTarget = 512, kWideMin = 16;
 constexpr float kUneven = 0.4f;
 
-// Tiles of kPairRows rows load and widen a block once for twice the rows: with
-// bf16 (float32 has no registers for it: 64 sequences of up to 8192 tokens, 24
-// rows on each of 8 heads of 128 dims, 279 and 295 us; in bf16 260 and 187), where
-// they still fill the card, or are kPairItems and full and see kPairBlocks (64
-// sequences, 64 rows on one head: 73 and 52; on the other side 16 of 2000 tokens,
-// 32 rows on each of 8: 23 and 28, and 32 of 4000, 20 rows: 53 and 60).
+// Tiles of kPairRows rows load and widen a block once for twice the rows: where
+// they still fill the card (64 sequences of up to 8192 tokens, 24 rows on each of 8
+// heads of 128 dims: bf16 260 us in tiles of 16 and 177, float32 279 and 210), or
+// are kPairItems and full and see kPairBlocks (64 sequences, 64 rows on one head:
+// 73 and 49; on the other side 16 of 2000 tokens, 32 rows on each of 8: 23 and 28,
+// and 32 of 4000, 20 rows: 53 and 60).
 constexpr int kPairItems = 96, kPairBlocks = 64;
 
 // How a call runs, from its sizes alone.
@@ -565,7 +570,7 @@ struct Shape {
 
 // Whether a call's tiles can have 32 rows, 128.
 bool may_be_pairs(const KvAttnArgs& a) {
-  return a.dtype == FA_DT_BF16 && a.c.nc <= 4 && a.c.rows * (a.H / a.c.hkv) > (int64_t)kTileRows * a.c.nseq;
+  return a.c.nc <= 4 && a.c.rows * (a.H / a.c.hkv) > (int64_t)kTileRows * a.c.nseq;
 }
 bool may_be_wide(const KvAttnArgs& a) {
   return a.c.nc <= 4 && a.c.rows * (a.H / a.c.hkv) > (int64_t)(a.dtype == FA_DT_BF16 ? 64 : 95) * a.c.nseq;
@@ -590,7 +595,7 @@ Shape shape_of(const KvAttnArgs& a, int tile = 0) {
     if (may_be_wide(a) && tiles(kTileRows) * a.c.hkv * seen(kTileRows) * a.c.nc >= kWideWork)
       r.tile = kWideRows;
     else if (may_be_pairs(a) &&
-             (pairs >= 256 * few_per_cu(a.c.nc) || (a.c.nc <= 2 && pairs >= kPairItems &&
+             (pairs >= 256 * few_per_cu(a.c.nc, 2) || (a.c.nc <= 2 && pairs >= kPairItems &&
                                                     seen(kPairRows) >= kPairBlocks && all >= kPairRows * nseq)))
       r.tile = kPairRows;
   }
@@ -599,7 +604,7 @@ Shape shape_of(const KvAttnArgs& a, int tile = 0) {
   const bool wide = r.tile == kWideRows;
   r.span = span(r.tile);
   const int64_t blocks = seen(r.tile);
-  const int per_cu = wide ? kv_tiles_per_cu(a.c.nc, a.dtype) : few_per_cu(a.c.nc);
+  const int per_cu = wide ? kv_tiles_per_cu(a.c.nc, a.dtype) : few_per_cu(a.c.nc, 2);  // (of pairs)
   r.target = wide ? 256 * per_cu : kTarget;
   r.least = kMinChunk;
   r.cap = wide ? 0 : kRound;
@@ -629,11 +634,9 @@ Shape shape_of(const KvAttnArgs& a, int tile = 0) {
 template <typename T, int TERMS>
 int few_t(fa_ctx* ctx, const AttnArgs& a, int64_t slots, hipStream_t s) {
   const dim3 grid = a.part ? dim3((unsigned)a.parts) : dim3((unsigned)slots, (unsigned)a.c.hkv);
-#define FA_KV_A(N)                                                                       \
-  if (TERMS == 1 && a.tile == kPairRows)                                                 \
-    kv_attn_kernel<T, TERMS, N, TERMS == 1 ? 2 : 1><<<grid, 256, 0, s>>>(a);             \
-  else                                                                                   \
-    kv_attn_kernel<T, TERMS, N, 1><<<grid, 256, 0, s>>>(a)
+#define FA_KV_A(N)                                                                    \
+  if (a.tile == kPairRows) kv_attn_kernel<T, TERMS, N, 2><<<grid, 256, 0, s>>>(a);    \
+  else kv_attn_kernel<T, TERMS, N, 1><<<grid, 256, 0, s>>>(a)
   if (a.c.nc == 1) { FA_KV_A(1); }
   else if (a.c.nc == 2) { FA_KV_A(2); }
   else if (a.c.nc == 3) { FA_KV_A(3); }

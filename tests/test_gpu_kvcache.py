@@ -790,21 +790,23 @@ def test_tiles_of_many_rows_cut_in_parts(ctx, dtype, D, H, lengths, ns, window, 
     attention_case(ctx, 54, dtype, D, H, H, lengths, ns, window=window, width=width, work=True)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("D,Hkv,G,lengths,ns,causal,window", [
     (64, 16, 4, [400] * 40, [5] * 40, True, 0), (64, 16, 5, [130, 0, 64, 65, 300] * 9, [7, 0, 1, 6, 5] * 9, True, 0),
     (128, 16, 20, [200, 90, 640, 33] * 8, [1] * 32, True, 0), (128, 16, 4, [200, 90, 640, 33] * 8, [8, 7, 6, 5] * 8, False, 60),
     (72, 8, 33, [4100, 4097] * 4, [1] * 8, True, 0), (70, 2, 16, [4500, 4300] * 12, [3] * 24, True, 4400),
     (192, 8, 24, [90, 300, 65] * 11, [1] * 33, True, 0), (256, 8, 5, [90, 300, 128] * 11, [4, 5, 8] * 11, True, 100),
     (200, 8, 16, [150, 80] * 16, [2] * 32, False, 0)])
-def test_tiles_of_32_rows(ctx, D, Hkv, G, lengths, ns, causal, window):
-    """More than 16 rows of a sequence and head, of bf16, on a full card."""
-    attention_case(ctx, 58, "bf16", D, Hkv * G, Hkv, lengths, ns, causal, window, work=True)
+def test_tiles_of_32_rows(ctx, D, Hkv, G, lengths, ns, causal, window, dtype):
+    """More than 16 rows of a sequence and head on a full card."""
+    attention_case(ctx, 58, dtype, D, Hkv * G, Hkv, lengths, ns, causal, window, work=True)
 
 
-def test_nan_in_tiles_of_32_rows(ctx):
+@pytest.mark.parametrize("dtype,D,Hkv", [("bf16", 64, 16), ("f32", 64, 16), ("bf16", 256, 8), ("f32", 200, 8)])
+def test_nan_in_tiles_of_32_rows(ctx, dtype, D, Hkv):
     """NaN values among drafted tokens reach the rows that see them and no others."""
     r = rng(59)
-    B, Hkv, G, D, n = 40, 16, 4, 64, 6
+    B, G, n = 40, 4, 6
     lengths = [int(x) for x in r.integers(n, 200, B)]
     blocks, tables = K.tables_for(r, lengths)
     cache, ref = K.Cache(ctx, blocks, Hkv, D), O.RefCache(blocks, Hkv, D)
@@ -813,11 +815,12 @@ def test_nan_in_tiles_of_32_rows(ctx):
     bad = [int(x) for x in r.integers(1, n, B)]  # the first of the last n tokens with NaN in dim 3 of its values
     for b in range(B):
         v[cu[b + 1] - n + bad[b], :, 3] = np.nan
-    k, v = S.f32_to_bf16(k), S.f32_to_bf16(v)
+    if dtype == "bf16":
+        k, v = S.f32_to_bf16(k), S.f32_to_bf16(v)
     full = K.Batch(ctx, tables, lengths, cu)
     K.write(cache, full, k, v)
     ref.write(tables, lengths, cu, K.wide(k), K.wide(v))
-    q = make(r, (B * n, Hkv * G, D), "bf16")
+    q = make(r, (B * n, Hkv * G, D), dtype)
     b = K.Batch(ctx, tables, lengths, K.cu_of([n] * B))
     got = K.wide(K.attend(cache, b, q, scale=0.125)).reshape(B, n, Hkv * G, D)
     for i in range(B):
@@ -828,7 +831,8 @@ def test_nan_in_tiles_of_32_rows(ctx):
         mask = O.sees(lengths[i], n, True, 0)
         qi = K.wide(q[i * n:(i + 1) * n])
         want, tol = O.attention(qi, kk, vv, mask, 0.125)
-        tol = tol + BF * O.attention(qi, kk, np.abs(vv), mask, 0.125)[0] + np.abs(want) * BF + 1e-37
+        half = BF if dtype == "bf16" else O.U
+        tol = tol + half * (O.attention(qi, kk, np.abs(vv), mask, 0.125)[0] + np.abs(want)) + 1e-37
         assert (np.abs(got[i] - want) <= tol)[~nan].all()
     for x in (full, b, cache):
         x.free()
