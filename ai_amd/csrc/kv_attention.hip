@@ -521,16 +521,16 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
   if (it.ok && it.chunks > 1 && r < s.n * a.G) join_row<T, 4>(a, s, it, r, r - tile * a.tile, threadIdx.x & 15);
 }
 
-// The kernel for many rows is taken where the work of 16-row tiles, tiles times
-// blocks times slices of 64 dims, is kWideWork or more, and a sequence and head has
-// over 64 rows in bf16, 95 in float32. Less work than that is over before its 128
-// rows and the launch that joins its parts pay. us by it and by the kernel for few
-// rows, with the work: bf16, 128 dims, 8 heads, 8000 tokens, 128 rows 32 and 30 (16 k),
-// 256 rows 39 and 40 (32 k), 512 rows 44 and 56; one head, 30000 tokens, 256 rows 54
-// and 29 (15 k); 64 sequences of 8192, one head, 80 rows 56 and 79 (82 k). float32, 256
-// dims, 16 sequences of 500, 4 heads, 128 rows 52 and 42 (16 k), 256 rows 56 and 88
-// (33 k). At 64 rows the two are within a fifth of each other either way.
-constexpr int kWideWork = 32768;
+// The kernel for many rows is taken where the work in 16-row tiles, tiles times
+// blocks, is kWideWork or more, and a sequence and head has over 64 rows in bf16, 95
+// in float32. Less work than that is over before its 128 rows and the launch that
+// joins its parts pay. us by it and by the kernel for few rows, with the work: bf16,
+// 128 dims, 8 heads, 8000 tokens, 128 rows 32 and 30 (8 k), 256 rows 38 and 39 (16 k),
+// 512 rows 45 and 54 (32 k); one head, 30000 tokens, 256 rows 54 and 29 (7.5 k); 64
+// sequences of 8192, one head, 80 rows 60 and 75 (45 k). float32, 256 dims, 16
+// sequences of 500, 4 heads, 128 rows 52 and 34 (4 k), 512 rows 62 and 131 (16 k). At
+// 64 rows the two are within a fifth of each other either way.
+constexpr int kWideWork = 16384;
 
 // Its tiles are split, in about a part for each workgroup that the card holds, where
 // they are fewer than kWideItems; beyond that, in kWideTarget, where plan_item's rule
@@ -592,7 +592,7 @@ Shape shape_of(const KvAttnArgs& a, int tile = 0) {
   if (!tile) {
     r.tile = kTileRows;
     const int64_t pairs = tiles(kPairRows) * a.c.hkv;
-    if (may_be_wide(a) && tiles(kTileRows) * a.c.hkv * seen(kTileRows) * a.c.nc >= kWideWork)
+    if (may_be_wide(a) && tiles(kTileRows) * a.c.hkv * seen(kTileRows) >= kWideWork)
       r.tile = kWideRows;
     else if (may_be_pairs(a) &&
              (pairs >= 256 * few_per_cu(a.c.nc, 2) || (a.c.nc <= 2 && pairs >= kPairItems &&

@@ -779,11 +779,11 @@ def test_captured_step_replays_with_new_contents(ctx):
 
 
 @pytest.mark.parametrize("dtype,D,H,lengths,ns,window,width", [
-    ("bf16", 64, 16, [2000, 1900, 2048, 70], [128, 100, 128, 70], 0, None),  # long enough to be split
-    ("bf16", 64, 16, [1000, 900, 64, 200], [128, 100, 64, 128], 0, 40),      # only the tables are
-    ("bf16", 64, 16, [2500, 2400, 2048, 2000], [100] * 4, 1700, None),
-    ("f32", 80, 16, [2000, 1900, 2048, 1990], [100] * 4, 0, None),
-    ("f32", 80, 8, [1900], [1900], 0, None),                                  # a prompt: later tiles see more
+    ("bf16", 64, 16, [2000, 1900, 2048, 70], [128, 100, 128, 70], 0, 64),  # long enough to be split
+    ("bf16", 64, 16, [1000, 900, 64, 200], [128, 100, 64, 128], 0, 64),    # only the tables are
+    ("bf16", 64, 16, [2500, 2400, 2048, 2000], [160] * 4, 1700, None),
+    ("f32", 80, 16, [2000, 1900, 2048, 1990], [130] * 4, 0, 64),
+    ("f32", 80, 9, [1900], [1900], 0, None),                               # a prompt: later tiles see more
     ("f32", 80, 8, [1900], [1900], 500, None)])
 def test_tiles_of_many_rows_cut_in_parts(ctx, dtype, D, H, lengths, ns, window, width):
     """128 work items and more of 128 rows, which are cut where the longest sequence is long."""
