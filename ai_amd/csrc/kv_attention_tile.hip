@@ -100,8 +100,8 @@ __device__ __forceinline__ f16x8 widen_f16(uint32_t a, uint32_t b) {
 // convert 2 * 64 * D codes for 32 rows, as many instructions as its softmax),
 // and two such workgroups fit a CU (bf16, up to 128 dims).
 //
-// A prompt of 8192 tokens, 32 heads on 8 of 128 dims in bf16: 519 to 551 us,
-// 1.0 to 1.06 PFLOP/s, where a large matrix product reaches 1.26. Bound by the
+// A prompt of 8192 tokens, 32 heads on 8 of 128 dims in bf16: 519 to 555 us,
+// 0.99 to 1.06 PFLOP/s, where a large matrix product reaches 1.26. Bound by the
 // card's power (1.95 GHz, matrix units busy 0.45 of the time beside softmax and
 // widening: a twelfth fewer vector instructions took as long).
 //
