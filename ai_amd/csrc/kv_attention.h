@@ -231,12 +231,19 @@ __device__ __forceinline__ kvf4 mfma(bf16x8 a, bf16x8 b, kvf4 c) {
 }
 
 // The bf16 terms of eight float32 values as operands: all 24 bits in three
-// (TERMS 3), or rounded to nearest (TERMS 1).
+// (TERMS 3), 17 in two (TERMS 2: the value rounded to nearest and what that
+// leaves, rounded again), or rounded to nearest (TERMS 1).
 template <int TERMS>
 __device__ __forceinline__ void terms_of(const float (&v)[8], bf16x8 (&t)[TERMS]) {
   if constexpr (TERMS == 1) {
 #pragma unroll
     for (int i = 0; i < 8; i++) t[0][i] = (__bf16)v[i];
+  } else if constexpr (TERMS == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      t[0][i] = (__bf16)v[i];
+      t[1][i] = (__bf16)(v[i] - (float)t[0][i]);
+    }
   } else {
     uint32_t w[3][4];
 #pragma unroll

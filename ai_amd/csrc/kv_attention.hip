@@ -13,7 +13,8 @@
 //
 // float32 queries, and the weights for them, enter as three exact bf16 terms
 // (24 bits, the whole range of float32), bf16 queries as they are and their
-// weights rounded to bf16, as many bits as the outputs keep. Scores,
+// weights as two (17 bits: one would put an error of an output's own rounding
+// beside it, relative to the sum of magnitudes and not to the output). Scores,
 // statistics and sums are float32.
 #include <algorithm>
 
@@ -115,6 +116,7 @@ constexpr int few_per_cu(int nc, int rt) { return nc * rt <= 4 ? 2 : 1; }
 // block ahead, 17.7 half a block and two workgroups a CU).
 template <typename T, int TERMS, int NC, int RT>
 __global__ __launch_bounds__(256, few_per_cu(NC, RT)) void kv_attn_kernel(AttnArgs a) {
+  constexpr int WT = TERMS == 3 ? 3 : 2;  // terms of a weight; TERMS: of a query
   constexpr int kRows = 16 * RT;
   constexpr bool AHEAD = NC * RT <= 2;  // loads a block ahead, else half of one
   constexpr int kWaves = 4, kThreads = kWaves * 64;
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(256, few_per_cu(NC, RT)) void kv_attn_kernel(AttnAr
     const float mul = a.scale2 * ks;
     const bool edge = j0 < alo || j0 + 64 > ahi;  // some row does not see some token
     const float f = vs * kWeightScale;
-    bf16x8 pt[RT][2][TERMS];  // weights as operands: two steps of 32 tokens
+    bf16x8 pt[RT][2][WT];  // weights as operands: two steps of 32 tokens
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
       float top = -__builtin_inff();
@@ -333,7 +335,7 @@ __global__ __launch_bounds__(256, few_per_cu(NC, RT)) void kv_attn_kernel(AttnAr
           l[rt] += x;
           w[i] = x * f;
         }
-        terms_of<TERMS>(w, pt[rt][st2]);
+        terms_of<WT>(w, pt[rt][st2]);
       }
     }
     // Tokens that no row of the tile sees may hold anything (a length ends
@@ -371,7 +373,7 @@ __global__ __launch_bounds__(256, few_per_cu(NC, RT)) void kv_attn_kernel(AttnAr
 #pragma unroll
       for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-        for (int k = 0; k < TERMS; k++) {
+        for (int k = 0; k < WT; k++) {
           acc[rt][dt] = mfma(v0, pt[rt][0][k], acc[rt][dt]);
           acc[rt][dt] = mfma(v1, pt[rt][1][k], acc[rt][dt]);
         }

@@ -109,12 +109,14 @@ __device__ __forceinline__ f16x8 widen_f16(uint32_t a, uint32_t b) {
 // to a largest magnitude of 2^13 .. 2^14: 22 bits of a value, or 2^-39 of the row's
 // largest, whichever is coarser (codes are exact in fp16, too). Its weights
 // keep three bf16 terms: with the value scales in them they need float32's range.
+// The weights of bf16 queries are two bf16 terms (17 bits).
 template <typename T, int TERMS, int NC>
 __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(AttnArgs a) {
   constexpr int W = 4, kThreads = W * 64, kRows = W * 32;
   constexpr int KS = NC * 4;            // steps of 16 dims
   constexpr int QT = TERMS == 3 ? 2 : 1;  // terms of a query
   using Op = typename std::conditional<TERMS == 3, f16x8, bf16x8>::type;
+  constexpr int WT = TERMS == 3 ? 3 : 2;  // terms of a weight
   constexpr int DT = NC * 2;            // tiles of 32 dims
   constexpr int kFrag = NC * 512;       // operands of a block's keys; as many of its values
   constexpr int kVals = (NC + 1) / 2;   // a thread's value loads of 2 x 16 codes; NC key loads of 16
@@ -410,12 +412,12 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
             sc[tt][j] = t >= rlo && t < rhi ? sc[tt][j] : -__builtin_inff();
           }
       }
-      // one term: the value scale enters the exponent (down to kLeastFactor:
+      // bf16: the value scale enters the exponent (down to kLeastFactor:
       // below it, weights that count in the row's sum would be lost), and the
       // sum of the scaled weights is scaled back once a block
       const float fe = TERMS == 1 ? (float)((int)(__float_as_uint(fmaxf(f, kLeastFactor)) >> 23) - 127) : 0.f;
       float part;
-      bf16x8 pt[4][TERMS];
+      bf16x8 pt[4][WT];
       auto weights = [&]() {
         const float mu = (m == -__builtin_inff() ? 0.f : m) - fe;
         part = 0.f;
@@ -428,7 +430,7 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
             part += y;
             x[i] = TERMS == 1 ? y : y * f;
           }
-          terms_of<TERMS>(x, pt[k]);
+          terms_of<WT>(x, pt[k]);
         }
         part *= TERMS == 1 ? __builtin_amdgcn_exp2f(-fe) : 1.f;
       };
@@ -456,7 +458,9 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
-          for (int i = 0; i < 8; i++) pt[k][0][i] = (__bf16)((float)pt[k][0][i] * rest);
+          for (int x = 0; x < WT; x++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) pt[k][x][i] = (__bf16)((float)pt[k][x][i] * rest);
       }
 #pragma unroll
       for (int k = 0; k < 4; k++)
@@ -465,12 +469,12 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
           const bf16x8 v0 = __builtin_bit_cast(bf16x8, vf[(k * DT + i) * 64 + lane]);
           const bf16x8 v1 = __builtin_bit_cast(bf16x8, vf[(k * DT + i + 1) * 64 + lane]);
 #pragma unroll
-          for (int x = 0; x < TERMS; x++) {
+          for (int x = 0; x < WT; x++) {
             acc[i] = mfma32(v0, pt[k][x], acc[i]);
             acc[i + 1] = mfma32(v1, pt[k][x], acc[i + 1]);
           }
         }
-      reads_ahead<4 * DT, TERMS>();
+      reads_ahead<4 * DT, WT>();
     }
     __syncthreads();
     ksv = ksv1;
