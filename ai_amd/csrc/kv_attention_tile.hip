@@ -1,7 +1,6 @@
 // Attention over the 8-bit key/value cache for many query rows (prompts and
 // chunks of them).
 #include <atomic>
-#include <type_traits>
 
 #include "kv_attention.h"
 
@@ -69,24 +68,9 @@ __device__ __forceinline__ Item whole_item(const AttnArgs& a, int w, int slots, 
 constexpr int per_cu(int nc, int terms) { return nc <= (terms == 1 ? 2 : 1) ? 2 : 1; }
 
 typedef float kvf16 __attribute__((ext_vector_type(16)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ kvf16 mfma32(bf16x8 a, bf16x8 b, kvf16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-
-__device__ __forceinline__ kvf16 mfma32(f16x8 a, f16x8 b, kvf16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// Eight codes (two dwords) as an fp16 operand.
-__device__ __forceinline__ f16x8 widen_f16(uint32_t a, uint32_t b) {
-  const f16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false);
-  const f16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true);
-  const f16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false);
-  const f16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true);
-  return f16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
 }
 
 // A workgroup of four waves takes 128 query rows of one key/value head, a wave
@@ -105,18 +89,13 @@ __device__ __forceinline__ f16x8 widen_f16(uint32_t a, uint32_t b) {
 // card's power (1.95 GHz, matrix units busy 0.45 of the time beside softmax and
 // widening: a twelfth fewer vector instructions took as long).
 //
-// A float32 query enters as two fp16 terms of its row scaled by a power of two
-// to a largest magnitude of 2^13 .. 2^14: 22 bits of a value, or 2^-39 of the row's
-// largest, whichever is coarser (codes are exact in fp16, too). Its weights
-// keep three bf16 terms: with the value scales in them they need float32's range.
-// The weights of bf16 queries are two bf16 terms (17 bits).
+// Terms as in the kernel for few rows: which of the two a call takes changes no
+// operand's bits.
 template <typename T, int TERMS, int NC>
 __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(AttnArgs a) {
   constexpr int W = 4, kThreads = W * 64, kRows = W * 32;
   constexpr int KS = NC * 4;            // steps of 16 dims
-  constexpr int QT = TERMS == 3 ? 2 : 1;  // terms of a query
-  using Op = typename std::conditional<TERMS == 3, f16x8, bf16x8>::type;
-  constexpr int WT = TERMS == 3 ? 3 : 2;  // terms of a weight
+  constexpr int WT = TERMS == 3 ? 3 : 2;  // terms of a weight; TERMS: of a query
   constexpr int DT = NC * 2;            // tiles of 32 dims
   constexpr int kFrag = NC * 512;       // operands of a block's keys; as many of its values
   constexpr int kVals = (NC + 1) / 2;   // a thread's value loads of 2 x 16 codes; NC key loads of 16
@@ -213,13 +192,8 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
     uint4* to = tile_lds + buf * 2 * kFrag;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
-      if constexpr (TERMS == 3) {
-        to[kto[i]] = __builtin_bit_cast(uint4, widen_f16(kraw[i].x, kraw[i].y));
-        to[kto[i] + 32] = __builtin_bit_cast(uint4, widen_f16(kraw[i].z, kraw[i].w));
-      } else {
-        to[kto[i]] = __builtin_bit_cast(uint4, widen(kraw[i].x, kraw[i].y));
-        to[kto[i] + 32] = __builtin_bit_cast(uint4, widen(kraw[i].z, kraw[i].w));
-      }
+      to[kto[i]] = __builtin_bit_cast(uint4, widen(kraw[i].x, kraw[i].y));
+      to[kto[i] + 32] = __builtin_bit_cast(uint4, widen(kraw[i].z, kraw[i].w));
     }
     const int j0 = p * 64;
     if (j0 < galo || j0 + 64 > gahi) {
@@ -270,42 +244,17 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
   }
 
   // queries as operands, in registers; a negative scale turns their sign
-  Op qf[KS][QT];
-  float back = 1.f;  // what a score is to be multiplied by
+  bf16x8 qf[KS][TERMS];
   {
     const float sign = a.scale2 < 0.f ? -1.f : 1.f;
     const T* p = (const T*)a.q + (s.row0 + tok) * a.q_st + head * a.q_sh;
-    if constexpr (TERMS == 3) {
-      float v[KS][8], top = 0.f;
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
+    for (int k = 0; k < KS; k++) {
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (on) load8(p, k * 16 + half * 8, a.c.D, a.vec, v);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[k][i] = 0.f;
-        if (on) load8(p, k * 16 + half * 8, a.c.D, a.vec, v[k]);
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(v[k][i]));
-      }
-      top = fmaxf(top, lane_xor32(top));
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 14), 254);
-      const float up = sign * __uint_as_float((uint32_t)(267 - e) << 23);  // 2^(140 - e): the row's largest to 2^13 .. 2^14
-      back = __uint_as_float((uint32_t)max(e - 13, 1) << 23);
-#pragma unroll
-      for (int k = 0; k < KS; k++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float y = v[k][i] * up;
-          qf[k][0][i] = (_Float16)y;
-          qf[k][1][i] = (_Float16)(y - (float)qf[k][0][i]);
-        }
-    } else {
-#pragma unroll
-      for (int k = 0; k < KS; k++) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (on) load8(p, k * 16 + half * 8, a.c.D, a.vec, v);
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] *= sign;
-        terms_of<1>(v, qf[k]);
-      }
+      for (int i = 0; i < 8; i++) v[i] *= sign;
+      terms_of<TERMS>(v, qf[k]);
     }
   }
 
@@ -381,15 +330,15 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
         for (int j = 0; j < 16; j++) sc[tt][j] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; k++) {
-        const Op k0 = __builtin_bit_cast(Op, kf[k * 128 + lane]);
-        const Op k1 = __builtin_bit_cast(Op, kf[k * 128 + 64 + lane]);
+        const bf16x8 k0 = __builtin_bit_cast(bf16x8, kf[k * 128 + lane]);
+        const bf16x8 k1 = __builtin_bit_cast(bf16x8, kf[k * 128 + 64 + lane]);
 #pragma unroll
-        for (int x = 0; x < QT; x++) {
+        for (int x = 0; x < TERMS; x++) {
           sc[0] = mfma32(k0, qf[k][x], sc[0]);
           sc[1] = mfma32(k1, qf[k][x], sc[1]);
         }
       }
-      reads_ahead<KS * 2, QT>();
+      reads_ahead<KS * 2, TERMS>();
     }
     if (p + 1 < pg1) {
       stage(buf ^ 1, p + 1);
@@ -401,7 +350,7 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
     }
     if (here) {
       // (not zero: a hidden score is -inf times it)
-      const float mul = fmaxf(fabsf(a.scale2) * ksv.x * back, 0x1p-126f);
+      const float mul = fmaxf(fabsf(a.scale2) * ksv.x, 0x1p-126f);
       const float f = ksv.y * kWeightScale;
       if (j0 < alo || j0 + 64 > ahi) {
 #pragma unroll

@@ -317,9 +317,8 @@ int fa_kv_read_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* bat
  * product with a block's key scale (and a float32 query) has to be in float32's
  * range. out: [rows][heads][head_dim]
  * contiguous, of dtype. Sums, statistics and scores are float32. With float32
- * tensors queries and weights enter the matrix units as three exact bf16 terms
- * (queries of many rows as two fp16 terms of the row scaled by a power of two, 22
- * bits), with bf16 tensors weights as two (17 bits).
+ * tensors queries and weights enter the matrix units as three exact bf16 terms,
+ * with bf16 tensors weights as two (17 bits).
  *
  * work (_dev): scratch of at least fa_kv_attention_work(...) bytes, 16-byte
  * aligned, of any contents, used until the call's work is done: calls that may overlap (graphs

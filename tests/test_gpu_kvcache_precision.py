@@ -3,7 +3,8 @@
 bf16 tensors: outputs are rounded to bf16 once, and nothing before them is. A
 weight enters as two bf16 terms: rounded to bf16 it leaves at most 2^-8 of
 itself, which is rounded again, so it is off by at most 2^-16 of itself, and a
-sum by 2^-16 of sum p |v|; the rest of the bound is float32's (kv_oracle)."""
+sum by 2^-16 of sum p |v|; the rest of the bound is float32's (kv_oracle).
+float32 tensors: three exact bf16 terms of queries and weights, in every kernel."""
 import numpy as np
 import pytest
 
@@ -70,5 +71,53 @@ def test_bf16_value_scales_far_apart(ctx):
             want, tol = O.attention(K.wide(q), wk, wv, mask, 0.125)
             tol = (tol + TWO * O.attention(K.wide(q), wk, np.abs(wv), mask, 0.125)[0]) * (1 + G.BF)
             G.close(got, want, tol, f"value scales, {heads} heads, window {window}")
+    b.free()
+    cache.free()
+
+
+def f32_bound(q, k, v, mask, scale):
+    """The reference's output and float32's bound without any loss of a query's bits: products of three bf16 terms are
+    exact, their sums of 3 D terms and the factors in float32 (as kv_oracle.attention states, whose bound grows with the
+    row's largest query value, too; this one only with the products)."""
+    n, H, D = q.shape
+    q = q.astype(np.float64)
+    with np.errstate(over="ignore"):  # (its bound)
+        out, tol = O.attention(q, k, v, mask, scale)
+        absv = O.attention(q, k, np.abs(v), mask, scale)[0]
+    for h in range(H):
+        kh = np.abs(k[:, h // (H // k.shape[1])])
+        mag = np.where(mask, np.abs(q[:, h]) @ kh.T, 0).max(1) * abs(scale)
+        ds = (3 * D + 4) * O.U * mag
+        rel = np.expm1(2 * ds) + 2.0 ** -22 + 2 * 150 * O.U + (3 * mask.sum(1) + 64) * O.U
+        tol[:, h] = rel[:, None] * absv[:, h]
+    return out, tol
+
+
+@pytest.mark.parametrize("D,H,Hkv,length,n,width", [(64, 2, 1, 200, 5, None), (64, 4, 1, 300, 257, 20000),
+                                                    (128, 2, 2, 300, 300, 20000), (256, 3, 1, 200, 200, 20000)])
+@pytest.mark.parametrize("large", [2.0 ** 30, 2.0 ** -60, 2.0 ** 90])
+def test_f32_queries_keep_their_bits(ctx, D, H, Hkv, length, n, width, large):
+    """A channel of the queries is far from the others and meets zero keys (2^-60: the others do, and it meets ones of
+    2^60): every other channel's 24 bits count, whichever kernel takes the call."""
+    r = G.rng(D + n)
+    blocks, tables = K.tables_for(r, [length], width=width)
+    cache, ref = K.Cache(ctx, blocks, Hkv, D), O.RefCache(blocks, Hkv, D)
+    k, v = G.make(r, (length, Hkv, D), "f32"), G.make(r, (length, Hkv, D), "f32")
+    q = G.make(r, (n, H, D), "f32")
+    if large > 1:
+        q[:, :, 3] *= np.float32(large)
+        k[:, :, 3] = 0
+    else:
+        q[:, :, :4] *= np.float32(large)
+        k[:, :, 4:] = 0
+        k *= np.float32(1 / large)
+    b = K.Batch(ctx, tables, [length], [0, length])
+    K.write(cache, b, k, v)
+    ref.write(tables, [length], [0, length], k, v)
+    b.free()
+    b = K.Batch(ctx, tables, [length], [0, n])
+    got = K.attend(cache, b, q, scale=0.125)
+    want, tol = f32_bound(q, *ref.tokens(tables[0], length), O.sees(length, n, True, 0), 0.125)
+    G.close(got, want, tol, f"D={D} n={n} large={large:g}")
     b.free()
     cache.free()
