@@ -349,8 +349,9 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
       }
     }
     if (here) {
-      // (not zero: a hidden score is -inf times it)
-      const float mul = fmaxf(fabsf(a.scale2) * ksv.x, 0x1p-126f);
+      // (not zero: a hidden score is -inf times it; the smallest float, under
+      // which a product with any other score is 2^-21 at most)
+      const float mul = fmaxf(fabsf(a.scale2) * ksv.x, 0x1p-149f);
       const float f = ksv.y * kWeightScale;
       if (j0 < alo || j0 + 64 > ahi) {
 #pragma unroll

@@ -121,3 +121,28 @@ def test_f32_queries_keep_their_bits(ctx, D, H, Hkv, length, n, width, large):
     G.close(got, want, tol, f"D={D} n={n} large={large:g}")
     b.free()
     cache.free()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n,width", [(5, None), (150, 20000), (150, 1000)])
+def test_scales_near_zero(ctx, dtype, n, width):
+    """Queries of 2^110 and scales down to 0, whose product with a block's key scale is below float32's normal numbers:
+    scores are that product's, in the kernel for many rows too."""
+    r = G.rng(70 + n)
+    D, H, length = 64, 2, 300
+    cache, ref, tables = G.fill(ctx, r, [length], 1, D, dtype, width=width)
+    wk, wv = ref.tokens(tables[0], length)
+    q = G.make(r, (n, H, D), "f32", 2.0 ** 112)
+    q = G.S.f32_to_bf16(q) if dtype == "bf16" else q
+    b = K.Batch(ctx, tables, [length], [0, n])
+    mask = O.sees(length, n, True, 0)
+    for scale in (0.0, 2.0 ** -122, -2.0 ** -120, 1e-45, 2.0 ** -114):
+        got = K.attend(cache, b, q, scale=scale)
+        want, tol = f32_bound(K.wide(q), wk, wv, mask, scale)
+        if dtype == "bf16":
+            tol = (tol + TWO * O.attention(K.wide(q), wk, np.abs(wv), mask, scale)[0]) * (1 + G.BF)
+        if 0 < abs(scale) < 2.0 ** -116:  # a factor with fewer than 24 bits: at most 2^-149 of a product under 2^128
+            tol = tol + 2.0 ** -20 * O.attention(K.wide(q), wk, np.abs(wv), mask, scale)[0]
+        G.close(got, want, tol, f"{dtype} n={n} scale={scale:g}")
+    b.free()
+    cache.free()
