@@ -23,6 +23,12 @@ constexpr float kLeastFactor = 0x1p-64f;
 // The largest sum of a lane's weights in a block, relative to its row's reference.
 constexpr float kMostWeight = 0x1p8f;
 
+// The word of the counters in which the kernel for many rows leaves the blocks
+// of a part for the launch that joins its parts: they come from sums and a
+// threshold in float32, and two kernels need not be compiled to the same
+// rounding. (Few rows count in words below 3080: kTarget and 2 kTarget items + 8.)
+constexpr int kPlanWord = kKvCountBytes / 4 - 1;
+
 // The work of one call: tiles of `tile` rows of a sequence's n * G, for
 // each key/value head, over the blocks they see; in a planned call the blocks
 // are cut into parts of about equal size over the whole batch.
@@ -35,7 +41,7 @@ struct AttnArgs {
   float scale2;  // scale * log2 e
   void* out;
   float* part;    // planned: [parts][tile][Dp] sums, then [parts][tile][2] maximum, sum
-  uint32_t* count;  // planned: per part 0 of a tile, how many of its parts are done
+  uint32_t* count;  // planned: per part 0 of a tile, how many of its parts are done; [kPlanWord]
   int64_t parts;  // parts that the scratch holds
   int32_t tile;   // query rows of a work item
   int32_t target, least, cap;  // planned: parts aimed at, blocks of a part at least
@@ -97,15 +103,11 @@ __device__ __forceinline__ Seen seen_by(const AttnArgs& a, int b) {
 struct Item {
   int b, tile, h, chunk, chunks;
   int64_t first;  // planned: the part of chunk 0
+  int len;        // planned: blocks of a part
   bool ok;
   KvSeq s;  // the sequence's rows and length
 };
 
-// Parts are numbered by sequence, tile, head, chunk. The item of part w, or
-// (w < 0) the first part of the tile and head that are asked for. Every wave
-// finds its own from the lengths, one load for up to 64 sequences (float32
-// sums in a fixed order: the same in every wave).
-//
 // A part has the batch's blocks over a.target, a.least at least; but up to
 // a.cap blocks, as many as leave one part for each CU: a part's beginning (its
 // lengths, its table entries, its first codes, each load after the one before)
@@ -116,9 +118,8 @@ struct Item {
 // not far from full) parts are made only where the longest tile's blocks times
 // the free share of the card are kWideGain or more: a tile counts whole, or less
 // by a.uneven of the part of its sequence that is new, whose tiles see less.
-__device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want_b, int want_tile, int want_h) {
+__device__ __forceinline__ int part_blocks(const AttnArgs& a, const Seen& first) {
   const int lane = threadIdx.x & 63;
-  const Seen first = seen_by(a, lane);
   float total = 0.f, tiles = 0.f, longest = 0.f, busy = 0.f;
   auto count = [&](const Seen& x) {
     const float t = (float)x.tiles, b = (float)x.blocks;
@@ -138,7 +139,20 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want
     busy = wave_sum(busy) * (float)a.c.hkv;
     if (!(wave_max(longest) * (a.places - busy) >= kWideGain * a.places)) chunk = 1 << 30;
   }
-  Item r = {0, 0, 0, 0, 1, 0, false, {0, 0, 0}};
+  return chunk;
+}
+
+// Parts are numbered by sequence, tile, head, chunk. The item of part w, or
+// (w < 0) the first part of the tile and head that are asked for, with parts of
+// `len` blocks as the kernel that wrote them had it. Every wave
+// finds its own from the lengths, one load for up to 64 sequences (float32
+// sums in a fixed order: the same in every wave of a kernel).
+__device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want_b, int want_tile, int want_h,
+                                          int len = 0) {
+  const int lane = threadIdx.x & 63;
+  const Seen first = seen_by(a, lane);
+  const int chunk = w < 0 ? len : part_blocks(a, first);
+  Item r = {0, 0, 0, 0, 1, 0, chunk, false, {0, 0, 0}};
   int64_t before = 0;
   for (int b0 = 0; b0 < a.c.nseq; b0 += 64) {
     const Seen x = b0 ? seen_by(a, b0 + lane) : first;
@@ -176,7 +190,7 @@ __device__ __forceinline__ Item plan_item(const AttnArgs& a, int64_t w, int want
 
 // Unplanned: the slots of sequence b's tiles of `rows` rows start at cu[b] * G / rows + b.
 __device__ __forceinline__ Item direct_item(const AttnArgs& a, int64_t slot, int h, int rows) {
-  Item r = {0, 0, h, 0, 1, 0, false, {0, 0, 0}};
+  Item r = {0, 0, h, 0, 1, 0, 0, false, {0, 0, 0}};
   const int G = a.G;
   auto base = [&](int32_t c, int b) { return (int64_t)((uint32_t)c * (uint32_t)G / (uint32_t)rows) + b; };
   const KvFound f = kv_find(a.c, slot, base);

@@ -519,7 +519,8 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
   if (!t.ok) return;
   const KvSeq s = t.s;
   const int r = t.tile * 16 + (threadIdx.x >> 4), tile = r / a.tile;
-  const Item it = plan_item(a, -1, t.b, tile, t.h);
+  const int len = __builtin_amdgcn_readfirstlane(a.count[kPlanWord]);
+  const Item it = plan_item(a, -1, t.b, tile, t.h, len);
   if (it.ok && it.chunks > 1 && r < s.n * a.G) join_row<T, 4>(a, s, it, r, r - tile * a.tile, threadIdx.x & 15);
 }
 

@@ -54,7 +54,7 @@ __device__ __forceinline__ Item whole_item(const AttnArgs& a, int w, int slots, 
     if (m) before = at;
     else before += __builtin_amdgcn_readlane(incl, 63);
   }
-  Item r = {0, 0, h, 0, 1, 0, false, {0, 0, 0}};
+  Item r = {0, 0, h, 0, 1, 0, 0, false, {0, 0, 0}};
   if (!m) return r;
   const int src = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)m) - 1);
   r.b = src;
@@ -108,6 +108,7 @@ __global__ __launch_bounds__(256, per_cu(NC, TERMS)) void kv_attn_tile_kernel(At
   // are 8 heads or a multiple.
   const Item it = planned ? plan_item(a, (int64_t)gridDim.x - 1 - blockIdx.x, 0, 0, 0)
                           : whole_item(a, blockIdx.x / a.c.hkv, gridDim.x / a.c.hkv, blockIdx.x % a.c.hkv);
+  if (planned && blockIdx.x == 0 && tid == 0) a.count[kPlanWord] = it.len;
   if (!it.ok) return;
   const KvSeq s = it.s;
   const int rows = s.n * a.G, r0 = it.tile * kRows;

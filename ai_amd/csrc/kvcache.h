@@ -45,7 +45,7 @@ struct KvAttnArgs {
   void* out;  // [rows][H][D]
 };
 // Scratch that a call needs (partial results of a split token axis); 0: none.
-// It begins with kKvCountBytes of counters that are zero between calls.
+// It begins with kKvCountBytes of counters that are zero between calls (the last word is no counter).
 constexpr size_t kKvCountBytes = 16384;
 size_t kv_attention_scratch(const KvAttnArgs& a);
 size_t kv_attention_scratch_any(KvAttnArgs a);  // enough for either type, any window, causal or not
