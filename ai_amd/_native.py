@@ -244,6 +244,11 @@ class Context:
 
     def close(self) -> None:
         if self.h:
+            # what is open on it first: a cache's device memory can only be freed through it
+            for r in reversed(_owners):
+                o = r()
+                if getattr(o, "ctx", None) is self:
+                    o.close()
             lib().fa_destroy(self.h)
             self.h = None
 

@@ -77,11 +77,18 @@ class KVCache:
         N.own(self)
 
     def close(self) -> None:
-        """Frees the device memory (also at interpreter exit, and with the context)."""
-        if self._codes and self.ctx.h:
-            N.lib().fa_device_free(self.ctx.h, self._codes)
-            N.lib().fa_device_free(self.ctx.h, self._scales)
-        self._codes = self._scales = N.vp()
+        """Frees the device memory (also when the cache is dropped, with its context, and at interpreter exit)."""
+        codes, scales = self._codes, self._scales
+        self._codes, self._scales = N.vp(), N.vp()
+        if codes and self.ctx.h:
+            N.lib().fa_device_free(self.ctx.h, codes)
+            N.lib().fa_device_free(self.ctx.h, scales)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # (a cache whose constructor raised has nothing to free)
+            pass
 
     def __enter__(self):
         return self
