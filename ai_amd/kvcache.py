@@ -169,15 +169,15 @@ class KVCache:
         if sum(need) > len(self._free):
             _fail(f"Append: {sum(need)} blocks needed, {len(self._free)} free")
         before = {s: self._lengths[s] for s in seqs}
-        for s, c, u in zip(seqs, counts, need):
-            self._tables[s].extend(self._free.pop() for _ in range(u))
-            self._lengths[s] += c
-        batch, keep = self._batch(seqs, counts)
         try:
+            for s, c, u in zip(seqs, counts, need):
+                self._tables[s].extend(self._free.pop() for _ in range(u))
+                self._lengths[s] += c
+            batch, keep = self._batch(seqs, counts)
             _call("KVWrite", self.ctx, N.lib().fa_kv_write(
                 self.ctx.h, N.C.byref(self.cache), N.C.byref(batch), _dtype(k), k.ctypes.data, *_strides(k),
                 v.ctypes.data, *_strides(v)))
-        except Exception:
+        except BaseException:
             for s in reversed(seqs):
                 self.Truncate(s, before[s])
             raise

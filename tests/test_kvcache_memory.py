@@ -82,3 +82,28 @@ def test_a_context_closes_its_caches_first(fake):
     assert not fake.held and [e for e, _ in fake.log].count("free") == 6
     other.close()
     assert [e for e in fake.log if e[0] == "destroy"] == [("destroy", 7), ("destroy", 8)]
+
+
+def test_a_call_that_fails_early_leaves_the_sequences(fake, monkeypatch):
+    """Whatever goes wrong after blocks were handed out, before the library is called or while it runs."""
+    c = M.KVCache(2, 64, 640, ctx=context(7))
+    a, b = c.Add(), c.Add()
+    x = np.zeros((100, 2, 64), np.float32)
+    c.Append([a], x[:70], x[:70], [70])
+
+    def fails(*args):
+        raise error
+
+    for error, name in ((MemoryError(), "_batch"), (KeyboardInterrupt(), "_batch"), (KeyboardInterrupt(), None)):
+        with monkeypatch.context() as m:
+            if name:
+                m.setattr(M.KVCache, name, fails)
+            else:
+                m.setattr(FakeLib, "fa_kv_write", fails)
+            with pytest.raises(type(error)):
+                c.Append([a, b], x, x, [60, 40])
+        assert (c.Len(a), c.Len(b), c.Room()) == (70, 0, 640 - 128)
+    c.Append([a, b], x, x, [60, 40])
+    assert (c.Len(a), c.Len(b), c.Room()) == (130, 40, 640 - 256)
+    c.close()
+    c.ctx.close()
