@@ -24,6 +24,7 @@ from . import _native as N
 from .tensor import TensorError, _call, default_context
 
 BLOCK = N.FA_KV_BLOCK
+_I32 = 2 ** 31 - 1
 
 
 def _fail(msg: str):
@@ -58,7 +59,8 @@ class KVCache:
         self.kv_heads, self.head_dim = int(kv_heads), int(head_dim)
         self.blocks = -(-int(tokens) // BLOCK)
         L = N.lib()
-        size = L.fa_kv_codes_bytes(self.blocks, self.kv_heads, self.head_dim) if self.blocks > 0 else 0
+        sizes = (self.blocks, self.kv_heads, self.head_dim)
+        size = L.fa_kv_codes_bytes(*sizes) if all(0 < x <= _I32 for x in sizes) else 0
         if size == 0:
             _fail(f"{kv_heads} heads of {head_dim} dims for {tokens} tokens")
         self.ctx = ctx or default_context()
@@ -190,12 +192,14 @@ class KVCache:
         seqs = list(seqs)
         q = _rows(q, "Attention", None, self.head_dim)
         counts = self._counts(seqs, len(q), counts, "Attention")
+        if not 0 <= int(window) <= _I32:
+            _fail(f"Attention: window {window}")
         scale = float(np.float32(1.0 / math.sqrt(self.head_dim))) if scale is None else float(scale)
         out = np.empty(q.shape, q.dtype)
         batch, keep = self._batch(seqs, counts)
         _call("KVAttention", self.ctx, N.lib().fa_kv_attention(
             self.ctx.h, N.C.byref(self.cache), N.C.byref(batch), _dtype(q), q.ctypes.data, *_strides(q), q.shape[1],
-            int(causal), int(window), scale, N.ptr(out)))
+            int(bool(causal)), int(window), scale, N.ptr(out)))
         del keep
         return out
 

@@ -107,3 +107,22 @@ def test_a_call_that_fails_early_leaves_the_sequences(fake, monkeypatch):
     assert (c.Len(a), c.Len(b), c.Room()) == (130, 40, 640 - 256)
     c.close()
     c.ctx.close()
+
+
+def test_sizes_past_their_integers_are_refused(fake):
+    """The library takes 32-bit sizes: larger ones are refused, not cut to their low bits."""
+    ctx = context(7)
+    for args in ((2 ** 32 + 2, 64, 640), (2, 2 ** 32 + 64, 640), (2, 64, 2 ** 38 + 64)):
+        with pytest.raises(TensorError):
+            M.KVCache(*args, ctx=ctx)
+    c = M.KVCache(2, 64, 640, ctx=ctx)
+    a = c.Add()
+    k = np.zeros((1, 2, 64), np.float32)
+    c.Append([a], k, k)
+    for window in (2 ** 31, 2 ** 32, -1, -2 ** 32 + 5):
+        with pytest.raises(TensorError, match="window"):
+            c.Attention([a], k, window=window)
+    c.Attention([a], k, window=2 ** 31 - 1)
+    c.close()
+    ctx.close()
+    assert not fake.held
