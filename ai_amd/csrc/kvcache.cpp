@@ -14,13 +14,19 @@ namespace {
 constexpr int64_t kMaxGrid = 0x7FFFFFFF;
 constexpr int32_t kMaxTable = (1 << 25) - 1;  // positions stay below 2^31
 
-int check_cache(fa_ctx* ctx, const char* op, const fa_kv_cache* c) {
+int check_cache_sizes(fa_ctx* ctx, const char* op, const fa_kv_cache* c) {
   if (!c) return set_error(ctx, FA_ERR_ARG, "%s: cache is NULL", op);
   if (c->blocks < 0) return set_error(ctx, FA_ERR_ARG, "%s: %d blocks", op, c->blocks);
   if (c->kv_heads < 1 || c->kv_heads > 65535)
     return set_error(ctx, FA_ERR_ARG, "%s: %d key/value heads outside 1..65535", op, c->kv_heads);
   if (c->head_dim < 1 || c->head_dim > fa::kKvMaxDim)
     return set_error(ctx, FA_ERR_ARG, "%s: head dimension %d outside 1..%d", op, c->head_dim, fa::kKvMaxDim);
+  return FA_OK;
+}
+
+int check_cache(fa_ctx* ctx, const char* op, const fa_kv_cache* c) {
+  const int rc = check_cache_sizes(ctx, op, c);
+  if (rc) return rc;
   if (c->blocks > 0 && (!c->codes || !c->scales)) return set_error(ctx, FA_ERR_ARG, "%s: NULL cache buffer", op);
   if ((reinterpret_cast<uintptr_t>(c->codes) & 15) || (reinterpret_cast<uintptr_t>(c->scales) & 7))
     return set_error(ctx, FA_ERR_ARG, "%s: the cache's codes must be 16-byte and its scales 8-byte aligned", op);
@@ -284,7 +290,7 @@ int fa_kv_attention_work(const fa_kv_cache* cache, const fa_kv_batch* batch, int
   if (!bytes) return set_error(nullptr, FA_ERR_ARG, "KVAttention: bytes is NULL");
   *bytes = 0;
   int rc;
-  if ((rc = check_cache(nullptr, "KVAttention", cache))) return rc;
+  if ((rc = check_cache_sizes(nullptr, "KVAttention", cache))) return rc;
   if (!batch || batch->nseq < 0 || batch->rows < 0 || batch->table_stride < 0 || batch->table_stride > kMaxTable)
     return set_error(nullptr, FA_ERR_ARG, "KVAttention: batch is NULL or has a negative size or too long table rows");
   if (heads < 1 || heads % cache->kv_heads != 0 || heads > 65535)
