@@ -226,6 +226,7 @@ int fa_sync(fa_ctx* ctx) {
 
 int fa_device_alloc(fa_ctx* ctx, size_t bytes, void** out) {
   if (!ctx || !out) return set_error(ctx, FA_ERR_ARG, "fa_device_alloc: NULL argument");
+  FA_HIP_CHECK(ctx, hipSetDevice(ctx->device));  // another context's may be current
   hipError_t e = hipMalloc(out, bytes ? bytes : 1);
   if (e != hipSuccess) return set_error(ctx, FA_ERR_OOM, "hipMalloc(%zu): %s", bytes, hipGetErrorString(e));
   return FA_OK;
