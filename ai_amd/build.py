@@ -42,7 +42,8 @@ ROCM_SOURCES = ["context.cpp", "matmul.cpp", "model.cpp", "plan.cpp", "gemm.hip"
 
 # Products whose accumulators arithmetic reads too (the softmax's scores) stay
 # in the ordinary registers: left to itself the compiler keeps them in the
-# accumulation registers and copies each value there and back.
+# accumulation registers and copies each value there and back. An option of this
+# compiler's own, for speed alone: one that does not know it builds without.
 SOURCE_FLAGS = {"kv_attention_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 
@@ -57,16 +58,26 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(out)
 
 
+def _known(flags: list[str]) -> list[str]:
+    """flags if the compiler takes them, else none."""
+    r = subprocess.run([HIPCC, f"--offload-arch={ARCH}", "-x", "hip", "--cuda-device-only", *flags, "-c", "-o",
+                        os.devnull, os.devnull], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        print(f"built without {' '.join(flags)}: {r.stdout.strip().splitlines()[:1]}", file=sys.stderr, flush=True)
+    return flags if r.returncode == 0 else []
+
+
 def build_rocm(verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIB, exist_ok=True)
     objs = []
     jobs = []
+    extra = {src: _known(flags) for src, flags in SOURCE_FLAGS.items()}
     for src in ROCM_SOURCES:
         obj = os.path.join(BUILD, src.replace(".", "_") + ".o")
         objs.append(obj)
         lang = ["-x", "hip"] if src.endswith(".hip") else []
-        jobs.append([HIPCC, *HIP_FLAGS, *SOURCE_FLAGS.get(src, []), *lang, "-c", os.path.join(CSRC, src), "-o", obj])
+        jobs.append([HIPCC, *HIP_FLAGS, *extra.get(src, []), *lang, "-c", os.path.join(CSRC, src), "-o", obj])
     workers = min(len(jobs), max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(workers) as ex:
         for f in [ex.submit(_run, j, verbose) for j in jobs]:
