@@ -1,5 +1,8 @@
 """The 8-bit key/value cache on the GPU: uses of its calls that go wrong silently where they go wrong."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -119,3 +122,94 @@ def test_row_starts_out_of_order_write_nothing_else(ctx, cu, dtype, width):
             np.testing.assert_array_equal(K.attend(cache, full, q, scale=0.125), before)
     for x in (full, codes, scales):
         x.free()
+
+# ---- many rows under capture -------------------------------------------------------------------
+
+HIP = {"hipStreamBeginCapture": [C.c_void_p, C.c_int], "hipStreamEndCapture": [C.c_void_p, C.POINTER(C.c_void_p)],
+       "hipGraphInstantiate": [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t],
+       "hipGraphLaunch": [C.c_void_p, C.c_void_p], "hipGraphDestroy": [C.c_void_p], "hipGraphExecDestroy": [C.c_void_p]}
+
+
+def captured_chunks(ctx, dtype, D, H, Hkv, width, split):
+    """A step of chunks (written, attended to) captured before any call of its kernels ran, replayed four times with other
+    tokens, lengths, row starts and tables, with eager calls and synchronisation between, against the eager calls."""
+    hip = C.CDLL("libamdhip64.so")
+    for name, types in HIP.items():
+        getattr(hip, name).argtypes = types
+    L, r, rows = N.lib(), G.rng(41), 600
+    plans = [([700, 400], [0, 350, 600]), ([1200, 290], [0, 310, 600]), ([300, 640], [0, 300, 590]),
+             ([64, 1270], [0, 3, 600])]
+    blocks = 2 * width if width < 100 else 60
+    cache = K.Cache(ctx, blocks, Hkv, D, fill=0)
+    b = K.Batch(ctx, np.full((2, width), -1, np.int32), plans[0][0], plans[0][1], rows=rows)
+    like = G.make(r, (1,), dtype)
+    bufs = {n: K.Buf(ctx, nbytes=rows * h * D * like.itemsize, fill=0) for n, h in
+            (("k", Hkv), ("v", Hkv), ("q", H), ("out", H))}
+    need = C.c_size_t(0)
+    N.check(ctx.h, L.fa_kv_attention_work(C.byref(cache.c), C.byref(b.b), H, C.byref(need)))
+    work = K.Buf(ctx, nbytes=need.value, fill=0)
+
+    def step(w, nbytes):
+        N.check(ctx.h, L.fa_kv_write_dev(ctx.h, C.byref(cache.c), C.byref(b.b), K.dt(like), bufs["k"].p, Hkv * D, D,
+                                         bufs["v"].p, Hkv * D, D))
+        N.check(ctx.h, L.fa_kv_attention_dev(ctx.h, C.byref(cache.c), C.byref(b.b), K.dt(like), bufs["q"].p, H * D, D, H,
+                                             1, 0, 0.09, bufs["out"].p, w, nbytes))
+
+    graph, ex = C.c_void_p(), C.c_void_p()
+    ctx.sync()
+    assert hip.hipStreamBeginCapture(ctx.stream, 2) == 0
+    step(work.p, need.value)
+    assert hip.hipStreamEndCapture(ctx.stream, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(ex), graph, None, None, 0) == 0
+    for turn, (lengths, cu) in enumerate(plans):
+        perm, t, at = r.permutation(blocks), np.full((2, width), -1, np.int32), 0
+        for i, length in enumerate(lengths):
+            u = -(-length // 64)
+            t[i, :u] = perm[at:at + u]
+            at += u
+        for x, y in zip(b.bufs, (t, np.array(lengths, np.int32), np.array(cu, np.int32))):
+            x.put(y)
+        for n, h in (("k", Hkv), ("v", Hkv), ("q", H)):
+            bufs[n].put(G.make(r, (rows, h, D), dtype))
+        if turn == 0:  # what the sequences hold before the step
+            for x in (cache.codes, cache.scales):
+                x.put(np.zeros(x.nbytes, np.uint8) if x is cache.codes else np.ones(x.nbytes // 4, np.float32))
+        state = cache.state()
+        bufs["out"].put(np.full(bufs["out"].nbytes, 0x5A, np.uint8))
+        assert hip.hipGraphLaunch(ex, ctx.stream) == 0
+        ctx.sync()
+        got, after = bufs["out"].get((rows, H, D), like.dtype), cache.state()
+        head = work.get((need.value // 4,), np.uint32)[:4096] if need.value else np.zeros(1, np.uint32)
+        assert (head[-1] > 0) == split  # the launch was cut in parts
+        cache.codes.put(state[0])
+        cache.scales.put(state[1])
+        bufs["out"].put(np.full(bufs["out"].nbytes, 0x5A, np.uint8))
+        step(None, 0)
+        ctx.sync()
+        np.testing.assert_array_equal(got.view(np.uint8), bufs["out"].get((rows, H, D), like.dtype).view(np.uint8))
+        for x0, x1 in zip(after, cache.state()):
+            np.testing.assert_array_equal(x0, x1)
+        assert np.isfinite(K.wide(got[:cu[-1]])).all() and (got[cu[-1]:].view(np.uint8) == 0x5A).all()
+    hip.hipGraphExecDestroy(ex)
+    hip.hipGraphDestroy(graph)
+    for x in (*bufs.values(), work, b, cache):
+        x.free()
+
+
+CHUNKS = [("bf16", 128, 8, 2, 200, True), ("f32", 128, 8, 2, 200, True), ("bf16", 64, 32, 32, 20, False),
+          ("f32", 192, 32, 32, 20, False)]
+
+
+@pytest.mark.parametrize("case", CHUNKS)
+def test_captured_chunks_replay_with_new_contents(ctx, case):
+    captured_chunks(ctx, *case)
+
+
+@pytest.mark.parametrize("case", [CHUNKS[0], CHUNKS[3]])
+def test_first_call_of_a_process_is_captured(case):
+    """The kernel's own setting is made where its first call is under capture."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = ("import sys; sys.path[:0] = ['tests', '.']; import test_gpu_kvcache_use as t; from ai_amd import _native as N; "
+            f"t.captured_chunks(N.Context(0), *{case!r}); print('done', flush=True)")
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip() == "done", r.stderr[-2000:]
