@@ -26,8 +26,8 @@ namespace {
 // Two floats of a part, written and read past the caches that XCDs do not
 // share (relaxed atomics of the device's scope): the workgroup that joins a
 // tile's parts may be on another XCD than those that wrote them, and a fence
-// for ordinary stores writes back a whole L2 (with one in each workgroup a
-// step of 16 sequences of 2048 tokens took 81 us instead of 16).
+// for ordinary stores writes back a whole L2 (one in each workgroup made a
+// step of 16 sequences of 2048 tokens 65 us longer).
 __device__ __forceinline__ void put2(float* p, float a, float b) {
   const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -107,13 +107,13 @@ constexpr int few_per_cu(int nc, int rt) { return nc * rt <= 4 ? 2 : 1; }
 // end. A wave loads a block's keys while it works on the scores of the block
 // before, and its values while it works on the next scores, so that about a
 // block (D = 128: 16 KB) is always under way: 64 sequences of up to 8192
-// tokens (606 MB) take 126 us, 4.8 TB/s, against 219 without, and a large copy
+// tokens (606 MB) take 127 us, 4.8 TB/s, against 219 without, and a large copy
 // moves 5.1 TB/s. Where registers for that leave room for fewer workgroups, one
 // set serves both (not AHEAD): a slice's values are loaded where its keys were,
 // the next block's keys where its values were, so half a block is under way
-// (64 sequences of 2000 tokens, 16 heads on 4 of 512 dims: 207 us without, 88;
-// drafts of 2 to 5 tokens on windows of 512, 8 heads on 2 of 256 dims: 19.1 us a
-// block ahead, 17.7 half a block and two workgroups a CU).
+// (64 sequences of 2000 tokens, 16 heads on 4 of 512 dims: 207 us without, 80;
+// drafts of 2 to 5 tokens on windows of 512, 8 heads on 2 of 256 dims: 18.0 us with
+// half a block and two workgroups a CU, 1.4 less than a block ahead).
 template <typename T, int TERMS, int NC, int RT>
 __global__ __launch_bounds__(256, few_per_cu(NC, RT)) void kv_attn_kernel(AttnArgs a) {
   constexpr int WT = TERMS == 3 ? 3 : 2;  // terms of a weight; TERMS: of a query
@@ -526,38 +526,44 @@ __global__ __launch_bounds__(256) void kv_join_kernel(AttnArgs a) {
 
 // The kernel for many rows is taken where the work in 16-row tiles, tiles times
 // blocks, is kWideWork or more, and a sequence and head has over 64 rows in bf16, 95
-// in float32. Less work than that is over before its 128 rows and the launch that
-// joins its parts pay. us by it and by the kernel for few rows, with the work: bf16,
-// 128 dims, 8 heads, 8000 tokens, 128 rows 32 and 30 (8 k), 256 rows 38 and 39 (16 k),
-// 512 rows 45 and 54 (32 k); one head, 30000 tokens, 256 rows 54 and 29 (7.5 k); 64
-// sequences of 8192, one head, 80 rows 60 and 75 (45 k). float32, 256 dims, 16
-// sequences of 500, 4 heads, 128 rows 52 and 34 (4 k), 512 rows 62 and 131 (16 k). At
-// 64 rows the two are within a fifth of each other either way.
+// in float32, in the mean of the batch. Less work than that is over before its 128 rows
+// and the launch that joins its parts pay. us by it and by the kernel for few rows, with
+// the work: bf16, 128 dims, 8 heads, 8000 tokens, 128 rows 32 and 30 (8 k), 256 rows 39
+// and 39 (16 k), 512 rows 49 and 51 (32 k); one head, 30000 tokens, 256 rows 54 and 29
+// (7.5 k); 64 sequences of 8192, one head, 80 rows 61 and 80 (45 k). float32, 256 dims,
+// 16 sequences of 500, 4 heads, 128 rows 57 and 32 (4 k), 500 rows 60 and 116 (16 k). At
+// 64 rows in bf16, 94 in float32, on 64 sequences: of 8192 tokens, one head 55 and 61, of
+// 2000, 4 heads 65 and 48, in float32 103 and 87.
+//
+// One kernel takes the whole call, so sequences of many rows beside others of one have
+// the form that the mean asks for (bf16, 32 heads on 8 of 128 dims, a prompt beside single
+// tokens of 200 to 4000: 2048 tokens and 200 others 269 us, apart 73 and 168; 512 and 64
+// others 67, apart 17 and 38; 512 and 16 others 26, apart 17 and 11).
 constexpr int kWideWork = 16384;
 
 // Its tiles are split, in about a part for each workgroup that the card holds, where
 // they are fewer than kWideItems; beyond that, in kWideTarget, where plan_item's rule
 // finds that a longest tile is long and the card far from full: every row of a part is
 // written, read and joined. Prompts of 8 x 1100 tokens, 139 tiles of float32 rows of
-// 256 dims on up to 18 blocks: 96 us whole, 114 in parts; 2 x 3000, 142 tiles on 47
-// blocks: 209 and 124. In bf16, 512 tokens on 8000, 32 heads on 8 of 128 dims, 136
-// tiles on 125 blocks: 173 and 96; 1536 on 3000, 392 tiles on 47: 86 and 101. Where
+// 256 dims on up to 18 blocks: 99 us whole, 93 in parts; 2 x 3000, 142 tiles on 47
+// blocks: 228 and 126. In bf16, 512 tokens on 8000, 32 heads on 8 of 128 dims, 136
+// tiles on 125 blocks: 224 and 109; 1536 on 3000, 392 tiles on 47: 100 and 120. Where
 // workgroups have a CU each, a prompt's later tiles leave the earlier ones' CUs idle
-// (kUneven: 8 heads on 2 of 256 dims, 4000 tokens, 252 tiles: 171 and 152 us); where
+// (kUneven: 8 heads on 2 of 256 dims, 4000 tokens, 252 tiles: 224 and 176 us); where
 // two share one, the longer has it to itself then (16 on 4 of 128, 4000 tokens,
-// 502 tiles: 104 and 120). Parts of fewer than kWideMin blocks cost more (2 x 3000
-// in float32: 139 us with 8, 124 with 16), and so do more of them than fit at once
-// (512 tokens on 8000, 3 heads on one of 256 dims in float32, 13 tiles: 62 us in 256
+// 502 tiles: 130 and 136). Parts of fewer than kWideMin blocks cost more (2 x 3000
+// in float32: 144 us with 8, 126 with 16), and so do more of them than fit at once
+// (512 tokens on 8000, 3 heads on one of 256 dims in float32, 13 tiles: 64 us in 256
 // parts, 90 in 512).
 constexpr int kWideItems = 128, kWideTarget = 512, kWideMin = 16;
 constexpr float kUneven = 0.4f;
 
 // Tiles of kPairRows rows load and widen a block once for twice the rows: where
 // they still fill the card (64 sequences of up to 8192 tokens, 24 rows on each of 8
-// heads of 128 dims: bf16 260 us in tiles of 16 and 177, float32 279 and 210), or
+// heads of 128 dims: bf16 228 us in tiles of 16 and 152, float32 246 and 176), or
 // are kPairItems and full and see kPairBlocks (64 sequences, 64 rows on one head:
-// 73 and 49; on the other side 16 of 2000 tokens, 32 rows on each of 8: 23 and 28,
-// and 32 of 4000, 20 rows: 53 and 60).
+// 63 and 43; on the other side 16 of 2000 tokens, 32 rows on each of 8: 25 and 29,
+// and 32 of 4000, 20 rows: 53 and 56).
 constexpr int kPairItems = 96, kPairBlocks = 64;
 
 // How a call runs, from its sizes alone.

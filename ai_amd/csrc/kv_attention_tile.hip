@@ -17,8 +17,8 @@ __device__ __forceinline__ uint32_t nan_drop(uint32_t w) {
 
 // Order of N operand reads from LDS and the M products that use each: the
 // reads kAhead products early (left to itself the compiler waits for each
-// pair of reads just before its products: 642 against 562 us for a prompt of
-// 8192 tokens, 32 heads on 8 of 128 dims).
+// pair of reads just before its products: 740 against 721 us for a prompt of
+// 8192 tokens, 308 against 296 for 4 chunks of 512, 32 heads on 8 of 128 dims).
 constexpr int kAhead = 4;
 template <int N, int M>
 __device__ __forceinline__ void reads_ahead() {
@@ -35,7 +35,7 @@ __device__ __forceinline__ void reads_ahead() {
 // most go first, by eighths of the most (finding the exact order takes longer),
 // and of one the later tiles, which see more if it is causal, so that the last
 // tiles to start are short: 4 chunks of 512 tokens on 2979 .. 8704, 32 heads on 8
-// of 128 dims in bf16, take 204 us from the longest down, 227 from the shortest
+// of 128 dims in bf16, take 296 us from the longest down, 323 from the shortest
 // up. Under kSortBlocks in their order; more sequences from the last to the first.
 constexpr int kSortBlocks = 16;
 __device__ __forceinline__ Item whole_item(const AttnArgs& a, int w, int slots, int h) {
@@ -84,10 +84,10 @@ __device__ __forceinline__ kvf16 mfma32(bf16x8 a, bf16x8 b, kvf16 c) {
 // convert 2 * 64 * D codes for 32 rows, as many instructions as its softmax),
 // and two such workgroups fit a CU (bf16, up to 128 dims).
 //
-// A prompt of 8192 tokens, 32 heads on 8 of 128 dims in bf16: 519 to 555 us,
-// 0.99 to 1.06 PFLOP/s, where a large matrix product reaches 1.26. Bound by the
-// card's power (1.95 GHz, matrix units busy 0.45 of the time beside softmax and
-// widening: a twelfth fewer vector instructions took as long).
+// A prompt of 8192 tokens, 32 heads on 8 of 128 dims in bf16: 712 to 727 us, with
+// two terms of the weights 1.13 to 1.16 PFLOP/s of products, where a large matrix
+// product reaches 1.26. Bound by the card's power (1.84 GHz, matrix units busy 0.52
+// of the time beside softmax and widening: a tenth fewer vector instructions took as long).
 //
 // Terms as in the kernel for few rows: which of the two a call takes changes no
 // operand's bits.

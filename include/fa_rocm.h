@@ -318,7 +318,9 @@ int fa_kv_read_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* bat
  * range. out: [rows][heads][head_dim]
  * contiguous, of dtype. Sums, statistics and scores are float32. With float32
  * tensors queries and weights enter the matrix units as three exact bf16 terms,
- * with bf16 tensors weights as two (17 bits).
+ * with bf16 tensors weights as two (17 bits). One kernel serves a call, chosen
+ * from its sizes: many rows of some sequences beside single ones of many others
+ * are often faster as two calls.
  *
  * work (_dev): scratch of at least fa_kv_attention_work(...) bytes, 16-byte
  * aligned, of any contents, used until the call's work is done: calls that may overlap (graphs
