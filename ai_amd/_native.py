@@ -68,6 +68,24 @@ class KvBatch(C.Structure):
                 ("rows", i64)]
 
 
+class KvRope(C.Structure):
+    """fa_kv_rope: rotary positions of keys and queries on the way into the cache."""
+    _fields_ = [("base", f64), ("dims", i32), ("positions", vp)]
+
+
+FA_F8_BLOCK = 128
+
+
+class F8Matrix(C.Structure):
+    """fa_f8_matrix: a matrix in 8 bits in device memory (codes, scale bytes, sizes)."""
+    _fields_ = [("codes", vp), ("scales", vp), ("n", i64), ("k", i64)]
+
+
+class Sampling(C.Structure):
+    """fa_sampling: settings of each row, NULL for the default."""
+    _fields_ = [("temperature", vp), ("top_k", vp), ("top_p", vp), ("min_p", vp)]
+
+
 class GemmaConfig(C.Structure):
     _fields_ = [("hidden_size", i32), ("num_hidden_layers", i32), ("num_attention_heads", i32),
                 ("num_key_value_heads", i32), ("head_dim", i32), ("intermediate_size", i32), ("vocab_size", i32),
@@ -81,6 +99,10 @@ class GemmaConfig(C.Structure):
 
 P_kvc = C.POINTER(KvCache)
 P_kvb = C.POINTER(KvBatch)
+P_kvr = C.POINTER(KvRope)
+P_f8 = C.POINTER(F8Matrix)
+P_epi = C.POINTER(Epilogue)
+P_smp = C.POINTER(Sampling)
 
 _SIGS = {
     "fa_create": (C.c_int, [C.c_int, C.POINTER(vp)]),
@@ -117,6 +139,21 @@ _SIGS = {
     "fa_kv_attention_dev": (C.c_int, [vp, P_kvc, P_kvb, C.c_int, vp, i64, i64, i32, C.c_int, i32, f32, vp, vp,
                                       C.c_size_t]),
     "fa_kv_attention_work": (C.c_int, [P_kvc, P_kvb, i32, C.POINTER(C.c_size_t)]),
+    "fa_kv_write_rope": (C.c_int, [vp, P_kvc, P_kvb, P_kvr, C.c_int, vp, i64, i64, i32, vp, vp, i64, i64, vp, i64, i64]),
+    "fa_kv_write_rope_dev": (C.c_int, [vp, P_kvc, P_kvb, P_kvr, C.c_int, vp, i64, i64, i32, vp, vp, i64, i64, vp, i64,
+                                       i64]),
+    "fa_f8_codes_bytes": (C.c_size_t, [i64, i64]),
+    "fa_f8_scales_bytes": (C.c_size_t, [i64, i64]),
+    "fa_f8_write": (C.c_int, [vp, P_f8, C.c_int, vp, i64]),
+    "fa_f8_write_dev": (C.c_int, [vp, P_f8, C.c_int, vp, i64]),
+    "fa_f8_read": (C.c_int, [vp, P_f8, C.c_int, vp, i64]),
+    "fa_f8_read_dev": (C.c_int, [vp, P_f8, C.c_int, vp, i64]),
+    "fa_matmul_f8": (C.c_int, [vp, i64, C.c_int, vp, i64, P_f8, P_epi, C.c_int, vp, i64]),
+    "fa_matmul_f8_dev": (C.c_int, [vp, i64, C.c_int, vp, i64, P_f8, P_epi, C.c_int, vp, i64, vp, C.c_size_t]),
+    "fa_matmul_f8_work": (C.c_int, [i64, P_f8, C.POINTER(C.c_size_t)]),
+    "fa_sample": (C.c_int, [vp, i64, i64, C.c_int, vp, i64, P_smp, vp, vp, vp]),
+    "fa_sample_dev": (C.c_int, [vp, i64, i64, C.c_int, vp, i64, P_smp, vp, vp, vp, vp, C.c_size_t]),
+    "fa_sample_work": (C.c_int, [i64, i64, C.POINTER(C.c_size_t)]),
     "fa_similarities_topk": (C.c_int, [vp, vp, i64, vp, i64, i32, i32, vp, vp]),
     "fa_similarities_topk_dev": (C.c_int, [vp, vp, i64, vp, i64, i32, i32, vp, vp]),
     "fa_similarities_topk_dev_noalloc": (C.c_int, [vp, vp, i64, vp, i64, i32, i32, vp, vp]),

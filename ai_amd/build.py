@@ -38,7 +38,8 @@ HIP_FLAGS = [
 ]
 
 ROCM_SOURCES = ["context.cpp", "matmul.cpp", "model.cpp", "plan.cpp", "gemm.hip", "gemm_h2.hip", "rowops.hip", "attention.hip", "attention_split.hip", "score.hip", "score_few.hip", "cluster.hip",
-                "kvcache.cpp", "kvcache.hip", "kv_attention.hip", "kv_attention_tile.hip"]
+                "kvcache.cpp", "kvcache.hip", "kv_attention.hip", "kv_attention_tile.hip", "f8.cpp", "f8.hip",
+                "sample.cpp", "sample.hip"]
 
 # Products whose accumulators arithmetic reads too (the softmax's scores) stay
 # in the ordinary registers: left to itself the compiler keeps them in the

@@ -60,6 +60,9 @@ enum : size_t {
   S_ATTN,                               // key and value images (attention drop-in)
   S_KV,                                 // batch arrays of the key/value cache's host entry points
   S_KV_PARTS,                           // parts of a split token axis (attention over the cache)
+  S_F8,                                 // quantised left operand (products with 8-bit weights)
+  S_SAMPLE,                             // a row's state between launches (sampling)
+  S_SAMPLE_IN,                          // settings and numbers of sampling's host entry point
   S_COUNT
 };
 }  // namespace slots

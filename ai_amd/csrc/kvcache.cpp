@@ -180,9 +180,8 @@ int attn_args(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, i
   return check_grid(ctx, op, fa::kv_attention_grid(*a));
 }
 
-int write_check(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, const void* k,
-                int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh) {
-  const char* op = "KVWrite";
+int write_check(fa_ctx* ctx, const char* op, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype,
+                const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh) {
   int rc;
   if ((rc = check_cache(ctx, op, cache)) || (rc = check_batch(ctx, op, batch, dtype)) ||
       (rc = check_strides(ctx, op, batch->rows, cache->kv_heads, k_st, k_sh)) ||
@@ -190,6 +189,46 @@ int write_check(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch,
       (rc = check_sizes(ctx, op, batch, cache->kv_heads)) || (rc = check_grid(ctx, op, fa::kv_grid(args_of(cache, batch)))))
     return rc;
   if (batch->rows > 0 && batch->nseq > 0 && (!k || !v)) return set_error(ctx, FA_ERR_ARG, "%s: NULL buffer", op);
+  return FA_OK;
+}
+
+int rope_check(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, const fa_kv_rope* rope, int dtype,
+               const void* q, int64_t q_st, int64_t q_sh, int32_t heads, const void* q_out, const void* k, int64_t k_st,
+               int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, fa::KvRopeArgs* r) {
+  const char* op = "KVWriteRoPE";
+  int rc;
+  if ((rc = write_check(ctx, op, cache, batch, dtype, k, k_st, k_sh, v, v_st, v_sh))) return rc;
+  if (!rope) return set_error(ctx, FA_ERR_ARG, "%s: rope is NULL", op);
+  if (!(rope->base > 0) || !std::isfinite(rope->base))
+    return set_error(ctx, FA_ERR_ARG, "%s: base %g is not finite and above 0", op, rope->base);
+  if (rope->dims < 2 || rope->dims % 2 != 0 || rope->dims > cache->head_dim)
+    return set_error(ctx, FA_ERR_ARG, "%s: %d rotary dims of %d, not even or outside 2..%d", op, rope->dims,
+                     cache->head_dim, cache->head_dim);
+  if (heads < 0 || heads % cache->kv_heads != 0)
+    return set_error(ctx, FA_ERR_ARG, "%s: %d query heads on %d key/value heads", op, heads, cache->kv_heads);
+  if ((int64_t)heads + 2 * cache->kv_heads > 65535)
+    return set_error(ctx, FA_ERR_ARG, "%s: %d query and %d key/value heads are more than one call takes", op, heads,
+                     cache->kv_heads);
+  if (heads > 0 && ((rc = check_strides(ctx, op, batch->rows, heads, q_st, q_sh)) ||
+                    (rc = check_sizes(ctx, op, batch, heads))))
+    return rc;
+  const bool some = batch->rows > 0 && batch->nseq > 0;
+  if (some && heads > 0 && (!q || !q_out)) return set_error(ctx, FA_ERR_ARG, "%s: NULL buffer", op);
+  if (heads == 0 && (q || q_out)) return set_error(ctx, FA_ERR_ARG, "%s: queries of no heads", op);
+  r->q = q;
+  r->q_st = q_st;
+  r->q_sh = q_sh;
+  r->H = heads;
+  r->q_out = const_cast<void*>(q_out);
+  r->k = k;
+  r->k_st = k_st;
+  r->k_sh = k_sh;
+  r->v = v;
+  r->v_st = v_st;
+  r->v_sh = v_sh;
+  r->positions = rope->positions;
+  r->half = rope->dims / 2;
+  for (int i = 0; i < r->half; i++) r->inv[i] = std::pow(rope->base, -(double)(2 * i) / (double)rope->dims);
   return FA_OK;
 }
 
@@ -231,7 +270,7 @@ size_t fa_kv_codes_bytes(int32_t blocks, int32_t kv_heads, int32_t head_dim) {
 
 int fa_kv_write_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, const void* k,
                     int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh) {
-  int rc = write_check(ctx, cache, batch, dtype, k, k_st, k_sh, v, v_st, v_sh);
+  int rc = write_check(ctx, "KVWrite", cache, batch, dtype, k, k_st, k_sh, v, v_st, v_sh);
   if (rc || (rc = need_ctx(ctx, "KVWrite")) || nothing(batch)) return rc;
   FA_HIP_CHECK(ctx, hipSetDevice(ctx->device));
   return fa::launch_kv_write(ctx, args_of(cache, batch), dtype, k, k_st, k_sh, v, v_st, v_sh, ctx->stream);
@@ -239,7 +278,7 @@ int fa_kv_write_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* ba
 
 int fa_kv_write(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, int dtype, const void* k,
                 int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh) {
-  int rc = write_check(ctx, cache, batch, dtype, k, k_st, k_sh, v, v_st, v_sh);
+  int rc = write_check(ctx, "KVWrite", cache, batch, dtype, k, k_st, k_sh, v, v_st, v_sh);
   if (rc || (rc = check_host_batch(ctx, "KVWrite", cache, batch, Use::Write)) || (rc = need_ctx(ctx, "KVWrite")) ||
       nothing(batch))
     return rc;
@@ -254,6 +293,51 @@ int fa_kv_write(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch,
   if ((rc = fa::stage_h2d(ctx, S_V, v, span(rows, cache->kv_heads, v_st, v_sh, cache->head_dim, dtype), &dv))) return rc;
   if ((rc = fa::launch_kv_write(ctx, args_of(cache, &dev), dtype, dk, k_st, k_sh, dv, v_st, v_sh, ctx->stream)))
     return rc;
+  FA_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
+  return FA_OK;
+}
+
+int fa_kv_write_rope_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, const fa_kv_rope* rope,
+                         int dtype, const void* q, int64_t q_st, int64_t q_sh, int32_t heads, void* q_out,
+                         const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh) {
+  fa::KvRopeArgs r;
+  int rc = rope_check(ctx, cache, batch, rope, dtype, q, q_st, q_sh, heads, q_out, k, k_st, k_sh, v, v_st, v_sh, &r);
+  if (rc || (rc = need_ctx(ctx, "KVWriteRoPE")) || nothing(batch)) return rc;
+  FA_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+  return fa::launch_kv_write_rope(ctx, args_of(cache, batch), dtype, r, ctx->stream);
+}
+
+int fa_kv_write_rope(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, const fa_kv_rope* rope, int dtype,
+                     const void* q, int64_t q_st, int64_t q_sh, int32_t heads, void* q_out, const void* k, int64_t k_st,
+                     int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh) {
+  const char* op = "KVWriteRoPE";
+  fa::KvRopeArgs r;
+  int rc = rope_check(ctx, cache, batch, rope, dtype, q, q_st, q_sh, heads, q_out, k, k_st, k_sh, v, v_st, v_sh, &r);
+  if (rc || (rc = check_host_batch(ctx, op, cache, batch, Use::Write)) || (rc = need_ctx(ctx, op)) || nothing(batch))
+    return rc;
+  const int64_t rows = batch->cu_rows[batch->nseq];
+  if (rows == 0) return FA_OK;
+  if ((rc = fa::refuse_capture(ctx, ctx->stream, op))) return rc;
+  FA_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+  fa_kv_batch dev;
+  void *dk, *dv, *dq = nullptr, *dp = nullptr;
+  const int32_t D = cache->head_dim;
+  if ((rc = stage_batch(ctx, batch, &dev))) return rc;
+  if ((rc = fa::stage_h2d(ctx, S_K, k, span(rows, cache->kv_heads, k_st, k_sh, D, dtype), &dk))) return rc;
+  if ((rc = fa::stage_h2d(ctx, S_V, v, span(rows, cache->kv_heads, v_st, v_sh, D, dtype), &dv))) return rc;
+  const size_t q_bytes = (size_t)rows * heads * D * elem(dtype);
+  if (heads > 0) {
+    if ((rc = fa::stage_h2d(ctx, S_Q, q, span(rows, heads, q_st, q_sh, D, dtype), &dq))) return rc;
+    if ((rc = ctx->slot(S_OUT).ensure(ctx, q_bytes))) return rc;
+    r.q_out = ctx->slot(S_OUT).ptr;
+  }
+  if (rope->positions && (rc = fa::stage_h2d(ctx, S_MASK, rope->positions, (size_t)rows * 4, &dp))) return rc;
+  r.q = dq;
+  r.k = dk;
+  r.v = dv;
+  r.positions = static_cast<const int32_t*>(dp);
+  if ((rc = fa::launch_kv_write_rope(ctx, args_of(cache, &dev), dtype, r, ctx->stream))) return rc;
+  if (heads > 0) FA_HIP_CHECK(ctx, hipMemcpyAsync(q_out, r.q_out, q_bytes, hipMemcpyDeviceToHost, ctx->stream));
   FA_HIP_CHECK(ctx, hipStreamSynchronize(ctx->stream));
   return FA_OK;
 }

@@ -1,17 +1,13 @@
 // The key/value cache in 8 bits: what its translation units share.
 #pragma once
 
+#include "e4m3.h"
 #include "fa_internal.h"
 
 namespace fa {
 
 constexpr int kKvBlock = FA_KV_BLOCK;  // tokens of a block, and of a scale
 constexpr int kKvMaxDim = 512;
-// Scale exponents. Above: the largest a finite float32 needs. Below: a
-// block whose largest magnitude is under 448 * 2^-80 (4e-22) keeps the
-// scale 2^-80, so that a scale times a softmax weight stays far from
-// float32's subnormals in attention.
-constexpr int kKvMinExp = -80, kKvMaxExp = 120;
 
 // Head dims as stored: whole slices of 64.
 inline int kv_slices(int head_dim) { return (head_dim + 63) / 64; }
@@ -31,6 +27,23 @@ struct KvArgs {
 
 int launch_kv_write(fa_ctx* ctx, const KvArgs& a, int dtype, const void* k, int64_t k_st, int64_t k_sh, const void* v,
                     int64_t v_st, int64_t v_sh, hipStream_t s);
+// fa_kv_write_rope: pair i < half of a head's first 2 * half dims turns by
+// position * inv[i].
+constexpr int kKvMaxPairs = kKvMaxDim / 2;
+struct KvRopeArgs {
+  const void* q;  // null: no queries
+  int64_t q_st, q_sh;
+  int32_t H;
+  void* q_out;  // [rows][H][D]
+  const void* k;
+  int64_t k_st, k_sh;
+  const void* v;
+  int64_t v_st, v_sh;
+  const int32_t* positions;  // null: a token's place in its sequence
+  int32_t half;
+  double inv[kKvMaxPairs];
+};
+int launch_kv_write_rope(fa_ctx* ctx, const KvArgs& a, int dtype, const KvRopeArgs& r, hipStream_t s);
 int64_t kv_grid(const KvArgs& a);  // workgroups of both along a grid's x
 int launch_kv_read(fa_ctx* ctx, const KvArgs& a, int dtype, void* k, void* v, hipStream_t s);
 

@@ -68,58 +68,17 @@ __device__ __forceinline__ KvUnit kv_unit(const KvArgs& a, int64_t u, bool by_ro
   return r;
 }
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
-
-// Four neighbouring values of a row, those past D as zeros. vec: the row
-// starts are aligned for one load.
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p, int d, int D, bool vec) {
-  f32x4 r = {0.f, 0.f, 0.f, 0.f};
-  if (vec && d + 4 <= D) {
-    if constexpr (sizeof(T) == 4) {
-      r = *reinterpret_cast<const f32x4*>(p + d);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(p + d);
-      r = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
-                __uint_as_float(w.y & 0xFFFF0000u)};
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (d + i < D) r[i] = to_f32(p[d + i]);
-  }
-  return r;
-}
-
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
-}
-__device__ __forceinline__ f32x4 unpack4(uint32_t w) {
-  auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-  auto b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  return f32x4{a[0], a[1], b[0], b[1]};
-}
 // Each code times 2^sh (sh <= 0), rounded to a code again.
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float f) {
   const f32x4 v = unpack4(w);
   return pack4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
 }
 
-// The smallest e with a <= 448 * 2^e (448 = 1.75 * 2^8), from a's bits.
-__device__ __forceinline__ int scale_exp(float a) {
-  const uint32_t u = __float_as_uint(a);
-  const int e = (int)(u >> 23) - 135 + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  return min(max(e, kKvMinExp), kKvMaxExp);
-}
 // The exponent of a stored scale (whatever the bits, a valid one).
 __device__ __forceinline__ int stored_exp(float s) {
   const int e = (int)((__float_as_uint(s) >> 23) & 255u) - 127;
-  return min(max(e, kKvMinExp), kKvMaxExp);
+  return min(max(e, kMinExp), kMaxExp);
 }
-__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-
 // A thread's share of a 64 x 64 slice: the tokens 16 a + 4 b + 0..3 and dims
 // 4 dq + 0..3, with dq = tid & 15, a = (tid >> 4) & 3, b = tid >> 6. A
 // wave's loads cover 256 (float32) or 128 (bf16) bytes of each of four
@@ -134,21 +93,13 @@ __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float((uint3
 // nothing of the next under way. Single tokens are bound by that chain and the
 // write-back of the 128 lines that one token's values touch in a head (64 sequences,
 // one float32 token each, written 7.1 us).
-template <typename T, int NCM>
-__global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __restrict__ k, int64_t k_st, int64_t k_sh,
-                                                       const T* __restrict__ v, int64_t v_st, int64_t v_sh,
-                                                       bool by_row, bool vec) {
+// load(row, d): four values of the part from dim d on in row `row`, zeros past D.
+template <int NCM, typename F>
+__device__ __forceinline__ void write_block(const KvArgs& a, const KvUnit& u, int id, int h, int part, F load) {
   __shared__ float red[4];
   __shared__ uint32_t tile[64 * 17];
-  const KvUnit u = kv_unit(a, blockIdx.x, by_row);
-  if (!u.ok) return;
-  const int id = kv_block(a, u.b, u.slot);
-  if (id < 0) return;
-  const int h = blockIdx.y, part = blockIdx.z;
   const int tid = threadIdx.x, dq = tid & 15, ta = (tid >> 4) & 3, tb = tid >> 6;
   const int t0 = ta * 16 + tb * 4;
-  const T* src = part ? v : k;
-  const int64_t st = part ? v_st : k_st, sh = part ? v_sh : k_sh;
   const int end = u.place + u.n;
   f32x4 x[NCM][4];
   float big = 0.f;
@@ -159,8 +110,7 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
       for (int i = 0; i < 4; i++) {
         const int t = t0 + i;
         x[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (t >= u.place && t < end)
-          x[c][i] = load4(src + (u.row + (t - u.place)) * st + h * sh, c * 64 + dq * 4, a.D, vec);
+        if (t >= u.place && t < end) x[c][i] = load(u.row + (t - u.place), c * 64 + dq * 4);
       }
 #pragma unroll
   for (int c = 0; c < NCM; c++)
@@ -169,15 +119,15 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
       for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          const float y = fabsf(x[c][i][j]);
-          if (y < __builtin_inff()) big = fmaxf(big, y);
-          else x[c][i][j] = __builtin_nanf("");  // not finite: stored as NaN
+          float y = x[c][i][j];
+          join_max(y, big);  // not finite: stored as NaN
+          x[c][i][j] = y;
         }
   uint8_t* dst = kv_part(a, id, h, part);
   const bool whole = u.place == 0 && end == 64;
   float* scale = a.scales + ((int64_t)id * a.hkv + h) * 2 + part;
   const bool keep = u.place > 0;  // tokens below the first new one stay
-  const int e_old = keep ? stored_exp(*scale) : kKvMinExp;
+  const int e_old = keep ? stored_exp(*scale) : kMinExp;
   big = wave_max(big);
   if ((tid & 63) == 0) red[tid >> 6] = big;
   __syncthreads();
@@ -186,16 +136,14 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
   const int e = max(e_new, e_old);
   const bool grow = keep && e > e_old;
   const float inv = exp2_int(-e), shrink = exp2_int(max(e_old - e, -126));
-  if (e == kKvMaxExp) {  // 256 * 2^120 and above would be read back as infinite
+  if (e == kMaxExp) {  // 256 * 2^120 and above would be read back as infinite
 #pragma unroll
     for (int c = 0; c < NCM; c++)
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float y = x[c][i][j], top = 240.f * exp2_int(kKvMaxExp);
-          if (c < a.nc) x[c][i][j] = y > top ? top : y < -top ? -top : y;
-        }
+        for (int j = 0; j < 4; j++)
+          if (c < a.nc) x[c][i][j] = clamp_top(x[c][i][j]);
   }
   if (tid == 0) *scale = exp2_int(e);  // (every thread read the old one before the maximum was joined)
   if (part == 1 && u.n <= 8 && !grow) {
@@ -263,28 +211,84 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
   }
 }
 
-__device__ __forceinline__ void store4(float* p, int d, int D, bool vec, const f32x4& v) {
-  if (vec && d + 4 <= D) {
-    *reinterpret_cast<f32x4*>(p + d) = v;
-  } else {
+template <typename T, int NCM>
+__global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __restrict__ k, int64_t k_st, int64_t k_sh,
+                                                       const T* __restrict__ v, int64_t v_st, int64_t v_sh,
+                                                       bool by_row, bool vec) {
+  const KvUnit u = kv_unit(a, blockIdx.x, by_row);
+  if (!u.ok) return;
+  const int id = kv_block(a, u.b, u.slot);
+  if (id < 0) return;
+  const int h = blockIdx.y, part = blockIdx.z;
+  const T* src = part ? v : k;
+  const int64_t st = part ? v_st : k_st, sh = part ? v_sh : k_sh;
+  write_block<NCM>(a, u, id, h, part, [&](int64_t row, int d) { return load4(src + row * st + h * sh, d, a.D, vec); });
+}
+
+// Four values of a head from dim d on, turned: dim i < half of the first 2 *
+// half becomes x_i cos - x_{i + half} sin, dim i + half x_{i + half} cos + x_i
+// sin, the angle position * inv_i in float64, cos and sin rounded to float32 (as
+// fa_rope's tables), the products exact in float64.
+template <typename T>
+__device__ __forceinline__ f32x4 load_turned(const KvRopeArgs& r, const T* p, int64_t position, int d, int D, bool vec) {
+  f32x4 x = load4(p, d, D, vec);
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (d + i < D) p[d + i] = v[i];
+  for (int j = 0; j < 4; j++) {
+    const int i = d + j;
+    if (i >= 2 * r.half) continue;
+    const bool up = i >= r.half;
+    const int pair = up ? i - r.half : i;
+    double sn, cs;
+    sincos((double)position * r.inv[pair], &sn, &cs);
+    const double c = (double)(float)cs, s = (double)(float)sn;
+    const double other = (double)to_f32(p[up ? pair : i + r.half]);
+    x[j] = (float)((double)x[j] * c + (up ? other : -other) * s);
   }
+  return x;
 }
-__device__ __forceinline__ uint16_t bf16_bits(float v) {
-  return __builtin_bit_cast(uint16_t, (__bf16)v);  // to nearest, ties to even
-}
-__device__ __forceinline__ void store4(uint16_t* p, int d, int D, bool vec, const f32x4& v) {
-  uint16_t b[4];
+
+template <typename T, int NCM>
+__global__ __launch_bounds__(256) void kv_write_rope_kernel(KvArgs a, KvRopeArgs r, bool by_row, bool vec) {
+  const KvUnit u = kv_unit(a, blockIdx.x, by_row);
+  if (!u.ok) return;
+  const int64_t first = u.slot * 64 + u.place;  // position of the unit's first row in its sequence
+  auto position = [&](int64_t row) { return r.positions ? (int64_t)r.positions[row] : first + (row - u.row); };
+  const int job = blockIdx.y;
+  if (job < 2 * a.hkv) {
+    const int id = kv_block(a, u.b, u.slot);
+    if (id < 0) return;
+    const int h = job >> 1, part = job & 1;
+    write_block<NCM>(a, u, id, h, part, [&](int64_t row, int d) {
+      if (part) return load4((const T*)r.v + row * r.v_st + h * r.v_sh, d, a.D, vec);
+      return load_turned(r, (const T*)r.k + row * r.k_st + h * r.k_sh, position(row), d, a.D, vec);
+    });
+    return;
+  }
+  // queries: a thread turns whole pairs, so that q_out may be q
+  const int h = job - 2 * a.hkv;
+  const int pairs = (r.half + 3) / 4, words = pairs + (a.D - 2 * r.half + 3) / 4;
+  const bool vec2 = vec && r.half % 4 == 0, vec_out = vec && a.D % 4 == 0;
+  for (int i = threadIdx.x; i < u.n * words; i += 256) {
+    const int64_t row = u.row + i / words;
+    const int w = i % words;
+    const T* p = (const T*)r.q + row * r.q_st + h * r.q_sh;
+    T* o = (T*)r.q_out + (row * r.H + h) * a.D;
+    if (w >= pairs) {
+      const int d = 2 * r.half + (w - pairs) * 4;
+      store4(o, d, a.D, vec_out && r.half % 2 == 0, load4(p, d, a.D, vec && r.half % 2 == 0));
+      continue;
+    }
+    f32x4 lo = load4(p, w * 4, r.half, vec), hi = load4(p + r.half, w * 4, r.half, vec2);
 #pragma unroll
-  for (int i = 0; i < 4; i++) b[i] = bf16_bits(v[i]);
-  if (vec && d + 4 <= D) {
-    *reinterpret_cast<uint2*>(p + d) = make_uint2(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (d + i < D) p[d + i] = b[i];
+    for (int j = 0; j < 4; j++) {
+      double sn, cs;
+      sincos((double)position(row) * r.inv[min(w * 4 + j, r.half - 1)], &sn, &cs);
+      const double c = (double)(float)cs, s = (double)(float)sn, x = (double)lo[j], y = (double)hi[j];
+      lo[j] = (float)(x * c - y * s);
+      hi[j] = (float)(y * c + x * s);
+    }
+    store4(o, w * 4, r.half, vec_out, lo);
+    store4(o + r.half, w * 4, r.half, vec_out && vec2, hi);
   }
 }
 
@@ -361,7 +365,27 @@ int write_t(fa_ctx* ctx, const KvArgs& a, const void* k, int64_t k_st, int64_t k
   return FA_OK;
 }
 
+template <typename T>
+int write_rope_t(fa_ctx* ctx, const KvArgs& a, const KvRopeArgs& r, hipStream_t s) {
+  bool by_row;
+  const int64_t units = kv_units(a.rows, a.nseq, &by_row);
+  const size_t al = 4 * sizeof(T);
+  const bool vec = aligned(r.k, al) && aligned(r.v, al) && (r.k_st | r.k_sh | r.v_st | r.v_sh) % 4 == 0 &&
+                   (!r.q || (aligned(r.q, al) && aligned(r.q_out, al) && (r.q_st | r.q_sh) % 4 == 0));
+  const dim3 grid((unsigned)units, (unsigned)(2 * a.hkv + r.H));
+  if (a.nc <= 1) kv_write_rope_kernel<T, 1><<<grid, 256, 0, s>>>(a, r, by_row, vec);
+  else if (a.nc <= 2) kv_write_rope_kernel<T, 2><<<grid, 256, 0, s>>>(a, r, by_row, vec);
+  else if (a.nc <= 4) kv_write_rope_kernel<T, 4><<<grid, 256, 0, s>>>(a, r, by_row, vec);
+  else kv_write_rope_kernel<T, 8><<<grid, 256, 0, s>>>(a, r, by_row, vec);
+  FA_CHECK_LAUNCH(ctx);
+  return FA_OK;
+}
+
 }  // namespace
+
+int launch_kv_write_rope(fa_ctx* ctx, const KvArgs& a, int dtype, const KvRopeArgs& r, hipStream_t s) {
+  return dtype == FA_DT_F32 ? write_rope_t<float>(ctx, a, r, s) : write_rope_t<uint16_t>(ctx, a, r, s);
+}
 
 int64_t kv_grid(const KvArgs& a) {
   bool by_row;

@@ -13,6 +13,7 @@ there is no CPU fallback. A shape error raises tensor.TensorError.
     out = cache.Attention([seq], q, [len(q)])        # and its queries
     cache.Append([seq], k1, v1)                      # the next token
     out1 = cache.Attention([seq], q1)
+    q2 = cache.AppendRoPE([seq], q2, k2, v2, base=1e6)  # rotary positions on the way
 """
 from __future__ import annotations
 
@@ -160,25 +161,63 @@ class KVCache:
 
     def Append(self, seqs, k, v, counts=None) -> None:
         """Adds k and v [rows, kv_heads, head_dim], counts[i] rows to sequence seqs[i] (one each by default)."""
+        self._append("Append", seqs, k, v, counts, lambda batch, k, v: _call("KVWrite", self.ctx, N.lib().fa_kv_write(
+            self.ctx.h, N.C.byref(self.cache), N.C.byref(batch), _dtype(k), k.ctypes.data, *_strides(k), v.ctypes.data,
+            *_strides(v))))
+
+    def AppendRoPE(self, seqs, q, k, v, counts=None, *, base: float, dims: int | None = None,
+                   positions=None) -> np.ndarray | None:
+        """Append with rotary positions (tensor.RoPE's, of the first dims dims of a head; all by default) on the way:
+        keys are rotated and added, the queries q [rows, heads, head_dim] (or None) rotated and returned. positions
+        [rows]: a token's place in its sequence by default."""
+        what = "AppendRoPE"
+        dims = self.head_dim if dims is None else int(dims)
+        if not -_I32 <= dims <= _I32:
+            _fail(f"{what}: {dims} rotary dims")
+        rows = len(np.asarray(k))
+        if q is not None:
+            q = _rows(q, what, None, self.head_dim)
+            if len(q) != rows:
+                _fail(f"{what}: {len(q)} queries for {rows} keys")
+        if positions is not None:
+            positions = np.asarray(positions)
+            if positions.shape != (rows,) or (rows and (positions.dtype.kind not in "iu" or positions.min() < -_I32 or
+                                                        positions.max() > _I32)):
+                _fail(f"{what}: want {rows} positions in 32 bits, got {list(positions.shape)} {positions.dtype}")
+            positions = np.ascontiguousarray(positions, np.int32)
+        out = None if q is None else np.empty(q.shape, q.dtype)
+
+        def write(batch, k, v):
+            if q is not None and q.dtype != k.dtype:
+                _fail(f"{what}: q is {q.dtype}, k is {k.dtype}")
+            rope = N.KvRope(float(base), dims, None if positions is None else positions.ctypes.data)
+            heads = 0 if q is None else q.shape[1]
+            _call("KVWriteRoPE", self.ctx, N.lib().fa_kv_write_rope(
+                self.ctx.h, N.C.byref(self.cache), N.C.byref(batch), N.C.byref(rope), _dtype(k),
+                q.ctypes.data if heads else None, *(_strides(q) if heads else (0, 0)), heads,
+                N.ptr(out) if heads else None, k.ctypes.data, *_strides(k), v.ctypes.data, *_strides(v)))
+
+        self._append(what, seqs, k, v, counts, write)
+        return out
+
+    def _append(self, what: str, seqs, k, v, counts, write) -> None:
         seqs = list(seqs)
-        k, v = (_rows(x, "Append", self.kv_heads, self.head_dim) for x in (k, v))
+        k, v = (_rows(x, what, self.kv_heads, self.head_dim) for x in (k, v))
         if len(k) != len(v) or k.dtype != v.dtype:
-            _fail(f"Append: k is {list(k.shape)} {k.dtype}, v is {list(v.shape)} {v.dtype}")
-        counts = self._counts(seqs, len(k), counts, "Append")
+            _fail(f"{what}: k is {list(k.shape)} {k.dtype}, v is {list(v.shape)} {v.dtype}")
+        counts = self._counts(seqs, len(k), counts, what)
         if len(set(seqs)) != len(seqs):
-            _fail("Append: a sequence is given twice")
+            _fail(f"{what}: a sequence is given twice")
         need = [-(-(self._lengths[s] + c) // BLOCK) - len(self._tables[s]) for s, c in zip(seqs, counts)]
         if sum(need) > len(self._free):
-            _fail(f"Append: {sum(need)} blocks needed, {len(self._free)} free")
+            _fail(f"{what}: {sum(need)} blocks needed, {len(self._free)} free")
         before = {s: self._lengths[s] for s in seqs}
         try:
             for s, c, u in zip(seqs, counts, need):
                 self._tables[s].extend(self._free.pop() for _ in range(u))
                 self._lengths[s] += c
             batch, keep = self._batch(seqs, counts)
-            _call("KVWrite", self.ctx, N.lib().fa_kv_write(
-                self.ctx.h, N.C.byref(self.cache), N.C.byref(batch), _dtype(k), k.ctypes.data, *_strides(k),
-                v.ctypes.data, *_strides(v)))
+            write(batch, k, v)
         except BaseException:
             for s in reversed(seqs):
                 self.Truncate(s, before[s])

@@ -21,8 +21,9 @@
  * documented as goroutine-safe either, models/gemma/embed.go:15). Distinct
  * contexts may be used from distinct threads.
  *
- * HIP graphs: fa_similarities_topk_dev_noalloc and the fa_kv_*_dev entry
- * points (fa_kv_attention_dev with work) can be captured. The others are not
+ * HIP graphs: fa_similarities_topk_dev_noalloc and the fa_kv_*_dev, fa_f8_*_dev,
+ * fa_matmul_f8_dev and fa_sample_dev entry points (those that take work: with
+ * work) can be captured. The others are not
  * capture-safe (they may grow device buffers on a call, and
  * fa_gemma_embed_ids_dev uploads its per-call plan from a pinned host buffer
  * that the next call rewrites and records events of the model): they check
@@ -334,6 +335,116 @@ int fa_kv_attention_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch
                         int64_t q_st, int64_t q_sh, int32_t heads, int causal, int32_t window, float scale, void* out,
                         void* work, size_t work_bytes);
 int fa_kv_attention_work(const fa_kv_cache* cache, const fa_kv_batch* batch, int32_t heads, size_t* bytes);
+
+/* Rotary positions of fa_kv_write_rope. */
+typedef struct fa_kv_rope {
+  double base;              /* finite, > 0: pair i turns by position * base^(-2 i / dims) */
+  int32_t dims;             /* even, 2..head_dim: dims i and i + dims / 2 are a pair; dims past it stay */
+  const int32_t* positions; /* [rows], or NULL: a token's place in its sequence */
+} fa_kv_rope;
+
+/* fa_kv_write with the rotary positions of fa_rope applied on the way: keys are
+ * rotated and written, values written as they are, and the step's queries (q:
+ * `heads` of them a row, any multiple of kv_heads; none with heads == 0 and q ==
+ * NULL) rotated into q_out, [rows][heads][head_dim] contiguous, of dtype, which
+ * may be q itself where q is laid out so, and else must not overlap it. Angles in
+ * float64, their cosines and sines rounded to float32 as fa_rope's, products and sums
+ * in float64, results rounded to float32 (the keys that are quantised; queries of
+ * bf16 tensors are rounded once more). A query is rotated whether or not its token
+ * has a block. positions is on the device in the _dev form, else on the host.
+ * 2 * kv_heads + heads <= 65535. */
+int fa_kv_write_rope(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, const fa_kv_rope* rope, int dtype,
+                     const void* q, int64_t q_st, int64_t q_sh, int32_t heads, void* q_out, const void* k, int64_t k_st,
+                     int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh);
+int fa_kv_write_rope_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, const fa_kv_rope* rope,
+                         int dtype, const void* q, int64_t q_st, int64_t q_sh, int32_t heads, void* q_out,
+                         const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh);
+
+/* ---- products with weights in 8 bits -------------------------------------- */
+
+/* A matrix [n x k] held as e4m3 codes with one scale, a power of two, for each
+ * block of FA_F8_BLOCK columns of a row (a value is code * scale): beside
+ * fa_matmul_fused, for layers that are bound by reading their weights, or by the
+ * matrix units. The caller allocates both buffers in device memory.
+ *
+ * codes:  fa_f8_codes_bytes: [n][kp], kp = k rounded up to whole blocks, zeros past k
+ * scales: fa_f8_scales_bytes: [n][ks] bytes 127 + e for the scale 2^e, ks = kp / 128
+ *         rounded up to a multiple of 4 (127 past kp / 128) */
+#define FA_F8_BLOCK 128
+typedef struct fa_f8_matrix {
+  void* codes;  /* device memory, 16-byte aligned, also in the host entry points */
+  void* scales; /* likewise, 4-byte aligned */
+  int64_t n, k; /* 0 <= n < 2^27, 0 <= k < 2^24 */
+} fa_f8_matrix;
+/* 0 for sizes outside the ranges above. */
+size_t fa_f8_codes_bytes(int64_t n, int64_t k);
+size_t fa_f8_scales_bytes(int64_t n, int64_t k);
+
+/* Quantises x [n x k] (dtype FA_DT_F32 or FA_DT_BF16, leading dimension ldx) into
+ * w. A block takes the smallest 2^e (-80 <= e <= 120) under which its largest finite
+ * magnitude is at most 448 (e4m3's largest); codes are rounded to nearest, ties to
+ * even: within 2^-4 of a value, or 2^-10 of the scale; magnitudes above 240 * 2^120
+ * (3.19e38) become that. NaN and infinities are stored as NaN. The same rule as
+ * the key/value cache's. */
+int fa_f8_write(fa_ctx* ctx, const fa_f8_matrix* w, int dtype, const void* x, int64_t ldx);
+int fa_f8_write_dev(fa_ctx* ctx, const fa_f8_matrix* w, int dtype, const void* x, int64_t ldx);
+/* out [n x k] = the values that w holds (exact in either type). */
+int fa_f8_read(fa_ctx* ctx, const fa_f8_matrix* w, int dtype, void* out, int64_t ldo);
+int fa_f8_read_dev(fa_ctx* ctx, const fa_f8_matrix* w, int dtype, void* out, int64_t ldo);
+
+/* C[m x n] = epilogue(A^ . W^T): A [m x k] of a_dtype (leading dimension lda) is
+ * quantised on the way by fa_f8_write's rule, per row and block, to A^; W [n x k]
+ * is held in 8 bits; C of c_dtype (ldc). The epilogue as fa_matmul_fused's, its
+ * arrays float32. A NaN or an infinity in a row of A makes that row of the product
+ * NaN. float32 results: products exact, sums float32. bf16 results: on the 8-bit
+ * matrix units, which cut every product toward zero to a multiple of 2^-13 of the
+ * power of two below the largest of its group of eight, and then add in float32: off
+ * by less than 2^-10 of the sum of the groups' largest magnitudes, and in 2-norm by
+ * 1/30 to 1/100 of what rounding the result to bf16 adds.
+ *
+ * The _dev form enqueues on fa_stream(ctx); work: scratch of at least
+ * fa_matmul_f8_work(...) bytes, 16-byte aligned, of any contents, used until the
+ * call's work is done (calls that may overlap need one each); NULL: the context's
+ * own, which may grow, so that a call under capture needs work (FA_ERR_STATE
+ * otherwise, if any is needed). m < 2^27, and tiles of 16 rows by 64 columns fewer than 2^24. */
+int fa_matmul_f8(fa_ctx* ctx, int64_t m, int a_dtype, const void* a, int64_t lda, const fa_f8_matrix* w,
+                 const fa_epilogue* e, int c_dtype, void* c, int64_t ldc);
+int fa_matmul_f8_dev(fa_ctx* ctx, int64_t m, int a_dtype, const void* a, int64_t lda, const fa_f8_matrix* w,
+                     const fa_epilogue* e, int c_dtype, void* c, int64_t ldc, void* work, size_t work_bytes);
+int fa_matmul_f8_work(int64_t m, const fa_f8_matrix* w, size_t* bytes);
+
+/* ---- the next token ------------------------------------------------------- */
+
+/* Settings of each row of fa_sample; NULL: the same for all, as stated. */
+typedef struct fa_sampling {
+  const float* temperature; /* [rows], finite, >= 0; NULL: 1 */
+  const int32_t* top_k;     /* [rows], <= 0: no limit; NULL: no limit */
+  const float* top_p;       /* [rows], 0..1; NULL: 1 */
+  const float* min_p;       /* [rows], 0..1; NULL: 0 */
+} fa_sampling;
+
+/* Draws a token from each row of logits [rows x vocab] (dtype FA_DT_F32 or
+ * FA_DT_BF16, leading dimension ld) with the row's number u in [0, 1). With M the
+ * row's largest logit and T its temperature, w = exp((l - M) / T). Of the tokens
+ * ordered by logit, falling, ties by the lower id, those stay that are among the
+ * first top_k, of these the shortest run whose weights make at least top_p of
+ * theirs (top_p 1: all), and of these the ones with w >= min_p; the first of the
+ * order always stays. ids[row] is the first token, by id, up to which the weights
+ * of those that stay exceed u times their sum, and logp[row] (logp may be NULL) the
+ * log of its share of that sum. T == 0: the first of the order, logp 0.
+ * Weights and sums in float64. NaN and -inf logits are never drawn and not
+ * counted; where infinite ones are the largest, they share the weight. A row of
+ * nothing but NaN and -inf gives the id -1 and NaN. s may be NULL.
+ *
+ * vocab: 1..2^24; rows < 2^20. Without _dev everything is host memory and
+ * settings or numbers u outside their ranges are FA_ERR_ARG; with _dev everything
+ * is device memory, such a row gives -1 and NaN, and the work is enqueued on
+ * fa_stream(ctx). work as in fa_matmul_f8, of fa_sample_work(...) bytes. */
+int fa_sample(fa_ctx* ctx, int64_t rows, int64_t vocab, int dtype, const void* logits, int64_t ld,
+              const fa_sampling* s, const float* u, int32_t* ids, float* logp);
+int fa_sample_dev(fa_ctx* ctx, int64_t rows, int64_t vocab, int dtype, const void* logits, int64_t ld,
+                  const fa_sampling* s, const float* u, int32_t* ids, float* logp, void* work, size_t work_bytes);
+int fa_sample_work(int64_t rows, int64_t vocab, size_t* bytes);
 
 /* Scores queries [nq x d] against docs [nd x d] (dot products, the rows
  * being unit length as cluster.Similarities requires, cluster.go:180-190) and
