@@ -15,6 +15,9 @@ int check_sizes(fa_ctx* ctx, int64_t rows, int64_t vocab) {
   if (rows < 0 || rows >= kMaxRows) return set_error(ctx, FA_ERR_ARG, "%s: %lld rows outside [0..2^20)", kOp, (long long)rows);
   if (vocab < 1 || vocab > kMaxVocab)
     return set_error(ctx, FA_ERR_ARG, "%s: a vocabulary of %lld outside 1..2^24", kOp, (long long)vocab);
+  if (fa::sample_grid(rows, vocab) >= (int64_t)1 << 23)
+    return set_error(ctx, FA_ERR_ARG, "%s: %lld rows of %lld are more than one call takes", kOp, (long long)rows,
+                     (long long)vocab);
   return FA_OK;
 }
 

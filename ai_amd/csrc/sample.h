@@ -16,6 +16,7 @@ struct SampleArgs {
   float* logp;  // may be null
 };
 size_t sample_scratch(int64_t rows, int64_t vocab);
+int64_t sample_grid(int64_t rows, int64_t vocab);  // workgroups of a launch
 int launch_sample(fa_ctx* ctx, const SampleArgs& a, void* work, hipStream_t s);
 
 }  // namespace fa
