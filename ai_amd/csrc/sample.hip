@@ -13,8 +13,8 @@
 // The logits are read once, by workgroups that each hold a slice of a row in
 // registers; a second, partial reading finds the few tokens near the bounds:
 //   scan    a slice's first token of the order, and the weight of all of it, or
-//           (where a filter is set) a histogram of counts and weights by z = l / T
-//           in steps of 1/8, on a grid that all slices share.
+//           (where a filter is set) a histogram of counts and weights by l / T in
+//           steps of 1/32, further down of 1, on grids that all slices share.
 //   join    adds up a row's histograms, which gives the steps in which its bounds lie.
 //   gather  slices that have tokens there list them.
 //   finish  finds the bounds among the listed tokens, weighs what stays of every
@@ -28,19 +28,19 @@ namespace fa {
 namespace {
 
 constexpr int kScan = 512;     // threads of scan and gather
-constexpr int kFinish = 1024;  // of finish
-constexpr int kBins = 512;     // steps of 1/8: weights down to e^-64, the last bin holds the rest
+constexpr int kFinish = 512;   // of finish
+constexpr int kFine = 768;     // bins of one step of 1/32: weights down to e^-24
+constexpr int kBins = 1024;    // and bins of 32 steps below: down to e^-280, the last holds the rest
 constexpr int kMaxSlices = 1024;
 constexpr int kSub = 2048;     // bins of a selection's pass
-constexpr int kCached = 4096;  // listed tokens that finish keeps in LDS
+constexpr int kCached = 8192;  // listed tokens that finish keeps in LDS
 
 // ---- a row's layout in the scratch ------------------------------------------------
 
 struct Slice {
-  uint64_t top;    // its first token of the order
-  double mass;     // weights of all its tokens, relative to the first
-  uint32_t count;  // tokens that can be drawn
-  int32_t bins;    // bins in use
+  uint64_t top;   // its first token of the order
+  double mass;    // the weight of all of it, relative to the first token
+  int32_t bins;   // bins in use
 };
 
 // Bins in which a row's bounds may lie. Tokens in listed bins are looked at one by one.
@@ -50,7 +50,8 @@ struct Cut {
   int k_rank;         // its rank there, from 1
   int p_lo, p_hi;     // bins of top_p's bound (kBins: none)
   int m_lo, m_hi;     // of min_p's
-  double step;        // of most
+  double step;        // the grid's step of most
+  double t;           // most on the grid
   double above_k, above_p;  // weights of the bins before k_bin, before p_lo
   double all;         // of all bins
   __device__ __forceinline__ bool listed(int b) const {
@@ -63,8 +64,8 @@ struct Plan {
   int vec;          // rows aligned for 16-byte loads
   Slice* slice;     // [rows][slices]
   Cut* cut;         // [rows]
-  uint64_t* mass;   // [rows][slices][kBins]
-  uint32_t* count;  // likewise
+  double* mass;     // [rows][slices][kBins] weights of the bins up to each, relative to the slice's first token
+  uint32_t* count;  // likewise tokens (without top-k: bins with tokens)
   uint32_t* listed; // [rows][slices]
   uint16_t* list;   // [rows][slices * per]
 };
@@ -136,18 +137,44 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t row) {
 __device__ __forceinline__ double weight(float l, float most, double inv, int scale = 0) {
   return l == most ? ldexp(1.0, scale) : exp_scaled(((double)l - (double)most) * inv, scale);
 }
-// Steps of 1/8 from the grid's step of `most` down to that of l.
-__device__ __forceinline__ int bin_of(float l, float most, double inv, double most_step) {
-  if (l == most) return 0;
-  return (int)fmin(most_step - floor((double)l * 8.0 * inv), (double)(kBins - 1));
+
+// The grid: t = 32 l / T, its steps whole numbers; 32 of them make a wide step.
+// Where the largest logit is infinite, only infinite ones count, at 0.
+__device__ __forceinline__ double grid_of(float l, double inv) { return l == __builtin_inff() ? 0.0 : (double)l * (32.0 * inv); }
+__device__ __forceinline__ bool counts(float l, float most) {
+  return most == __builtin_inff() ? l == most : l > -__builtin_inff();
 }
-__device__ __forceinline__ double step_of(float l, double inv) { return floor((double)l * 8.0 * inv); }
-// Weights in bin b are below 2^-bin_exp(b): l / T is more than (b - 1) / 8 below.
-__device__ __forceinline__ int bin_exp(int b) { return b > 1 ? (int)((float)(b - 1) * 0.18033f) : 0; }
+// The bin of step `at` below the top step: by steps up to kFine of them, then by wide ones.
+__device__ __forceinline__ int bin_of_step(double at, double top) {
+  const double down = top - at;
+  if (down < (double)kFine) return (int)down;
+  const double wide = floor(top * 0.03125) - floor(at * 0.03125);  // at least kFine / 32
+  return (int)fmin(wide + (double)(kFine - kFine / 32), (double)(kBins - 1));
+}
+// The lowest step of bin b of those counted from `top`.
+__device__ __forceinline__ double last_step(int b, double top) {
+  return b < kFine ? top - (double)b : (floor(top * 0.03125) - (double)(b - (kFine - kFine / 32))) * 32.0;
+}
+__device__ __forceinline__ int bin_of(float l, double inv, double top) { return bin_of_step(floor(grid_of(l, inv)), top); }
+// From here on unequal logits are 2^16 steps and more apart, and t is taken as it is.
+constexpr double kFar = 0x1p40;
+// Weight in the middle of bin b of steps counted from `top`, beside the logit at t.
+__device__ __forceinline__ double middle(int b, double top, double t) {
+  if (!(fabs(t) < kFar)) return b == 0 && top == floor(t) ? 1.0 : 0.0;
+  double at = top - (double)b + 0.5;
+  if (b >= kFine) at = (floor(top * 0.03125) - (double)(b - (kFine - kFine / 32))) * 32.0 + 16.0;
+  return exp_scaled((at - t) * 0.03125, 0);
+}
+// Weights in bin b are below 2^-bin_exp(b): (b - 1) / 32 below the first, or a wide step less than wide steps.
+__device__ __forceinline__ int bin_exp(int b) {
+  if (b < kFine) return b > 1 ? (int)((float)(b - 1) * 0.04508f) : 0;
+  return (int)((float)(b - (kFine - kFine / 32) - 1) * 1.4426f);
+}
 // A number below 2^51 as an integer, to nearest.
 __device__ __forceinline__ uint64_t to_int(double x) {
   return (uint64_t)__double_as_longlong(x + 0x1p52) - (uint64_t)0x4330000000000000ull;
 }
+constexpr int kUnit = 48;  // a bin's weights are held in units of 2^-48 of its middle: 2^14 of them fit
 
 // ---- a workgroup's sums and scans, in a fixed order -----------------------------------------
 
@@ -239,61 +266,103 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs a, Plan p) {
   if (!r.sound) return;
   Held<T, E> h;
   h.load((const T*)a.logits + row * a.ld + first, min(p.per, (int)a.vocab - first), p.vec);
-  mass[tid] = 0;
-  count[tid] = 0;
-  uint64_t top = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++) top = max(top, order_of(h.v[e], first + Held<T, E>::at(e)));
-  top = block_join<kScan>(top, red, Max());
-  const float most = logit_of(top);
-  if (r.greedy || most == -__builtin_inff()) {
-    if (tid == 0) *out = {top, 0.0, 0, 0};
+  for (int i = 0; i < kBins / kScan; i++) mass[i * kScan + tid] = 0, count[i * kScan + tid] = 0;
+  float most = -__builtin_inff();
+#pragma unroll
+  for (int e = 0; e < E; e++) most = fmaxf(most, h.v[e]);
+  most = block_join<kScan>(most, (float*)red, Max());
+  if (most == -__builtin_inff()) {
+    if (tid == 0) *out = {0, 0.0, 0};
+    return;
+  }
+  int id = 0x7FFFFFFF;  // the lowest of those equal to it
+#pragma unroll
+  for (int e = 0; e < E; e++)
+    if (h.v[e] == most) id = min(id, first + Held<T, E>::at(e));
+  const uint64_t top = order_of(most, block_join<kScan>(id, (int*)redd, Min()));
+  if (r.greedy) {
+    if (tid == 0) *out = {top, 0.0, 0};
     return;
   }
   if (!r.cut) {
     double sum = 0;
 #pragma unroll
     for (int e = 0; e < E; e++)
-      if (h.v[e] > -__builtin_inff()) sum += weight(h.v[e], most, r.inv);
+      if (counts(h.v[e], most)) sum += weight(h.v[e], most, r.inv);
     sum = block_join<kScan>(sum, redd, Add());
-    if (tid == 0) *out = {top, sum, 0, 0};
+    if (tid == 0) *out = {top, sum, 0};
     return;
   }
-  const double step = step_of(most, r.inv);
-  uint64_t last = 0, valid = 0;
+  const double c = 32.0 * r.inv, step = floor(grid_of(most, r.inv)), near = fabs(step) < kFar ? 1.0 : 0.0;
+  const bool counted = r.top_k < a.vocab;
 #pragma unroll
-  for (int e = 0; e < E; e++)
-    if (h.v[e] > -__builtin_inff()) {
-      const int b = bin_of(h.v[e], most, r.inv, step);
-      // up to 2^14 tokens of less than 2^49 each
-      atomicAdd((unsigned long long*)&mass[b], to_int(weight(h.v[e], most, r.inv, 48 + bin_exp(b))));
-      atomicAdd(&count[b], 1u);
-      valid++;
+  for (int e = 0; e < E; e++) {
+#pragma clang fp contract(off)  // (t - floor(t) is exact, and the rounding of t is added by itself)
+    const float v = h.v[e];
+    if (!counts(v, most)) continue;
+    const double t = grid_of(v, r.inv), whole = floor(t), down = step - whole;
+    int b;
+    uint64_t w;
+    if (down < (double)kFine) {
+      b = (int)down;
+      const double rest = v == __builtin_inff() ? 0.0 : fma((double)v, c, -t);
+      // 2^48 e^d to d^6, |d| <= 1/64: the next term is 5e-17
+      const double d = near != 0 ? ((t - whole) - 0.5 + rest) * 0.03125 : 0.0;
+      double x = 1.0 / 720.0;
+      x = fma(x, d, 1.0 / 120.0);
+      x = fma(x, d, 1.0 / 24.0);
+      x = fma(x, d, 1.0 / 6.0);
+      x = fma(x, d, 0.5);
+      x = fma(x, d, 1.0);
+      x = fma(x, d, 1.0);
+      w = to_int(x * 0x1p48);
+    } else {
+      // 4e-11 of the slice's first weight and less: seven digits of them are enough
+      b = bin_of_step(whole, step);
+      const float d = (float)(t * 0.03125 - floor(t * 0.03125)) - 0.5f;
+      w = b == kBins - 1 ? 0 : to_int((double)__builtin_amdgcn_exp2f(d * 1.4426950408889634f) * 0x1p48);
     }
-  __syncthreads();
-  const uint64_t m = mass[tid];
-  const uint32_t c = count[tid];
-  if (c) last = tid + 1;
-  last = block_join<kScan>(last, red, Max());
-  valid = block_join<kScan>(valid, red, Add());
-  const double all = block_join<kScan>(ldexp((double)m, -48 - bin_exp(tid)), redd, Add());
-  const int64_t at = (row * p.slices + s) * kBins + tid;
-  if (tid < (int)last) {
-    p.mass[at] = m;
-    p.count[at] = c;
+    atomicAdd((unsigned long long*)&mass[b], (unsigned long long)w);
+    if (counted) atomicAdd(&count[b], 1u);
   }
-  if (tid == 0) *out = {top, all, (uint32_t)valid, (int32_t)last};
+  __syncthreads();
+  // running sums over the bins (two neighbours a thread); without top-k, whether there are tokens in a bin is all that is asked
+  static_assert(kBins == 2 * kScan, "two bins a thread");
+  const double t0 = grid_of(most, r.inv);
+  uint64_t w[2];
+  double m[2];
+  uint32_t n[2];
+  int last = 0;
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int b = 2 * tid + i;
+    w[i] = mass[b];
+    n[i] = counted ? count[b] : w[i] != 0;
+    m[i] = w[i] ? ldexp((double)w[i], -kUnit) * middle(b, step, t0) : 0.0;
+    if (n[i]) last = b + 1;
+  }
+  last = block_join<kScan>(last, (int*)red, Max());
+  double all_m;
+  uint32_t all_n;
+  const double m0 = block_scan<kScan>(m[0] + m[1], redd, &all_m);
+  const uint32_t n0 = block_scan<kScan>(n[0] + n[1], (uint32_t*)red, &all_n);
+  const int64_t at = (row * p.slices + s) * kBins + 2 * tid;
+  if (2 * tid < last) {
+    *reinterpret_cast<double2*>(p.mass + at) = make_double2(m0 + m[0], m0 + m[0] + m[1]);
+    *reinterpret_cast<uint2*>(p.count + at) = make_uint2(n0 + n[0], n0 + n[0] + n[1]);
+  }
+  if (tid == 0) *out = {top, all_m, last};
 }
 
 // ---- a row's histograms joined ----------------------------------------------------------------------
 
-// Bins that a slice whose first token has logit l lies below the row's.
-__device__ __forceinline__ int slice_offset(float l, float most, double step, double inv) {
-  if (l == most) return 0;
-  if (l == -__builtin_inff()) return kBins;
-  return (int)fmin(step - step_of(l, inv), (double)kBins);
+// The row's bin of a slice's bin b: the slice's steps are counted from `own`, the row's from `top`.
+__device__ __forceinline__ int row_bin(int b, double own, double top) {
+  if (b < kFine) return bin_of_step(own - (double)b, top);
+  const double wide = floor(top * 0.03125) - floor(own * 0.03125);
+  return (int)fmin((double)b + wide, (double)(kBins - 1));
 }
-
 template <int NT>
 __device__ __forceinline__ uint64_t row_top(const Plan& p, int64_t row, uint64_t* red) {
   uint64_t top = 0;
@@ -301,77 +370,82 @@ __device__ __forceinline__ uint64_t row_top(const Plan& p, int64_t row, uint64_t
   return block_join<NT>(top, red, Max());
 }
 
-// One workgroup a row, a thread a bin. Slices are taken kChunk at a time: their
-// heads first, then all their bins, so that loads do not wait for one another.
-constexpr int kChunk = 64;
+// One workgroup a row, a thread a bin: what the slices have down to the last step of
+// each. Slices are taken kChunk at a time, their heads first, and the sums of kAtOnce
+// slices are under way at once.
+constexpr int kChunk = 64, kAtOnce = 16;
 __global__ __launch_bounds__(kBins) void join_kernel(SampleArgs a, Plan p) {
   constexpr int NT = kBins;
-  __shared__ double redd[NT / 64], sums[kBins], scale[kChunk];
-  __shared__ uint64_t red[NT / 64];
-  __shared__ int found[4], offset[kChunk], bins[kChunk];
+  __shared__ double sums[kBins], scale[kChunk];
+  __shared__ uint64_t red[NT / 64], counts_to[kBins];
+  __shared__ int found[4], bins[kChunk], below[kChunk], wide_below[kChunk];
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const Row r = row_of(a, row);
   if (!r.sound || r.greedy || !r.cut) return;
   const Slice* slice = p.slice + row * p.slices;
   const float most = logit_of(row_top<NT>(p, row, red));
-  if (most == -__builtin_inff()) return;
+  if (!(most > -__builtin_inff())) return;
   Cut c;
   c.most = most;
-  c.step = step_of(most, r.inv);
+  c.t = grid_of(most, r.inv);
+  c.step = floor(c.t);
   c.k_bin = c.p_lo = c.m_lo = kBins;
   c.p_hi = c.m_hi = -1;
   c.k_rank = 0;
   c.above_k = c.above_p = 0;
-  double m = 0, far_m = 0;
-  uint64_t n = 0, far_n = 0;
+  const int down = (int)fmin(c.step - last_step(tid, c.step), 0x1p24);  // steps to the last of this bin
+  double m = 0;
+  uint64_t n = 0;
   for (int s0 = 0; s0 < p.slices; s0 += kChunk) {
-    const int many = min(kChunk, p.slices - s0);
     __syncthreads();
-    if (tid < many) {
-      const Slice x = slice[s0 + tid];
-      const float l = logit_of(x.top);
-      int off = kBins, used = 0;
-      double w = 0;
-      if (x.bins) {
-        off = slice_offset(l, most, c.step, r.inv);
-        w = weight(l, most, r.inv);
-        if (off >= kBins - 1) far_m += x.mass * w, far_n += x.count;  // all of it past the row's last bin
-        else used = x.bins;
+    if (tid < kChunk) {
+      bins[tid] = below[tid] = wide_below[tid] = 0;
+      scale[tid] = 0;
+      if (s0 + tid < p.slices) {
+        const Slice x = slice[s0 + tid];
+        const float l = logit_of(x.top);
+        if (x.bins && counts(l, most)) {
+          // the slice's first step below the row's, in steps and in wide ones
+          const double own = floor(grid_of(l, r.inv));
+          below[tid] = (int)fmin(c.step - own, 0x1p25);
+          wide_below[tid] = (int)fmin(floor(c.step * 0.03125) - floor(own * 0.03125), 0x1p20);
+          scale[tid] = weight(l, most, r.inv);
+          bins[tid] = x.bins;
+        }
       }
-      offset[tid] = off;
-      bins[tid] = used;
-      scale[tid] = w;
     }
     __syncthreads();
     const int64_t at = (row * p.slices + s0) * kBins;
-#pragma unroll 8
-    for (int s = 0; s < many; s++) {
-      const int j = tid - offset[s];
-      const bool in = tid < kBins - 1 && j >= 0 && j < bins[s];
-      const int64_t i = at + (int64_t)s * kBins + (in ? j : 0);
-      const uint64_t mass = p.mass[i];
-      const uint32_t count = p.count[i];
-      if (in) m += ldexp((double)mass, -48 - bin_exp(j)) * scale[s], n += count;
-    }
-    for (int s = 0; s < many; s++)
-      for (int i = kBins - 1 - offset[s] + tid; i < bins[s]; i += NT) {  // past the row's last bin
-        far_m += ldexp((double)p.mass[at + (int64_t)s * kBins + i], -48 - bin_exp(i)) * scale[s];
-        far_n += p.count[at + (int64_t)s * kBins + i];
+    const int many = min(kChunk, p.slices - s0);
+    for (int s = 0; s < many; s += kAtOnce) {
+      double mass[kAtOnce];
+      uint32_t count[kAtOnce];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; i++) {
+        const int q = min(s + i, kChunk - 1), d = down - below[q];  // (of slices past the last: no bins)
+        int j = d < kFine ? d : tid - wide_below[q];
+        if (tid == kBins - 1) j = kBins - 1;
+        const bool in = bins[q] > 0 && j >= 0;
+        const int64_t from = at + min(s + i, many - 1) * kBins + (in ? min(j, bins[q] - 1) : 0);
+        mass[i] = p.mass[from];
+        count[i] = p.count[from];
+        if (!in) mass[i] = 0, count[i] = 0;
       }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; i++) m = fma(mass[i], scale[min(s + i, kChunk - 1)], m), n += count[i];
+    }
   }
-  far_m = block_join<NT>(far_m, redd, Add());
-  far_n = block_join<NT>(far_n, red, Add());
-  if (tid == kBins - 1) m = far_m, n = far_n;
-  uint64_t tokens;
-  const double before = block_scan<NT>(m, redd, &c.all);
-  const uint64_t n_before = block_scan<NT>(n, red, &tokens);
-  sums[tid] = before;
+  sums[tid] = m;
+  counts_to[tid] = n;
   if (tid < 4) found[tid] = tid == 1 ? 0 : kBins;
   __syncthreads();
+  const double before = tid ? sums[tid - 1] : 0.0;
+  const uint64_t n_before = tid ? counts_to[tid - 1] : 0, tokens = counts_to[kBins - 1];
+  c.all = sums[kBins - 1];
   // top-k: the bin of the top_k-th token, if there are more
   const uint64_t k = (uint64_t)r.top_k;
-  if (n_before < k && n_before + n >= k && tokens > k) {
+  if (k < (uint64_t)a.vocab && n_before < k && n >= k && tokens > k) {
     found[0] = tid;
     found[1] = (int)(k - n_before);
   }
@@ -380,26 +454,25 @@ __global__ __launch_bounds__(kBins) void join_kernel(SampleArgs a, Plan p) {
   c.k_rank = found[1];
   double k_least = c.all, k_most = c.all;  // weight of the top_k tokens
   if (c.k_bin < kBins) {
-    c.above_k = k_least = sums[c.k_bin];
-    k_most = c.k_bin + 1 < kBins ? sums[c.k_bin + 1] : c.all;
+    c.above_k = k_least = c.k_bin ? sums[c.k_bin - 1] : 0.0;
+    k_most = sums[c.k_bin];
   }
-  // top-p: sums of bins are right to 1e-14 or so, the margin of 1e-12 keeps to either side
+  // top-p: sums are right to 1e-14 or so, the margin of 1e-12 keeps to either side
   if (r.top_p < 1.f) {
     const double least = (double)r.top_p * k_least * (1 - 1e-12), want = (double)r.top_p * k_most * (1 + 1e-12);
-    if (n > 0) {
-      if (before + m >= least) atomicMin(&found[2], tid);
-      if (before + m >= want) atomicMin(&found[3], tid);
-    }
+    if (before < least && m >= least) atomicMin(&found[2], tid);
+    if (before < want && m >= want) atomicMin(&found[3], tid);
     __syncthreads();
-    c.p_lo = min(found[2], min(c.k_bin, kBins - 1));
-    c.p_hi = min(found[3], min(c.k_bin, kBins - 1));
-    c.above_p = sums[c.p_lo];
+    const int end = min(c.k_bin, kBins - 1);
+    c.p_lo = least > 0 ? min(found[2], end) : 0;
+    c.p_hi = want > 0 ? min(found[3], end) : 0;
+    c.above_p = c.p_lo ? sums[c.p_lo - 1] : 0.0;
   }
   // min-p: l >= most + T ln(min_p), in the step of that bound or the next
   if (r.min_p > 0.f) {
-    const int b = most == __builtin_inff() ? 0 : (int)fmin(-8.0 * log((double)r.min_p), (double)kBins);
-    c.m_lo = max(0, b - 1);
-    c.m_hi = b + 2;
+    const double down = most == __builtin_inff() ? 0.0 : -32.0 * log((double)r.min_p);
+    c.m_lo = max(0, bin_of_step(c.step - floor(down), c.step) - 1);
+    c.m_hi = bin_of_step(c.step - floor(down) - 2.0, c.step) + 1;
   }
   if (tid == 0) p.cut[row] = c;
 }
@@ -418,11 +491,14 @@ __global__ __launch_bounds__(kScan) void gather_kernel(SampleArgs a, Plan p) {
   }
   const Cut c = p.cut[row];
   const float most = c.most;
-  const int off = slice_offset(logit_of(x.top), most, c.step, r.inv);
+  const float own = logit_of(x.top);
+  const double step = floor(grid_of(own, r.inv));
   const int64_t at = (row * p.slices + s) * kBins;
   // does the slice have tokens in listed bins?
-  bool any = off >= kBins - 1 && c.listed(kBins - 1);
-  if (off < kBins - 1 && tid < x.bins) any = p.count[at + tid] && c.listed(min(tid + off, kBins - 1));
+  bool any = false;
+  if (counts(own, most))
+    for (int b = tid; b < x.bins; b += kScan)
+      if (c.listed(row_bin(b, step, c.step))) any |= p.count[at + b] != (b ? p.count[at + b - 1] : 0);
   if (tid == 0) n_listed = 0;
   if (__syncthreads_or(any)) {
     Held<T, E> h;
@@ -430,9 +506,9 @@ __global__ __launch_bounds__(kScan) void gather_kernel(SampleArgs a, Plan p) {
     uint16_t* list = p.list + (row * p.slices + s) * p.per;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-      const bool in = h.v[e] > -__builtin_inff() && c.listed(bin_of(h.v[e], most, r.inv, c.step));
+      const bool in = counts(h.v[e], most) && c.listed(bin_of(h.v[e], r.inv, c.step));
       const uint64_t mask = __ballot(in);
-      if (mask == 0) continue;
+      if (mask == 0) continue;  // (uniform in the wave)
       uint32_t base = 0;
       if ((tid & 63) == 0) base = atomicAdd(&n_listed, (uint32_t)__popcll(mask));
       base = __builtin_amdgcn_readfirstlane(base);
@@ -448,85 +524,109 @@ __global__ __launch_bounds__(kScan) void gather_kernel(SampleArgs a, Plan p) {
 struct FinishMem {
   double redd[kFinish / 64];
   uint64_t red[kFinish / 64];
-  int found[4];
-  uint64_t token[kCached];   // the row's listed tokens, if they fit
+  uint64_t token[kCached];         // the row's listed tokens, if they fit
   uint64_t sub_mass[kSub];
   uint32_t sub_count[kSub];
   uint32_t start[kMaxSlices + 1];  // of a slice's listed tokens among the row's
-  double keep[kMaxSlices];   // weight that stays of each slice
-  uint64_t part[kMaxSlices]; // of its listed tokens
-  int pick;
-  uint64_t one;
-  uint64_t pass[3];
+  uint64_t part[kMaxSlices];       // weight of the listed tokens of each slice that stay
+  int found;
+  double found_before;
+  uint64_t one, pass[3];
 };
 
+constexpr int kAhead = 4;
 // The listed tokens of a row, each given to f as its number in the order.
 template <typename T, typename F>
-__device__ __forceinline__ void each_listed(const SampleArgs& a, const Plan& p, int64_t row, const FinishMem& mem,
-                                            uint32_t n, F f) {
-  if (n <= kCached) {
-    for (uint32_t i = threadIdx.x; i < n; i += kFinish) f(mem.token[i], i);
-    return;
-  }
+__device__ __forceinline__ void each_in_memory(const SampleArgs& a, const Plan& p, int64_t row, const FinishMem& mem, F f) {
   const T* l = (const T*)a.logits + row * a.ld;
   for (int s = threadIdx.x >> 6; s < p.slices; s += kFinish / 64) {
     const uint32_t from = mem.start[s], m = mem.start[s + 1] - from;
     const uint16_t* list = p.list + (row * p.slices + s) * p.per;
-    for (uint32_t i = threadIdx.x & 63; i < m; i += 64) {
-      const int id = s * p.per + list[i];
-      f(order_of(value_of(l[id]), id), from + i);
+    for (uint32_t i = threadIdx.x & 63; i < m; i += 64 * kAhead) {  // several under way at once
+      int id[kAhead];
+      T v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) id[j] = s * p.per + list[min(i + 64 * j, m - 1)];
+#pragma unroll
+      for (int j = 0; j < kAhead; j++) v[j] = l[id[j]];
+#pragma unroll
+      for (int j = 0; j < kAhead; j++)
+        if (i + 64 * j < m) f(order_of(value_of(v[j]), id[j]), from + i + 64 * j);
     }
   }
 }
+template <typename T, typename F>
+__device__ __forceinline__ void each_listed(const SampleArgs& a, const Plan& p, int64_t row, const FinishMem& mem,
+                                            uint32_t n, F f) {
+  if (n > kCached) {
+    each_in_memory<T>(a, p, row, mem, [&](uint64_t o, uint32_t) { f(o); });
+    return;
+  }
+  for (uint32_t i = threadIdx.x; i < n; i += kFinish) f(mem.token[i]);
+}
 
-// Of the listed tokens that `in` takes, the one down to which there are `rank`
+// Of the listed tokens from hi down to lo, the one down to which there are `rank`
 // (by count), or down to which weights and `above` make `want`. Weights count in
 // units of 2^-unit. The last of them if there are not so many.
-template <typename T, bool MASS, typename IN>
-__device__ uint64_t select_token(const SampleArgs& a, const Plan& p, int64_t row, FinishMem& mem, uint32_t n, IN in,
-                                 float most, double inv, int unit, uint64_t rank, double above, double want) {
+template <typename T, bool MASS>
+__device__ uint64_t select_token(const SampleArgs& a, const Plan& p, int64_t row, FinishMem& mem, uint32_t n, uint64_t lo,
+                                 uint64_t hi, float most, double inv, int unit, uint64_t rank, double above, double want) {
+  constexpr int W = kSub / kFinish;  // bins of a thread
   const int tid = threadIdx.x;
-  uint64_t hi = 0, lo = ~0ull;
-  each_listed<T>(a, p, row, mem, n, [&](uint64_t o, uint32_t) {
-    if (in(o)) hi = max(hi, o), lo = min(lo, o);
-  });
-  hi = block_join<kFinish>(hi, mem.red, Max());
-  lo = block_join<kFinish>(lo, mem.red, Min());
   uint64_t before = 0, count_before = 0;  // integer weight and tokens above hi
+  want = fmax(want, above + ldexp(1.0, -unit));  // (top_p = 0: the first token all the same)
   while (lo < hi) {
     const int shift = max(0, 64 - (int)__builtin_clzll(hi - lo) - 11);
-    for (int i = tid; i < kSub; i += kFinish) mem.sub_mass[i] = 0, mem.sub_count[i] = 0;
+    for (int i = tid; i < kSub; i += kFinish) {
+      mem.sub_count[i] = 0;
+      if (MASS) mem.sub_mass[i] = 0;
+    }
+    if (tid == 0) mem.found = -1;
     __syncthreads();
-    each_listed<T>(a, p, row, mem, n, [&](uint64_t o, uint32_t) {
-      if (o < lo || o > hi || !in(o)) return;
+    each_listed<T>(a, p, row, mem, n, [&](uint64_t o) {
+      if (o < lo || o > hi) return;
       const int i = (int)((hi - o) >> shift);
       atomicAdd(&mem.sub_count[i], 1u);
       if (MASS) atomicAdd((unsigned long long*)&mem.sub_mass[i], to_int(weight(logit_of(o), most, inv, unit)));
     });
     __syncthreads();
-    // each thread two bins
-    const uint64_t m0 = mem.sub_mass[2 * tid], m1 = mem.sub_mass[2 * tid + 1];
-    const uint64_t c0 = mem.sub_count[2 * tid], c1 = mem.sub_count[2 * tid + 1];
-    uint64_t all;
-    uint64_t cb = block_scan<kFinish>(c0 + c1, mem.red, &all);
-    uint64_t mb = MASS ? block_scan<kFinish>(m0 + m1, mem.red, &all) : 0;
-    if (tid == 0) mem.found[0] = kSub, mem.found[1] = -1;
-    __syncthreads();
+    uint64_t c[W], w[W], cs = 0, ws = 0, all;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      c[i] = mem.sub_count[W * tid + i];
+      w[i] = MASS ? mem.sub_mass[W * tid + i] : 0;
+      cs += c[i];
+      ws += w[i];
+    }
+    uint64_t cb = block_scan<kFinish>(cs, mem.red, &all);
+    uint64_t wb = MASS ? block_scan<kFinish>(ws, mem.red, &all) : 0;
     auto reached = [&](uint64_t count, uint64_t mass) {
       return MASS ? above + ldexp((double)(before + mass), -unit) >= want : count_before + count >= rank;
     };
-    if (c0) atomicMax(&mem.found[1], 2 * tid);
-    if (c1) atomicMax(&mem.found[1], 2 * tid + 1);
-    if (c0 && reached(cb + c0, mb + m0)) atomicMin(&mem.found[0], 2 * tid);
-    else if (c1 && reached(cb + c0 + c1, mb + m0 + m1)) atomicMin(&mem.found[0], 2 * tid + 1);
-    __syncthreads();
-    const int pick = mem.found[0] < kSub ? mem.found[0] : mem.found[1];
-    if (pick >> 1 == tid) {
-      mem.pass[0] = pick & 1 ? cb + c0 : cb;
-      mem.pass[1] = pick & 1 ? mb + m0 : mb;
-      mem.pass[2] = pick & 1 ? c1 : c0;
+    const int last_used = block_join<kFinish>(cs ? tid : -1, (int*)mem.redd, Max());
+    // the one thread before whose tokens the aim is not reached and with them is, or the last of any
+    const bool open = !reached(cb, wb) || count_before + cb == 0;
+    if (cs && open && (reached(cb + cs, wb + ws) || tid == last_used)) {
+      int pick = -1;
+#pragma unroll
+      for (int i = 0; i < W; i++) {
+        if (pick >= 0 || c[i] == 0) continue;
+        bool more = false;  // tokens of this thread after bin i
+#pragma unroll
+        for (int j = 0; j < W; j++) more |= j > i && c[j] != 0;
+        if (reached(cb + c[i], wb + w[i]) || !more) {
+          pick = W * tid + i;
+          mem.found = pick;
+          mem.pass[0] = cb;
+          mem.pass[1] = wb;
+          mem.pass[2] = c[i];
+        }
+        cb += c[i];
+        wb += w[i];
+      }
     }
     __syncthreads();
+    const int pick = mem.found;
     count_before += mem.pass[0];
     before += mem.pass[1];
     const bool single = mem.pass[2] == 1;
@@ -534,8 +634,8 @@ __device__ uint64_t select_token(const SampleArgs& a, const Plan& p, int64_t row
     const uint64_t width = 1ull << shift;
     if (hi - lo >= width) lo = hi - width + 1;
     if (single && lo < hi) {
-      each_listed<T>(a, p, row, mem, n, [&](uint64_t o, uint32_t) {
-        if (o >= lo && o <= hi && in(o)) mem.one = o;
+      each_listed<T>(a, p, row, mem, n, [&](uint64_t o) {
+        if (o >= lo && o <= hi) mem.one = o;
       });
       __syncthreads();
       hi = lo = mem.one;
@@ -545,7 +645,7 @@ __device__ uint64_t select_token(const SampleArgs& a, const Plan& p, int64_t row
   return hi;
 }
 
-template <typename T>
+template <typename T, int E>
 __global__ __launch_bounds__(kFinish) void finish_kernel(SampleArgs a, Plan p) {
   __shared__ FinishMem mem;
   const int64_t row = blockIdx.x;
@@ -554,7 +654,7 @@ __global__ __launch_bounds__(kFinish) void finish_kernel(SampleArgs a, Plan p) {
   uint64_t top = 0;
   if (r.sound) top = row_top<kFinish>(p, row, mem.red);
   const float most = logit_of(top);
-  const bool none = !r.sound || most == -__builtin_inff();
+  const bool none = !r.sound || !(most > -__builtin_inff());
   if (none || r.greedy) {
     if (tid == 0) {
       a.ids[row] = none ? -1 : id_of(top);
@@ -564,155 +664,213 @@ __global__ __launch_bounds__(kFinish) void finish_kernel(SampleArgs a, Plan p) {
   }
   const Slice* slice = p.slice + row * p.slices;
   const T* l = (const T*)a.logits + row * a.ld;
-  uint64_t bound = 0;     // tokens at or above it stay (but for min_p)
-  int whole = kBins;      // bins before it stay whole, listed tokens of the others are asked
+  uint64_t bound = 0;  // tokens at or above it stay (but for min_p)
+  int whole = kBins;   // bins before it stay whole, listed tokens of the others are asked
+  int unit = 0;        // mem.part counts 2^-unit
+  double step = 0;
   if (r.cut) {
     const Cut c = p.cut[row];
-    const uint32_t mine = tid < p.slices ? p.listed[row * p.slices + tid] : 0;
-    uint32_t n;
-    const uint32_t start = block_scan<kFinish>(mine, (uint32_t*)mem.red, &n);
-    if (tid < p.slices) mem.start[tid] = start, mem.part[tid] = 0;
+    step = c.step;
+    // where each slice's listed tokens go
+    uint32_t n = 0;
+    for (int s0 = 0; s0 < p.slices; s0 += kFinish) {
+      const int s = s0 + tid;
+      const uint32_t mine = s < p.slices ? p.listed[row * p.slices + s] : 0;
+      uint32_t all;
+      const uint32_t start = block_scan<kFinish>(mine, (uint32_t*)mem.red, &all);
+      if (s < p.slices) mem.start[s] = n + start, mem.part[s] = 0;
+      n += all;
+    }
     if (tid == 0) mem.start[p.slices] = n;
     __syncthreads();
-    if (n <= kCached) {
-      for (int s = wave; s < p.slices; s += kFinish / 64) {
-        const uint32_t from = mem.start[s], m = mem.start[s + 1] - from;
-        const uint16_t* list = p.list + (row * p.slices + s) * p.per;
-        for (uint32_t i = lane; i < m; i += 64) {
-          const int id = s * p.per + list[i];
-          mem.token[from + i] = order_of(value_of(l[id]), id);
-        }
-      }
-      __syncthreads();
-    }
-    auto bin = [&](uint64_t o) { return bin_of(logit_of(o), most, r.inv, c.step); };
-    // integer weights: n of them, each below 2^(bits + 1), stay below 2^63
+    auto bin = [&](uint64_t o) { return bin_of(logit_of(o), r.inv, step); };
+    uint64_t k_hi = 0, k_lo = ~0ull, p_hi = 0, p_lo = ~0ull;
+    each_in_memory<T>(a, p, row, mem, [&](uint64_t o, uint32_t i) {
+      if (n <= kCached) mem.token[i] = o;
+      const int b = bin(o);
+      if (b == c.k_bin) k_hi = max(k_hi, o), k_lo = min(k_lo, o);
+      if (b >= c.p_lo && b <= c.p_hi) p_hi = max(p_hi, o), p_lo = min(p_lo, o);
+    });
+    __syncthreads();
+    // integer weights: n of them, each below 2^bits, stay below 2^62
     const int bits = min(49, 61 - (32 - __builtin_clz(n | 1)));
     double k_mass = c.all;
     if (c.k_bin < kBins) {
-      const int b = c.k_bin;
-      bound = select_token<T, false>(a, p, row, mem, n, [&](uint64_t o) { return bin(o) == b; }, most, r.inv, 0,
-                                     (uint64_t)c.k_rank, 0, 0);
-      uint64_t sum = 0;
-      const int unit = bits + bin_exp(b);
-      each_listed<T>(a, p, row, mem, n, [&](uint64_t o, uint32_t) {
-        if (o >= bound && bin(o) == b) sum += to_int(weight(logit_of(o), most, r.inv, unit));
-      });
-      sum = block_join<kFinish>(sum, mem.red, Add());
-      k_mass = c.above_k + ldexp((double)sum, -unit);
-      whole = b;
+      k_hi = block_join<kFinish>(k_hi, mem.red, Max());
+      k_lo = block_join<kFinish>(k_lo, mem.red, Min());
+      bound = select_token<T, false>(a, p, row, mem, n, k_lo, k_hi, most, r.inv, 0, (uint64_t)c.k_rank, 0, 0);
+      whole = c.k_bin;
+      if (r.top_p < 1.f) {
+        uint64_t sum = 0;
+        const int u = bits + bin_exp(c.k_bin);
+        each_listed<T>(a, p, row, mem, n, [&](uint64_t o) {
+          if (o >= bound && o <= k_hi) sum += to_int(weight(logit_of(o), most, r.inv, u));
+        });
+        sum = block_join<kFinish>(sum, mem.red, Add());
+        k_mass = c.above_k + ldexp((double)sum, -u);
+      }
     }
     if (r.top_p < 1.f) {
-      const uint64_t o_k = bound;
-      const int unit = bits + bin_exp(c.p_lo);
-      const uint64_t o_p = select_token<T, true>(
-          a, p, row, mem, n, [&](uint64_t o) { const int b = bin(o); return o >= o_k && b >= c.p_lo && b <= c.p_hi; }, most,
-          r.inv, unit, 0, c.above_p, (double)r.top_p * k_mass);
-      bound = max(bound, o_p);
-      whole = min(whole, bin(o_p));
+      p_hi = block_join<kFinish>(p_hi, mem.red, Max());
+      p_lo = max(bound, block_join<kFinish>(p_lo, mem.red, Min()));
+      if (p_lo <= p_hi) {
+        bound = select_token<T, true>(a, p, row, mem, n, p_lo, p_hi, most, r.inv, bits + bin_exp(c.p_lo), 0, c.above_p,
+                                      (double)r.top_p * k_mass);
+        whole = min(whole, bin(bound));
+      }
     }
     whole = min(whole, c.m_lo);
-    // what stays of each slice: its whole bins, then its listed tokens
-    for (int s = wave; s < p.slices; s += kFinish / 64) {
-      const Slice x = slice[s];
-      const int off = slice_offset(logit_of(x.top), most, c.step, r.inv);
-      const int64_t at = (row * p.slices + s) * kBins;
-      double m = 0;
-      for (int i = lane; i < x.bins && min(i + off, kBins - 1) < whole; i += 64)
-        m += ldexp((double)p.mass[at + i], -48 - bin_exp(i));
+    unit = bits + bin_exp(whole);
+    auto stays = [&](uint64_t o) -> uint64_t {
+      if (o < bound || bin(o) < whole) return 0;
+      const double w = weight(logit_of(o), most, r.inv);
+      return w >= (double)r.min_p ? to_int(ldexp(w, unit)) : 0;
+    };
+    if (n <= kCached) {
+      for (int s = wave; s < p.slices; s += kFinish / 64) {
+        const uint32_t from = mem.start[s], to = mem.start[s + 1];
+        if (from == to) continue;
+        uint64_t sum = 0;
+        for (uint32_t i = from + lane; i < to; i += 64) sum += stays(mem.token[i]);
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
-      if (lane == 0) mem.keep[s] = m * weight(logit_of(x.top), most, r.inv);
-    }
-    const int unit = bits + bin_exp(whole);
-    each_listed<T>(a, p, row, mem, n, [&](uint64_t o, uint32_t) {
-      if (o < bound || bin(o) < whole) return;
-      const double w = weight(logit_of(o), most, r.inv);
-      if (w >= (double)r.min_p)
-        atomicAdd((unsigned long long*)&mem.part[id_of(o) / p.per], to_int(ldexp(w, unit)));
-    });
-    __syncthreads();
-    for (int s = tid; s < p.slices; s += kFinish) mem.keep[s] += ldexp((double)mem.part[s], -unit);
-  } else {
-    for (int s = tid; s < p.slices; s += kFinish) {
-      const float first = logit_of(slice[s].top);
-      mem.keep[s] = first == -__builtin_inff() ? 0.0 : slice[s].mass * weight(first, most, r.inv);
-    }
-  }
-  // a slice whose first token stays has some weight, however small
-  __syncthreads();
-  double mine = 0;
-  if (tid < p.slices) {
-    mine = mem.keep[tid];
-    const uint64_t o = slice[tid].top;
-    if (logit_of(o) > -__builtin_inff() && o >= bound) {
-      const double w = weight(logit_of(o), most, r.inv);
-      if (w >= (double)r.min_p) mine = fmax(mine, w);
-      else mine = 0;
+        for (int k = 32; k > 0; k >>= 1) sum += __shfl_xor(sum, k, 64);
+        if (lane == 0) mem.part[s] = sum;
+      }
     } else {
-      mine = 0;
+      each_in_memory<T>(a, p, row, mem, [&](uint64_t o, uint32_t) {
+        const uint64_t w = stays(o);
+        if (w) atomicAdd((unsigned long long*)&mem.part[id_of(o) / p.per], (unsigned long long)w);
+      });
     }
+    __syncthreads();
   }
-  double total;
-  const double before = block_scan<kFinish>(mine, mem.redd, &total);
+  // the slice that the number falls into
+  double total = 0;
+  auto keep = [&](int s) {
+    if (s >= p.slices) return 0.0;
+    const Slice x = slice[s];
+    const float first = logit_of(x.top);
+    if (!counts(first, most) || x.top < bound) return 0.0;
+    const double w = weight(first, most, r.inv);
+    if (w < (double)r.min_p) return 0.0;
+    double m = x.mass;
+    if (r.cut) {
+      const double own = floor(grid_of(first, r.inv)), to = last_step(whole - 1, step);
+      if (whole < kBins) {
+        m = 0;
+        if (whole > 0 && x.bins > 0 && to <= own)
+          m = p.mass[(row * p.slices + s) * kBins + min(bin_of_step(to, own), x.bins - 1)];
+      }
+      m = m * w + ldexp((double)mem.part[s], -unit);
+    } else {
+      m *= w;
+    }
+    return fmax(w, m);  // (a slice whose first token stays has some weight, however small)
+  };
+  double mine[kMaxSlices / kFinish], at[kMaxSlices / kFinish];
+#pragma unroll
+  for (int i = 0; i < kMaxSlices / kFinish; i++) {
+    mine[i] = at[i] = 0;
+    if (i * kFinish >= p.slices) continue;
+    mine[i] = keep(i * kFinish + tid);
+    double all;
+    at[i] = total + block_scan<kFinish>(mine[i], mem.redd, &all);
+    total += all;
+  }
   const double aim = (double)r.u * total;
-  if (tid == 0) mem.found[0] = kMaxSlices, mem.found[1] = 0;
+  if (tid == 0) mem.found = -1;
   __syncthreads();
-  if (mine > 0) {
-    atomicMax(&mem.found[1], tid);
-    if (before + mine > aim) atomicMin(&mem.found[0], tid);
+#pragma unroll
+  for (int i = 0; i < kMaxSlices / kFinish; i++)
+    if (at[i] <= aim && at[i] + mine[i] > aim) mem.found = i * kFinish + tid, mem.found_before = at[i];
+  __syncthreads();
+  int s = mem.found;
+  if (s < 0) {  // (rounding: the last slice of any weight)
+    int last = -1;
+#pragma unroll
+    for (int i = 0; i < kMaxSlices / kFinish; i++)
+      if (mine[i] > 0) last = i * kFinish + tid;
+    s = block_join<kFinish>(last, (int*)mem.red, Max());
+#pragma unroll
+    for (int i = 0; i < kMaxSlices / kFinish; i++)
+      if (s == i * kFinish + tid) mem.found_before = at[i];
+    __syncthreads();
   }
-  __syncthreads();
-  const int s = mem.found[0] < kMaxSlices ? mem.found[0] : mem.found[1];
-  if (tid == s) mem.keep[0] = before;
-  __syncthreads();
-  // the walk: each thread a run of the slice's ids
-  const double rest = aim - mem.keep[0];
-  const int first = s * p.per, end = min((int)a.vocab, first + p.per), each = p.per / kFinish;
-  const int i0 = min(end, first + tid * each), i1 = min(end, i0 + each);
-  auto share = [&](int i) {
-    const float v = value_of(l[i]);
-    const uint64_t o = order_of(v, i);
-    if (o < bound || !(v > -__builtin_inff())) return 0.0;
+  // the walk: each wave weighs a run of the slice's ids, the one that the number falls into goes along it
+  const double rest = aim - mem.found_before;
+  const int first = s * p.per + wave * 64 * E + lane, end = (int)a.vocab;
+  auto share = [&](float v, int id) {
+    if (id >= end || !counts(v, most) || order_of(v, id) < bound) return 0.0;
     const double w = weight(v, most, r.inv);
     return w >= (double)r.min_p ? w : 0.0;
   };
   double run = 0;
-  for (int i = i0; i < i1; i++) run += share(i);
-  double unused;
-  const double at0 = block_scan<kFinish>(run, mem.redd, &unused);
-  __syncthreads();
-  if (tid == 0) mem.found[0] = kFinish, mem.found[1] = 0;
-  __syncthreads();
-  if (run > 0) {
-    atomicMax(&mem.found[1], tid);
-    if (at0 + run > rest) atomicMin(&mem.found[0], tid);
+#pragma unroll 1
+  for (int e = 0; e < E; e += kAhead) {
+    float v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) v[i] = value_of(l[min(first + (e + i) * 64, end - 1)]);
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) run += share(v[i], first + (e + i) * 64);
   }
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) run += __shfl_xor(run, k, 64);
   __syncthreads();
-  if (tid == (mem.found[0] < kFinish ? mem.found[0] : mem.found[1])) {
-    double at = at0;
-    int id = -1;
-    for (int i = i0; i < i1; i++) {
-      const double w = share(i);
-      if (w > 0) {
-        id = i;
-        at += w;
-        if (at > rest) break;
+  if (lane == 0) mem.redd[wave] = run;
+  __syncthreads();
+  int who = -1;
+  double before = 0, sum = 0;
+#pragma unroll
+  for (int i = 0; i < kFinish / 64; i++) {
+    const double x = mem.redd[i];
+    if (x > 0 && (who < 0 || sum <= rest)) who = i, before = sum;  // (the last of any weight, should none reach it)
+    sum += x;
+  }
+  if (wave != who) return;
+  int id = -1;
+  float x = most;
+  bool done = false;
+#pragma unroll 1
+  for (int e = 0; e < E && !done; e += kAhead) {
+    float v[kAhead];
+    double w[kAhead], upto[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) v[i] = value_of(l[min(first + (e + i) * 64, end - 1)]);
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) upto[i] = w[i] = share(v[i], first + (e + i) * 64);
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1)
+#pragma unroll
+      for (int i = 0; i < kAhead; i++) {
+        const double y = __shfl_up(upto[i], k, 64);
+        if (lane >= k) upto[i] += y;
       }
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+      const uint64_t any = __ballot(w[i] > 0), past = __ballot(w[i] > 0 && before + upto[i] > rest);
+      if (any && !done) {
+        const int pick = past ? __ffsll((unsigned long long)past) - 1 : 63 - __builtin_clzll(any);
+        id = __builtin_amdgcn_readlane(first + (e + i) * 64, pick);
+        x = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v[i]), pick));
+      }
+      done |= past != 0;
+      before += __shfl(upto[i], 63, 64);
     }
+  }
+  if (lane == 0) {
     a.ids[row] = id;
-    const float v = value_of(l[max(id, 0)]);
-    if (a.logp) a.logp[row] = (float)((v == most ? 0.0 : ((double)v - (double)most) * r.inv) - log(total));
+    if (a.logp) a.logp[row] = (float)((x == most ? 0.0 : ((double)x - (double)most) * r.inv) - log(total));
   }
 }
 
 // ---- the division of rows ----------------------------------------------------------------------------
 
 int per_of(int64_t rows, int64_t vocab) {
-  // few workgroups: shorter slices; a row has no more than kMaxSlices
-  if (vocab > (int64_t)kMaxSlices * 16 * kScan) return 32 * kScan;
-  return rows * ((vocab + 16 * kScan - 1) / (16 * kScan)) < 256 && vocab <= (int64_t)kMaxSlices * 8 * kScan ? 8 * kScan
-                                                                                                             : 16 * kScan;
+  // few workgroups: shorter slices, but not so many that joining them takes longer (64 of a row: 17 us, 32: 9); a row has
+  // no more than kMaxSlices
+  const auto slices = [&](int e) { return (vocab + e * kScan - 1) / (e * kScan); };
+  if (slices(8) <= 16 && (rows * slices(8) <= 1024 || slices(8) == 1)) return 8 * kScan;
+  return slices(16) <= kMaxSlices ? 16 * kScan : 32 * kScan;
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -729,7 +887,7 @@ size_t lay_out(int64_t rows, int64_t vocab, char* work, Plan* p) {
   Plan q = {per, (int)slices, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   q.slice = (Slice*)take(all * sizeof(Slice));
   q.cut = (Cut*)take(rows * sizeof(Cut));
-  q.mass = (uint64_t*)take(all * kBins * 8);
+  q.mass = (double*)take(all * kBins * 8);
   q.count = (uint32_t*)take(all * kBins * 4);
   q.listed = (uint32_t*)take(all * 4);
   q.list = (uint16_t*)take(all * per * 2);
@@ -745,7 +903,7 @@ void launch_e(const SampleArgs& a, const Plan& p, hipStream_t s) {
     join_kernel<<<(unsigned)a.rows, kBins, 0, s>>>(a, p);
     gather_kernel<T, E><<<grid, kScan, 0, s>>>(a, p);
   }
-  finish_kernel<T><<<(unsigned)a.rows, kFinish, 0, s>>>(a, p);
+  finish_kernel<T, E * kScan / kFinish><<<(unsigned)a.rows, kFinish, 0, s>>>(a, p);
 }
 
 template <typename T>
