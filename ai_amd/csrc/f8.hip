@@ -9,14 +9,18 @@
 // results need the sums that lose nothing: a code times its scale is exact in bf16,
 // so they come from the bf16 units, whose products are exact and sums float32.
 #include <algorithm>
+#include <type_traits>
 
 #include "f8.h"
+#include "gemm_common.h"
 
 namespace fa {
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -63,70 +67,431 @@ __global__ __launch_bounds__(256) void f8_read_kernel(F8View w, T* __restrict__ 
   }
 }
 
-// The epilogue of one value.
-__device__ __forceinline__ float epilogue(const fa_epilogue& e, float v, int64_t row, int64_t col) {
-  if (e.bias) v = v + e.bias[col];
-  if (e.row_scale) v = v * e.row_scale[row];
-  if (e.act == FA_ACT_RELU) v = fmaxf(v, 0.f);
-  else if (e.act == FA_ACT_GELU) v = gelu_tanh_ref(v);
-  else if (e.act == FA_ACT_TANH) v = tanh_ref(v);
-  if (e.mul) v = v * e.mul[row * e.ldm + col];
-  if (e.residual) v = v + e.residual[row * e.ldr + col];
-  return v;
-}
-__device__ __forceinline__ void put(float* c, float v) { *c = v; }
-__device__ __forceinline__ void put(uint16_t* c, float v) { *c = bf16_bits(v); }
-
 struct GemmParams {
-  int64_t m, n;
-  int kb, ks;
+  int64_t m, n, k;
+  int kb, ks;  // blocks of a row, its scale bytes
   const uint8_t *a, *as, *w, *ws;  // codes and scale bytes
+  const void* raw;                 // A before it is quantised (few rows)
+  int64_t ldr;
+  int vec;                         // raw rows aligned for 16-byte loads
   fa_epilogue e;
+  int vec_bias, vec_mul, vec_residual, vec_c;  // aligned for four values at a time
   int64_t ldc;
+  int split;                       // waves that share a row's blocks (few rows)
 };
 
-// 8 codes times a power of two, exact in bf16.
-__device__ __forceinline__ bf16x8 widen8(uint2 w, float s) {
-  const f32x4 a = unpack4(w.x) * s, b = unpack4(w.y) * s;
-  bf16x8 r;
+// Two codes times a power of two, exact in bf16.
+__device__ __forceinline__ uint32_t widen2(uint32_t w, float s, bool hi) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 r = hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false);
+  return __builtin_bit_cast(uint32_t, r);
+}
+// Eight codes as an operand of the bf16 units.
+__device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float s) {
+  const uint4 r = make_uint4(widen2(lo, s, false), widen2(lo, s, true), widen2(hi, s, false), widen2(hi, s, true));
+  return __builtin_bit_cast(bf16x8, r);
+}
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }  // 2^(byte - 127)
+
+// R rows of C, four neighbouring values of each, through the epilogue: what it reads of
+// all of them under way at once. Rows and columns past C are left out.
+template <int R, typename T>
+__device__ __forceinline__ void put4(const GemmParams& p, T* c, const int64_t (&row)[R], int64_t col, f32x4 (&v)[R]) {
+  const int n = (int)p.n, at = (int)col;
+  f32x4 bias = {0.f, 0.f, 0.f, 0.f}, mul[R], residual[R];
+  float scale[R];
+  if (p.e.bias) bias = load4(p.e.bias, at, n, p.vec_bias);
 #pragma unroll
-  for (int i = 0; i < 4; i++) r[i] = (__bf16)a[i], r[4 + i] = (__bf16)b[i];
-  return r;
+  for (int i = 0; i < R; i++) {
+    const int64_t r = min(row[i], p.m - 1);
+    scale[i] = 1.f;
+    if (p.e.row_scale) scale[i] = p.e.row_scale[r];
+    if (p.e.mul) mul[i] = load4(p.e.mul + r * p.e.ldm, at, n, p.vec_mul);
+    if (p.e.residual) residual[i] = load4(p.e.residual + r * p.e.ldr, at, n, p.vec_residual);
+  }
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    if (p.e.bias) v[i] = v[i] + bias;
+    if (p.e.row_scale) v[i] = v[i] * scale[i];
+  }
+  if (p.e.act != FA_ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < R; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float x = v[i][j];
+        v[i][j] = p.e.act == FA_ACT_RELU ? fmaxf(x, 0.f) : p.e.act == FA_ACT_GELU ? gelu_tanh_ref(x) : tanh_ref(x);
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    if (p.e.mul) v[i] = v[i] * mul[i];
+    if (p.e.residual) v[i] = v[i] + residual[i];
+    if (row[i] < p.m) store4(c + row[i] * p.ldc, at, n, p.vec_c, v[i]);
+  }
 }
 
-// One wave computes a tile of 16 x 16, its operands straight from memory.
+// ---- few rows -----------------------------------------------------------------------
+
+// A block of 32 codes of this lane (row r of 16, columns 32 g .. of the block): A
+// quantised on the way. Lanes r, r + 16, r + 32, r + 48 hold a row's block.
 template <typename T>
-__global__ __launch_bounds__(256) void f8_gemm_kernel(GemmParams p, T* __restrict__ c) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-  const int64_t cols = (p.n + 63) / 64;
-  const int64_t m0 = blockIdx.x / cols * 16, n0 = (blockIdx.x % cols) * 64 + wave * 16;
-  if (n0 >= p.n) return;
-  const int64_t ar = min(m0 + r, p.m - 1), wr = min(n0 + r, p.n - 1);
-  const int64_t kp = (int64_t)p.kb * kF8Block;
-  const uint8_t *a = p.a + ar * kp + g * 32, *w = p.w + wr * kp + g * 32;
-  const uint8_t *as = p.as + ar * p.ks, *ws = p.ws + wr * p.ks;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int b = 0; b < p.kb; b++) {
-    const uint8_t *ab = a + (int64_t)b * kF8Block, *wb = w + (int64_t)b * kF8Block;
-    if constexpr (sizeof(T) == 2) {
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(*reinterpret_cast<const i32x8*>(ab),
-                                                             *reinterpret_cast<const i32x8*>(wb), acc, 0, 0, 0,
-                                                             (int)as[b], 0, (int)ws[b]);
-    } else {
-      const float sa = exp2_int((int)as[b] - 127), sw = exp2_int((int)ws[b] - 127);
+__device__ __forceinline__ float quantize_block(const T* x, int d, int k, bool vec, uint32_t (&code)[8]) {
+  f32x4 v[8];
+  float big = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; i++)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8(*reinterpret_cast<const uint2*>(ab + i * 8), sa),
-                                                      widen8(*reinterpret_cast<const uint2*>(wb + i * 8), sw), acc, 0,
-                                                      0, 0);
+  for (int i = 0; i < 8; i++) {
+    v[i] = load4(x, d + 4 * i, k, vec);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      float y = v[i][j];
+      join_max(y, big);
+      v[i][j] = y;
     }
   }
-  const int64_t col = n0 + r;
+  big = fmaxf(big, lane_xor16(big));
+  big = fmaxf(big, lane_xor32(big));
+  const int e = scale_exp(big);
+  const float inv = exp2_int(-e);
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int64_t row = m0 + g * 4 + i;
-    if (row < p.m && col < p.n) put(c + row * p.ldc + col, epilogue(p.e, acc[i], row, col));
+  for (int i = 0; i < 8; i++) {
+    if (e == kMaxExp) v[i] = f32x4{clamp_top(v[i][0]), clamp_top(v[i][1]), clamp_top(v[i][2]), clamp_top(v[i][3])};
+    code[i] = pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
   }
+  return exp2_int(e);
+}
+
+// Up to 16 MT rows. A wave computes 16 CN columns of C over every split-th block of
+// 128, on the bf16 units (whose operands, codes times powers of two, are exact: the
+// time goes into reading W, not into products); the waves of a column group add up
+// through LDS, in their order. W comes straight from memory in the units' order: 16
+// rows of 128 bytes a block, kDeep blocks under way. A: quantised here (RAW: up to 16
+// rows, where a launch of its own would cost more), or codes.
+constexpr int kFewWaves = 8, kDeep = 4;
+template <typename TA, typename TC, int MT, int CN, bool RAW>
+__device__ __forceinline__ void f8_few(const GemmParams& p, TC* c) {
+  __shared__ f32x4 part[kFewWaves][MT * CN][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+  const int group = wave / p.split, ks = wave % p.split;  // split divides kFewWaves
+  const int64_t n0 = ((int64_t)blockIdx.x * (kFewWaves / p.split) + group) * (16 * CN);
+  const int64_t kp = (int64_t)p.kb * kF8Block;
+  const uint8_t *w[CN], *ws[CN], *a[MT], *as[MT];
+#pragma unroll
+  for (int j = 0; j < CN; j++) {
+    const int64_t row = min(n0 + j * 16 + r, p.n - 1);
+    w[j] = p.w + row * kp + g * 32;
+    ws[j] = p.ws + row * p.ks;
+  }
+#pragma unroll
+  for (int i = 0; i < MT; i++) {
+    const int64_t row = min((int64_t)i * 16 + r, p.m - 1);
+    a[i] = RAW ? reinterpret_cast<const uint8_t*>(static_cast<const TA*>(p.raw) + row * p.ldr) : p.a + row * kp + g * 32;
+    as[i] = p.as + row * p.ks;
+  }
+  f32x4 acc[MT][CN] = {};
+  uint4 cw[kDeep][CN][2];
+  uint32_t cs[kDeep][CN];
+  auto load = [&](int d, int b) {  // (blocks past the last: the last again, not used)
+    const int at = min(b, p.kb - 1);
+#pragma unroll
+    for (int j = 0; j < CN; j++) {
+      const uint4* q = reinterpret_cast<const uint4*>(w[j] + (int64_t)at * kF8Block);
+      cw[d][j][0] = q[0];
+      cw[d][j][1] = q[1];
+      cs[d][j] = ws[j][at];
+    }
+  };
+  if (p.kb > 0) {
+#pragma unroll
+    for (int d = 0; d < kDeep; d++) load(d, ks + d * p.split);
+  }
+  for (int b0 = ks; b0 < p.kb; b0 += kDeep * p.split) {
+#pragma unroll
+    for (int d = 0; d < kDeep; d++) {
+      const int b = b0 + d * p.split;
+      if (b >= p.kb) break;  // (uniform in the wave)
+      bf16x8 ww[CN][4];
+#pragma unroll
+      for (int j = 0; j < CN; j++) {
+        const float s = scale_of(cs[d][j]);
+        ww[j][0] = widen8(cw[d][j][0].x, cw[d][j][0].y, s);
+        ww[j][1] = widen8(cw[d][j][0].z, cw[d][j][0].w, s);
+        ww[j][2] = widen8(cw[d][j][1].x, cw[d][j][1].y, s);
+        ww[j][3] = widen8(cw[d][j][1].z, cw[d][j][1].w, s);
+      }
+      load(d, b + kDeep * p.split);
+#pragma unroll
+      for (int i = 0; i < MT; i++) {
+        uint32_t code[8];
+        float s;
+        if constexpr (RAW) {
+          s = quantize_block(reinterpret_cast<const TA*>(a[i]), b * kF8Block + g * 32, (int)p.k, p.vec, code);
+        } else {
+          const uint4* q = reinterpret_cast<const uint4*>(a[i] + (int64_t)b * kF8Block);
+          const uint4 x = q[0], y = q[1];
+          code[0] = x.x, code[1] = x.y, code[2] = x.z, code[3] = x.w;
+          code[4] = y.x, code[5] = y.y, code[6] = y.z, code[7] = y.w;
+          s = scale_of(as[i][b]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const bf16x8 aa = widen8(code[2 * q], code[2 * q + 1], s);
+#pragma unroll
+          for (int j = 0; j < CN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[j][q], aa, acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+  }
+  // lane: row r of A, columns 4 g .. + 3
+  if (p.split > 1) {
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < CN; j++) part[wave][i * CN + j][lane] = acc[i][j];
+    __syncthreads();
+    // the waves of a group share its tiles
+    for (int t = ks; t < MT * CN; t += p.split) {
+      f32x4 v = part[group * p.split][t][lane];
+      for (int s = 1; s < p.split; s++) v = v + part[group * p.split + s][t][lane];
+      const int64_t row[1] = {(int64_t)(t / CN) * 16 + r}, col = n0 + (t % CN) * 16 + g * 4;
+      f32x4 one[1] = {v};
+      if (col < p.n) put4(p, c, row, col, one);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int j = 0; j < CN; j++) {
+        const int64_t row[1] = {(int64_t)i * 16 + r}, col = n0 + j * 16 + g * 4;
+        f32x4 one[1] = {acc[i][j]};
+        if (col < p.n) put4(p, c, row, col, one);
+      }
+  }
+}
+
+template <typename TA, typename TC, int MT, int CN, bool RAW>
+__global__ __launch_bounds__(kFewWaves * 64) void f8_few_kernel(GemmParams p, TC* c) {
+  f8_few<TA, TC, MT, CN, RAW>(p, c);
+}
+
+// ---- tiles ---------------------------------------------------------------------------------
+
+// Workgroup barrier after the wave's direct loads to LDS have landed and its LDS reads are done.
+__device__ __forceinline__ void tile_barrier() {
+  __builtin_amdgcn_s_waitcnt(0);  // every counter
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// Order of a half block's READS reads of operands, LOADS loads to LDS and PRODUCTS
+// products (0: left to the compiler): the reads in turn with products, so that they
+// arrive under them, the loads among the first half of these (at the next meeting
+// every load has to have landed).
+template <int READS, int LOADS, int PRODUCTS>
+__device__ __forceinline__ void mix() {
+  constexpr int R = PRODUCTS ? (READS + PRODUCTS - 1) / PRODUCTS : 0, L = PRODUCTS ? (2 * LOADS + PRODUCTS - 1) / PRODUCTS : 0;
+#pragma unroll
+  for (int i = 0; i < PRODUCTS; i++) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    if (i * R < READS) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    if (i * L < LOADS) __builtin_amdgcn_sched_group_barrier(0x20, L, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Four waves, each a quarter (BM / 2 x BN / 2) of the tile in 32 x 32 products. A
+// block of both operands (128 bytes of each row) goes straight from memory to LDS, two
+// blocks held: at the middle of a block the waves have read all of it, meet once,
+// and start the loads of the block after next into its place. Rows lie 128 bytes
+// apart, their 16-byte pieces permuted by the row (piece j at j ^ (row & 7)), so that
+// eight lanes reading the same piece of eight rows use all banks. Operands of the
+// next half block are read while the products of this one run.
+template <int BM, int BN, typename TC>
+__device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m, int tiles_n) {
+  constexpr int FM = BM / 64, FN = BN / 64, NA = BM * 8 / 256, NB = BN * 8 / 256;
+  constexpr bool F8 = sizeof(TC) == 2;  // on the 8-bit units
+  constexpr int kStage = (BM + BN) * kF8Block;
+  __shared__ __attribute__((aligned(16))) uint8_t S0[kStage], S1[kStage];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+  const int64_t kp = (int64_t)p.kb * kF8Block;
+  // Tiles of an XCD's run are taken in groups of 8 tile rows, down the columns: the
+  // ones that run together share their rows of A and of W in its L2.
+  int tm, tn;
+  {
+    const int tile = xcd_tile(tiles_m, tiles_n);
+    constexpr int G = 8;
+    const int group = tile / (G * tiles_n), rows = min(G, tiles_m - group * G), at = tile - group * G * tiles_n;
+    tm = group * G + at % rows;
+    tn = at / rows;
+  }
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  // the tile's first rows (the same for the workgroup), and a thread's pieces from there
+  const uint8_t *a0 = p.a + m0 * kp, *b0 = p.w + n0 * kp;
+  uint32_t ga[NA], gb[NB];
+  {
+    const int row = tid >> 3, piece = (tid & 7) ^ (row & 7);
+    const int rows_a = (int)min(p.m - m0, (int64_t)BM) - 1, rows_b = (int)min(p.n - n0, (int64_t)BN) - 1;
+#pragma unroll
+    for (int i = 0; i < NA; i++) ga[i] = (uint32_t)min(i * 32 + row, rows_a) * (uint32_t)kp + piece * 16;
+#pragma unroll
+    for (int i = 0; i < NB; i++) gb[i] = (uint32_t)min(i * 32 + row, rows_b) * (uint32_t)kp + piece * 16;
+  }
+  auto stage = [&](uint8_t* s, int b) {
+    const uint8_t *a = a0 + (int64_t)b * kF8Block, *w = b0 + (int64_t)b * kF8Block;
+#pragma unroll
+    for (int i = 0; i < NA; i++)
+      __builtin_amdgcn_global_load_lds(a + ga[i], (__attribute__((address_space(3))) void*)(s + (i * 256 + wave * 64) * 16), 16, 0, 0);
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+      __builtin_amdgcn_global_load_lds(
+          w + gb[i], (__attribute__((address_space(3))) void*)(s + BM * kF8Block + (i * 256 + wave * 64) * 16), 16, 0, 0);
+  };
+  // operands: row lane % 32, bytes 32 (lane / 32) .. + 31 of each half block
+  const int row = lane & 31, half = lane >> 5;
+  const int a_at = (wm * (BM / 2) + row) * kF8Block, b_at = BM * kF8Block + (wn * (BN / 2) + row) * kF8Block;
+  int piece[2][2];
+#pragma unroll
+  for (int h = 0; h < 2; h++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) piece[h][j] = ((h * 4 + half * 2 + j) ^ (row & 7)) * 16;
+  struct Ops {
+    i32x8 a[FM], b[FN];
+  };
+  auto two = [&](const uint8_t* s, int h) {
+    const i32x4 x = *reinterpret_cast<const i32x4*>(s + piece[h][0]), y = *reinterpret_cast<const i32x4*>(s + piece[h][1]);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto read = [&](const uint8_t* s, int h, Ops& o) {
+#pragma unroll
+    for (int f = 0; f < FN; f++) o.b[f] = two(s + b_at + f * 32 * kF8Block, h);
+#pragma unroll
+    for (int f = 0; f < FM; f++) o.a[f] = two(s + a_at + f * 32 * kF8Block, h);
+  };
+  // scale bytes of four blocks at a time
+  const uint8_t *as0 = p.as + m0 * p.ks, *bs0 = p.ws + n0 * p.ks;
+  uint32_t sa[FM], sb[FN];
+#pragma unroll
+  for (int f = 0; f < FM; f++)
+    sa[f] = (uint32_t)min((int64_t)(wm * (BM / 2) + f * 32 + row), p.m - 1 - m0) * (uint32_t)p.ks;
+#pragma unroll
+  for (int f = 0; f < FN; f++)
+    sb[f] = (uint32_t)min((int64_t)(wn * (BN / 2) + f * 32 + row), p.n - 1 - n0) * (uint32_t)p.ks;
+  uint32_t xa[FM], xb[FN], na[FM], nb[FN];
+  auto scales = [&](int b) {  // (rows of scale bytes are whole groups of four)
+    const int at = min(b, p.ks - 4);
+#pragma unroll
+    for (int f = 0; f < FM; f++) na[f] = *reinterpret_cast<const uint32_t*>(as0 + at + sa[f]);
+#pragma unroll
+    for (int f = 0; f < FN; f++) nb[f] = *reinterpret_cast<const uint32_t*>(bs0 + at + sb[f]);
+  };
+  f32x16 acc[FM][FN] = {};
+  auto multiply = [&](const Ops& o, auto sel) {
+    constexpr int SEL = decltype(sel)::value;  // the block's byte of the scales
+    if constexpr (F8) {
+#pragma unroll
+      for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(o.a[i], o.b[j], acc[i][j], 0, 0, SEL, (int)xa[i], SEL, (int)xb[j]);
+    } else {
+      float ea[FM], eb[FN];
+#pragma unroll
+      for (int i = 0; i < FM; i++) ea[i] = scale_of(xa[i] >> (8 * SEL) & 255);
+#pragma unroll
+      for (int j = 0; j < FN; j++) eb[j] = scale_of(xb[j] >> (8 * SEL) & 255);
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        bf16x8 x[FM], y[FN];
+#pragma unroll
+        for (int i = 0; i < FM; i++) x[i] = widen8((uint32_t)o.a[i][2 * q], (uint32_t)o.a[i][2 * q + 1], ea[i]);
+#pragma unroll
+        for (int j = 0; j < FN; j++) y[j] = widen8((uint32_t)o.b[j][2 * q], (uint32_t)o.b[j][2 * q + 1], eb[j]);
+#pragma unroll
+        for (int i = 0; i < FM; i++)
+#pragma unroll
+          for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[i], y[j], acc[i][j], 0, 0, 0);
+      }
+    }
+  };
+  Ops X, Y;
+  // Block b, in s (its first half in X already); the next one is in `next`. Past the
+  // last block the last is loaded again and not used: no branch in the loop.
+  auto block = [&](uint8_t* s, uint8_t* next, int b, auto sel) {
+    read(s, 1, Y);
+    multiply(X, sel);
+    mix<2 * (FM + FN), 0, F8 ? FM * FN : 0>();
+    tile_barrier();
+    stage(s, min(b + 2, p.kb - 1));
+    read(next, 0, X);
+    multiply(Y, sel);
+    mix<2 * (FM + FN), NA + NB, F8 ? FM * FN : 0>();
+  };
+  using std::integral_constant;
+  if (p.kb > 0) {
+    scales(0);
+    stage(S0, 0);
+    stage(S1, min(1, p.kb - 1));
+    tile_barrier();
+    read(S0, 0, X);
+    int b = 0;
+    for (; b + 4 <= p.kb; b += 4) {
+#pragma unroll
+      for (int f = 0; f < FM; f++) xa[f] = na[f];
+#pragma unroll
+      for (int f = 0; f < FN; f++) xb[f] = nb[f];
+      scales(b + 4);
+      block(S0, S1, b, integral_constant<int, 0>());
+      block(S1, S0, b + 1, integral_constant<int, 1>());
+      block(S0, S1, b + 2, integral_constant<int, 2>());
+      block(S1, S0, b + 3, integral_constant<int, 3>());
+    }
+#pragma unroll
+    for (int f = 0; f < FM; f++) xa[f] = na[f];
+#pragma unroll
+    for (int f = 0; f < FN; f++) xb[f] = nb[f];
+    if (b < p.kb) block(S0, S1, b, integral_constant<int, 0>());
+    if (b + 1 < p.kb) block(S1, S0, b + 1, integral_constant<int, 1>());
+    if (b + 2 < p.kb) block(S0, S1, b + 2, integral_constant<int, 2>());
+    tile_barrier();  // (the loads that are not used)
+  }
+  // through LDS, 32 rows of the wave at a time, so that rows of C are written whole
+  __syncthreads();
+  constexpr int kRow = BN / 2 + 4;
+  static_assert(4 * 32 * kRow * 4 <= 2 * kStage, "the tile's rows fit");
+  float* mine = reinterpret_cast<float*>(wave < 2 ? S0 : S1) + (wave & 1) * 32 * kRow;
+#pragma unroll
+  for (int i = 0; i < FM; i++) {
+#pragma unroll
+    for (int j = 0; j < FN; j++)
+#pragma unroll
+      for (int q = 0; q < 16; q++) mine[((q >> 2) * 8 + half * 4 + (q & 3)) * kRow + j * 32 + row] = acc[i][j][q];
+    __syncthreads();
+    constexpr int kLanes = BN / 8, kRows = 64 / kLanes, R = 4;  // lanes of a row, rows at once, of those under way
+    const int tc = lane % kLanes * 4;
+    const int64_t col = n0 + wn * (BN / 2) + tc;
+#pragma unroll 1
+    for (int t = 0; t < 32; t += kRows * R) {
+      int64_t at[R];
+      f32x4 v[R];
+#pragma unroll
+      for (int k = 0; k < R; k++) {
+        const int tr = t + k * kRows + lane / kLanes;
+        at[k] = m0 + wm * (BM / 2) + i * 32 + tr;
+        v[k] = *reinterpret_cast<const f32x4*>(mine + tr * kRow + tc);
+      }
+      if (col < p.n) put4(p, c, at, col, v);
+    }
+    __syncthreads();
+  }
+}
+
+// (A kernel whose own body holds arrays of dependent bounds in lambdas loses its host stub.)
+template <int BM, int BN, typename TC>
+__global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void f8_tile_kernel(GemmParams p, TC* c, int tiles_m,
+                                                                                 int tiles_n) {
+  f8_tile<BM, BN, TC>(p, c, tiles_m, tiles_n);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -157,22 +522,80 @@ int launch_f8_read(fa_ctx* ctx, const F8View& w, int dtype, void* out, int64_t l
   return FA_OK;
 }
 
+// Up to kRawRows rows A is quantised by the product itself, up to kFewRows a wave
+// takes all the rows of its columns.
+constexpr int64_t kRawRows = 16, kFewRows = 64;
+
 size_t f8_scratch(int64_t m, int64_t n, int64_t k) {
+  if (m <= kRawRows) return 0;
   return align256((size_t)m * f8_kp(k)) + align256((size_t)m * f8_ks(k));
 }
 
 int64_t f8_grid(int64_t m, int64_t n) { return ((m + 15) / 16) * ((n + 63) / 64); }
 
+namespace {
+
+template <typename TA, typename TC>
+void launch_gemm_t(const GemmParams& p, TC* c, int cus, hipStream_t s) {
+  if (p.m <= kFewRows) {
+    GemmParams q = p;
+    const int64_t groups = (p.n + 15) / 16;
+    q.split = 8;
+    while (q.split > 1 && (groups * q.split > 4096 * 2 || q.split > std::max(1, p.kb))) q.split /= 2;
+    const unsigned grid = (unsigned)((groups * q.split + kFewWaves - 1) / kFewWaves);
+    if (p.m <= kRawRows) f8_few_kernel<TA, TC, 1, 1, true><<<grid, kFewWaves * 64, 0, s>>>(q, c);
+    else if (p.m <= 32) f8_few_kernel<TA, TC, 2, 1, false><<<grid, kFewWaves * 64, 0, s>>>(q, c);
+    else f8_few_kernel<TA, TC, 4, 1, false><<<grid, kFewWaves * 64, 0, s>>>(q, c);
+    return;
+  }
+  const int64_t big = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+  if (sizeof(TC) == 2 && big >= cus) {
+    const int tm = (int)((p.m + 255) / 256), tn = (int)((p.n + 255) / 256);
+    f8_tile_kernel<256, 256, uint16_t><<<(unsigned)(tm * tn), 256, 0, s>>>(p, (uint16_t*)c, tm, tn);
+  } else {
+    const int tm = (int)((p.m + 127) / 128), tn = (int)((p.n + 127) / 128);
+    f8_tile_kernel<128, 128, TC><<<(unsigned)(tm * tn), 256, 0, s>>>(p, c, tm, tn);
+  }
+}
+
+}  // namespace
+
 int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s) {
   const int64_t k = g.w.k;
-  F8View a = {static_cast<uint8_t*>(work), static_cast<uint8_t*>(work) + align256((size_t)g.m * f8_kp(k)), g.m, k};
-  int rc;
-  if (k > 0 && (rc = launch_f8_write(ctx, a, g.a_dtype, g.a, g.lda, s))) return rc;
-  const GemmParams p = {g.m, g.w.n, (int)(f8_kp(k) / kF8Block), (int)f8_ks(k), a.codes, a.scales, g.w.codes, g.w.scales,
-                        g.e, g.ldc};
-  const unsigned grid = (unsigned)f8_grid(g.m, g.w.n);
-  if (g.c_dtype == FA_DT_F32) f8_gemm_kernel<float><<<grid, 256, 0, s>>>(p, (float*)g.c);
-  else f8_gemm_kernel<uint16_t><<<grid, 256, 0, s>>>(p, (uint16_t*)g.c);
+  F8View a = {nullptr, nullptr, g.m, k};
+  if (g.m > kRawRows && k > 0) {
+    a.codes = static_cast<uint8_t*>(work);
+    a.scales = a.codes + align256((size_t)g.m * f8_kp(k));
+    const int rc = launch_f8_write(ctx, a, g.a_dtype, g.a, g.lda, s);
+    if (rc) return rc;
+  }
+  GemmParams p = {};
+  p.m = g.m;
+  p.n = g.w.n;
+  p.k = k;
+  p.kb = (int)(f8_kp(k) / kF8Block);
+  p.ks = (int)f8_ks(k);
+  p.a = a.codes;
+  p.as = a.scales;
+  p.w = g.w.codes;
+  p.ws = g.w.scales;
+  p.raw = g.a;
+  p.ldr = g.lda;
+  p.vec = g.lda % 4 == 0 && aligned(g.a, g.a_dtype == FA_DT_F32 ? 16 : 8);
+  p.e = g.e;
+  p.vec_bias = aligned(g.e.bias, 16);
+  p.vec_mul = g.e.ldm % 4 == 0 && aligned(g.e.mul, 16);
+  p.vec_residual = g.e.ldr % 4 == 0 && aligned(g.e.residual, 16);
+  p.vec_c = g.ldc % 4 == 0 && aligned(g.c, g.c_dtype == FA_DT_F32 ? 16 : 8);
+  p.ldc = g.ldc;
+  const bool af = g.a_dtype == FA_DT_F32;
+  if (g.c_dtype == FA_DT_F32) {
+    if (af) launch_gemm_t<float>(p, (float*)g.c, ctx->cu_count, s);
+    else launch_gemm_t<uint16_t>(p, (float*)g.c, ctx->cu_count, s);
+  } else {
+    if (af) launch_gemm_t<float>(p, (uint16_t*)g.c, ctx->cu_count, s);
+    else launch_gemm_t<uint16_t>(p, (uint16_t*)g.c, ctx->cu_count, s);
+  }
   FA_CHECK_LAUNCH(ctx);
   return FA_OK;
 }
