@@ -24,33 +24,66 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-// One 32-lane half of a wave takes a block of 128 columns, four values a lane.
-// The lane of a row's last block also writes the scale bytes that pad the row.
-template <typename T>
+// 16 lanes take a block of 128 columns, eight values a lane, a wave 4 U neighbouring
+// blocks, all their loads under way at once. The lanes of a row's last block also
+// write the scale bytes that pad the row.
+template <typename T, int U>
 __global__ __launch_bounds__(256) void f8_write_kernel(F8View w, const T* __restrict__ x, int64_t ldx, int kb, int ks,
                                                        bool vec) {
-  const int64_t blocks = w.n * kb;
-  const int lane = threadIdx.x & 31;
-  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < blocks; i += (int64_t)gridDim.x * 8) {
-    const int64_t row = i / kb;
-    const int b = (int)(i - row * kb), d = b * kF8Block + lane * 4;
-    f32x4 v = load4(x + row * ldx, d, (int)w.k, vec);
+  const int lane = threadIdx.x & 63, l = lane & 15;
+  const int64_t first = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * (4 * U);
+  const int64_t blocks = w.n * kb, row0 = blocks >> 32 ? first / kb : (uint32_t)first / (uint32_t)kb;
+  const uint32_t b0 = (uint32_t)(first - row0 * kb);
+  f32x4 v[U][2];
+  int64_t row[U];
+  int b[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) {
+    const uint32_t at = b0 + u * 4 + (lane >> 4);
+    row[u] = row0 + at / (uint32_t)kb;
+    b[u] = (int)(at % (uint32_t)kb);
+    const bool in = first + u * 4 + (lane >> 4) < blocks;
+    const T* from = x + min(row[u], w.n - 1) * ldx;
+    const int d = b[u] * kF8Block + l * 8, k = in ? (int)w.k : 0;
+    if constexpr (sizeof(T) == 2) {
+      if (vec && d + 8 <= k) {
+        const uint4 q = *reinterpret_cast<const uint4*>(from + d);
+        v[u][0] = f32x4{__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xFFFF0000u), __uint_as_float(q.y << 16),
+                        __uint_as_float(q.y & 0xFFFF0000u)};
+        v[u][1] = f32x4{__uint_as_float(q.z << 16), __uint_as_float(q.z & 0xFFFF0000u), __uint_as_float(q.w << 16),
+                        __uint_as_float(q.w & 0xFFFF0000u)};
+        continue;
+      }
+    }
+    v[u][0] = load4(from, d, k, vec && sizeof(T) == 4);
+    v[u][1] = load4(from, d + 4, k, vec && sizeof(T) == 4);
+  }
+#pragma unroll
+  for (int u = 0; u < U; u++) {
     float big = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      float y = v[j];
+    for (int j = 0; j < 8; j++) {
+      float y = v[u][j >> 2][j & 3];
       join_max(y, big);
-      v[j] = y;
+      v[u][j >> 2][j & 3] = y;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 32));
+    // over the 16 lanes: rotations of a row of lanes
+    big = fmaxf(big, dpp_f32<0x128>(big));
+    big = fmaxf(big, dpp_f32<0x124>(big));
+    big = fmaxf(big, dpp_f32<0x122>(big));
+    big = fmaxf(big, dpp_f32<0x121>(big));
     const int e = scale_exp(big);
-    if (e == kMaxExp) v = f32x4{clamp_top(v[0]), clamp_top(v[1]), clamp_top(v[2]), clamp_top(v[3])};
+    if (e == kMaxExp) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[u][j >> 2][j & 3] = clamp_top(v[u][j >> 2][j & 3]);
+    }
     const float inv = exp2_int(-e);
-    reinterpret_cast<uint32_t*>(w.codes + row * kb * kF8Block)[b * 32 + lane] =
-        pack4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-    if (lane == 0) w.scales[row * ks + b] = (uint8_t)(e + 127);
-    if (b == kb - 1 && kb + lane < ks) w.scales[row * ks + kb + lane] = 127;
+    if (first + u * 4 + (lane >> 4) >= blocks) continue;
+    *reinterpret_cast<uint2*>(w.codes + (row[u] * kb + b[u]) * kF8Block + l * 8) =
+        make_uint2(pack4(v[u][0][0] * inv, v[u][0][1] * inv, v[u][0][2] * inv, v[u][0][3] * inv),
+                   pack4(v[u][1][0] * inv, v[u][1][1] * inv, v[u][1][2] * inv, v[u][1][3] * inv));
+    if (l == 0) w.scales[row[u] * ks + b[u]] = (uint8_t)(e + 127);
+    if (b[u] == kb - 1 && kb + l < ks) w.scales[row[u] * ks + kb + l] = 127;
   }
 }
 
@@ -71,9 +104,6 @@ struct GemmParams {
   int64_t m, n, k;
   int kb, ks;  // blocks of a row, its scale bytes
   const uint8_t *a, *as, *w, *ws;  // codes and scale bytes
-  const void* raw;                 // A before it is quantised (few rows)
-  int64_t ldr;
-  int vec;                         // raw rows aligned for 16-byte loads
   fa_epilogue e;
   int vec_bias, vec_mul, vec_residual, vec_c;  // aligned for four values at a time
   int64_t ldc;
@@ -93,185 +123,144 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi, float s) {
 }
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }  // 2^(byte - 127)
 
-// R rows of C, four neighbouring values of each, through the epilogue: what it reads of
-// all of them under way at once. Rows and columns past C are left out.
+// Bias, row scale and activation of four neighbouring values.
+__device__ __forceinline__ f32x4 before_mul(const GemmParams& p, f32x4 v, int64_t row, int col) {
+  if (p.e.bias) v = v + load4(p.e.bias, col, (int)p.n, p.vec_bias);
+  if (p.e.row_scale) v = v * p.e.row_scale[min(row, p.m - 1)];
+  if (p.e.act == FA_ACT_RELU) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = fmaxf(v[j], 0.f);
+  } else if (p.e.act != FA_ACT_NONE) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const float x = v[j];
+      v[j] = p.e.act == FA_ACT_GELU ? gelu_tanh_ref(x) : tanh_ref(x);
+    }
+  }
+  return v;
+}
+
+// R rows of C, four neighbouring values of each, through the rest of the epilogue:
+// what it reads of all of them under way at once. Rows and columns past C are left out.
 template <int R, typename T>
 __device__ __forceinline__ void put4(const GemmParams& p, T* c, const int64_t (&row)[R], int64_t col, f32x4 (&v)[R]) {
   const int n = (int)p.n, at = (int)col;
-  f32x4 bias = {0.f, 0.f, 0.f, 0.f}, mul[R], residual[R];
-  float scale[R];
-  if (p.e.bias) bias = load4(p.e.bias, at, n, p.vec_bias);
+  if (p.e.mul) {
+    f32x4 x[R];
 #pragma unroll
-  for (int i = 0; i < R; i++) {
-    const int64_t r = min(row[i], p.m - 1);
-    scale[i] = 1.f;
-    if (p.e.row_scale) scale[i] = p.e.row_scale[r];
-    if (p.e.mul) mul[i] = load4(p.e.mul + r * p.e.ldm, at, n, p.vec_mul);
-    if (p.e.residual) residual[i] = load4(p.e.residual + r * p.e.ldr, at, n, p.vec_residual);
+    for (int i = 0; i < R; i++) x[i] = load4(p.e.mul + min(row[i], p.m - 1) * p.e.ldm, at, n, p.vec_mul);
+#pragma unroll
+    for (int i = 0; i < R; i++) v[i] = v[i] * x[i];
+  }
+  if (p.e.residual) {
+    f32x4 x[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) x[i] = load4(p.e.residual + min(row[i], p.m - 1) * p.e.ldr, at, n, p.vec_residual);
+#pragma unroll
+    for (int i = 0; i < R; i++) v[i] = v[i] + x[i];
   }
 #pragma unroll
-  for (int i = 0; i < R; i++) {
-    if (p.e.bias) v[i] = v[i] + bias;
-    if (p.e.row_scale) v[i] = v[i] * scale[i];
-  }
-  if (p.e.act != FA_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < R; i++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float x = v[i][j];
-        v[i][j] = p.e.act == FA_ACT_RELU ? fmaxf(x, 0.f) : p.e.act == FA_ACT_GELU ? gelu_tanh_ref(x) : tanh_ref(x);
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < R; i++) {
-    if (p.e.mul) v[i] = v[i] * mul[i];
-    if (p.e.residual) v[i] = v[i] + residual[i];
+  for (int i = 0; i < R; i++)
     if (row[i] < p.m) store4(c + row[i] * p.ldc, at, n, p.vec_c, v[i]);
-  }
 }
 
 // ---- few rows -----------------------------------------------------------------------
 
-// A block of 32 codes of this lane (row r of 16, columns 32 g .. of the block): A
-// quantised on the way. Lanes r, r + 16, r + 32, r + 48 hold a row's block.
-template <typename T>
-__device__ __forceinline__ float quantize_block(const T* x, int d, int k, bool vec, uint32_t (&code)[8]) {
-  f32x4 v[8];
-  float big = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    v[i] = load4(x, d + 4 * i, k, vec);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      float y = v[i][j];
-      join_max(y, big);
-      v[i][j] = y;
-    }
-  }
-  big = fmaxf(big, lane_xor16(big));
-  big = fmaxf(big, lane_xor32(big));
-  const int e = scale_exp(big);
-  const float inv = exp2_int(-e);
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    if (e == kMaxExp) v[i] = f32x4{clamp_top(v[i][0]), clamp_top(v[i][1]), clamp_top(v[i][2]), clamp_top(v[i][3])};
-    code[i] = pack4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv);
-  }
-  return exp2_int(e);
-}
-
-// Up to 16 MT rows. A wave computes 16 CN columns of C over every split-th block of
+// Up to 16 MT rows. A wave computes 16 columns of C over every split-th block of
 // 128, on the bf16 units (whose operands, codes times powers of two, are exact: the
 // time goes into reading W, not into products); the waves of a column group add up
-// through LDS, in their order. W comes straight from memory in the units' order: 16
-// rows of 128 bytes a block, kDeep blocks under way. A: quantised here (RAW: up to 16
-// rows, where a launch of its own would cost more), or codes.
-constexpr int kFewWaves = 8, kDeep = 4;
-template <typename TA, typename TC, int MT, int CN, bool RAW>
+// through LDS, in their order. Both operands come straight from memory in the units'
+// order, DEEP blocks of W under way: a lane (row r of 16, g of 4) holds bytes 16 g ..
+// and 64 + 16 g .. of its row's block, so that four lanes read 64 bytes together.
+constexpr int kFewWaves = 8;
+template <typename TC, int MT, int DEEP>
 __device__ __forceinline__ void f8_few(const GemmParams& p, TC* c) {
-  __shared__ f32x4 part[kFewWaves][MT * CN][64];
+  __shared__ f32x4 part[kFewWaves][MT][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int group = wave / p.split, ks = wave % p.split;  // split divides kFewWaves
-  const int64_t n0 = ((int64_t)blockIdx.x * (kFewWaves / p.split) + group) * (16 * CN);
+  const int64_t n0 = ((int64_t)blockIdx.x * (kFewWaves / p.split) + group) * 16;
   const int64_t kp = (int64_t)p.kb * kF8Block;
-  const uint8_t *w[CN], *ws[CN], *a[MT], *as[MT];
-#pragma unroll
-  for (int j = 0; j < CN; j++) {
-    const int64_t row = min(n0 + j * 16 + r, p.n - 1);
-    w[j] = p.w + row * kp + g * 32;
-    ws[j] = p.ws + row * p.ks;
-  }
+  const int64_t n_row = min(n0 + r, p.n - 1);
+  const uint8_t *w = p.w + n_row * kp + g * 16, *ws = p.ws + n_row * p.ks, *a[MT], *as[MT];
 #pragma unroll
   for (int i = 0; i < MT; i++) {
     const int64_t row = min((int64_t)i * 16 + r, p.m - 1);
-    a[i] = RAW ? reinterpret_cast<const uint8_t*>(static_cast<const TA*>(p.raw) + row * p.ldr) : p.a + row * kp + g * 32;
+    a[i] = p.a + row * kp + g * 16;
     as[i] = p.as + row * p.ks;
   }
-  f32x4 acc[MT][CN] = {};
-  uint4 cw[kDeep][CN][2];
-  uint32_t cs[kDeep][CN];
-  auto load = [&](int d, int b) {  // (blocks past the last: the last again, not used)
-    const int at = min(b, p.kb - 1);
-#pragma unroll
-    for (int j = 0; j < CN; j++) {
-      const uint4* q = reinterpret_cast<const uint4*>(w[j] + (int64_t)at * kF8Block);
-      cw[d][j][0] = q[0];
-      cw[d][j][1] = q[1];
-      cs[d][j] = ws[j][at];
-    }
+  struct Block {
+    uint4 lo, hi;
+    uint32_t s;
   };
-  if (p.kb > 0) {
+  auto get = [](const uint8_t* codes, const uint8_t* scales, int b) {
+    const uint8_t* q = codes + (int64_t)b * kF8Block;
+    return Block{*reinterpret_cast<const uint4*>(q), *reinterpret_cast<const uint4*>(q + 64), scales[b]};
+  };
+  auto widen = [](const Block& x, bf16x8 (&o)[4]) {
+    const float s = scale_of(x.s);
+    o[0] = widen8(x.lo.x, x.lo.y, s);
+    o[1] = widen8(x.lo.z, x.lo.w, s);
+    o[2] = widen8(x.hi.x, x.hi.y, s);
+    o[3] = widen8(x.hi.z, x.hi.w, s);
+  };
+  f32x4 acc[MT] = {};
+  Block cw[DEEP], ca[DEEP][MT];
 #pragma unroll
-    for (int d = 0; d < kDeep; d++) load(d, ks + d * p.split);
-  }
-  for (int b0 = ks; b0 < p.kb; b0 += kDeep * p.split) {
+  for (int d = 0; d < DEEP; d++)
+    if (ks + d * p.split < p.kb) {
+      cw[d] = get(w, ws, ks + d * p.split);
 #pragma unroll
-    for (int d = 0; d < kDeep; d++) {
-      const int b = b0 + d * p.split;
+      for (int i = 0; i < MT; i++) ca[d][i] = get(a[i], as[i], ks + d * p.split);
+    }
+  for (int b0 = ks; b0 < p.kb; b0 += DEEP * p.split) {
+#pragma unroll
+    for (int d = 0; d < DEEP; d++) {
+      const int b = b0 + d * p.split, next = b + DEEP * p.split;
       if (b >= p.kb) break;  // (uniform in the wave)
-      bf16x8 ww[CN][4];
+      bf16x8 x[4], y[MT][4];
+      widen(cw[d], x);
 #pragma unroll
-      for (int j = 0; j < CN; j++) {
-        const float s = scale_of(cs[d][j]);
-        ww[j][0] = widen8(cw[d][j][0].x, cw[d][j][0].y, s);
-        ww[j][1] = widen8(cw[d][j][0].z, cw[d][j][0].w, s);
-        ww[j][2] = widen8(cw[d][j][1].x, cw[d][j][1].y, s);
-        ww[j][3] = widen8(cw[d][j][1].z, cw[d][j][1].w, s);
+      for (int i = 0; i < MT; i++) widen(ca[d][i], y[i]);
+      if (next < p.kb) {
+        cw[d] = get(w, ws, next);
+#pragma unroll
+        for (int i = 0; i < MT; i++) ca[d][i] = get(a[i], as[i], next);
       }
-      load(d, b + kDeep * p.split);
 #pragma unroll
-      for (int i = 0; i < MT; i++) {
-        uint32_t code[8];
-        float s;
-        if constexpr (RAW) {
-          s = quantize_block(reinterpret_cast<const TA*>(a[i]), b * kF8Block + g * 32, (int)p.k, p.vec, code);
-        } else {
-          const uint4* q = reinterpret_cast<const uint4*>(a[i] + (int64_t)b * kF8Block);
-          const uint4 x = q[0], y = q[1];
-          code[0] = x.x, code[1] = x.y, code[2] = x.z, code[3] = x.w;
-          code[4] = y.x, code[5] = y.y, code[6] = y.z, code[7] = y.w;
-          s = scale_of(as[i][b]);
-        }
+      for (int q = 0; q < 4; q++)
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-          const bf16x8 aa = widen8(code[2 * q], code[2 * q + 1], s);
-#pragma unroll
-          for (int j = 0; j < CN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[j][q], aa, acc[i][j], 0, 0, 0);
-        }
-      }
+        for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[q], y[i][q], acc[i], 0, 0, 0);
     }
   }
   // lane: row r of A, columns 4 g .. + 3
+  const int64_t col = n0 + g * 4;
   if (p.split > 1) {
 #pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int j = 0; j < CN; j++) part[wave][i * CN + j][lane] = acc[i][j];
+    for (int i = 0; i < MT; i++) part[wave][i][lane] = acc[i];
     __syncthreads();
     // the waves of a group share its tiles
-    for (int t = ks; t < MT * CN; t += p.split) {
-      f32x4 v = part[group * p.split][t][lane];
-      for (int s = 1; s < p.split; s++) v = v + part[group * p.split + s][t][lane];
-      const int64_t row[1] = {(int64_t)(t / CN) * 16 + r}, col = n0 + (t % CN) * 16 + g * 4;
-      f32x4 one[1] = {v};
-      if (col < p.n) put4(p, c, row, col, one);
+    for (int t = ks; t < MT; t += p.split) {
+      f32x4 one[1] = {part[group * p.split][t][lane]};
+      for (int s = 1; s < p.split; s++) one[0] = one[0] + part[group * p.split + s][t][lane];
+      const int64_t row[1] = {(int64_t)t * 16 + r};
+      if (col >= p.n) continue;
+      one[0] = before_mul(p, one[0], row[0], (int)col);
+      put4(p, c, row, col, one);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int j = 0; j < CN; j++) {
-        const int64_t row[1] = {(int64_t)i * 16 + r}, col = n0 + j * 16 + g * 4;
-        f32x4 one[1] = {acc[i][j]};
-        if (col < p.n) put4(p, c, row, col, one);
-      }
+    for (int i = 0; i < MT; i++) {
+      const int64_t row[1] = {(int64_t)i * 16 + r};
+      if (col >= p.n) continue;
+      f32x4 one[1] = {before_mul(p, acc[i], row[0], (int)col)};
+      put4(p, c, row, col, one);
+    }
   }
 }
 
-template <typename TA, typename TC, int MT, int CN, bool RAW>
+template <typename TC, int MT, int DEEP>
 __global__ __launch_bounds__(kFewWaves * 64) void f8_few_kernel(GemmParams p, TC* c) {
-  f8_few<TA, TC, MT, CN, RAW>(p, c);
+  f8_few<TC, MT, DEEP>(p, c);
 }
 
 // ---- tiles ---------------------------------------------------------------------------------
@@ -456,34 +445,49 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
     if (b + 2 < p.kb) block(S0, S1, b + 2, integral_constant<int, 2>());
     tile_barrier();  // (the loads that are not used)
   }
-  // through LDS, 32 rows of the wave at a time, so that rows of C are written whole
-  __syncthreads();
-  constexpr int kRow = BN / 2 + 4;
-  static_assert(4 * 32 * kRow * 4 <= 2 * kStage, "the tile's rows fit");
+  // Through LDS, 32 rows of the wave at a time, so that rows of C are written whole. One
+  // copy of what follows the writes: jumping over code that is not needed costs
+  // as much as running it.
+  constexpr int kRow = BN / 2 + 8;  // (lanes 32 apart, four rows on, write to the other half of the banks)
+  static_assert(2 * 32 * kRow * 4 <= kStage, "the waves' rows fit");
   float* mine = reinterpret_cast<float*>(wave < 2 ? S0 : S1) + (wave & 1) * 32 * kRow;
-#pragma unroll
-  for (int i = 0; i < FM; i++) {
+  constexpr int kLanes = BN / 8, kRows = 64 / kLanes, R = 32 / kRows < 8 ? 32 / kRows : 8;  // lanes of a row, rows at once, of those under way
+  const int tr = lane / kLanes, tc = lane % kLanes * 4;
+  const int64_t col = n0 + wn * (BN / 2) + tc;
+  auto spread = [&](const f32x16 (&x)[FN]) {
 #pragma unroll
     for (int j = 0; j < FN; j++)
 #pragma unroll
-      for (int q = 0; q < 16; q++) mine[((q >> 2) * 8 + half * 4 + (q & 3)) * kRow + j * 32 + row] = acc[i][j][q];
-    __syncthreads();
-    constexpr int kLanes = BN / 8, kRows = 64 / kLanes, R = 4;  // lanes of a row, rows at once, of those under way
-    const int tc = lane % kLanes * 4;
-    const int64_t col = n0 + wn * (BN / 2) + tc;
+      for (int q = 0; q < 16; q++) mine[((q >> 2) * 8 + half * 4 + (q & 3)) * kRow + j * 32 + row] = x[j][q];
+  };
+#pragma unroll 1
+  for (int i = 0; i < FM; i++) {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);  // (a wave's own rows: its LDS accesses keep their order)
+    if (i == 0) spread(acc[0]);
+    if constexpr (FM > 1) { if (i == 1) spread(acc[1]); }
+    if constexpr (FM > 2) { if (i == 2) spread(acc[2]); }
+    if constexpr (FM > 3) { if (i == 3) spread(acc[3]); }
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    if (col >= p.n) continue;
+    const int64_t first = m0 + wm * (BM / 2) + i * 32 + tr;
+    if (p.e.bias || p.e.row_scale || p.e.act != FA_ACT_NONE) {
+#pragma unroll 1
+      for (int t = 0; t < 32; t += kRows) {
+        f32x4* at = reinterpret_cast<f32x4*>(mine + (t + tr) * kRow + tc);
+        *at = before_mul(p, *at, first + t, (int)col);
+      }
+    }
 #pragma unroll 1
     for (int t = 0; t < 32; t += kRows * R) {
       int64_t at[R];
       f32x4 v[R];
 #pragma unroll
       for (int k = 0; k < R; k++) {
-        const int tr = t + k * kRows + lane / kLanes;
-        at[k] = m0 + wm * (BM / 2) + i * 32 + tr;
-        v[k] = *reinterpret_cast<const f32x4*>(mine + tr * kRow + tc);
+        at[k] = first + t + k * kRows;
+        v[k] = *reinterpret_cast<const f32x4*>(mine + (t + k * kRows + tr) * kRow + tc);
       }
-      if (col < p.n) put4(p, c, at, col, v);
+      put4(p, c, at, col, v);
     }
-    __syncthreads();
   }
 }
 
@@ -500,12 +504,22 @@ size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 int launch_f8_write(fa_ctx* ctx, const F8View& w, int dtype, const void* x, int64_t ldx, hipStream_t s) {
   const int kb = (int)(f8_kp(w.k) / kF8Block), ks = (int)f8_ks(w.k);
-  const unsigned grid = (unsigned)std::min<int64_t>((w.n * kb + 7) / 8, 1 << 20);
-  const bool vec = ldx % 4 == 0;
-  if (dtype == FA_DT_F32)
-    f8_write_kernel<float><<<grid, 256, 0, s>>>(w, (const float*)x, ldx, kb, ks, vec && aligned(x, 16));
-  else
-    f8_write_kernel<uint16_t><<<grid, 256, 0, s>>>(w, (const uint16_t*)x, ldx, kb, ks, vec && aligned(x, 8));
+  // few blocks: one to 16 lanes, so that they spread over the card
+  const int64_t blocks = w.n * kb, per = blocks > 65536 ? 64 : 16, units = (blocks + per - 1) / per;
+  if (units >= (int64_t)1 << 24)
+    return set_error(ctx, FA_ERR_ARG, "F8Write: [%lld x %lld] is more than one call takes", (long long)w.n, (long long)w.k);
+  const unsigned grid = (unsigned)units;
+  if (dtype == FA_DT_F32) {
+    const float* f = (const float*)x;
+    const bool vec = ldx % 4 == 0 && aligned(x, 16);
+    if (per == 64) f8_write_kernel<float, 4><<<grid, 256, 0, s>>>(w, f, ldx, kb, ks, vec);
+    else f8_write_kernel<float, 1><<<grid, 256, 0, s>>>(w, f, ldx, kb, ks, vec);
+  } else {
+    const uint16_t* h = (const uint16_t*)x;
+    const bool vec = ldx % 8 == 0 && aligned(x, 16);
+    if (per == 64) f8_write_kernel<uint16_t, 4><<<grid, 256, 0, s>>>(w, h, ldx, kb, ks, vec);
+    else f8_write_kernel<uint16_t, 1><<<grid, 256, 0, s>>>(w, h, ldx, kb, ks, vec);
+  }
   FA_CHECK_LAUNCH(ctx);
   return FA_OK;
 }
@@ -522,12 +536,9 @@ int launch_f8_read(fa_ctx* ctx, const F8View& w, int dtype, void* out, int64_t l
   return FA_OK;
 }
 
-// Up to kRawRows rows A is quantised by the product itself, up to kFewRows a wave
-// takes all the rows of its columns.
-constexpr int64_t kRawRows = 16, kFewRows = 64;
+constexpr int64_t kFewRows = 64;  // up to so many rows a wave takes all the rows of its columns
 
 size_t f8_scratch(int64_t m, int64_t n, int64_t k) {
-  if (m <= kRawRows) return 0;
   return align256((size_t)m * f8_kp(k)) + align256((size_t)m * f8_ks(k));
 }
 
@@ -535,26 +546,29 @@ int64_t f8_grid(int64_t m, int64_t n) { return ((m + 15) / 16) * ((n + 63) / 64)
 
 namespace {
 
-template <typename TA, typename TC>
+template <typename TC>
 void launch_gemm_t(const GemmParams& p, TC* c, int cus, hipStream_t s) {
   if (p.m <= kFewRows) {
     GemmParams q = p;
     const int64_t groups = (p.n + 15) / 16;
-    q.split = 8;
-    while (q.split > 1 && (groups * q.split > 4096 * 2 || q.split > std::max(1, p.kb))) q.split /= 2;
+    q.split = kFewWaves;
+    while (q.split > 1 && (groups * q.split > 8192 || q.split > std::max(1, p.kb))) q.split /= 2;
     const unsigned grid = (unsigned)((groups * q.split + kFewWaves - 1) / kFewWaves);
-    if (p.m <= kRawRows) f8_few_kernel<TA, TC, 1, 1, true><<<grid, kFewWaves * 64, 0, s>>>(q, c);
-    else if (p.m <= 32) f8_few_kernel<TA, TC, 2, 1, false><<<grid, kFewWaves * 64, 0, s>>>(q, c);
-    else f8_few_kernel<TA, TC, 4, 1, false><<<grid, kFewWaves * 64, 0, s>>>(q, c);
+    if (p.m <= 16) f8_few_kernel<TC, 1, 4><<<grid, kFewWaves * 64, 0, s>>>(q, c);
+    else if (p.m <= 32) f8_few_kernel<TC, 2, 3><<<grid, kFewWaves * 64, 0, s>>>(q, c);
+    else f8_few_kernel<TC, 4, 2><<<grid, kFewWaves * 64, 0, s>>>(q, c);
     return;
   }
   const int64_t big = ((p.m + 255) / 256) * ((p.n + 255) / 256);
   if (sizeof(TC) == 2 && big >= cus) {
     const int tm = (int)((p.m + 255) / 256), tn = (int)((p.n + 255) / 256);
     f8_tile_kernel<256, 256, uint16_t><<<(unsigned)(tm * tn), 256, 0, s>>>(p, (uint16_t*)c, tm, tn);
-  } else {
+  } else if (((p.m + 127) / 128) * ((p.n + 127) / 128) >= cus) {
     const int tm = (int)((p.m + 127) / 128), tn = (int)((p.n + 127) / 128);
     f8_tile_kernel<128, 128, TC><<<(unsigned)(tm * tn), 256, 0, s>>>(p, c, tm, tn);
+  } else {
+    const int tm = (int)((p.m + 63) / 64), tn = (int)((p.n + 63) / 64);
+    f8_tile_kernel<64, 64, TC><<<(unsigned)(tm * tn), 256, 0, s>>>(p, c, tm, tn);
   }
 }
 
@@ -563,7 +577,7 @@ void launch_gemm_t(const GemmParams& p, TC* c, int cus, hipStream_t s) {
 int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s) {
   const int64_t k = g.w.k;
   F8View a = {nullptr, nullptr, g.m, k};
-  if (g.m > kRawRows && k > 0) {
+  if (k > 0) {
     a.codes = static_cast<uint8_t*>(work);
     a.scales = a.codes + align256((size_t)g.m * f8_kp(k));
     const int rc = launch_f8_write(ctx, a, g.a_dtype, g.a, g.lda, s);
@@ -579,23 +593,14 @@ int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s) 
   p.as = a.scales;
   p.w = g.w.codes;
   p.ws = g.w.scales;
-  p.raw = g.a;
-  p.ldr = g.lda;
-  p.vec = g.lda % 4 == 0 && aligned(g.a, g.a_dtype == FA_DT_F32 ? 16 : 8);
   p.e = g.e;
   p.vec_bias = aligned(g.e.bias, 16);
   p.vec_mul = g.e.ldm % 4 == 0 && aligned(g.e.mul, 16);
   p.vec_residual = g.e.ldr % 4 == 0 && aligned(g.e.residual, 16);
   p.vec_c = g.ldc % 4 == 0 && aligned(g.c, g.c_dtype == FA_DT_F32 ? 16 : 8);
   p.ldc = g.ldc;
-  const bool af = g.a_dtype == FA_DT_F32;
-  if (g.c_dtype == FA_DT_F32) {
-    if (af) launch_gemm_t<float>(p, (float*)g.c, ctx->cu_count, s);
-    else launch_gemm_t<uint16_t>(p, (float*)g.c, ctx->cu_count, s);
-  } else {
-    if (af) launch_gemm_t<float>(p, (uint16_t*)g.c, ctx->cu_count, s);
-    else launch_gemm_t<uint16_t>(p, (uint16_t*)g.c, ctx->cu_count, s);
-  }
+  if (g.c_dtype == FA_DT_F32) launch_gemm_t(p, (float*)g.c, ctx->cu_count, s);
+  else launch_gemm_t(p, (uint16_t*)g.c, ctx->cu_count, s);
   FA_CHECK_LAUNCH(ctx);
   return FA_OK;
 }
