@@ -18,19 +18,28 @@ constexpr int kMinExp = -80, kMaxExp = 120;
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
 
+// Four neighbouring values as one aligned load brings them.
+template <typename T>
+struct Four { using type = f32x4; };
+template <>
+struct Four<uint16_t> { using type = uint2; };
+template <typename T>
+using Raw4 = typename Four<T>::type;
+template <typename T>
+__device__ __forceinline__ Raw4<T> raw4(const T* p) { return *reinterpret_cast<const Raw4<T>*>(p); }
+__device__ __forceinline__ f32x4 widen(f32x4 x) { return x; }
+__device__ __forceinline__ f32x4 widen(uint2 w) {
+  return f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
+               __uint_as_float(w.y & 0xFFFF0000u)};
+}
+
 // Four neighbouring values of a row, those past D as zeros. vec: the row
 // starts are aligned for one load.
 template <typename T>
 __device__ __forceinline__ f32x4 load4(const T* p, int d, int D, bool vec) {
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
   if (vec && d + 4 <= D) {
-    if constexpr (sizeof(T) == 4) {
-      r = *reinterpret_cast<const f32x4*>(p + d);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(p + d);
-      r = f32x4{__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
-                __uint_as_float(w.y & 0xFFFF0000u)};
-    }
+    r = widen(raw4(p + d));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; i++)

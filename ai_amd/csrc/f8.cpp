@@ -35,7 +35,7 @@ int check_ld(fa_ctx* ctx, const char* op, int64_t rows, int64_t cols, int64_t ld
 }
 
 fa::F8View view_of(const fa_f8_matrix* w) {
-  return {static_cast<uint8_t*>(w->codes), static_cast<uint8_t*>(w->scales), w->n, w->k};
+  return {static_cast<uint8_t*>(w->codes), static_cast<uint8_t*>(w->scales), w->n, w->k, fa::f8_kp(w->k)};
 }
 
 size_t elem(int dtype) { return dtype == FA_DT_F32 ? 4 : 2; }

@@ -13,9 +13,9 @@ inline int64_t f8_ks(int64_t k) { return (f8_kp(k) / kF8Block + 3) / 4 * 4; }
 
 // A matrix [n x k] in 8 bits on the device (fa_f8_matrix).
 struct F8View {
-  uint8_t* codes;   // [n][kp]
+  uint8_t* codes;   // [n][stride], kp of them used
   uint8_t* scales;  // [n][ks]
-  int64_t n, k;
+  int64_t n, k, stride;
 };
 int launch_f8_write(fa_ctx* ctx, const F8View& w, int dtype, const void* x, int64_t ldx, hipStream_t s);
 int launch_f8_read(fa_ctx* ctx, const F8View& w, int dtype, void* out, int64_t ldo, hipStream_t s);

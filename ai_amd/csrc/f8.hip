@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void f8_write_kernel(F8View w, const T* __rest
     }
     const float inv = exp2_int(-e);
     if (first + u * 4 + (lane >> 4) >= blocks) continue;
-    *reinterpret_cast<uint2*>(w.codes + (row[u] * kb + b[u]) * kF8Block + l * 8) =
+    *reinterpret_cast<uint2*>(w.codes + row[u] * w.stride + b[u] * kF8Block + l * 8) =
         make_uint2(pack4(v[u][0][0] * inv, v[u][0][1] * inv, v[u][0][2] * inv, v[u][0][3] * inv),
                    pack4(v[u][1][0] * inv, v[u][1][1] * inv, v[u][1][2] * inv, v[u][1][3] * inv));
     if (l == 0) w.scales[row[u] * ks + b[u]] = (uint8_t)(e + 127);
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(256) void f8_read_kernel(F8View w, T* __restrict__ 
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / (kb * 32);
     const int word = (int)(i - row * (kb * 32));
-    const f32x4 v = unpack4(reinterpret_cast<const uint32_t*>(w.codes)[i]);
+    const f32x4 v = unpack4(*reinterpret_cast<const uint32_t*>(w.codes + row * w.stride + word * 4));
     const float s = exp2_int((int)w.scales[row * ks + (word >> 5)] - 127);
     store4(out + row * ldo, word * 4, (int)w.k, vec, v * s);
   }
@@ -102,7 +102,8 @@ __global__ __launch_bounds__(256) void f8_read_kernel(F8View w, T* __restrict__ 
 
 struct GemmParams {
   int64_t m, n, k;
-  int kb, ks;  // blocks of a row, its scale bytes
+  int kb, ks;   // blocks of a row, its scale bytes
+  int64_t a_st;  // bytes from a row of A's codes to the next
   const uint8_t *a, *as, *w, *ws;  // codes and scale bytes
   fa_epilogue e;
   int vec_bias, vec_mul, vec_residual, vec_c;  // aligned for four values at a time
@@ -185,7 +186,7 @@ __device__ __forceinline__ void f8_few(const GemmParams& p, TC* c) {
 #pragma unroll
   for (int i = 0; i < MT; i++) {
     const int64_t row = min((int64_t)i * 16 + r, p.m - 1);
-    a[i] = p.a + row * kp + g * 16;
+    a[i] = p.a + row * p.a_st + g * 16;
     as[i] = p.as + row * p.ks;
   }
   struct Block {
@@ -305,25 +306,25 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
   const int64_t kp = (int64_t)p.kb * kF8Block;
-  // Tiles of an XCD's run are taken in groups of 8 tile rows, down the columns: the
+  // Tiles of an XCD's run are taken in groups of 4 tile rows, down the columns: the
   // ones that run together share their rows of A and of W in its L2.
   int tm, tn;
   {
     const int tile = xcd_tile(tiles_m, tiles_n);
-    constexpr int G = 8;
+    constexpr int G = 4;
     const int group = tile / (G * tiles_n), rows = min(G, tiles_m - group * G), at = tile - group * G * tiles_n;
     tm = group * G + at % rows;
     tn = at / rows;
   }
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   // the tile's first rows (the same for the workgroup), and a thread's pieces from there
-  const uint8_t *a0 = p.a + m0 * kp, *b0 = p.w + n0 * kp;
+  const uint8_t *a0 = p.a + m0 * p.a_st, *b0 = p.w + n0 * kp;
   uint32_t ga[NA], gb[NB];
   {
     const int row = tid >> 3, piece = (tid & 7) ^ (row & 7);
     const int rows_a = (int)min(p.m - m0, (int64_t)BM) - 1, rows_b = (int)min(p.n - n0, (int64_t)BN) - 1;
 #pragma unroll
-    for (int i = 0; i < NA; i++) ga[i] = (uint32_t)min(i * 32 + row, rows_a) * (uint32_t)kp + piece * 16;
+    for (int i = 0; i < NA; i++) ga[i] = (uint32_t)min(i * 32 + row, rows_a) * (uint32_t)p.a_st + piece * 16;
 #pragma unroll
     for (int i = 0; i < NB; i++) gb[i] = (uint32_t)min(i * 32 + row, rows_b) * (uint32_t)kp + piece * 16;
   }
@@ -538,8 +539,12 @@ int launch_f8_read(fa_ctx* ctx, const F8View& w, int dtype, void* out, int64_t l
 
 constexpr int64_t kFewRows = 64;  // up to so many rows a wave takes all the rows of its columns
 
+// Rows of A's codes a multiple of 2 KB apart would lie in few of the L2's channels:
+// a block more between them (8192 x 8192 x 8192 504 -> 496 us).
+int64_t a_stride(int64_t k) { return f8_kp(k) + (f8_kp(k) % 2048 == 0 ? kF8Block : 0); }
+
 size_t f8_scratch(int64_t m, int64_t n, int64_t k) {
-  return align256((size_t)m * f8_kp(k)) + align256((size_t)m * f8_ks(k));
+  return align256((size_t)m * a_stride(k)) + align256((size_t)m * f8_ks(k));
 }
 
 int64_t f8_grid(int64_t m, int64_t n) { return ((m + 15) / 16) * ((n + 63) / 64); }
@@ -576,10 +581,10 @@ void launch_gemm_t(const GemmParams& p, TC* c, int cus, hipStream_t s) {
 
 int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s) {
   const int64_t k = g.w.k;
-  F8View a = {nullptr, nullptr, g.m, k};
+  F8View a = {nullptr, nullptr, g.m, k, a_stride(k)};
   if (k > 0) {
     a.codes = static_cast<uint8_t*>(work);
-    a.scales = a.codes + align256((size_t)g.m * f8_kp(k));
+    a.scales = a.codes + align256((size_t)g.m * a.stride);
     const int rc = launch_f8_write(ctx, a, g.a_dtype, g.a, g.lda, s);
     if (rc) return rc;
   }
@@ -590,6 +595,7 @@ int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s) 
   p.kb = (int)(f8_kp(k) / kF8Block);
   p.ks = (int)f8_ks(k);
   p.a = a.codes;
+  p.a_st = a.stride;
   p.as = a.scales;
   p.w = g.w.codes;
   p.ws = g.w.scales;

@@ -14,6 +14,9 @@
 //           lane group b of a wave holds tokens 4 b .. 4 b + 3 of each 16 in
 //           the layout in which it gets their scores, so weights meet values
 //           without leaving their registers.
+#include <algorithm>
+#include <atomic>
+
 #include "device_math.h"
 #include "kvcache.h"
 
@@ -93,9 +96,9 @@ __device__ __forceinline__ int stored_exp(float s) {
 // nothing of the next under way. Single tokens are bound by that chain and the
 // write-back of the 128 lines that one token's values touch in a head (64 sequences,
 // one float32 token each, written 7.1 us).
-// load(row, d): four values of the part from dim d on in row `row`, zeros past D.
-template <int NCM, typename F>
-__device__ __forceinline__ void write_block(const KvArgs& a, const KvUnit& u, int id, int h, int part, F load) {
+// at(row): a row's values. vec: fours of them are aligned.
+template <typename T, int NCM, typename F>
+__device__ __forceinline__ void write_block(const KvArgs& a, const KvUnit& u, int id, int h, int part, bool vec, F at) {
   __shared__ float red[4];
   __shared__ uint32_t tile[64 * 17];
   const int tid = threadIdx.x, dq = tid & 15, ta = (tid >> 4) & 3, tb = tid >> 6;
@@ -103,14 +106,27 @@ __device__ __forceinline__ void write_block(const KvArgs& a, const KvUnit& u, in
   const int end = u.place + u.n;
   f32x4 x[NCM][4];
   float big = 0.f;
+  Raw4<T> raw[NCM][4];  // (all loads under way before the first is widened)
 #pragma unroll
   for (int c = 0; c < NCM; c++)
-    if (c < a.nc)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int t = t0 + i, d = c * 64 + dq * 4;
+      raw[c][i] = Raw4<T>{};
+      if (c < a.nc && vec && t >= u.place && t < end && d + 4 <= a.D) raw[c][i] = raw4(at(u.row + (t - u.place)) + d);
+    }
+#pragma unroll
+  for (int c = 0; c < NCM; c++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[c][i] = widen(raw[c][i]);
+  if (!vec || a.D % 4 != 0)
+#pragma unroll
+    for (int c = 0; c < NCM; c++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int t = t0 + i;
-        x[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (t >= u.place && t < end) x[c][i] = load(u.row + (t - u.place), c * 64 + dq * 4);
+        const int t = t0 + i, d = c * 64 + dq * 4;
+        if (t >= u.place && t < end && !(vec && d + 4 <= a.D))
+          x[c][i] = load4(at(u.row + (t - u.place)), d, a.D, false);
       }
 #pragma unroll
   for (int c = 0; c < NCM; c++)
@@ -222,74 +238,195 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, const T* __rest
   const int h = blockIdx.y, part = blockIdx.z;
   const T* src = part ? v : k;
   const int64_t st = part ? v_st : k_st, sh = part ? v_sh : k_sh;
-  write_block<NCM>(a, u, id, h, part, [&](int64_t row, int d) { return load4(src + row * st + h * sh, d, a.D, vec); });
+  write_block<T, NCM>(a, u, id, h, part, vec, [&](int64_t row) { return src + row * st + h * sh; });
 }
 
-// Four values of a head from dim d on, turned: dim i < half of the first 2 *
-// half becomes x_i cos - x_{i + half} sin, dim i + half x_{i + half} cos + x_i
-// sin, the angle position * inv_i in float64, cos and sin rounded to float32 (as
-// fa_rope's tables), the products exact in float64.
-template <typename T>
-__device__ __forceinline__ f32x4 load_turned(const KvRopeArgs& r, const T* p, int64_t position, int d, int D, bool vec) {
-  f32x4 x = load4(p, d, D, vec);
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    const int i = d + j;
-    if (i >= 2 * r.half) continue;
-    const bool up = i >= r.half;
-    const int pair = up ? i - r.half : i;
-    double sn, cs;
-    sincos((double)position * r.inv[pair], &sn, &cs);
-    const double c = (double)(float)cs, s = (double)(float)sn;
-    const double other = (double)to_f32(p[up ? pair : i + r.half]);
-    x[j] = (float)((double)x[j] * c + (up ? other : -other) * s);
+// ---- rotary positions on the way ---------------------------------------------------
+
+// Cosine and sine of an angle in float64, rounded to float32 as fa_rope's tables. a -
+// n pi / 2 with pi / 2 in two parts (the products exact in the fma), then
+// the series of both to a^11 and a^12: the next terms are below 2^-36. |a| < 2^31;
+// WIDE: any angle.
+template <bool WIDE>
+__device__ __forceinline__ float2 cos_sin(double a) {
+  if (WIDE) {
+    double s, c;
+    sincos(a, &s, &c);
+    return make_float2((float)c, (float)s);
   }
-  return x;
+  const double n = rint(a * 0.63661977236758134);
+  double r = fma(-n, 1.5707963267948966, a);
+  r = fma(-n, 6.123233995736766e-17, r);
+  const double x = r * r;
+  double s = -1.0 / 39916800.0, c = 1.0 / 479001600.0;
+  c = fma(c, x, -1.0 / 3628800.0);
+  s = fma(s, x, 1.0 / 362880.0);
+  c = fma(c, x, 1.0 / 40320.0);
+  s = fma(s, x, -1.0 / 5040.0);
+  c = fma(c, x, -1.0 / 720.0);
+  s = fma(s, x, 1.0 / 120.0);
+  c = fma(c, x, 1.0 / 24.0);
+  s = fma(s, x, -1.0 / 6.0);
+  c = fma(c, x, -0.5);
+  s = fma(s * x, r, r);
+  c = fma(c, x, 1.0);
+  const int q = (int)n;
+  const float fs = (float)s, fc = (float)c;
+  const float u = q & 1 ? fs : fc, v = q & 1 ? fc : fs;
+  return make_float2((q + 1) & 2 ? -u : u, q & 2 ? -v : v);
 }
 
-template <typename T, int NCM>
-__global__ __launch_bounds__(256) void kv_write_rope_kernel(KvArgs a, KvRopeArgs r, bool by_row, bool vec) {
+// x_i cos - x_{i + half} sin of a pair and x_{i + half} cos + x_i sin. EXACT: products
+// of float32 are exact in float64, so that each is rounded once there and once to
+// float32; otherwise one product is rounded to float32 and then the sum.
+template <bool EXACT>
+__device__ __forceinline__ void turn(float& lo, float& hi, float2 cs) {
+  if (EXACT) {
+    const double x = (double)lo, y = (double)hi, c = (double)cs.x, s = (double)cs.y;
+    lo = (float)(x * c - y * s);
+    hi = (float)(y * c + x * s);
+  } else {
+    const float x = lo, y = hi;
+    lo = fmaf(x, cs.x, -(y * cs.y));
+    hi = fmaf(y, cs.x, x * cs.y);
+  }
+}
+
+// Rows i0 .. i1 - 1 of a unit, heads h0 .. h1 - 1 of src, turned into put(i, h, d,
+// end, four values): dims d .. end - 1, four at most. A thread holds the cosines and
+// sines of four pairs of a row and goes through heads with them, HEADS at once, the
+// next loads under way; a pair is read and written by one thread, so the target may be
+// the source. Rows fill the threads first, then heads. WHOLE: fours of values are
+// aligned, and whole.
+template <typename T, bool WIDE, bool EXACT, int HEADS, bool WHOLE, typename F>
+__device__ __forceinline__ void turn_rows(const KvArgs& a, const KvRopeArgs& r, const KvUnit& u, int64_t first,
+                                          const T* src, int64_t st, int64_t sh, int i0, int i1, int h0, int h1, F put) {
+  // slots of a row's head: fours of pairs, then fours of the dims that stay (at most 129)
+  const int pairs = (r.half + 3) / 4, slots = pairs + (a.D - 2 * r.half + 3) / 4;
+  const int items = 256 / slots, at_once = min(items, i1 - i0), runs = items / at_once;
+  const int item = (int)threadIdx.x / slots, slot = (int)threadIdx.x - item * slots;
+  if (item >= at_once * runs) return;
+  const int run = item % runs;
+  const bool rest = slot >= pairs;
+  // this thread's dims d .. end - 1 and d2 .. end2 - 1; the same where nothing turns
+  const int d = rest ? 2 * r.half + (slot - pairs) * 4 : slot * 4, end = rest ? a.D : r.half;
+  const int d2 = rest ? d : d + r.half, end2 = rest ? a.D : 2 * r.half;
+  double inv[4];
+#pragma unroll
+  for (int j = 0; j < 4; j++) inv[j] = r.inv[min(d + j, r.half - 1)];
+  Raw4<T> x[HEADS], y[HEADS];
+  auto fetch = [&](int i, int h) {
+    const T* p = src + (u.row + i) * st;
+#pragma unroll
+    for (int k = 0; k < HEADS; k++) {
+      const T* from = p + min(h + k * runs, h1 - 1) * sh;
+      x[k] = raw4(from + d);
+      y[k] = raw4(from + d2);
+    }
+  };
+  int i = i0 + item / runs, h = h0 + run;
+  if (h >= h1) return;
+  if (WHOLE && i < i1) fetch(i, h);
+  float2 cs[4];
+  while (i < i1) {
+    if (h == h0 + run) {
+      const double pos = (double)(r.positions ? (int64_t)r.positions[u.row + i] : first + i);
+#pragma unroll
+      for (int j = 0; j < 4; j++) cs[j] = cos_sin<WIDE>(pos * inv[j]);
+    }
+    f32x4 lo[HEADS], hi[HEADS];
+#pragma unroll
+    for (int k = 0; k < HEADS; k++) {
+      if (WHOLE) {
+        lo[k] = widen(x[k]);
+        hi[k] = widen(y[k]);
+      } else {
+        const T* from = src + (u.row + i) * st + min(h + k * runs, h1 - 1) * sh;
+        lo[k] = load4(from, d, end, false);
+        hi[k] = load4(from, d2, end2, false);
+      }
+    }
+    const int at = i, head = h;
+    h += runs * HEADS;
+    if (h >= h1) {
+      h = h0 + run;
+      i += at_once;
+    }
+    if (WHOLE && i < i1) fetch(i, h);
+#pragma unroll
+    for (int k = 0; k < HEADS; k++) {
+      if (head + k * runs >= h1) break;
+      if (!rest)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          float l = lo[k][j], g = hi[k][j];
+          turn<EXACT>(l, g, cs[j]);
+          lo[k][j] = l;
+          hi[k][j] = g;
+        }
+      put(at, head + k * runs, d, end, lo[k]);
+      put(at, head + k * runs, d2, end2, hi[k]);
+    }
+  }
+}
+
+// Jobs of a unit along the grid's y: key heads, value heads, then q_parts parts of the
+// rows (one pass of the threads each) by groups of q_heads query heads. Keys are turned
+// into float32 in LDS, each pair by one thread, and stored from there as the writer's.
+//
+// Bound by memory: prompts (16 of up to 2048 tokens, 32 query and 8 key/value heads of
+// 128 dims in bf16) take 138 us, 3.8 TB/s, where a large copy's rate gives 105; the
+// queries alone take 92 of 77, the keys and values 56 of 29 (values 23). Chunks of 512
+// in float32, half of each head turning: 14 us of 8. Single tokens wait for the chain
+// sequence, block, row, store: 64 sequences 9.2 us, one 8.4. What it took, in us of the
+// prompts: keys turned where the writer loads them, each pair twice, and queries by a
+// thread per four dims 326; cosines shared by heads and pairs turned once, but loads
+// waited for one by one 212; cosines' factors and all loads of a thread under way
+// before the first is used 161; the next heads' loads too, 16 heads a job 138 (8 heads
+// 146: more cosines; 32 leave too few workgroups: the queries alone by 13% slower).
+template <typename T, int NCM, bool WIDE>
+__global__ __launch_bounds__(256, NCM <= 2 ? 4 : 2) void kv_write_rope_kernel(KvArgs a, KvRopeArgs r, int q_parts,
+                                                                              int q_heads, bool by_row, bool vec,
+                                                                              bool whole, bool whole_q) {
+  extern __shared__ float keys[];  // [token of the unit][dim], rows of whole fours + 4
   const KvUnit u = kv_unit(a, blockIdx.x, by_row);
   if (!u.ok) return;
-  const int64_t first = u.slot * 64 + u.place;  // position of the unit's first row in its sequence
-  auto position = [&](int64_t row) { return r.positions ? (int64_t)r.positions[row] : first + (row - u.row); };
-  const int job = blockIdx.y;
-  if (job < 2 * a.hkv) {
-    const int id = kv_block(a, u.b, u.slot);
-    if (id < 0) return;
-    const int h = job >> 1, part = job & 1;
-    write_block<NCM>(a, u, id, h, part, [&](int64_t row, int d) {
-      if (part) return load4((const T*)r.v + row * r.v_st + h * r.v_sh, d, a.D, vec);
-      return load_turned(r, (const T*)r.k + row * r.k_st + h * r.k_sh, position(row), d, a.D, vec);
-    });
+  const int64_t first = u.slot * 64 + u.place;
+  int job = blockIdx.y;
+  if (job >= 2 * a.hkv) {
+    job -= 2 * a.hkv;
+    const int part = job % q_parts, group = job / q_parts, n = (64 + q_parts - 1) / q_parts;
+    const int i0 = part * n, i1 = q_parts == 1 ? u.n : min(u.n, i0 + n);
+    if (i0 >= i1) return;
+    const int h0 = group * q_heads, h1 = min(r.H, h0 + q_heads);
+    auto put = [&](bool v4, int i, int h, int d, int end, f32x4 x) {
+      store4((T*)r.q_out + ((u.row + i) * r.H + h) * a.D, d, end, v4, x);
+    };
+    if (whole_q)
+      turn_rows<T, WIDE, false, 4, true>(a, r, u, first, (const T*)r.q, r.q_st, r.q_sh, i0, i1, h0, h1,
+                                         [&](int i, int h, int d, int end, f32x4 x) { put(true, i, h, d, end, x); });
+    else
+      turn_rows<T, WIDE, false, 1, false>(a, r, u, first, (const T*)r.q, r.q_st, r.q_sh, i0, i1, h0, h1,
+                                          [&](int i, int h, int d, int end, f32x4 x) { put(false, i, h, d, end, x); });
     return;
   }
-  // queries: a thread turns whole pairs, so that q_out may be q
-  const int h = job - 2 * a.hkv;
-  const int pairs = (r.half + 3) / 4, words = pairs + (a.D - 2 * r.half + 3) / 4;
-  const bool vec2 = vec && r.half % 4 == 0, vec_out = vec && a.D % 4 == 0;
-  for (int i = threadIdx.x; i < u.n * words; i += 256) {
-    const int64_t row = u.row + i / words;
-    const int w = i % words;
-    const T* p = (const T*)r.q + row * r.q_st + h * r.q_sh;
-    T* o = (T*)r.q_out + (row * r.H + h) * a.D;
-    if (w >= pairs) {
-      const int d = 2 * r.half + (w - pairs) * 4;
-      store4(o, d, a.D, vec_out && r.half % 2 == 0, load4(p, d, a.D, vec && r.half % 2 == 0));
-      continue;
-    }
-    f32x4 lo = load4(p, w * 4, r.half, vec), hi = load4(p + r.half, w * 4, r.half, vec2);
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      double sn, cs;
-      sincos((double)position(row) * r.inv[min(w * 4 + j, r.half - 1)], &sn, &cs);
-      const double c = (double)(float)cs, s = (double)(float)sn, x = (double)lo[j], y = (double)hi[j];
-      lo[j] = (float)(x * c - y * s);
-      hi[j] = (float)(y * c + x * s);
-    }
-    store4(o, w * 4, r.half, vec_out, lo);
-    store4(o + r.half, w * 4, r.half, vec_out && vec2, hi);
+  const int id = kv_block(a, u.b, u.slot);
+  if (id < 0) return;
+  const int h = job % a.hkv;
+  if (job >= a.hkv) {
+    write_block<T, NCM>(a, u, id, h, 1, vec, [&](int64_t row) { return (const T*)r.v + row * r.v_st + h * r.v_sh; });
+    return;
   }
+  const int stride = (a.D + 3) / 4 * 4 + 4;
+  if (whole)
+    turn_rows<T, WIDE, true, 1, true>(a, r, u, first, (const T*)r.k, r.k_st, r.k_sh, 0, u.n, h, h + 1,
+                                      [&](int i, int, int d, int, f32x4 x) { *(f32x4*)(keys + i * stride + d) = x; });
+  else
+    turn_rows<T, WIDE, true, 1, false>(
+        a, r, u, first, (const T*)r.k, r.k_st, r.k_sh, 0, u.n, h, h + 1,
+        [&](int i, int, int d, int end, f32x4 x) { store4(keys + i * stride, d, end, false, x); });
+  __syncthreads();
+  write_block<float, NCM>(a, u, id, h, 0, true, [&](int64_t row) { return keys + (row - u.row) * stride; });
 }
 
 // One workgroup reads back one (block, head, keys or values): the thread
@@ -365,20 +502,43 @@ int write_t(fa_ctx* ctx, const KvArgs& a, const void* k, int64_t k_st, int64_t k
   return FA_OK;
 }
 
-template <typename T>
-int write_rope_t(fa_ctx* ctx, const KvArgs& a, const KvRopeArgs& r, hipStream_t s) {
+template <typename T, int NCM, bool WIDE>
+int write_rope_nc(fa_ctx* ctx, const KvArgs& a, const KvRopeArgs& r, hipStream_t s) {
   bool by_row;
   const int64_t units = kv_units(a.rows, a.nseq, &by_row);
   const size_t al = 4 * sizeof(T);
-  const bool vec = aligned(r.k, al) && aligned(r.v, al) && (r.k_st | r.k_sh | r.v_st | r.v_sh) % 4 == 0 &&
-                   (!r.q || (aligned(r.q, al) && aligned(r.q_out, al) && (r.q_st | r.q_sh) % 4 == 0));
-  const dim3 grid((unsigned)units, (unsigned)(2 * a.hkv + r.H));
-  if (a.nc <= 1) kv_write_rope_kernel<T, 1><<<grid, 256, 0, s>>>(a, r, by_row, vec);
-  else if (a.nc <= 2) kv_write_rope_kernel<T, 2><<<grid, 256, 0, s>>>(a, r, by_row, vec);
-  else if (a.nc <= 4) kv_write_rope_kernel<T, 4><<<grid, 256, 0, s>>>(a, r, by_row, vec);
-  else kv_write_rope_kernel<T, 8><<<grid, 256, 0, s>>>(a, r, by_row, vec);
+  const bool vec = aligned(r.k, al) && aligned(r.v, al) && (r.k_st | r.k_sh | r.v_st | r.v_sh) % 4 == 0;
+  const bool vec_q = r.q && aligned(r.q, al) && aligned(r.q_out, al) && (r.q_st | r.q_sh) % 4 == 0;
+  const bool fours = a.D % 4 == 0 && r.half % 4 == 0;
+  const int slots = (r.half + 3) / 4 + (a.D - 2 * r.half + 3) / 4;
+  const int q_parts = by_row ? 1 : (64 + 256 / slots - 1) / (256 / slots);
+  int q_heads = 16;  // (a grid's y holds 65535)
+  while (2 * a.hkv + (int64_t)q_parts * ((r.H + q_heads - 1) / q_heads) > 65535) q_heads *= 2;
+  const size_t lds = (size_t)64 * ((a.D + 3) / 4 * 4 + 4) * sizeof(float);
+  auto kernel = kv_write_rope_kernel<T, NCM, WIDE>;
+  static std::atomic<uint64_t> ready{0};  // devices that know of more than 64 KB, the first 64
+  const uint64_t bit = ctx->device < 64 ? uint64_t(1) << ctx->device : 0;
+  if (lds > 48 * 1024 && !(ready.load() & bit)) {
+    FA_HIP_CHECK(ctx, hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                          64 * (2 * kKvMaxPairs + 4) * (int)sizeof(float)));
+    ready.fetch_or(bit);
+  }
+  const unsigned jobs = (unsigned)(2 * a.hkv + q_parts * ((r.H + q_heads - 1) / q_heads));
+  kernel<<<dim3((unsigned)units, jobs), 256, lds, s>>>(a, r, q_parts, q_heads, by_row, vec, vec && fours,
+                                                       vec_q && fours);
   FA_CHECK_LAUNCH(ctx);
   return FA_OK;
+}
+
+template <typename T>
+int write_rope_t(fa_ctx* ctx, const KvArgs& a, const KvRopeArgs& r, hipStream_t s) {
+  // bases below 1 alone turn by more than the position, which is below 2^31
+  const double most = std::max(r.inv[0], r.inv[r.half - 1]);
+  return most > 1      ? write_rope_nc<T, 8, true>(ctx, a, r, s)
+         : a.nc <= 1   ? write_rope_nc<T, 1, false>(ctx, a, r, s)
+         : a.nc <= 2   ? write_rope_nc<T, 2, false>(ctx, a, r, s)
+         : a.nc <= 4   ? write_rope_nc<T, 4, false>(ctx, a, r, s)
+                       : write_rope_nc<T, 8, false>(ctx, a, r, s);
 }
 
 }  // namespace

@@ -348,9 +348,9 @@ typedef struct fa_kv_rope {
  * `heads` of them a row, any multiple of kv_heads; none with heads == 0 and q ==
  * NULL) rotated into q_out, [rows][heads][head_dim] contiguous, of dtype, which
  * may be q itself where q is laid out so, and else must not overlap it. Angles in
- * float64, their cosines and sines rounded to float32 as fa_rope's, products and sums
- * in float64, results rounded to float32 (the keys that are quantised; queries of
- * bf16 tensors are rounded once more). A query is rotated whether or not its token
+ * float64, their cosines and sines rounded to float32 as fa_rope's. Keys: products and
+ * sums in float64, rounded to float32 and quantised. Queries: in float32, one product
+ * rounded and then the sum, rounded to bf16 once more where dtype says so. A query is rotated whether or not its token
  * has a block. positions is on the device in the _dev form, else on the host.
  * 2 * kv_heads + heads <= 65535. */
 int fa_kv_write_rope(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch* batch, const fa_kv_rope* rope, int dtype,
