@@ -327,4 +327,19 @@ __device__ __forceinline__ void residual_norm_row(const float* __restrict__ o, c
   }
 }
 
+// Two floats of a part, written and read past the caches that XCDs do not
+// share (relaxed atomics of the device's scope): the workgroup that joins a
+// tile's parts may be on another XCD than those that wrote them, and a fence
+// for ordinary stores writes back a whole L2 (one in each workgroup made a
+// step of 16 sequences of 2048 tokens 65 us longer).
+__device__ __forceinline__ void put2(float* p, float a, float b) {
+  const uint64_t v = (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float* p) {
+  const uint64_t v =
+      __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
 }  // namespace fa

@@ -17,7 +17,9 @@ struct F8View {
   uint8_t* scales;  // [n][ks]
   int64_t n, k, stride;
 };
-int launch_f8_write(fa_ctx* ctx, const F8View& w, int dtype, const void* x, int64_t ldx, hipStream_t s);
+// zeros words from `zero` on are set to 0 on the way.
+int launch_f8_write(fa_ctx* ctx, const F8View& w, int dtype, const void* x, int64_t ldx, hipStream_t s,
+                    uint32_t* zero = nullptr, int zeros = 0);
 int launch_f8_read(fa_ctx* ctx, const F8View& w, int dtype, void* out, int64_t ldo, hipStream_t s);
 
 struct F8GemmArgs {
@@ -31,7 +33,7 @@ struct F8GemmArgs {
   void* c;
   int64_t ldc;
 };
-// Scratch of a product of m rows: A in 8 bits.
+// Scratch of a product of m rows: A in 8 bits, sums of a split K.
 size_t f8_scratch(int64_t m, int64_t n, int64_t k);
 int64_t f8_grid(int64_t m, int64_t n);
 int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s);

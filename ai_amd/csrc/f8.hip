@@ -29,7 +29,8 @@ bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 // write the scale bytes that pad the row.
 template <typename T, int U>
 __global__ __launch_bounds__(256) void f8_write_kernel(F8View w, const T* __restrict__ x, int64_t ldx, int kb, int ks,
-                                                       bool vec) {
+                                                       bool vec, uint32_t* zero, int zeros) {
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < zeros; i += gridDim.x * 256) zero[i] = 0;
   const int lane = threadIdx.x & 63, l = lane & 15;
   const int64_t first = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * (4 * U);
   const int64_t blocks = w.n * kb, row0 = blocks >> 32 ? first / kb : (uint32_t)first / (uint32_t)kb;
@@ -109,6 +110,9 @@ struct GemmParams {
   int vec_bias, vec_mul, vec_residual, vec_c;  // aligned for four values at a time
   int64_t ldc;
   int split;                       // waves that share a row's blocks (few rows)
+  int parts, per;                  // parts of K, each of `per` blocks (a multiple of 4) or what is left
+  float* part;                     // [tile][part][BM * BN], in the order of the threads that hold them
+  uint32_t* count;                 // [tile] parts that are there
 };
 
 // Two codes times a power of two, exact in bf16.
@@ -167,28 +171,23 @@ __device__ __forceinline__ void put4(const GemmParams& p, T* c, const int64_t (&
 
 // ---- few rows -----------------------------------------------------------------------
 
-// Up to 16 MT rows. A wave computes 16 columns of C over every split-th block of
-// 128, on the bf16 units (whose operands, codes times powers of two, are exact: the
-// time goes into reading W, not into products); the waves of a column group add up
-// through LDS, in their order. Both operands come straight from memory in the units'
-// order, DEEP blocks of W under way: a lane (row r of 16, g of 4) holds bytes 16 g ..
-// and 64 + 16 g .. of its row's block, so that four lanes read 64 bytes together.
-constexpr int kFewWaves = 8;
-template <typename TC, int MT, int DEEP>
+// Up to 16 rows. A wave computes 16 columns of C over every split-th block of 128, on
+// the bf16 units (whose operands, codes times powers of two, are exact: the time goes
+// into reading W, not into products); the waves of a column group add up through LDS, in
+// their order. Both operands come straight from memory in the units' order, four blocks
+// under way: a lane (row r of 16, g of 4) holds bytes 16 g .. and 64 + 16 g .. of its
+// row's block, so that four lanes read 64 bytes together. Bound by latencies: 16 x 4096 x
+// 4096 takes 12 us, 5 of them the launch before it, which quantises A.
+constexpr int kFewWaves = 8, kFewDeep = 4;
+template <typename TC>
 __device__ __forceinline__ void f8_few(const GemmParams& p, TC* c) {
-  __shared__ f32x4 part[kFewWaves][MT][64];
+  __shared__ f32x4 part[kFewWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
   const int group = wave / p.split, ks = wave % p.split;  // split divides kFewWaves
   const int64_t n0 = ((int64_t)blockIdx.x * (kFewWaves / p.split) + group) * 16;
-  const int64_t kp = (int64_t)p.kb * kF8Block;
-  const int64_t n_row = min(n0 + r, p.n - 1);
-  const uint8_t *w = p.w + n_row * kp + g * 16, *ws = p.ws + n_row * p.ks, *a[MT], *as[MT];
-#pragma unroll
-  for (int i = 0; i < MT; i++) {
-    const int64_t row = min((int64_t)i * 16 + r, p.m - 1);
-    a[i] = p.a + row * p.a_st + g * 16;
-    as[i] = p.as + row * p.ks;
-  }
+  const int64_t n_row = min(n0 + r, p.n - 1), m_row = min((int64_t)r, p.m - 1);
+  const uint8_t *w = p.w + n_row * p.kb * kF8Block + g * 16, *ws = p.ws + n_row * p.ks;
+  const uint8_t *a = p.a + m_row * p.a_st + g * 16, *as = p.as + m_row * p.ks;
   struct Block {
     uint4 lo, hi;
     uint32_t s;
@@ -204,71 +203,54 @@ __device__ __forceinline__ void f8_few(const GemmParams& p, TC* c) {
     o[2] = widen8(x.hi.x, x.hi.y, s);
     o[3] = widen8(x.hi.z, x.hi.w, s);
   };
-  f32x4 acc[MT] = {};
-  Block cw[DEEP], ca[DEEP][MT];
+  f32x4 acc = {};
+  Block cw[kFewDeep], ca[kFewDeep];
 #pragma unroll
-  for (int d = 0; d < DEEP; d++)
+  for (int d = 0; d < kFewDeep; d++)
     if (ks + d * p.split < p.kb) {
       cw[d] = get(w, ws, ks + d * p.split);
-#pragma unroll
-      for (int i = 0; i < MT; i++) ca[d][i] = get(a[i], as[i], ks + d * p.split);
+      ca[d] = get(a, as, ks + d * p.split);
     }
-  for (int b0 = ks; b0 < p.kb; b0 += DEEP * p.split) {
+  for (int b0 = ks; b0 < p.kb; b0 += kFewDeep * p.split) {
 #pragma unroll
-    for (int d = 0; d < DEEP; d++) {
-      const int b = b0 + d * p.split, next = b + DEEP * p.split;
+    for (int d = 0; d < kFewDeep; d++) {
+      const int b = b0 + d * p.split, next = b + kFewDeep * p.split;
       if (b >= p.kb) break;  // (uniform in the wave)
-      bf16x8 x[4], y[MT][4];
+      bf16x8 x[4], y[4];
       widen(cw[d], x);
-#pragma unroll
-      for (int i = 0; i < MT; i++) widen(ca[d][i], y[i]);
+      widen(ca[d], y);
       if (next < p.kb) {
         cw[d] = get(w, ws, next);
-#pragma unroll
-        for (int i = 0; i < MT; i++) ca[d][i] = get(a[i], as[i], next);
+        ca[d] = get(a, as, next);
       }
 #pragma unroll
-      for (int q = 0; q < 4; q++)
-#pragma unroll
-        for (int i = 0; i < MT; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[q], y[i][q], acc[i], 0, 0, 0);
+      for (int q = 0; q < 4; q++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[q], y[q], acc, 0, 0, 0);
     }
   }
+  part[wave][lane] = acc;
+  __syncthreads();
   // lane: row r of A, columns 4 g .. + 3
   const int64_t col = n0 + g * 4;
-  if (p.split > 1) {
-#pragma unroll
-    for (int i = 0; i < MT; i++) part[wave][i][lane] = acc[i];
-    __syncthreads();
-    // the waves of a group share its tiles
-    for (int t = ks; t < MT; t += p.split) {
-      f32x4 one[1] = {part[group * p.split][t][lane]};
-      for (int s = 1; s < p.split; s++) one[0] = one[0] + part[group * p.split + s][t][lane];
-      const int64_t row[1] = {(int64_t)t * 16 + r};
-      if (col >= p.n) continue;
-      one[0] = before_mul(p, one[0], row[0], (int)col);
-      put4(p, c, row, col, one);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < MT; i++) {
-      const int64_t row[1] = {(int64_t)i * 16 + r};
-      if (col >= p.n) continue;
-      f32x4 one[1] = {before_mul(p, acc[i], row[0], (int)col)};
-      put4(p, c, row, col, one);
-    }
-  }
+  if (ks != 0 || col >= p.n) return;
+  f32x4 one[1] = {part[wave][lane]};
+  for (int s = 1; s < p.split; s++) one[0] = one[0] + part[wave + s][lane];
+  const int64_t row[1] = {r};
+  one[0] = before_mul(p, one[0], r, (int)col);
+  put4(p, c, row, col, one);
 }
 
-template <typename TC, int MT, int DEEP>
+template <typename TC>
 __global__ __launch_bounds__(kFewWaves * 64) void f8_few_kernel(GemmParams p, TC* c) {
-  f8_few<TC, MT, DEEP>(p, c);
+  f8_few(p, c);
 }
 
 // ---- tiles ---------------------------------------------------------------------------------
 
-// Workgroup barrier after the wave's direct loads to LDS have landed and its LDS reads are done.
+// Workgroup barrier after the wave's LDS reads are done and its direct loads to LDS have
+// landed but for the LEFT last ones.
+template <int LEFT = 0>
 __device__ __forceinline__ void tile_barrier() {
-  __builtin_amdgcn_s_waitcnt(0);  // every counter
+  __builtin_amdgcn_s_waitcnt((LEFT & 15) | (LEFT >> 4) << 14);  // (the other counters to 0)
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
   __builtin_amdgcn_s_barrier();
   __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -290,27 +272,69 @@ __device__ __forceinline__ void mix() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Four waves, each a quarter (BM / 2 x BN / 2) of the tile in 32 x 32 products. A
-// block of both operands (128 bytes of each row) goes straight from memory to LDS, two
-// blocks held: at the middle of a block the waves have read all of it, meet once,
-// and start the loads of the block after next into its place. Rows lie 128 bytes
+// Leaves a thread's sums of a part of K beside the other parts' of the tile. The
+// workgroup that comes last (true) adds them up, in their order: the result does not
+// depend on which one that is. last: a word of LDS.
+template <int SIZE>
+__device__ __forceinline__ bool join(const GemmParams& p, f32x16& x, int tile, int part, int* last) {
+  float* to = p.part + ((int64_t)tile * p.parts + part) * SIZE + threadIdx.x * 2;
+#pragma unroll
+  for (int q = 0; q < 8; q++) put2(to + q * 512, x[2 * q], x[2 * q + 1]);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this thread's are where every workgroup finds them
+  __syncthreads();
+  if (threadIdx.x == 0)
+    *last = __hip_atomic_fetch_add(p.count + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)p.parts - 1;
+  __syncthreads();
+  if (!*last) return false;
+  const float* from = p.part + (int64_t)tile * p.parts * SIZE + threadIdx.x * 2;
+  x = f32x16{};
+  for (int s = 0; s < p.parts; s++, from += SIZE) {
+    float2 y[8];
+#pragma unroll
+    for (int q = 0; q < 8; q++) y[q] = get2(from + q * 512);
+#pragma unroll
+    for (int q = 0; q < 8; q++) {
+      x[2 * q] += y[q].x;
+      x[2 * q + 1] += y[q].y;
+    }
+  }
+  return true;
+}
+
+// Four waves, WM of them one below the other, each with its part of the tile in 32 x 32
+// products. A block of both operands (128 bytes of each row) goes straight from memory
+// to LDS, D blocks held: at the middle of a block the waves have read all of it, meet
+// once, and start the loads of the block D on into its place. Rows lie 128 bytes
 // apart, their 16-byte pieces permuted by the row (piece j at j ^ (row & 7)), so that
 // eight lanes reading the same piece of eight rows use all banks. Operands of the
 // next half block are read while the products of this one run.
-template <int BM, int BN, typename TC>
+//
+// Large tiles are bound by products and two blocks are enough: 8192 x 8192 x 8192 with a
+// residual takes 550 us, 2.0 PFLOP/s (its products alone at 2.76), 4096^3 81. Small ones
+// wait for memory, a latency for each D - 1 blocks: 128 x 4096 x 4096 22 us with two
+// blocks, 14 with four. 1 x 262144 x 768 in float32 takes 46 us, 4.4 TB/s; 16 x 16384 x
+// 4096 16 us, 4.1 TB/s.
+template <int BM, int BN, int WM, int D, typename TC>
 __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m, int tiles_n) {
-  constexpr int FM = BM / 64, FN = BN / 64, NA = BM * 8 / 256, NB = BN * 8 / 256;
+  constexpr int WN = 4 / WM, MW = BM / WM, NW = BN / WN;  // waves each way, their parts of the tile
+  constexpr int FM = MW / 32, FN = NW / 32, NA = BM * 8 / 256, NB = BN * 8 / 256;
   constexpr bool F8 = sizeof(TC) == 2;  // on the 8-bit units
   constexpr int kStage = (BM + BN) * kF8Block;
-  __shared__ __attribute__((aligned(16))) uint8_t S0[kStage], S1[kStage];
+  __shared__ __attribute__((aligned(16))) uint8_t S0[kStage], S1[kStage], S2[D > 2 ? kStage : 16],
+      S3[D > 2 ? kStage : 16];  // (arrays of their own: reads of one need not wait for loads to another)
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave >> 1, wn = wave & 1;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
   const int64_t kp = (int64_t)p.kb * kF8Block;
   // Tiles of an XCD's run are taken in groups of 4 tile rows, down the columns: the
   // ones that run together share their rows of A and of W in its L2.
-  int tm, tn;
+  int tm, tn, tile, part = 0;
   {
-    const int tile = xcd_tile(tiles_m, tiles_n);
+    if (D > 2 && p.parts > 1) {
+      tile = blockIdx.x % (tiles_m * tiles_n);
+      part = blockIdx.x / (tiles_m * tiles_n);
+    } else {
+      tile = xcd_tile(tiles_m, tiles_n);
+    }
     constexpr int G = 4;
     const int group = tile / (G * tiles_n), rows = min(G, tiles_m - group * G), at = tile - group * G * tiles_n;
     tm = group * G + at % rows;
@@ -318,7 +342,9 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
   }
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   // the tile's first rows (the same for the workgroup), and a thread's pieces from there
-  const uint8_t *a0 = p.a + m0 * p.a_st, *b0 = p.w + n0 * kp;
+  const int first_block = part * p.per, kb = min(p.kb - first_block, p.per);
+  const int64_t skip = (int64_t)first_block * kF8Block;
+  const uint8_t *a0 = p.a + m0 * p.a_st + skip, *b0 = p.w + n0 * kp + skip;
   uint32_t ga[NA], gb[NB];
   {
     const int row = tid >> 3, piece = (tid & 7) ^ (row & 7);
@@ -340,7 +366,7 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
   };
   // operands: row lane % 32, bytes 32 (lane / 32) .. + 31 of each half block
   const int row = lane & 31, half = lane >> 5;
-  const int a_at = (wm * (BM / 2) + row) * kF8Block, b_at = BM * kF8Block + (wn * (BN / 2) + row) * kF8Block;
+  const int a_at = (wm * MW + row) * kF8Block, b_at = BM * kF8Block + (wn * NW + row) * kF8Block;
   int piece[2][2];
 #pragma unroll
   for (int h = 0; h < 2; h++)
@@ -360,17 +386,17 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
     for (int f = 0; f < FM; f++) o.a[f] = two(s + a_at + f * 32 * kF8Block, h);
   };
   // scale bytes of four blocks at a time
-  const uint8_t *as0 = p.as + m0 * p.ks, *bs0 = p.ws + n0 * p.ks;
+  const uint8_t *as0 = p.as + m0 * p.ks + first_block, *bs0 = p.ws + n0 * p.ks + first_block;
   uint32_t sa[FM], sb[FN];
 #pragma unroll
   for (int f = 0; f < FM; f++)
-    sa[f] = (uint32_t)min((int64_t)(wm * (BM / 2) + f * 32 + row), p.m - 1 - m0) * (uint32_t)p.ks;
+    sa[f] = (uint32_t)min((int64_t)(wm * MW + f * 32 + row), p.m - 1 - m0) * (uint32_t)p.ks;
 #pragma unroll
   for (int f = 0; f < FN; f++)
-    sb[f] = (uint32_t)min((int64_t)(wn * (BN / 2) + f * 32 + row), p.n - 1 - n0) * (uint32_t)p.ks;
+    sb[f] = (uint32_t)min((int64_t)(wn * NW + f * 32 + row), p.n - 1 - n0) * (uint32_t)p.ks;
   uint32_t xa[FM], xb[FN], na[FM], nb[FN];
   auto scales = [&](int b) {  // (rows of scale bytes are whole groups of four)
-    const int at = min(b, p.ks - 4);
+    const int at = min(b, p.ks - 4 - first_block);
 #pragma unroll
     for (int f = 0; f < FM; f++) na[f] = *reinterpret_cast<const uint32_t*>(as0 + at + sa[f]);
 #pragma unroll
@@ -408,53 +434,64 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
   Ops X, Y;
   // Block b, in s (its first half in X already); the next one is in `next`. Past the
   // last block the last is loaded again and not used: no branch in the loop.
+  static_assert(D == 2 || D == 4, "a group of four blocks goes through the places evenly");
+  uint8_t *const s2 = D > 2 ? S2 : S0, *const s3 = D > 2 ? S3 : S1;
   auto block = [&](uint8_t* s, uint8_t* next, int b, auto sel) {
     read(s, 1, Y);
     multiply(X, sel);
     mix<2 * (FM + FN), 0, F8 ? FM * FN : 0>();
-    tile_barrier();
-    stage(s, min(b + 2, p.kb - 1));
+    tile_barrier<(D - 2) * (NA + NB)>();
+    stage(s, min(b + D, kb - 1));
     read(next, 0, X);
     multiply(Y, sel);
     mix<2 * (FM + FN), NA + NB, F8 ? FM * FN : 0>();
   };
   using std::integral_constant;
-  if (p.kb > 0) {
+  if (kb > 0) {
     scales(0);
     stage(S0, 0);
-    stage(S1, min(1, p.kb - 1));
-    tile_barrier();
+    stage(S1, min(1, kb - 1));
+    if constexpr (D > 2) {
+      stage(S2, min(2, kb - 1));
+      stage(S3, min(3, kb - 1));
+    }
+    tile_barrier<(D - 1) * (NA + NB)>();
     read(S0, 0, X);
     int b = 0;
-    for (; b + 4 <= p.kb; b += 4) {
+    for (; b + 4 <= kb; b += 4) {
 #pragma unroll
       for (int f = 0; f < FM; f++) xa[f] = na[f];
 #pragma unroll
       for (int f = 0; f < FN; f++) xb[f] = nb[f];
       scales(b + 4);
       block(S0, S1, b, integral_constant<int, 0>());
-      block(S1, S0, b + 1, integral_constant<int, 1>());
-      block(S0, S1, b + 2, integral_constant<int, 2>());
-      block(S1, S0, b + 3, integral_constant<int, 3>());
+      block(S1, s2, b + 1, integral_constant<int, 1>());
+      block(s2, s3, b + 2, integral_constant<int, 2>());
+      block(s3, S0, b + 3, integral_constant<int, 3>());
     }
 #pragma unroll
     for (int f = 0; f < FM; f++) xa[f] = na[f];
 #pragma unroll
     for (int f = 0; f < FN; f++) xb[f] = nb[f];
-    if (b < p.kb) block(S0, S1, b, integral_constant<int, 0>());
-    if (b + 1 < p.kb) block(S1, S0, b + 1, integral_constant<int, 1>());
-    if (b + 2 < p.kb) block(S0, S1, b + 2, integral_constant<int, 2>());
+    if (b < kb) block(S0, S1, b, integral_constant<int, 0>());
+    if (b + 1 < kb) block(S1, s2, b + 1, integral_constant<int, 1>());
+    if (b + 2 < kb) block(s2, s3, b + 2, integral_constant<int, 2>());
     tile_barrier();  // (the loads that are not used)
+  }
+  if constexpr (D > 2) {
+    static_assert(FM * FN == 1, "one product's sums a wave");
+    static_assert(2 * 32 * (NW + 8) * 4 + 16 <= kStage, "a word that the epilogue leaves");
+    if (p.parts > 1 && !join<BM * BN>(p, acc[0][0], tile, part, reinterpret_cast<int*>(S0 + kStage - 16))) return;
   }
   // Through LDS, 32 rows of the wave at a time, so that rows of C are written whole. One
   // copy of what follows the writes: jumping over code that is not needed costs
   // as much as running it.
-  constexpr int kRow = BN / 2 + 8;  // (lanes 32 apart, four rows on, write to the other half of the banks)
+  constexpr int kRow = NW + 8;  // (lanes 32 apart, four rows on, write to the other half of the banks)
   static_assert(2 * 32 * kRow * 4 <= kStage, "the waves' rows fit");
   float* mine = reinterpret_cast<float*>(wave < 2 ? S0 : S1) + (wave & 1) * 32 * kRow;
-  constexpr int kLanes = BN / 8, kRows = 64 / kLanes, R = 32 / kRows < 8 ? 32 / kRows : 8;  // lanes of a row, rows at once, of those under way
+  constexpr int kLanes = NW / 4, kRows = 64 / kLanes, R = 32 / kRows < 8 ? 32 / kRows : 8;  // lanes of a row, rows at once, of those under way
   const int tr = lane / kLanes, tc = lane % kLanes * 4;
-  const int64_t col = n0 + wn * (BN / 2) + tc;
+  const int64_t col = n0 + wn * NW + tc;
   auto spread = [&](const f32x16 (&x)[FN]) {
 #pragma unroll
     for (int j = 0; j < FN; j++)
@@ -470,7 +507,7 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
     if constexpr (FM > 3) { if (i == 3) spread(acc[3]); }
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     if (col >= p.n) continue;
-    const int64_t first = m0 + wm * (BM / 2) + i * 32 + tr;
+    const int64_t first = m0 + wm * MW + i * 32 + tr;
     if (p.e.bias || p.e.row_scale || p.e.act != FA_ACT_NONE) {
 #pragma unroll 1
       for (int t = 0; t < 32; t += kRows) {
@@ -493,17 +530,18 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
 }
 
 // (A kernel whose own body holds arrays of dependent bounds in lambdas loses its host stub.)
-template <int BM, int BN, typename TC>
+template <int BM, int BN, int WM, int D, typename TC>
 __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void f8_tile_kernel(GemmParams p, TC* c, int tiles_m,
                                                                                  int tiles_n) {
-  f8_tile<BM, BN, TC>(p, c, tiles_m, tiles_n);
+  f8_tile<BM, BN, WM, D, TC>(p, c, tiles_m, tiles_n);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 }  // namespace
 
-int launch_f8_write(fa_ctx* ctx, const F8View& w, int dtype, const void* x, int64_t ldx, hipStream_t s) {
+int launch_f8_write(fa_ctx* ctx, const F8View& w, int dtype, const void* x, int64_t ldx, hipStream_t s, uint32_t* zero,
+                    int zeros) {
   const int kb = (int)(f8_kp(w.k) / kF8Block), ks = (int)f8_ks(w.k);
   // few blocks: one to 16 lanes, so that they spread over the card
   const int64_t blocks = w.n * kb, per = blocks > 65536 ? 64 : 16, units = (blocks + per - 1) / per;
@@ -513,13 +551,13 @@ int launch_f8_write(fa_ctx* ctx, const F8View& w, int dtype, const void* x, int6
   if (dtype == FA_DT_F32) {
     const float* f = (const float*)x;
     const bool vec = ldx % 4 == 0 && aligned(x, 16);
-    if (per == 64) f8_write_kernel<float, 4><<<grid, 256, 0, s>>>(w, f, ldx, kb, ks, vec);
-    else f8_write_kernel<float, 1><<<grid, 256, 0, s>>>(w, f, ldx, kb, ks, vec);
+    if (per == 64) f8_write_kernel<float, 4><<<grid, 256, 0, s>>>(w, f, ldx, kb, ks, vec, zero, zeros);
+    else f8_write_kernel<float, 1><<<grid, 256, 0, s>>>(w, f, ldx, kb, ks, vec, zero, zeros);
   } else {
     const uint16_t* h = (const uint16_t*)x;
     const bool vec = ldx % 8 == 0 && aligned(x, 16);
-    if (per == 64) f8_write_kernel<uint16_t, 4><<<grid, 256, 0, s>>>(w, h, ldx, kb, ks, vec);
-    else f8_write_kernel<uint16_t, 1><<<grid, 256, 0, s>>>(w, h, ldx, kb, ks, vec);
+    if (per == 64) f8_write_kernel<uint16_t, 4><<<grid, 256, 0, s>>>(w, h, ldx, kb, ks, vec, zero, zeros);
+    else f8_write_kernel<uint16_t, 1><<<grid, 256, 0, s>>>(w, h, ldx, kb, ks, vec, zero, zeros);
   }
   FA_CHECK_LAUNCH(ctx);
   return FA_OK;
@@ -537,43 +575,82 @@ int launch_f8_read(fa_ctx* ctx, const F8View& w, int dtype, void* out, int64_t l
   return FA_OK;
 }
 
-constexpr int64_t kFewRows = 64;  // up to so many rows a wave takes all the rows of its columns
-
 // Rows of A's codes a multiple of 2 KB apart would lie in few of the L2's channels:
 // a block more between them (8192 x 8192 x 8192 504 -> 496 us).
 int64_t a_stride(int64_t k) { return f8_kp(k) + (f8_kp(k) % 2048 == 0 ? kF8Block : 0); }
 
+namespace {
+
+// Tiles of a product, and the parts that K is split into. us, measured on both sides:
+// - Up to 16 rows and 2^24 weights the kernel for few rows, else tiles: 16 x 4096 x 4096
+//   12.4 and 13.6, 1 x 4096 x 4096 11.5 and 14; 1 x 32768 x 1024 16.7 and 11.4, 1 x 262144
+//   x 768 51 and 46.
+// - Tiles of 128 and of 256 (bf16) where they fill the card: 2048^3 is 24 in tiles of 128.
+//   Below, tiles of 64, and of 32 x 128 up to 32 rows: 32 x 262144 x 768 57 and 63 in
+//   tiles of 64, 1 x 262144 x 768 46 and 56 (two of either fit in a CU's LDS).
+// - Where these do not fill the card either, K in up to 8 parts of 8 blocks or more, which
+//   pays for joining them: 128 x 1152 x 16384 in float32 46 whole, 21 in parts; 32 x 4096 x
+//   4096 15.5 and 12.6; 512 x 512 x 4096 17.5 and 15.7, parts of 4 blocks there 18, 32 x
+//   1152 x 16384 42 whole, 17 in 8 parts, 19 in 16, 28 in twice the card's workgroups.
+constexpr int kCUs = 256;  // of the card
+struct Plan {
+  int tile;  // 256, 128, 64, 32 (x 128); 0: few rows
+  int parts, per;
+  int64_t tiles;
+};
+Plan plan_of(int64_t m, int64_t n, int64_t k, bool bf16) {
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
+  const int kb = (int)(f8_kp(k) / kF8Block);
+  Plan p = {0, 1, kb, 0};
+  if (m <= 16 && n * kb <= 131072) return p;
+  if (m > 64 && tiles(128, 128) >= kCUs) {
+    p.tile = bf16 && m > 128 && tiles(256, 256) >= kCUs ? 256 : 128;
+    return p;
+  }
+  p.tile = m > 32 ? 64 : 32;
+  p.tiles = m > 32 ? tiles(64, 64) : tiles(32, 128);
+  const int64_t most = std::min<int64_t>(kCUs / p.tiles, std::min(kb / 8, 8));
+  if (most > 1) {
+    p.per = (int)((kb + most - 1) / most + 3) / 4 * 4;
+    p.parts = (kb + p.per - 1) / p.per;
+  }
+  return p;
+}
+
+}  // namespace
+
 size_t f8_scratch(int64_t m, int64_t n, int64_t k) {
-  return align256((size_t)m * a_stride(k)) + align256((size_t)m * f8_ks(k));
+  const Plan p = plan_of(m, n, k, false);
+  const size_t joined = p.parts > 1 ? align256((size_t)p.tiles * 4) + (size_t)p.tiles * p.parts * 4096 * 4 : 0;
+  return align256((size_t)m * a_stride(k)) + align256((size_t)m * f8_ks(k)) + joined;
 }
 
 int64_t f8_grid(int64_t m, int64_t n) { return ((m + 15) / 16) * ((n + 63) / 64); }
 
 namespace {
 
+template <int BM, int BN, int WM, int D, typename TC>
+void launch_tiles(const GemmParams& p, TC* c, hipStream_t s) {
+  const int tm = (int)((p.m + BM - 1) / BM), tn = (int)((p.n + BN - 1) / BN);
+  f8_tile_kernel<BM, BN, WM, D, TC><<<(unsigned)(tm * tn * p.parts), 256, 0, s>>>(p, c, tm, tn);
+}
+
 template <typename TC>
-void launch_gemm_t(const GemmParams& p, TC* c, int cus, hipStream_t s) {
-  if (p.m <= kFewRows) {
-    GemmParams q = p;
-    const int64_t groups = (p.n + 15) / 16;
-    q.split = kFewWaves;
-    while (q.split > 1 && (groups * q.split > 8192 || q.split > std::max(1, p.kb))) q.split /= 2;
-    const unsigned grid = (unsigned)((groups * q.split + kFewWaves - 1) / kFewWaves);
-    if (p.m <= 16) f8_few_kernel<TC, 1, 4><<<grid, kFewWaves * 64, 0, s>>>(q, c);
-    else if (p.m <= 32) f8_few_kernel<TC, 2, 3><<<grid, kFewWaves * 64, 0, s>>>(q, c);
-    else f8_few_kernel<TC, 4, 2><<<grid, kFewWaves * 64, 0, s>>>(q, c);
-    return;
-  }
-  const int64_t big = ((p.m + 255) / 256) * ((p.n + 255) / 256);
-  if (sizeof(TC) == 2 && big >= cus) {
-    const int tm = (int)((p.m + 255) / 256), tn = (int)((p.n + 255) / 256);
-    f8_tile_kernel<256, 256, uint16_t><<<(unsigned)(tm * tn), 256, 0, s>>>(p, (uint16_t*)c, tm, tn);
-  } else if (((p.m + 127) / 128) * ((p.n + 127) / 128) >= cus) {
-    const int tm = (int)((p.m + 127) / 128), tn = (int)((p.n + 127) / 128);
-    f8_tile_kernel<128, 128, TC><<<(unsigned)(tm * tn), 256, 0, s>>>(p, c, tm, tn);
+void launch_gemm_t(const GemmParams& p, TC* c, int tile, hipStream_t s) {
+  if (tile == 256) {
+    launch_tiles<256, 256, 2, 2>(p, (uint16_t*)c, s);
+  } else if (tile == 128) {
+    launch_tiles<128, 128, 2, 2>(p, c, s);
+  } else if (tile == 64) {
+    launch_tiles<64, 64, 2, 4>(p, c, s);
+  } else if (tile == 32) {
+    launch_tiles<32, 128, 1, 4>(p, c, s);
   } else {
-    const int tm = (int)((p.m + 63) / 64), tn = (int)((p.n + 63) / 64);
-    f8_tile_kernel<64, 64, TC><<<(unsigned)(tm * tn), 256, 0, s>>>(p, c, tm, tn);
+    GemmParams q = p;
+    q.split = kFewWaves;
+    while (q.split > std::max(1, p.kb)) q.split /= 2;
+    const int columns = 16 * kFewWaves / q.split;
+    f8_few_kernel<<<(unsigned)((p.n + columns - 1) / columns), kFewWaves * 64, 0, s>>>(q, c);
   }
 }
 
@@ -581,14 +658,21 @@ void launch_gemm_t(const GemmParams& p, TC* c, int cus, hipStream_t s) {
 
 int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s) {
   const int64_t k = g.w.k;
+  const Plan plan = plan_of(g.m, g.w.n, k, g.c_dtype != FA_DT_F32);
   F8View a = {nullptr, nullptr, g.m, k, a_stride(k)};
+  GemmParams p = {};
+  p.parts = plan.parts;
+  p.per = plan.per;
   if (k > 0) {
     a.codes = static_cast<uint8_t*>(work);
     a.scales = a.codes + align256((size_t)g.m * a.stride);
-    const int rc = launch_f8_write(ctx, a, g.a_dtype, g.a, g.lda, s);
+    if (p.parts > 1) {
+      p.count = reinterpret_cast<uint32_t*>(a.scales + align256((size_t)g.m * f8_ks(k)));
+      p.part = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(p.count) + align256((size_t)plan.tiles * 4));
+    }
+    const int rc = launch_f8_write(ctx, a, g.a_dtype, g.a, g.lda, s, p.count, p.parts > 1 ? (int)plan.tiles : 0);
     if (rc) return rc;
   }
-  GemmParams p = {};
   p.m = g.m;
   p.n = g.w.n;
   p.k = k;
@@ -605,8 +689,8 @@ int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s) 
   p.vec_residual = g.e.ldr % 4 == 0 && aligned(g.e.residual, 16);
   p.vec_c = g.ldc % 4 == 0 && aligned(g.c, g.c_dtype == FA_DT_F32 ? 16 : 8);
   p.ldc = g.ldc;
-  if (g.c_dtype == FA_DT_F32) launch_gemm_t(p, (float*)g.c, ctx->cu_count, s);
-  else launch_gemm_t(p, (uint16_t*)g.c, ctx->cu_count, s);
+  if (g.c_dtype == FA_DT_F32) launch_gemm_t(p, (float*)g.c, plan.tile, s);
+  else launch_gemm_t(p, (uint16_t*)g.c, plan.tile, s);
   FA_CHECK_LAUNCH(ctx);
   return FA_OK;
 }

@@ -329,3 +329,27 @@ def test_work_is_checked(ctx):
     np.testing.assert_array_equal(c.get((500, 600), np.float32), 300)
     for b in (a, c, w, held):
         b.free()
+
+
+# ---- K in parts --------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("cdt", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(17, 1, 2048), (20, 200, 2088), (32, 129, 4096), (33, 70, 5000), (64, 65, 2176),
+                                   (130, 300, 3333), (1, 3000, 8192), (16, 1100, 16000), (200, 64, 9000)])
+def test_long_rows(ctx, m, n, k, cdt):
+    """Few tiles and long rows: parts of K that several workgroups sum, an uneven last part among them."""
+    case(ctx, m, n, k, "bf16", cdt, work=k % 2 == 0, epi=("bias", 2, "mul", "residual"), pad=3)
+
+
+def test_long_rows_give_the_same_bits(ctx):
+    """Whichever workgroup joins the parts; and on work that held another call's counts."""
+    r = G.rng(91)
+    held = [Held(ctx, n, k).write(r.standard_normal((n, k)).astype(np.float32)) for n, k in ((300, 8192), (100, 5000))]
+    a = [r.standard_normal((m, h.k)).astype(np.float32) for m, h in zip((40, 20), held)]
+    first = [product(ctx, h, x, "f32") for h, x in zip(held, a)]
+    for i in range(12):
+        for h, x, want in zip(held, a, first):
+            np.testing.assert_array_equal(product(ctx, h, x, "f32", work=i % 3 == 0), want)
+    for h in held:
+        h.free()
