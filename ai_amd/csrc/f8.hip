@@ -319,6 +319,7 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
   constexpr int WN = 4 / WM, MW = BM / WM, NW = BN / WN;  // waves each way, their parts of the tile
   constexpr int FM = MW / 32, FN = NW / 32, NA = BM * 8 / 256, NB = BN * 8 / 256;
   constexpr bool F8 = sizeof(TC) == 2;  // on the 8-bit units
+  constexpr bool kJoins = FM * FN == 1;  // K may be split
   constexpr int kStage = (BM + BN) * kF8Block;
   __shared__ __attribute__((aligned(16))) uint8_t S0[kStage], S1[kStage], S2[D > 2 ? kStage : 16],
       S3[D > 2 ? kStage : 16];  // (arrays of their own: reads of one need not wait for loads to another)
@@ -329,7 +330,7 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
   // ones that run together share their rows of A and of W in its L2.
   int tm, tn, tile, part = 0;
   {
-    if (D > 2 && p.parts > 1) {
+    if (kJoins && p.parts > 1) {
       tile = blockIdx.x % (tiles_m * tiles_n);
       part = blockIdx.x / (tiles_m * tiles_n);
     } else {
@@ -478,8 +479,7 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
     if (b + 2 < kb) block(s2, s3, b + 2, integral_constant<int, 2>());
     tile_barrier();  // (the loads that are not used)
   }
-  if constexpr (D > 2) {
-    static_assert(FM * FN == 1, "one product's sums a wave");
+  if constexpr (kJoins) {
     static_assert(2 * 32 * (NW + 8) * 4 + 16 <= kStage, "a word that the epilogue leaves");
     if (p.parts > 1 && !join<BM * BN>(p, acc[0][0], tile, part, reinterpret_cast<int*>(S0 + kStage - 16))) return;
   }
@@ -531,7 +531,7 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
 
 // (A kernel whose own body holds arrays of dependent bounds in lambdas loses its host stub.)
 template <int BM, int BN, int WM, int D, typename TC>
-__global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void f8_tile_kernel(GemmParams p, TC* c, int tiles_m,
+__global__ __launch_bounds__(256, (BM + BN) * D > 512 ? 1 : 2) void f8_tile_kernel(GemmParams p, TC* c, int tiles_m,
                                                                                  int tiles_n) {
   f8_tile<BM, BN, WM, D, TC>(p, c, tiles_m, tiles_n);
 }
@@ -585,7 +585,10 @@ namespace {
 // - Up to 16 rows and 2^24 weights the kernel for few rows, else tiles: 16 x 4096 x 4096
 //   12.4 and 13.6, 1 x 4096 x 4096 11.5 and 14; 1 x 32768 x 1024 16.7 and 11.4, 1 x 262144
 //   x 768 51 and 46.
-// - Tiles of 128 and of 256 (bf16) where they fill the card: 2048^3 is 24 in tiles of 128.
+// - Tiles of 128 and of 256 (bf16) where they fill the card; of 128 with four blocks held,
+//   for bf16, where they are at most one for each CU, and that for 3 of 4: 512 x 8192 x
+//   8192 61 and 47, 896 x 4096 x 4096 in tiles of 64 40, so 29, but 512 x 4096 x 4096 (128
+//   tiles) 23 and 26, and in float32, bound by widening, 384 x 8192 x 8192 67 and 68.
 //   Below, tiles of 64, and of 32 x 128 up to 32 rows: 32 x 262144 x 768 57 and 63 in
 //   tiles of 64, 1 x 262144 x 768 46 and 56 (two of either fit in a CU's LDS).
 // - Where these do not fill the card either, K in up to 8 parts of 8 blocks or more, which
@@ -594,17 +597,20 @@ namespace {
 //   1152 x 16384 42 whole, 17 in 8 parts, 19 in 16, 28 in twice the card's workgroups.
 constexpr int kCUs = 256;  // of the card
 struct Plan {
-  int tile;  // 256, 128, 64, 32 (x 128); 0: few rows
+  int tile;   // 256, 128, 64, 32 (x 128); 0: few rows
+  bool deep;  // four blocks held of tiles of 128
   int parts, per;
   int64_t tiles;
 };
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool bf16) {
   auto tiles = [&](int64_t bm, int64_t bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
   const int kb = (int)(f8_kp(k) / kF8Block);
-  Plan p = {0, 1, kb, 0};
+  Plan p = {0, false, 1, kb, 0};
   if (m <= 16 && n * kb <= 131072) return p;
-  if (m > 64 && tiles(128, 128) >= kCUs) {
+  const int64_t large = m > 64 ? tiles(128, 128) : 0;
+  if (large >= kCUs || (bf16 && large * 4 >= kCUs * 3)) {
     p.tile = bf16 && m > 128 && tiles(256, 256) >= kCUs ? 256 : 128;
+    p.deep = bf16 && large <= kCUs;
     return p;
   }
   p.tile = m > 32 ? 64 : 32;
@@ -636,9 +642,12 @@ void launch_tiles(const GemmParams& p, TC* c, hipStream_t s) {
 }
 
 template <typename TC>
-void launch_gemm_t(const GemmParams& p, TC* c, int tile, hipStream_t s) {
+void launch_gemm_t(const GemmParams& p, TC* c, const Plan& plan, hipStream_t s) {
+  const int tile = plan.tile;
   if (tile == 256) {
     launch_tiles<256, 256, 2, 2>(p, (uint16_t*)c, s);
+  } else if (plan.deep) {
+    launch_tiles<128, 128, 2, 4>(p, (uint16_t*)c, s);
   } else if (tile == 128) {
     launch_tiles<128, 128, 2, 2>(p, c, s);
   } else if (tile == 64) {
@@ -689,8 +698,8 @@ int launch_f8_gemm(fa_ctx* ctx, const F8GemmArgs& g, void* work, hipStream_t s) 
   p.vec_residual = g.e.ldr % 4 == 0 && aligned(g.e.residual, 16);
   p.vec_c = g.ldc % 4 == 0 && aligned(g.c, g.c_dtype == FA_DT_F32 ? 16 : 8);
   p.ldc = g.ldc;
-  if (g.c_dtype == FA_DT_F32) launch_gemm_t(p, (float*)g.c, plan.tile, s);
-  else launch_gemm_t(p, (uint16_t*)g.c, plan.tile, s);
+  if (g.c_dtype == FA_DT_F32) launch_gemm_t(p, (float*)g.c, plan, s);
+  else launch_gemm_t(p, (uint16_t*)g.c, plan, s);
   FA_CHECK_LAUNCH(ctx);
   return FA_OK;
 }
