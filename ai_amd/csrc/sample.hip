@@ -253,6 +253,9 @@ struct Held {
   }
 };
 
+// Bound by its arithmetic where rows are many: an exponential in float64 and two
+// additions in LDS a token (256 rows of 262144 in float32 125 us, 2.1 TB/s, where the
+// bytes take 54; without filters nothing is added in LDS). One such row: 9 us, latencies.
 template <typename T, int E>
 __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs a, Plan p) {
   __shared__ uint64_t red[kScan / 64];
@@ -372,7 +375,8 @@ __device__ __forceinline__ uint64_t row_top(const Plan& p, int64_t row, uint64_t
 
 // One workgroup a row, a thread a bin: what the slices have down to the last step of
 // each. Slices are taken kChunk at a time, their heads first, and the sums of kAtOnce
-// slices are under way at once.
+// slices are under way at once. A chain of loads and scans in one workgroup: 10 us for 8
+// slices, 12 for 32, 15 for 256 rows of 32.
 constexpr int kChunk = 64, kAtOnce = 16;
 __global__ __launch_bounds__(kBins) void join_kernel(SampleArgs a, Plan p) {
   constexpr int NT = kBins;
@@ -477,6 +481,8 @@ __global__ __launch_bounds__(kBins) void join_kernel(SampleArgs a, Plan p) {
   if (tid == 0) p.cut[row] = c;
 }
 
+// Slices without such tokens are left after their head. 256 rows of 262144 in float32 66 us,
+// 4.1 TB/s; one 7.
 template <typename T, int E>
 __global__ __launch_bounds__(kScan) void gather_kernel(SampleArgs a, Plan p) {
   __shared__ uint32_t n_listed;
@@ -645,6 +651,9 @@ __device__ uint64_t select_token(const SampleArgs& a, const Plan& p, int64_t row
   return hi;
 }
 
+// One workgroup a row, bound by its own chain: two selections, each of passes over the
+// listed tokens, the slices' weights, the walk. One row of 262144 21 us, 64 of 32000 31, 256
+// of 262144 91; 37 of 49999 without filters 11.
 template <typename T, int E>
 __global__ __launch_bounds__(kFinish) void finish_kernel(SampleArgs a, Plan p) {
   __shared__ FinishMem mem;
@@ -866,8 +875,8 @@ __global__ __launch_bounds__(kFinish) void finish_kernel(SampleArgs a, Plan p) {
 // ---- the division of rows ----------------------------------------------------------------------------
 
 int per_of(int64_t rows, int64_t vocab) {
-  // few workgroups: shorter slices, but not so many that joining them takes longer (64 of a row: 17 us, 32: 9); a row has
-  // no more than kMaxSlices
+  // few workgroups: shorter slices, but not so many that joining them takes longer (64 of a
+  // row: 17 us, 32: 9); a row has no more than kMaxSlices
   const auto slices = [&](int e) { return (vocab + e * kScan - 1) / (e * kScan); };
   if (slices(8) <= 16 && (rows * slices(8) <= 1024 || slices(8) == 1)) return 8 * kScan;
   return slices(16) <= kMaxSlices ? 16 * kScan : 32 * kScan;

@@ -359,3 +359,9 @@ def test_long_rows_give_the_same_bits(ctx):
 @pytest.mark.parametrize("m,n,k", [(1700, 2000, 700), (100, 26000, 130), (1000, 4100, 1153), (300, 32768, 260)])
 def test_tiles_about_as_many_as_cus(ctx, m, n, k, cdt):
     case(ctx, m, n, k, "bf16", cdt, epi=("residual",))
+
+
+@pytest.mark.parametrize("cdt", ["f32", "bf16"])
+@pytest.mark.parametrize("m", [3, 20, 70])
+def test_very_long_rows(ctx, m, cdt):
+    case(ctx, m, 3, 200001, "f32", cdt, work=True)
