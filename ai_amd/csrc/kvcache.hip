@@ -90,12 +90,11 @@ __device__ __forceinline__ int stored_exp(float s) {
 // One workgroup writes one (block, head, keys or values): all its new values
 // in registers, one reduction for the scale, one store. Bytes are read and
 // written once. Prompts (16 of up to 2048 tokens, 8 heads of 128 dims in bf16) take
-// 42 us after other work, 33 one after another, where the bytes take 28 at a large
-// copy's rate (in float32 41 one after another, of 46): each of 6288 workgroups waits
-// for its sequence, its block and its rows in turn, then reduces and stores with
-// nothing of the next under way. Single tokens are bound by that chain and the
-// write-back of the 128 lines that one token's values touch in a head (64 sequences,
-// one float32 token each, written 7.1 us).
+// 29 us one after another, where the bytes take 28 at a large copy's rate (42 with each
+// load widened, and so waited for, before the next). Single tokens are bound by the
+// chain of dependent loads (sequence, block, row) and the write-back of the 128 lines
+// that one token's values touch in a head (64 sequences, one float32 token each,
+// written 7.1 us).
 // at(row): a row's values. vec: fours of them are aligned.
 template <typename T, int NCM, typename F>
 __device__ __forceinline__ void write_block(const KvArgs& a, const KvUnit& u, int id, int h, int part, bool vec, F at) {
