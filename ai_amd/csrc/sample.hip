@@ -175,6 +175,10 @@ __device__ __forceinline__ uint64_t to_int(double x) {
   return (uint64_t)__double_as_longlong(x + 0x1p52) - (uint64_t)0x4330000000000000ull;
 }
 constexpr int kUnit = 48;  // a bin's weights are held in units of 2^-48 of its middle: 2^14 of them fit
+// Sums are right to 1e-13: weights to 2^-48, a thousand additions. Two that the definition
+// has equal (of equal logits, whose weights are 1) may differ by that much either way, so
+// a sum reaches a bound from this much below it on.
+constexpr double kNear = 1e-12;
 
 // ---- a workgroup's sums and scans, in a fixed order -----------------------------------------
 
@@ -461,9 +465,9 @@ __global__ __launch_bounds__(kBins) void join_kernel(SampleArgs a, Plan p) {
     c.above_k = k_least = c.k_bin ? sums[c.k_bin - 1] : 0.0;
     k_most = sums[c.k_bin];
   }
-  // top-p: sums are right to 1e-14 or so, the margin of 1e-12 keeps to either side
+  // top-p: the aim is taken kNear lower from other sums, a margin of that keeps to either side
   if (r.top_p < 1.f) {
-    const double least = (double)r.top_p * k_least * (1 - 1e-12), want = (double)r.top_p * k_most * (1 + 1e-12);
+    const double least = (double)r.top_p * k_least * (1 - 2 * kNear), want = (double)r.top_p * k_most * (1 + kNear);
     if (before < least && m >= least) atomicMin(&found[2], tid);
     if (before < want && m >= want) atomicMin(&found[3], tid);
     __syncthreads();
@@ -580,7 +584,7 @@ __device__ uint64_t select_token(const SampleArgs& a, const Plan& p, int64_t row
   constexpr int W = kSub / kFinish;  // bins of a thread
   const int tid = threadIdx.x;
   uint64_t before = 0, count_before = 0;  // integer weight and tokens above hi
-  want = fmax(want, above + ldexp(1.0, -unit));  // (top_p = 0: the first token all the same)
+  want = fmax(want * (1 - kNear), above + ldexp(1.0, -unit));  // (top_p = 0: the first token all the same)
   while (lo < hi) {
     const int shift = max(0, 64 - (int)__builtin_clzll(hi - lo) - 11);
     for (int i = tid; i < kSub; i += kFinish) {

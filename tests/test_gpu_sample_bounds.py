@@ -1,0 +1,34 @@
+"""Sampling where sums meet their bounds exactly: equal logits, whose weights
+are 1, so that the definition's sums have no rounding and say which tokens stay
+and which is drawn."""
+import numpy as np
+import pytest
+
+import test_gpu_kvcache as G
+import test_gpu_sample as T
+from ai_amd import synth as S
+
+pytestmark = pytest.mark.gpu
+INF = np.inf
+
+
+def some_equal(r, rows, n, vocab, dtype, spread=3.0):
+    """Rows of n equal logits at places of their own, -inf elsewhere."""
+    l = np.full((rows, vocab), -INF, np.float32)
+    for x in l:
+        x[r.permutation(vocab)[:n]] = np.float32(r.standard_normal() * spread)
+    return S.f32_to_bf16(l) if dtype == "bf16" else l
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [2, 4, 8, 1000])
+def test_top_p_of_equal_logits(ctx, n, dtype):
+    """A share of n tokens that is a whole number of them is reached by that many."""
+    r = G.rng(n)
+    rows = 240
+    l = some_equal(r, rows, n, n + 37, dtype)
+    top_p = r.choice([0.25, 0.5, 0.75], rows).astype(np.float32)
+    temperature = r.choice([1e-3, 0.2, 0.7, 1.0, 1.7], rows).astype(np.float32)
+    for u in (0.0, 0.3, 0.9, 1 - 2.0 ** -24):
+        u = np.full(rows, u, np.float32)
+        T.check(T.draw(ctx, l, u, top_p=top_p, temperature=temperature), l, u, top_p=top_p, temperature=temperature)
