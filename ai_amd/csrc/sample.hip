@@ -51,7 +51,6 @@ struct Cut {
   int p_lo, p_hi;     // bins of top_p's bound (kBins: none)
   int m_lo, m_hi;     // of min_p's
   double step;        // the grid's step of most
-  double t;           // most on the grid
   double above_k, above_p;  // weights of the bins before k_bin, before p_lo
   double all;         // of all bins
   __device__ __forceinline__ bool listed(int b) const {
@@ -158,12 +157,15 @@ __device__ __forceinline__ double last_step(int b, double top) {
 __device__ __forceinline__ int bin_of(float l, double inv, double top) { return bin_of_step(floor(grid_of(l, inv)), top); }
 // From here on unequal logits are 2^16 steps and more apart, and t is taken as it is.
 constexpr double kFar = 0x1p40;
-// Weight in the middle of bin b of steps counted from `top`, beside the logit at t.
-__device__ __forceinline__ double middle(int b, double top, double t) {
+// Weight in the middle of bin b of steps counted from `top`, beside the logit l. The
+// distance takes l's place on the grid unrounded: 2^39 steps from zero its rounding is 2e-6
+// of the weight.
+__device__ __forceinline__ double middle(int b, double top, float l, double inv) {
+  const double t = grid_of(l, inv);
   if (!(fabs(t) < kFar)) return b == 0 && top == floor(t) ? 1.0 : 0.0;
   double at = top - (double)b + 0.5;
   if (b >= kFine) at = (floor(top * 0.03125) - (double)(b - (kFine - kFine / 32))) * 32.0 + 16.0;
-  return exp_scaled((at - t) * 0.03125, 0);
+  return exp_scaled(fma(l == __builtin_inff() ? 0.0 : -(double)l, 32.0 * inv, at) * 0.03125, 0);
 }
 // Weights in bin b are below 2^-bin_exp(b): (b - 1) / 32 below the first, or a wide step less than wide steps.
 __device__ __forceinline__ int bin_exp(int b) {
@@ -336,7 +338,6 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs a, Plan p) {
   __syncthreads();
   // running sums over the bins (two neighbours a thread); without top-k, whether there are tokens in a bin is all that is asked
   static_assert(kBins == 2 * kScan, "two bins a thread");
-  const double t0 = grid_of(most, r.inv);
   uint64_t w[2];
   double m[2];
   uint32_t n[2];
@@ -346,7 +347,7 @@ __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs a, Plan p) {
     const int b = 2 * tid + i;
     w[i] = mass[b];
     n[i] = counted ? count[b] : w[i] != 0;
-    m[i] = w[i] ? ldexp((double)w[i], -kUnit) * middle(b, step, t0) : 0.0;
+    m[i] = w[i] ? ldexp((double)w[i], -kUnit) * middle(b, step, most, r.inv) : 0.0;
     if (n[i]) last = b + 1;
   }
   last = block_join<kScan>(last, (int*)red, Max());
@@ -396,8 +397,7 @@ __global__ __launch_bounds__(kBins) void join_kernel(SampleArgs a, Plan p) {
   if (!(most > -__builtin_inff())) return;
   Cut c;
   c.most = most;
-  c.t = grid_of(most, r.inv);
-  c.step = floor(c.t);
+  c.step = floor(grid_of(most, r.inv));
   c.k_bin = c.p_lo = c.m_lo = kBins;
   c.p_hi = c.m_hi = -1;
   c.k_rank = 0;

@@ -32,3 +32,16 @@ def test_top_p_of_equal_logits(ctx, n, dtype):
     for u in (0.0, 0.3, 0.9, 1 - 2.0 ** -24):
         u = np.full(rows, u, np.float32)
         T.check(T.draw(ctx, l, u, top_p=top_p, temperature=temperature), l, u, top_p=top_p, temperature=temperature)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_shares_where_logits_are_many_steps_from_zero(ctx, dtype):
+    """Logits that are up to 2^39 steps of 1/32 of the temperature from zero share the weight as others do."""
+    r = G.rng(5)
+    rows, n = 120, 6
+    l = some_equal(r, rows, n, 90, dtype, spread=1000.0)
+    temperature = (10.0 ** r.uniform(-7, 0, rows)).astype(np.float32)
+    u = (np.arange(rows) % n / n + 0.01).astype(np.float32)
+    for s in (dict(min_p=0.5), dict(top_p=0.999), dict(top_p=0.5), dict(top_k=20, min_p=0.1)):
+        s = {k: np.full(rows, v, np.int32 if k == "top_k" else np.float32) for k, v in s.items()}
+        T.check(T.draw(ctx, l, u, temperature=temperature, **s), l, u, temperature=temperature, **s)
