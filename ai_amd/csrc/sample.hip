@@ -179,7 +179,7 @@ __device__ __forceinline__ uint64_t to_int(double x) {
 constexpr int kUnit = 48;  // a bin's weights are held in units of 2^-48 of its middle: 2^14 of them fit
 // Sums are right to 1e-13: weights to 2^-48, a thousand additions. Two that the definition
 // has equal (of equal logits, whose weights are 1) may differ by that much either way, so
-// a sum reaches a bound from this much below it on.
+// a sum reaches a bound from this much below it on, and exceeds it from this much above.
 constexpr double kNear = 1e-12;
 
 // ---- a workgroup's sums and scans, in a fixed order -----------------------------------------
@@ -790,7 +790,7 @@ __global__ __launch_bounds__(kFinish) void finish_kernel(SampleArgs a, Plan p) {
     at[i] = total + block_scan<kFinish>(mine[i], mem.redd, &all);
     total += all;
   }
-  const double aim = (double)r.u * total;
+  const double aim = (double)r.u * total * (1 + kNear);  // (equal to a running sum: not exceeded by it)
   if (tid == 0) mem.found = -1;
   __syncthreads();
 #pragma unroll

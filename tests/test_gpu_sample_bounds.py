@@ -45,3 +45,17 @@ def test_shares_where_logits_are_many_steps_from_zero(ctx, dtype):
     for s in (dict(min_p=0.5), dict(top_p=0.999), dict(top_p=0.5), dict(top_k=20, min_p=0.1)):
         s = {k: np.full(rows, v, np.int32 if k == "top_k" else np.float32) for k, v in s.items()}
         T.check(T.draw(ctx, l, u, temperature=temperature, **s), l, u, temperature=temperature, **s)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("s", [dict(min_p=0.5), dict(top_p=0.999), dict(top_k=16), {}])
+@pytest.mark.parametrize("n", [2, 4, 16])
+def test_numbers_on_the_border_of_two_tokens(ctx, n, s, dtype):
+    """u times the sum equal to a running sum draws the token after it: the sum does not exceed it."""
+    r = G.rng(n + 100)
+    rows = 160
+    l = some_equal(r, rows, n, n + 50, dtype)
+    u = (np.arange(rows) % n / n).astype(np.float32)
+    s = {k: np.full(rows, v, np.int32 if k == "top_k" else np.float32) for k, v in s.items()}
+    s["temperature"] = r.choice([0.3, 0.7, 1.0, 1.9], rows).astype(np.float32)
+    T.check(T.draw(ctx, l, u, **s), l, u, **s)
