@@ -791,24 +791,21 @@ __global__ __launch_bounds__(kFinish) void finish_kernel(SampleArgs a, Plan p) {
     total += all;
   }
   const double aim = (double)r.u * total * (1 + kNear);  // (equal to a running sum: not exceeded by it)
-  if (tid == 0) mem.found = -1;
-  __syncthreads();
+  // the first slice whose end is past it: one thread's answer, also where the sums before two
+  // neighbours, which come from different trees of additions, overlap or leave a gap
+  int s = kMaxSlices, last = -1;
+#pragma unroll
+  for (int i = 0; i < kMaxSlices / kFinish; i++) {
+    if (!(mine[i] > 0)) continue;
+    if (at[i] + mine[i] > aim) s = min(s, i * kFinish + tid);
+    last = i * kFinish + tid;
+  }
+  s = block_join<kFinish>(s, (int*)mem.redd, Min());
+  if (s == kMaxSlices) s = block_join<kFinish>(last, (int*)mem.redd, Max());  // (rounding: the last slice of any weight)
 #pragma unroll
   for (int i = 0; i < kMaxSlices / kFinish; i++)
-    if (at[i] <= aim && at[i] + mine[i] > aim) mem.found = i * kFinish + tid, mem.found_before = at[i];
+    if (s == i * kFinish + tid) mem.found_before = at[i];
   __syncthreads();
-  int s = mem.found;
-  if (s < 0) {  // (rounding: the last slice of any weight)
-    int last = -1;
-#pragma unroll
-    for (int i = 0; i < kMaxSlices / kFinish; i++)
-      if (mine[i] > 0) last = i * kFinish + tid;
-    s = block_join<kFinish>(last, (int*)mem.red, Max());
-#pragma unroll
-    for (int i = 0; i < kMaxSlices / kFinish; i++)
-      if (s == i * kFinish + tid) mem.found_before = at[i];
-    __syncthreads();
-  }
   // the walk: each wave weighs a run of the slice's ids, the one that the number falls into goes along it
   const double rest = aim - mem.found_before;
   const int first = s * p.per + wave * 64 * E + lane, end = (int)a.vocab;

@@ -59,3 +59,20 @@ def test_numbers_on_the_border_of_two_tokens(ctx, n, s, dtype):
     s = {k: np.full(rows, v, np.int32 if k == "top_k" else np.float32) for k, v in s.items()}
     s["temperature"] = r.choice([0.3, 0.7, 1.0, 1.9], rows).astype(np.float32)
     T.check(T.draw(ctx, l, u, **s), l, u, **s)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("s", [{}, dict(min_p=0.5), dict(top_p=0.5), dict(top_k=2 ** 19 + 8192)])
+def test_numbers_on_the_border_of_two_slices(ctx, s, dtype):
+    """Rows of 128 slices, all logits equal: slices found by different waves, at each border, beside it and within."""
+    rows, vocab = 24, 2 ** 20
+    keep = vocab if "min_p" in s or not s else 2 ** 19 if "top_p" in s else s["top_k"]
+    at = np.concatenate([np.arange(8) * 8192 * 16, np.arange(8) * 8192 * 16 + 8191, np.arange(8) * 65536 + 70000]) % keep
+    l = np.full((rows, vocab), -2.5, np.float32)
+    l = S.f32_to_bf16(l) if dtype == "bf16" else l
+    u = (at / np.float64(keep)).astype(np.float32)
+    want = np.floor(np.float64(u) * keep).astype(np.int32)  # (u rounds where keep is no power of two)
+    s = {k: np.full(rows, v, np.int32 if k == "top_k" else np.float32) for k, v in s.items()}
+    ids, logp = T.draw(ctx, l, u, temperature=np.full(rows, 0.7, np.float32), **s)
+    np.testing.assert_array_equal(ids, want)
+    assert np.abs(logp + np.log(keep)).max() <= 2.0 ** -24 * np.log(keep) + 1e-9
