@@ -70,16 +70,20 @@ bool unregister_model(fa_model* m) {
   return take(*g_models, [m](const std::pair<fa_model*, fa_ctx*>& e) { return e.first == m; });
 }
 
-int refuse_capture(fa_ctx* ctx, hipStream_t s, const char* op) {
+int refuse_capture(fa_ctx* ctx, hipStream_t s, const char* op, const char* work_size) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   const hipError_t e = hipStreamIsCapturing(s, &st);
   if (e != hipSuccess) return set_error(ctx, FA_ERR_HIP, "%s: hipStreamIsCapturing: %s", op, hipGetErrorString(e));
-  if (st != hipStreamCaptureStatusNone)
+  if (st == hipStreamCaptureStatusNone) return FA_OK;
+  if (work_size)
     return set_error(ctx, FA_ERR_STATE,
-                     "%s: the context's stream is being captured into a HIP graph; this entry point may allocate "
-                     "and upload per-call data and cannot be captured (fa_similarities_topk_dev_noalloc can)",
-                     op);
-  return FA_OK;
+                     "%s: the context's stream is being captured into a HIP graph, which would keep the address of "
+                     "the context's scratch while a later call may replace it: pass work (%s)",
+                     op, work_size);
+  return set_error(ctx, FA_ERR_STATE,
+                   "%s: the context's stream is being captured into a HIP graph; this entry point may allocate "
+                   "and upload per-call data and cannot be captured (fa_similarities_topk_dev_noalloc can)",
+                   op);
 }
 
 int set_error(fa_ctx* ctx, int code, const char* fmt, ...) {

@@ -157,7 +157,7 @@ int fa_matmul_f8_dev(fa_ctx* ctx, int64_t m, int a_dtype, const void* a, int64_t
       return set_error(ctx, FA_ERR_ARG, "MatMulF8: work of %zu bytes, 16-byte aligned, is needed (%zu given)", need,
                        work_bytes);
   } else if (need) {
-    if ((rc = fa::refuse_capture(ctx, ctx->stream, "MatMulF8 without work"))) return rc;
+    if ((rc = fa::refuse_capture(ctx, ctx->stream, "MatMulF8", "fa_matmul_f8_work"))) return rc;
     if ((rc = ctx->slot(S_F8).ensure(ctx, need))) return rc;
     work = ctx->slot(S_F8).ptr;
   }

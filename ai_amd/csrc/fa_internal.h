@@ -91,8 +91,9 @@ bool unregister_model(fa_model* m);
 void model_release(fa_model* m);
 
 // FA_ERR_STATE when stream s is being captured into a HIP graph: the entry
-// points that grow buffers or upload per-call plans cannot be captured.
-int refuse_capture(fa_ctx* ctx, hipStream_t s, const char* op);
+// points that grow buffers or upload per-call plans cannot be captured. work_size:
+// the function that gives the size of the work with which this one can.
+int refuse_capture(fa_ctx* ctx, hipStream_t s, const char* op, const char* work_size = nullptr);
 
 // Copies host data into scratch slot `slot` (grown as needed) and returns
 // the device pointer via *out.

@@ -401,7 +401,7 @@ int fa_kv_attention_dev(fa_ctx* ctx, const fa_kv_cache* cache, const fa_kv_batch
                        work_bytes);
     if (need && (rc = fa::launch_zero(ctx, work, fa::kKvCountBytes, ctx->stream))) return rc;
   } else if (need) {
-    if ((rc = fa::refuse_capture(ctx, ctx->stream, "KVAttention without work"))) return rc;
+    if ((rc = fa::refuse_capture(ctx, ctx->stream, "KVAttention", "fa_kv_attention_work"))) return rc;
     if ((rc = own_parts(ctx, need, &work))) return rc;
   }
   return fa::launch_kv_attention(ctx, a, work, ctx->stream);

@@ -72,7 +72,7 @@ int fa_sample_dev(fa_ctx* ctx, int64_t rows, int64_t vocab, int dtype, const voi
       return set_error(ctx, FA_ERR_ARG, "%s: work of %zu bytes, 16-byte aligned, is needed (%zu given)", kOp, need,
                        work_bytes);
   } else if (need) {
-    if ((rc = fa::refuse_capture(ctx, ctx->stream, "Sample without work"))) return rc;
+    if ((rc = fa::refuse_capture(ctx, ctx->stream, kOp, "fa_sample_work"))) return rc;
     if ((rc = ctx->slot(S_SAMPLE).ensure(ctx, need))) return rc;
     work = ctx->slot(S_SAMPLE).ptr;
   }
