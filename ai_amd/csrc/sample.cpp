@@ -57,7 +57,7 @@ int fa_sample_work(int64_t rows, int64_t vocab, size_t* bytes) {
   *bytes = 0;
   const int rc = check_sizes(nullptr, rows, vocab);
   if (rc || rows == 0) return rc;
-  *bytes = fa::sample_scratch(rows, vocab);
+  *bytes = fa::sample_scratch(rows, vocab, true);
   return FA_OK;
 }
 
@@ -66,7 +66,8 @@ int fa_sample_dev(fa_ctx* ctx, int64_t rows, int64_t vocab, int dtype, const voi
   int rc = check(ctx, rows, vocab, dtype, logits, ld, u, ids);
   if (rc || rows == 0) return rc;
   FA_HIP_CHECK(ctx, hipSetDevice(ctx->device));
-  const size_t need = fa::sample_scratch(rows, vocab);
+  const fa_sampling h = s ? *s : fa_sampling{};
+  const size_t need = fa::sample_scratch(rows, vocab, fa::sample_filters(h));
   if (work) {
     if (work_bytes < need || (reinterpret_cast<uintptr_t>(work) & 15))
       return set_error(ctx, FA_ERR_ARG, "%s: work of %zu bytes, 16-byte aligned, is needed (%zu given)", kOp, need,
@@ -76,7 +77,7 @@ int fa_sample_dev(fa_ctx* ctx, int64_t rows, int64_t vocab, int dtype, const voi
     if ((rc = ctx->slot(S_SAMPLE).ensure(ctx, need))) return rc;
     work = ctx->slot(S_SAMPLE).ptr;
   }
-  const fa::SampleArgs a = {rows, vocab, dtype, logits, ld, s ? *s : fa_sampling{}, u, ids, logp};
+  const fa::SampleArgs a = {rows, vocab, dtype, logits, ld, h, u, ids, logp};
   return fa::launch_sample(ctx, a, work, ctx->stream);
 }
 
@@ -102,7 +103,7 @@ int fa_sample(fa_ctx* ctx, int64_t rows, int64_t vocab, int dtype, const void* l
     if (from[i])
       FA_HIP_CHECK(ctx, hipMemcpyAsync(d + i * rows, from[i], (size_t)rows * 4, hipMemcpyHostToDevice, ctx->stream));
   }
-  if ((rc = ctx->slot(S_SAMPLE).ensure(ctx, fa::sample_scratch(rows, vocab)))) return rc;
+  if ((rc = ctx->slot(S_SAMPLE).ensure(ctx, fa::sample_scratch(rows, vocab, fa::sample_filters(h))))) return rc;
   fa::SampleArgs a = {rows, vocab, dtype, dl, ld, {}, (const float*)at[4], (int32_t*)(d + 5 * rows), d + 6 * rows};
   a.s = {(const float*)at[0], (const int32_t*)at[1], (const float*)at[2], (const float*)at[3]};
   if ((rc = fa::launch_sample(ctx, a, ctx->slot(S_SAMPLE).ptr, ctx->stream))) return rc;

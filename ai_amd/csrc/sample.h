@@ -15,7 +15,9 @@ struct SampleArgs {
   int32_t* ids;
   float* logp;  // may be null
 };
-size_t sample_scratch(int64_t rows, int64_t vocab);
+// Whether tokens may be dropped from any row.
+inline bool sample_filters(const fa_sampling& s) { return s.top_k || s.top_p || s.min_p; }
+size_t sample_scratch(int64_t rows, int64_t vocab, bool filtered);
 int64_t sample_grid(int64_t rows, int64_t vocab);  // workgroups of a launch
 int launch_sample(fa_ctx* ctx, const SampleArgs& a, void* work, hipStream_t s);
 

@@ -60,13 +60,14 @@ struct Cut {
 
 struct Plan {
   int per, slices;  // tokens of a slice (a power of two), slices of a row
+  int room;         // tokens that a slice may list: all of its own
   int vec;          // rows aligned for 16-byte loads
   Slice* slice;     // [rows][slices]
   Cut* cut;         // [rows]
   double* mass;     // [rows][slices][kBins] weights of the bins up to each, relative to the slice's first token
   uint32_t* count;  // likewise tokens (without top-k: bins with tokens)
   uint32_t* listed; // [rows][slices]
-  uint16_t* list;   // [rows][slices * per]
+  uint16_t* list;   // [rows][slices * room]
 };
 
 // ---- order, weights, bins --------------------------------------------------------------
@@ -513,7 +514,7 @@ __global__ __launch_bounds__(kScan) void gather_kernel(SampleArgs a, Plan p) {
   if (__syncthreads_or(any)) {
     Held<T, E> h;
     h.load((const T*)a.logits + row * a.ld + first, min(p.per, (int)a.vocab - first), p.vec);
-    uint16_t* list = p.list + (row * p.slices + s) * p.per;
+    uint16_t* list = p.list + (row * p.slices + s) * p.room;
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const bool in = counts(h.v[e], most) && c.listed(bin_of(h.v[e], r.inv, c.step));
@@ -551,7 +552,7 @@ __device__ __forceinline__ void each_in_memory(const SampleArgs& a, const Plan& 
   const T* l = (const T*)a.logits + row * a.ld;
   for (int s = threadIdx.x >> 6; s < p.slices; s += kFinish / 64) {
     const uint32_t from = mem.start[s], m = mem.start[s + 1] - from;
-    const uint16_t* list = p.list + (row * p.slices + s) * p.per;
+    const uint16_t* list = p.list + (row * p.slices + s) * p.room;
     for (uint32_t i = threadIdx.x & 63; i < m; i += 64 * kAhead) {  // several under way at once
       int id[kAhead];
       T v[kAhead];
@@ -885,7 +886,8 @@ int per_of(int64_t rows, int64_t vocab) {
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-size_t lay_out(int64_t rows, int64_t vocab, char* work, Plan* p) {
+// What rows without filters use comes first, and is all that they need.
+size_t lay_out(int64_t rows, int64_t vocab, bool filtered, char* work, Plan* p) {
   const int per = per_of(rows, vocab);
   const int64_t slices = (vocab + per - 1) / per, all = rows * slices;
   size_t at = 0;
@@ -894,13 +896,16 @@ size_t lay_out(int64_t rows, int64_t vocab, char* work, Plan* p) {
     at += align256(bytes);
     return work ? work + here : nullptr;
   };
-  Plan q = {per, (int)slices, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+  const int room = (int)std::min<int64_t>(per, vocab);
+  Plan q = {per, (int)slices, room, 0, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
   q.slice = (Slice*)take(all * sizeof(Slice));
-  q.cut = (Cut*)take(rows * sizeof(Cut));
-  q.mass = (double*)take(all * kBins * 8);
-  q.count = (uint32_t*)take(all * kBins * 4);
-  q.listed = (uint32_t*)take(all * 4);
-  q.list = (uint16_t*)take(all * per * 2);
+  if (filtered) {
+    q.cut = (Cut*)take(rows * sizeof(Cut));
+    q.mass = (double*)take(all * kBins * 8);
+    q.count = (uint32_t*)take(all * kBins * 4);
+    q.listed = (uint32_t*)take(all * 4);
+    q.list = (uint16_t*)take(all * room * 2);
+  }
   if (p) *p = q;
   return at;
 }
@@ -909,7 +914,7 @@ template <typename T, int E>
 void launch_e(const SampleArgs& a, const Plan& p, hipStream_t s) {
   const unsigned grid = (unsigned)(a.rows * p.slices);
   scan_kernel<T, E><<<grid, kScan, 0, s>>>(a, p);
-  if (a.s.top_k || a.s.top_p || a.s.min_p) {
+  if (sample_filters(a.s)) {
     join_kernel<<<(unsigned)a.rows, kBins, 0, s>>>(a, p);
     gather_kernel<T, E><<<grid, kScan, 0, s>>>(a, p);
   }
@@ -926,7 +931,9 @@ void launch_t(const SampleArgs& a, Plan p, hipStream_t s) {
 
 }  // namespace
 
-size_t sample_scratch(int64_t rows, int64_t vocab) { return lay_out(rows, vocab, nullptr, nullptr); }
+size_t sample_scratch(int64_t rows, int64_t vocab, bool filtered) {
+  return lay_out(rows, vocab, filtered, nullptr, nullptr);
+}
 
 int64_t sample_grid(int64_t rows, int64_t vocab) {
   const int per = per_of(rows, vocab);
@@ -935,7 +942,7 @@ int64_t sample_grid(int64_t rows, int64_t vocab) {
 
 int launch_sample(fa_ctx* ctx, const SampleArgs& a, void* work, hipStream_t s) {
   Plan p;
-  lay_out(a.rows, a.vocab, static_cast<char*>(work), &p);
+  lay_out(a.rows, a.vocab, sample_filters(a.s), static_cast<char*>(work), &p);
   if (a.dtype == FA_DT_F32) launch_t<float>(a, p, s);
   else launch_t<uint16_t>(a, p, s);
   FA_CHECK_LAUNCH(ctx);
