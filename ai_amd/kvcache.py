@@ -174,7 +174,7 @@ class KVCache:
         dims = self.head_dim if dims is None else int(dims)
         if not -_I32 <= dims <= _I32:
             _fail(f"{what}: {dims} rotary dims")
-        rows = len(np.asarray(k))
+        rows = len(np.atleast_1d(k))
         if q is not None:
             q = _rows(q, what, None, self.head_dim)
             if len(q) != rows:
