@@ -181,7 +181,7 @@ class KVCache:
                 _fail(f"{what}: {len(q)} queries for {rows} keys")
         if positions is not None:
             positions = np.asarray(positions)
-            if positions.shape != (rows,) or (rows and (positions.dtype.kind not in "iu" or positions.min() < -_I32 or
+            if positions.shape != (rows,) or (rows and (positions.dtype.kind not in "iu" or positions.min() < -_I32 - 1 or
                                                         positions.max() > _I32)):
                 _fail(f"{what}: want {rows} positions in 32 bits, got {list(positions.shape)} {positions.dtype}")
             positions = np.ascontiguousarray(positions, np.int32)

@@ -24,3 +24,14 @@ def test_keys_of_another_shape(cache, k):
     """An error of the cache's kind, whatever is given for rows."""
     with pytest.raises(TensorError, match="want"):
         cache.AppendRoPE([cache.Add()], None, k, k, base=1e4)
+
+
+def test_positions_of_all_32_bits(cache):
+    """Both ends reach the library (which has no context here); one past either is refused."""
+    s = cache.Add()
+    k = np.zeros((2, 1, 8), np.float32)
+    with pytest.raises(TensorError, match="ctx is NULL"):
+        cache.AppendRoPE([s], None, k, k, [2], base=1e4, positions=[2 ** 31 - 1, -2 ** 31])
+    for p in (2 ** 31, -2 ** 31 - 1):
+        with pytest.raises(TensorError, match="positions"):
+            cache.AppendRoPE([s], None, k, k, [2], base=1e4, positions=[0, p])
