@@ -88,6 +88,8 @@ __global__ __launch_bounds__(256) void f8_write_kernel(F8View w, const T* __rest
   }
 }
 
+// Bound by memory, a word of four codes a thread: 8192 x 8192 to float32 68 us, 4.9 TB/s, to
+// bf16 38.
 template <typename T>
 __global__ __launch_bounds__(256) void f8_read_kernel(F8View w, T* __restrict__ out, int64_t ldo, int kb, int ks,
                                                       bool vec) {
@@ -176,8 +178,10 @@ __device__ __forceinline__ void put4(const GemmParams& p, T* c, const int64_t (&
 // into reading W, not into products); the waves of a column group add up through LDS, in
 // their order. Both operands come straight from memory in the units' order, four blocks
 // under way: a lane (row r of 16, g of 4) holds bytes 16 g .. and 64 + 16 g .. of its
-// row's block, so that four lanes read 64 bytes together. Bound by latencies: 16 x 4096 x
-// 4096 takes 9.8 us (and the launch before it, which quantises A, 2.8).
+// row's block, so that four lanes read 64 bytes together. 16 x 4096 x 4096 takes 9.7 us (and
+// the launch before it, which quantises A, 3.0): each wave's four blocks are one round of
+// loads, so what is left is that round (16 rows an instruction, a byte for each scale),
+// widening both operands and the join; which of them was not taken apart.
 constexpr int kFewWaves = 8, kFewDeep = 4;
 template <typename TC>
 __device__ __forceinline__ void f8_few(const GemmParams& p, TC* c) {
@@ -310,10 +314,12 @@ __device__ __forceinline__ bool join(const GemmParams& p, f32x16& x, int tile, i
 // next half block are read while the products of this one run.
 //
 // Large tiles are bound by products and two blocks are enough: 8192 x 8192 x 8192 with a
-// residual takes 550 us, 2.0 PFLOP/s (its products alone at 2.76), 4096^3 81. Small ones
+// residual takes 545 to 560 us, 2.0 PFLOP/s (its products alone at 2.76), without it 509,
+// 4096^3 76 (quantising A among each: 38 of 8192^3). Small ones
 // wait for memory, a latency for each D - 1 blocks: 128 x 4096 x 4096 22 us with two
-// blocks, 14 with four. 1 x 262144 x 768 in float32 takes 46 us, 4.4 TB/s; 16 x 16384 x
-// 4096 16 us, 4.1 TB/s.
+// blocks, 13 with four. 1 x 262144 x 768 in float32 takes 45 us, 4.6 TB/s; 16 x 16384 x
+// 4096 16 us, 4.1 TB/s. float32 results, whose operands every wave widens for itself:
+// 8192^3 991 us, 1.1 PFLOP/s, 4096^3 146.
 template <int BM, int BN, int WM, int D, typename TC>
 __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m, int tiles_n) {
   constexpr int WN = 4 / WM, MW = BM / WM, NW = BN / WN;  // waves each way, their parts of the tile

@@ -90,10 +90,10 @@ __device__ __forceinline__ int stored_exp(float s) {
 // One workgroup writes one (block, head, keys or values): all its new values
 // in registers, one reduction for the scale, one store. Bytes are read and
 // written once. Prompts (16 of up to 2048 tokens, 8 heads of 128 dims in bf16) take
-// 29 us one after another, where the bytes take 28 at a large copy's rate (42 with each
-// load widened, and so waited for, before the next; over head dims of 32 to 512 in either
-// type that order of loads is 0.99 to 1.33 times as fast for prompts and chunks, and costs
-// one token up to 0.13 of 4 us). Slices that a head does not have are jumped over as a
+// 35 us, where the bytes take 28 at a large copy's rate (43 with each load widened, and so
+// waited for, before the next; over head dims of 32 to 512 in either type that order of
+// loads is 1.0 to 1.3 times as fast for prompts and chunks, and costs one token up to 0.13
+// of 4 us). Slices that a head does not have are jumped over as a
 // whole (64 single tokens of 320 dims 7.7 -> 7.4 us). Single tokens are bound by the
 // chain of dependent loads (sequence, block, row) and the write-back of the 128 lines
 // that one token's values touch in a head (64 sequences, one float32 token each,
@@ -387,15 +387,18 @@ __device__ __forceinline__ void turn_rows(const KvArgs& a, const KvRopeArgs& r, 
 // into float32 in LDS, each pair by one thread, and stored from there as the writer's.
 //
 // Bound by memory: prompts (16 of up to 2048 tokens, 32 query and 8 key/value heads of
-// 128 dims in bf16) take 138 us, 3.8 TB/s, where a large copy's rate gives 105; the
-// queries alone take 92 of 77, the keys and values 56 of 29 (values 23). Chunks of 512
-// in float32, half of each head turning: 14 us of 8. Single tokens wait for the chain
-// sequence, block, row, store: 64 sequences 9.2 us, one 8.4. What it took, in us of the
+// 128 dims in bf16) take 129 us, 4.0 TB/s, where a large copy's rate gives 102. With 16
+// query and 4 key/value heads of 256 dims 154 us of 102, 230 of 195 in float32; 8 and 2
+// of 512 dims 233 of 102 and 287 of 195: every workgroup is held to the keys' LDS (68 KB
+// at 256 dims, two on a CU; 132 at 512, one). Chunks of 512
+// in float32, half of each head turning: 13 us of 8. Single tokens wait for the chain
+// sequence, block, row, store: 64 sequences 8.2 us, one 7.0. What it took, in us of the
 // prompts: keys turned where the writer loads them, each pair twice, and queries by a
 // thread per four dims 326; cosines shared by heads and pairs turned once, but loads
 // waited for one by one 212; cosines' factors and all loads of a thread under way
 // before the first is used 161; the next heads' loads too, 16 heads a job 138 (8 heads
-// 146: more cosines; 32 leave too few workgroups: the queries alone by 13% slower).
+// 146: more cosines; 32 leave too few workgroups: the queries alone by 13% slower);
+// all of a value job's loads under way too 129.
 template <typename T, int NCM, bool WIDE>
 __global__ __launch_bounds__(256, NCM <= 2 ? 4 : 2) void kv_write_rope_kernel(KvArgs a, KvRopeArgs r, int q_parts,
                                                                               int q_heads, bool by_row, bool vec,

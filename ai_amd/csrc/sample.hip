@@ -261,8 +261,8 @@ struct Held {
 };
 
 // Bound by its arithmetic where rows are many: an exponential in float64 and two
-// additions in LDS a token (256 rows of 262144 in float32 125 us, 2.1 TB/s, where the
-// bytes take 54; without filters nothing is added in LDS). One such row: 9 us, latencies.
+// additions in LDS a token (256 rows of 262144 in float32 124 us, 2.2 TB/s, where the
+// bytes take 53; without filters nothing is added in LDS). One such row: 9 us, latencies.
 template <typename T, int E>
 __global__ __launch_bounds__(kScan) void scan_kernel(SampleArgs a, Plan p) {
   __shared__ uint64_t red[kScan / 64];
@@ -657,8 +657,9 @@ __device__ uint64_t select_token(const SampleArgs& a, const Plan& p, int64_t row
 }
 
 // One workgroup a row, bound by its own chain: two selections, each of passes over the
-// listed tokens, the slices' weights, the walk. One row of 262144 21 us, 64 of 32000 31, 256
-// of 262144 91; 37 of 49999 without filters 11.
+// listed tokens, the slices' weights, the walk. One row of 262144 22 us, 64 of 32000 31, 256
+// of 262144 92 (rows of more than kCached listed tokens read them from memory in every
+// pass, and the slowest row is the launch's time); 37 of 49999 without filters 12.
 template <typename T, int E>
 __global__ __launch_bounds__(kFinish) void finish_kernel(SampleArgs a, Plan p) {
   __shared__ FinishMem mem;
