@@ -311,7 +311,7 @@ __device__ __forceinline__ bool join(const GemmParams& p, f32x16& x, int tile, i
 // once, and start the loads of the block D on into its place. Rows lie 128 bytes
 // apart, their 16-byte pieces permuted by the row (piece j at j ^ (row & 7)), so that
 // eight lanes reading the same piece of eight rows use all banks. Operands of the
-// next half block are read while the products of this one run.
+// next half block are read while the products of this one run. F8: on the 8-bit units.
 //
 // Large tiles are bound by products and two blocks are enough: 8192 x 8192 x 8192 with a
 // residual takes 545 to 560 us, 2.0 PFLOP/s (its products alone at 2.76), without it 509,
@@ -320,11 +320,10 @@ __device__ __forceinline__ bool join(const GemmParams& p, f32x16& x, int tile, i
 // blocks, 13 with four. 1 x 262144 x 768 in float32 takes 45 us, 4.6 TB/s; 16 x 16384 x
 // 4096 16 us, 4.1 TB/s. float32 results, whose operands every wave widens for itself:
 // 8192^3 991 us, 1.1 PFLOP/s, 4096^3 146.
-template <int BM, int BN, int WM, int D, typename TC>
+template <int BM, int BN, int WM, int D, bool F8, typename TC>
 __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m, int tiles_n) {
   constexpr int WN = 4 / WM, MW = BM / WM, NW = BN / WN;  // waves each way, their parts of the tile
   constexpr int FM = MW / 32, FN = NW / 32, NA = BM * 8 / 256, NB = BN * 8 / 256;
-  constexpr bool F8 = sizeof(TC) == 2;  // on the 8-bit units
   constexpr bool kJoins = FM * FN == 1;  // K may be split
   constexpr int kStage = (BM + BN) * kF8Block;
   __shared__ __attribute__((aligned(16))) uint8_t S0[kStage], S1[kStage], S2[D > 2 ? kStage : 16],
@@ -536,10 +535,10 @@ __device__ __forceinline__ void f8_tile(const GemmParams& p, TC* c, int tiles_m,
 }
 
 // (A kernel whose own body holds arrays of dependent bounds in lambdas loses its host stub.)
-template <int BM, int BN, int WM, int D, typename TC>
+template <int BM, int BN, int WM, int D, bool F8, typename TC>
 __global__ __launch_bounds__(256, (BM + BN) * D > 512 ? 1 : 2) void f8_tile_kernel(GemmParams p, TC* c, int tiles_m,
                                                                                  int tiles_n) {
-  f8_tile<BM, BN, WM, D, TC>(p, c, tiles_m, tiles_n);
+  f8_tile<BM, BN, WM, D, F8, TC>(p, c, tiles_m, tiles_n);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -588,9 +587,15 @@ int64_t a_stride(int64_t k) { return f8_kp(k) + (f8_kp(k) % 2048 == 0 ? kF8Block
 namespace {
 
 // Tiles of a product, and the parts that K is split into. us, measured on both sides:
-// - Up to 16 rows and 2^24 weights the kernel for few rows, else tiles: 16 x 4096 x 4096
-//   12.4 and 13.6, 1 x 4096 x 4096 11.5 and 14; 1 x 32768 x 1024 16.7 and 11.4, 1 x 262144
-//   x 768 51 and 46.
+// - Up to 16 rows and 2^24 weights, whose reading takes about a launch's time, on the bf16
+//   units whatever the result's type. Of these the kernel for few rows while its workgroups of 16
+//   columns are at most two for each CU and a wave has at most six blocks, else tiles of 32
+//   x 128: 16 x 4096 x 4096 10.9 and 11.2, 1 x 4096 x 4096 8.7 and 10.8, 1 x 2048 x 2048 7.2
+//   and 9.3; 16 x 8192 x 1024 7.2 and 7.7, 16 x 9000 x 1024 8.4 and 7.8, 16 x 16384 x 1024
+//   10.5 and 8.0; 1 x 1024 x 6144 9.7 and 11.1 (16 rows 12.4 and 11.5), 1 x 512 x 8192 11.5
+//   and 11.6 (16 rows 15.9 and 12.1), 16 x 1024 x 16384 26.7 and 14.7. Above 2^24 weights:
+//   16 x 5000 x 4096 16.2 and 11.8, 1 x 4096 x 8192 12.8 and 14.9, 16 rows 16.7 and 15.5, 1 x
+//   32768 x 1024 14.4 and 9.9.
 // - Tiles of 128 and of 256 (bf16) where they fill the card; of 128 with four blocks held,
 //   for bf16, where they are at most one for each CU, and that for 3 of 4: 512 x 8192 x
 //   8192 61 and 47, 896 x 4096 x 4096 in tiles of 64 40, so 29, but 512 x 4096 x 4096 (128
@@ -605,14 +610,16 @@ constexpr int kCUs = 256;  // of the card
 struct Plan {
   int tile;   // 256, 128, 64, 32 (x 128); 0: few rows
   bool deep;  // four blocks held of tiles of 128
+  bool exact;  // on the bf16 units
   int parts, per;
   int64_t tiles;
 };
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool bf16) {
   auto tiles = [&](int64_t bm, int64_t bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
   const int kb = (int)(f8_kp(k) / kF8Block);
-  Plan p = {0, false, 1, kb, 0};
-  if (m <= 16 && n * kb <= 131072) return p;
+  const bool few = m <= 16 && n * kb <= 131072;
+  Plan p = {0, false, few || !bf16, 1, kb, 0};
+  if (few && n <= 8192 && kb <= 48) return p;
   const int64_t large = m > 64 ? tiles(128, 128) : 0;
   if (large >= kCUs || (bf16 && large * 4 >= kCUs * 3)) {
     p.tile = bf16 && m > 128 && tiles(256, 256) >= kCUs ? 256 : 128;
@@ -641,10 +648,10 @@ int64_t f8_grid(int64_t m, int64_t n) { return ((m + 15) / 16) * ((n + 63) / 64)
 
 namespace {
 
-template <int BM, int BN, int WM, int D, typename TC>
+template <int BM, int BN, int WM, int D, typename TC, bool F8 = sizeof(TC) == 2>
 void launch_tiles(const GemmParams& p, TC* c, hipStream_t s) {
   const int tm = (int)((p.m + BM - 1) / BM), tn = (int)((p.n + BN - 1) / BN);
-  f8_tile_kernel<BM, BN, WM, D, TC><<<(unsigned)(tm * tn * p.parts), 256, 0, s>>>(p, c, tm, tn);
+  f8_tile_kernel<BM, BN, WM, D, F8, TC><<<(unsigned)(tm * tn * p.parts), 256, 0, s>>>(p, c, tm, tn);
 }
 
 template <typename TC>
@@ -659,7 +666,8 @@ void launch_gemm_t(const GemmParams& p, TC* c, const Plan& plan, hipStream_t s) 
   } else if (tile == 64) {
     launch_tiles<64, 64, 2, 4>(p, c, s);
   } else if (tile == 32) {
-    launch_tiles<32, 128, 1, 4>(p, c, s);
+    if (plan.exact) launch_tiles<32, 128, 1, 4, TC, false>(p, c, s);
+    else launch_tiles<32, 128, 1, 4>(p, c, s);
   } else {
     GemmParams q = p;
     q.split = kFewWaves;
