@@ -178,7 +178,8 @@ __device__ __forceinline__ uint64_t to_int(double x) {
   return (uint64_t)__double_as_longlong(x + 0x1p52) - (uint64_t)0x4330000000000000ull;
 }
 constexpr int kUnit = 48;  // a bin's weights are held in units of 2^-48 of its middle: 2^14 of them fit
-// Sums are right to 1e-13: weights to 2^-48, a thousand additions. Two that the definition
+// Sums are right to 1e-13: weights to 2^-48, a thousand additions (of more than 2^19 listed
+// tokens to 2^-37, but for weights of 1, which are whole numbers). Two that the definition
 // has equal (of equal logits, whose weights are 1) may differ by that much either way, so
 // a sum reaches a bound from this much below it on, and exceeds it from this much above.
 constexpr double kNear = 1e-12;
